@@ -17,7 +17,7 @@ own = False
 
 DTYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
 CODES = {"f32": 0, "f16": 1, "bf16": 30}      # ggml type numbers
-EPS = 1e-5
+EPS = torch.tensor(1e-5, dtype=torch.float32).item()      # as the call takes it
 
 
 def listed():
