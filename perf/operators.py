@@ -192,7 +192,7 @@ def _plain_norm(c, s):
         rows, n, win = c["rows"], c["n"], c["window"]
         pad = -n % win
         amax = torch.nn.functional.pad(y.abs(), (0, pad)).view(rows, -1, win).amax(-1)
-        step = amax / 127.0
+        step = amax / torch.full_like(amax, 127.0)      # (by a number, torch multiplies by its reciprocal)
         inv = torch.where(step != 0, 1.0 / step, torch.zeros_like(step))
         of = torch.arange(n, device="cuda") // win
         v = y * inv[:, of]
@@ -306,8 +306,8 @@ def exact(case, seed):
             full = torch.zeros(rows, nw * win, device="cuda")
             full[:, :n] = yf
             parts = full.view(rows, nw, win)
-            step = parts.abs().max(-1, keepdim=True).values / 127.0
-            v = (parts * torch.where(step > 0, step.reciprocal(), step)).double()
+            step = (parts.abs().max(-1, keepdim=True).values.double() / 127.0).float()
+            v = (parts * torch.where(step > 0, step.double().reciprocal().float(), step)).double()
             q = torch.sign(v) * torch.floor(v.abs() + 0.5)
             vals = (q * step.double()).view(rows, -1)[:, :n]
             scales = step.expand(rows, nw, win // 32).reshape(rows, -1)[:, : n // 32]
