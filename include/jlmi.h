@@ -42,11 +42,12 @@ extern "C" {
 #define JL_ERR_HIP (-2)
 #define JL_ERR_NOMEM (-3)
 
-#define JL_TYPE_F32 0   /* router weights only (jl_moe_logits_dev) */
+#define JL_TYPE_F32 0   /* plain values: router weights (jl_moe_logits_dev), normed rows, adapters */
 #define JL_TYPE_F16 1
 #define JL_TYPE_Q8_0 8
 #define JL_TYPE_Q4_K 12
 #define JL_TYPE_Q6_K 14
+#define JL_TYPE_BF16 30 /* normed rows and adapters */
 #define JL_TYPE_MXFP4 39
 
 typedef struct jl_ctx jl_ctx;
@@ -221,6 +222,36 @@ int jl_matmul_packed(jl_ctx *ctx, float *out, int type, const uint32_t *qs, cons
 int jl_quantize_act_dev(jl_ctx *ctx, const float *x, int ntok, int k, int8_t *q,
                         float *as, float *sum16, void *stream);
 
+/* Rows normed between two projections: the block's residual add, RMSNorm and the activation quantizer in one pass over any
+ * number of rows (RMSNormQuantRows, jit/gpu/kernels/elem.go:252-267; one row of a decode matvec can have its norm ride on the
+ * launch instead, jl_matvec_group_dev).  For each row of n elements
+ *     h = resid + alpha * x                  f32, product and sum each rounded; resid null: h = x
+ *     y = f32(h * w / sqrt(mean(h^2) + eps)) in f64, narrowed once; w null: ones
+ * x [rows][x_stride] of x_type and y [rows][y_stride] of y_type (JL_TYPE_F32, _F16, _BF16; strides in elements, 0 = n);
+ * resid and resid_out [rows][resid_stride] f32, w [n] f32.  Outputs, each null where it is not wanted, one at least:
+ * resid_out receives h (it may be resid; only with resid given), y the normed row rounded to its type, q / as / sum16 (all or none; n % 32 == 0, q 16-byte
+ * aligned) the int8 form jl_quantize_act_dev makes of the f32 y, bit for bit, with the context's activation window.  y may be
+ * x where type and stride are the same; no other operands overlap.  What lies between a row's end and the next is left as it
+ * was.  Rows on 16-byte boundaries are read in 16-byte loads, any others an element at a time.  n <= 65536. */
+typedef struct jl_norm_rows {
+    int rows, n;
+    const void *x;
+    int x_type;
+    size_t x_stride;
+    const float *resid;
+    size_t resid_stride;
+    float alpha;
+    float *resid_out;
+    const float *w;
+    float eps;
+    void *y;
+    int y_type;
+    size_t y_stride;
+    int8_t *q;
+    float *as, *sum16;
+} jl_norm_rows;
+int jl_norm_rows_dev(jl_ctx *ctx, const jl_norm_rows *g, void *stream);
+
 /* quant.Dequant32 (format/quant/dequant.go:50): n elements of GGUF blocks -> f32,
  * bit-identical to the reference decoder. */
 int jl_dequant_dev(jl_ctx *ctx, int type, const void *src, float *dst, size_t n,
@@ -335,6 +366,38 @@ int jl_matvec_packed_group(jl_ctx *ctx, int n, float *const *outs, const int *ty
                            const uint32_t *const *qs, const uint32_t *const *d, const uint32_t *const *sc,
                            const int *row, const int *stride, const int *rows, const float *x, int k,
                            const float *act_up, int act, float *resid, float alpha);
+
+/* Low-rank adapters of many requests beside the projections they share: token t with id a = ids[t] gets
+ *     out[i][t] = base[i][t] + scale[a] * B_i[a] (A_i[a] x[t])
+ * for n <= JL_MAX_GROUP projections that read one x (a block's q, k and v; its gate and up; one projection) -- base[i] is what
+ * jl_matmul_dev, jl_matvec_group_dev or their packed and MXFP4 forms made of the shared weights, [ntok][rows[i]] f32; it may be
+ * out[i] (added in place), and null stands for zeros.  a[i] [n_adapter][rank][k] and b[i] [n_adapter][rows[i]][rank] of `type`
+ * (JL_TYPE_F32, _F16, _BF16); x [ntok][k] of x_type (the same three).  ranks, when given, holds each adapter's own rank (more
+ * than `rank` counts as `rank`): rows of A and columns of B from there on are not used.  scale null: ones.  A token whose id is
+ * n_adapter or more has no adapter and gets base alone, as does one whose adapter has rank 0.  ids, ranks and scale are device
+ * memory, read by the kernels.  Products and sums are f32 whatever the types.  k % 32 == 0, rank <= 512; a, b and x 16-byte
+ * aligned.  The workspace (ntok * n * rank floats at most) is the context's, grown on demand; a buffer that is outgrown lives until the
+ * context goes, so a captured graph that holds its address stays valid.  jl_reserve_adapters sizes it ahead of time.
+ * No counterpart in the reference. */
+typedef struct jl_adapter_group {
+    int n;
+    float *out[JL_MAX_GROUP];
+    const float *base[JL_MAX_GROUP];
+    int rows[JL_MAX_GROUP];
+    const void *a[JL_MAX_GROUP], *b[JL_MAX_GROUP];
+    int type;
+    int n_adapter, rank;
+    const uint32_t *ranks;
+    const float *scale;
+    const void *x;
+    int x_type;
+    int k;
+    const uint32_t *ids;
+    int ntok;
+} jl_adapter_group;
+int jl_adapter_group_dev(jl_ctx *ctx, const jl_adapter_group *g, void *stream);
+/* Sizes the workspace for jl_adapter_group_dev calls of up to max_tok tokens, n projections and rank max_rank. */
+int jl_reserve_adapters(jl_ctx *ctx, int max_tok, int n, int max_rank);
 
 /* JIT.MatMulPacked / MatMul semantics on resident operands (engine/nn/packedmm.go:23,
  * matmul.go:27): x [ntok][k] f32 -> out [ntok][nrows], every token quantized on
@@ -527,6 +590,33 @@ int jl_moe_logits_dev(jl_ctx *ctx, float *logits, int wtype, const void *w, cons
  * of each row) and wt [rows][k_used].  n_expert <= 1024, k_used <= 16. */
 int jl_moe_route_dev(jl_ctx *ctx, const float *logits, int rows, int n_expert, int k_used,
                      uint32_t *sel, int sel_stride, float *wt, void *stream);
+
+/* The router in its general form, beside jl_moe_route_dev (softmax, no bias, no groups; the reference's MoERouter has the fields
+ * internal/oracle/moe.go:197-327 describes).  Per row of logits [rows][n_expert]:
+ *     s = softmax over all experts (JL_SCORE_SOFTMAX) or 1 / (1 + e^-l) (JL_SCORE_SIGMOID), in f64, narrowed to f32
+ *     c = s + bias[e]                                (f32; bias null: c = s): what the selection goes by, never the weight
+ *     n_group > 1: expert e is of group e / (n_expert / n_group); a group is worth its best c (group_top 1) or the sum of its
+ *         two best (2; a missing second adds nothing), and only the k_group best groups' experts are selected from
+ *     the k_used largest c by (c descending, index ascending); groups likewise
+ *     weight = s / (sum of the selected s in selection order + 1e-20) where renorm is not 0, else s; times scale
+ * An expert whose logit is -infinity, or whose c is -infinity (a bias of -infinity takes it out of service) or no number, is
+ * never selected; a softmax row that holds a NaN or +infinity has no numbers and selects nothing.  A row with fewer experts to
+ * select than k_used has the id n_expert and weight 0 in the places left over -- an id no expert has, which
+ * jl_moe_ffn_dev and the grouping leave out.  Fills sel [rows][sel_stride] (first k_used of each row) and wt [rows][k_used].
+ * n_expert <= 1024, k_used <= 16, n_group <= 64 and a divisor of n_expert, k_used <= k_group * (n_expert / n_group);
+ * n_group 0 or 1: no groups. */
+#define JL_SCORE_SOFTMAX 0
+#define JL_SCORE_SIGMOID 1
+typedef struct jl_moe_select {
+    int score;
+    const float *bias;
+    int n_group, k_group, group_top;
+    int k_used;
+    int renorm;
+    float scale;
+} jl_moe_select;
+int jl_moe_select_dev(jl_ctx *ctx, const float *logits, int rows, int n_expert, const jl_moe_select *plan,
+                      uint32_t *sel, int sel_stride, float *wt, void *stream);
 
 /* The grouping the device tier runs before a batched mixture (kernels.ExpertGroup*,
  * jit/gpu/kernels/moesort.go:12-31; specification groupPairs,

@@ -60,6 +60,31 @@ class LayerPlan(C.Structure):
 
 LAYER_DENSE, LAYER_MOE = 0, 1
 
+
+class NormRows(C.Structure):
+    """jl_norm_rows."""
+    _fields_ = [("rows", C.c_int), ("n", C.c_int), ("x", C.c_void_p), ("x_type", C.c_int), ("x_stride", C.c_size_t),
+                ("resid", C.c_void_p), ("resid_stride", C.c_size_t), ("alpha", C.c_float), ("resid_out", C.c_void_p),
+                ("w", C.c_void_p), ("eps", C.c_float), ("y", C.c_void_p), ("y_type", C.c_int), ("y_stride", C.c_size_t),
+                ("q", C.c_void_p), ("a_s", C.c_void_p), ("sum16", C.c_void_p)]
+
+
+class MoeSelect(C.Structure):
+    """jl_moe_select."""
+    _fields_ = [("score", C.c_int), ("bias", C.c_void_p), ("n_group", C.c_int), ("k_group", C.c_int), ("group_top", C.c_int),
+                ("k_used", C.c_int), ("renorm", C.c_int), ("scale", C.c_float)]
+
+
+class AdapterGroup(C.Structure):
+    """jl_adapter_group."""
+    _fields_ = [("n", C.c_int), ("out", C.c_void_p * MAX_GROUP), ("base", C.c_void_p * MAX_GROUP), ("rows", C.c_int * MAX_GROUP),
+                ("a", C.c_void_p * MAX_GROUP), ("b", C.c_void_p * MAX_GROUP), ("type", C.c_int), ("n_adapter", C.c_int),
+                ("rank", C.c_int), ("ranks", C.c_void_p), ("scale", C.c_void_p), ("x", C.c_void_p), ("x_type", C.c_int),
+                ("k", C.c_int), ("ids", C.c_void_p), ("ntok", C.c_int)]
+
+
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
+
 # name -> (restype, argtypes); every symbol include/jlmi.h declares
 SIGNATURES = {
     "jl_hip_runtime": (C.c_char_p, []),
@@ -118,6 +143,10 @@ SIGNATURES = {
     "jl_matmul_mxfp4_packed_bf16_dev": (_int, [_vp, _vp, _vp, _vp, _int, _int, _vp, _int, _int, _int, _vp]),
     "jl_moe_logits_dev": (_int, [_vp, _vp, _int, _vp, _vp, _int, _int, _int, _vp]),
     "jl_moe_route_dev": (_int, [_vp, _vp, _int, _int, _int, _vp, _int, _vp, _vp]),
+    "jl_norm_rows_dev": (_int, [_vp, C.POINTER(NormRows), _vp]),
+    "jl_moe_select_dev": (_int, [_vp, _vp, _int, _int, C.POINTER(MoeSelect), _vp, _int, _vp, _vp]),
+    "jl_adapter_group_dev": (_int, [_vp, C.POINTER(AdapterGroup), _vp]),
+    "jl_reserve_adapters": (_int, [_vp, _int, _int, _int]),
     "jl_moe_group_dev": (_int, [_vp, _vp, _int, _int, _int, _int, _vp, _vp, _vp, _vp]),
     "jl_moe_matvec_dev": (_int, [_vp, _vp, _vp, _int, _vp, _vp, _vp, _vp, _vp, _vp, _int, _int, _int, _int, _vp]),
     "jl_moe_matvec_packed_dev": (_int, [_vp, _vp, _vp, _int, C.POINTER(PackedBank), C.POINTER(PackedBank), _vp, _vp, _vp,

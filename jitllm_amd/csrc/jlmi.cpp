@@ -206,6 +206,12 @@ struct jl_ctx {
     void* moe_route_ws = nullptr;
     size_t moe_route_ws_bytes = 0;
 
+    // u = scale * A x of an adapter call, and the buffers it outgrew (a captured graph may hold their addresses)
+    void* adapter_ws = nullptr;
+    size_t adapter_ws_bytes = 0;
+    void* adapter_old[64] = {};   // (each at least twice the one before)
+    int adapter_olds = 0;
+
     // host-pointer seam state
     std::map<const void*, Resident> resident;
     void* stage_x = nullptr;    // device
@@ -2228,6 +2234,13 @@ int jl_ctx_create(jl_ctx** out, const jl_options* opts) {
     std::vector<std::string> names = {"jl_quantize_act", "jl_dequant", "jl_matvec_q4k_r1_pq", "jl_matvec_q4k_r1_pq_res", "jl_matvec_q8_0_r1_pq", "jl_matvec_q8_0_r1_pq_res", "jl_matvec_q6k_r1_pq", "jl_matvec_q6k_r1_pq_res", "jl_matvec_q8_0p_r1_pq", "jl_matvec_q8_0p_r1_pq_res", "jl_matvec_q4k_r1_res", "jl_matvec_q4k_r1_x4_res", "jl_matvec_q8_0_r1_res", "jl_matvec_q8_0_r1_x4_res", "jl_matvec_q6k_r1_res", "jl_matvec_q6k_r1_x4_res", "jl_matvec_q8_0p_r1_res", "jl_matvec_q8_0p_r1_x4_res", "jl_matvec_q8_0p_r1", "jl_matvec_q8_0p_r2", "jl_matvec_q8_0p_r4", "jl_gemm_prep_q4k", "jl_gemm_prep_q4k_w16", "jl_gemm_q4k_r64", "jl_gemm_q4k_r128", "jl_gemm_q4k_wide", "jl_gemm_prep_q4k_fold", "jl_gemm_q4k_fold_wide", "jl_gemm_q4k_fold_wide4", "jl_gemm_q4k_k2", "jl_gemm_q4k_k2_planes", "jl_gemm_prep_q4k_planes", "jl_gemm_q4k_r64_planes", "jl_gemm_q4k_wide_planes", "jl_gemm_w16_prep_q4k", "jl_gemm_q4k_w16", "jl_gemm_q4k_few32", "jl_moe_route", "jl_moe_route_g2", "jl_moe_route_g4", "jl_moe_logits", "jl_moe_logits_e2", "jl_moe_logits_e2_f16", "jl_moe_logits_e4", "jl_moe_logits_e4_f16", "jl_moe_logits_e8", "jl_moe_logits_e8_f16", "jl_moe_group", "jl_moe_group2", "jl_moe_quant", "jl_moe_matvec_planes_q4k", "jl_moe_combine", "jl_moe_worklist", "jl_moe_gemm_prep", "jl_moe_gemm_prep_planes", "jl_moe_gemm_q4k", "jl_moe_g16_prep", "jl_moe_g16_prep_planes", "jl_moe_g16_c1", "jl_moe_g16_c2", "jl_moe_g16_c3", "jl_moe_g16_f1", "jl_moe_g16_f2", "jl_moe_g16_f3", "jl_moe_g16_g1", "jl_moe_g16_g2", "jl_moe_g16_g3", "jl_moe_g16_d1", "jl_moe_g16_d2", "jl_moe_g16_d3", "jl_moe_g16p_c1", "jl_moe_g16p_c2", "jl_moe_g16p_c3", "jl_moe_g16p_f1", "jl_moe_g16p_f2", "jl_moe_g16p_f3", "jl_moe_g16p_g1", "jl_moe_g16p_g2", "jl_moe_g16p_g3", "jl_moe_g16p_d1", "jl_moe_g16p_d2", "jl_moe_g16p_d3", "jl_moe_gemm_r64", "jl_moe_gemm_r64_planes", "jl_mxfp4_prep", "jl_mxfp4_prep_few", "jl_mxfp4_few_t1", "jl_mxfp4_few_t2", "jl_mxfp4_few_t3", "jl_mxfp4_few_t4", "jl_mxfp4_few_planes_t1", "jl_mxfp4_few_planes_t2", "jl_mxfp4_few_planes_t3", "jl_mxfp4_few_planes_t4", "jl_mxfp4_few_c3", "jl_mxfp4_few_c4", "jl_mxfp4_few_planes_c3", "jl_mxfp4_few_planes_c4", "jl_mxfp4_gemm", "jl_mxfp4_gemm_r96", "jl_mxfp4_matvec", "jl_mxfp4_matvec1_b1", "jl_mxfp4_matvec1_b2", "jl_mxfp4_matvec1_b3", "jl_mxfp4_scaled_prep", "jl_mxfp4_scaled_gemm", "jl_mxfp4_planes_prep", "jl_mxfp4_planes_gemm", "jl_mxfp4_planes_gemm_r96", "jl_mxfp4_matvec_planes_r64", "jl_mxfp4_matvec_planes_r32", "jl_mxfp4_matvec_planes_r16", "jl_unpack_mxfp4", "jl_sum_parts", "jl_silu_mul", "jl_add_rows", "jl_host_in", "jl_host_done", "jl_q4k_fold_range", "jl_probe_read", "jl_probe_empty", "jl_probe_wait", "jl_probe_mfma", "jl_probe_mfma_v5",
                                       "jl_pack_weights", "jl_unpack_q4k", "jl_unpack_q6k", "jl_unpack_q8_0"};
     names.push_back("jl_few_prep");
+    for (const char* form : {"l16_1", "l32_1", "l64_1", "l64_2", "l64_4", "wg_1", "wg_2", "wg_4", "wg_8", "wg_16"})
+        for (const char* any : {"", "_any"}) names.push_back(std::string("jl_norm_rows_") + form + any);
+    for (const char* g : {"g2", "g4", "g8", "g16"}) names.push_back(std::string("jl_moe_select_") + g);
+    for (const char* t : {"f32", "f16", "bf16"}) {
+        for (const char* xt : {"f32", "f16", "bf16"}) names.push_back(std::string("jl_adapter_down_") + t + "_" + xt);
+        names.push_back(std::string("jl_adapter_up_") + t);
+    }
     for (const char* pl : {"", "planes_"})
         for (int nt = 1; nt <= 4; nt++)
             for (int rt = 1; rt <= 2; rt++) names.push_back(std::string("jl_mxfp4_one_") + pl + "t" + std::to_string(nt) + "r" + std::to_string(rt));
@@ -2354,6 +2367,8 @@ void jl_ctx_destroy(jl_ctx* c) {
     if (c->act_ws) (void)H->Free(c->act_ws);
     if (c->layer_ws) (void)H->Free(c->layer_ws);
     if (c->moe_route_ws) (void)H->Free(c->moe_route_ws);
+    if (c->adapter_ws) (void)H->Free(c->adapter_ws);
+    for (int i = 0; i < c->adapter_olds; i++) (void)H->Free(c->adapter_old[i]);
     for (auto& kv : c->layers)
         if (kv.second.mem) (void)H->Free(kv.second.mem);
     if (c->one_group) (void)H->Free(c->one_group);
@@ -2448,6 +2463,113 @@ int jl_quantize_act_dev(jl_ctx* c, const float* x, int ntok, int k, int8_t* q, f
     void* params[] = {(void*)&x, (void*)&q, (void*)&as, (void*)&sum16, (void*)&k, (void*)&per, (void*)&no_gate};
     unsigned gx = (unsigned)((k / 4 + 255) / 256);  // one thread per four elements
     return launch(c, "jl_quantize_act", gx, (unsigned)ntok, 256, 0, pick_stream(c, stream), params);
+}
+
+namespace {
+// Plain types of the calls around the projections: bytes an element, 0 for any other type.
+int plain_bytes(int type) { return type == JL_TYPE_F32 ? 4 : type == JL_TYPE_F16 || type == JL_TYPE_BF16 ? 2 : 0; }
+const char* plain_tag(int type) { return type == JL_TYPE_F32 ? "f32" : type == JL_TYPE_F16 ? "f16" : "bf16"; }
+}  // namespace
+
+int jl_norm_rows_dev(jl_ctx* c, const jl_norm_rows* g, void* stream) {
+    if (!c) return JL_ERR_ARG;
+    if (!g || !g->x || g->rows <= 0 || g->n <= 0) return fail(c, JL_ERR_ARG, "norm rows: bad operand");
+    if (!g->resid_out && !g->y && !g->q) return fail(c, JL_ERR_ARG, "norm rows: no output");
+    if (g->resid_out && !g->resid) return fail(c, JL_ERR_ARG, "norm rows: resid_out without resid");
+    if ((g->q && (!g->as || !g->sum16)) || (!g->q && (g->as || g->sum16)))
+        return fail(c, JL_ERR_ARG, "norm rows: q, as and sum16 come together");
+    if (!(g->eps >= 0.f)) return fail(c, JL_ERR_ARG, "norm rows: eps=%g", (double)g->eps);
+    const size_t n = (size_t)g->n;
+    const size_t xs = g->x_stride ? g->x_stride : n, rs = g->resid_stride ? g->resid_stride : n, ys = g->y_stride ? g->y_stride : n;
+    if (xs < n || rs < n || ys < n) return fail(c, JL_ERR_ARG, "norm rows: a stride is shorter than a row");
+    const int xb = plain_bytes(g->x_type), yb = g->y ? plain_bytes(g->y_type) : 4;
+    if (!xb || !yb || g->n > 65536) return JL_DECLINED;
+    if (((uintptr_t)g->x & (xb - 1)) || ((uintptr_t)g->y & (yb - 1)) || (((uintptr_t)g->resid | (uintptr_t)g->resid_out | (uintptr_t)g->w | (uintptr_t)g->as | (uintptr_t)g->sum16) & 3))
+        return JL_DECLINED;
+    if (g->q && (g->n % 32 != 0 || !aligned16(g->q))) return JL_DECLINED;
+    NormRowsArgs a;
+    a.x = g->x; a.resid = g->resid; a.resid_out = g->resid_out; a.w = g->w; a.y = g->y; a.q = g->q; a.as = g->as; a.s16 = g->sum16;
+    a.x_stride = xs; a.resid_stride = rs; a.y_stride = ys;
+    a.rows = g->rows; a.n = g->n; a.x_type = g->x_type; a.y_type = g->y ? g->y_type : JL_TYPE_F32; a.per = c->act_window / 32;
+    a.alpha = g->alpha; a.eps = g->eps; a.threads = 256;
+    const bool vec = n % 4 == 0 && xs % 4 == 0 && (!g->resid || rs % 4 == 0) && (!g->y || ys % 4 == 0) && !((uintptr_t)g->x & (4 * xb - 1)) &&
+                     !((uintptr_t)g->y & (4 * yb - 1)) && aligned16(g->resid) && aligned16(g->resid_out) && aligned16(g->w);
+    const int quads = (g->n + 3) / 4;   // groups of four elements
+    Name name;
+    name << "jl_norm_rows_";
+    unsigned grid, block = 256, lds = 0;
+    if (quads <= 256) {   // a wavefront a row, or a part of one
+        const int lanes = quads <= 16 ? 16 : quads <= 32 ? 32 : 64;
+        name << "l" << lanes << "_" << (quads <= 64 ? 1 : quads <= 128 ? 2 : 4);
+        grid = (unsigned)(((long)g->rows + 256 / lanes - 1) / (256 / lanes));
+    } else {              // a workgroup a row
+        int ni = 1;
+        while (quads > 1024 * ni) ni *= 2;
+        if (g->rows > c->num_cu && ni < 4) ni = 4;
+        block = (unsigned)((quads + 64 * ni - 1) / (64 * ni) * 64);
+        name << "wg_" << ni;
+        grid = (unsigned)g->rows;
+        lds = 16 * sizeof(double);
+    }
+    if ((unsigned long long)grid * block > 0xffffffffull) return JL_DECLINED;   // threads a launch can have
+    if (!vec) name << "_any";
+    a.threads = (int)block;
+    void* params[] = {&a};
+    HIP_TRY(c, H->SetDevice(c->device));
+    return launch(c, name, grid, 1, block, lds, pick_stream(c, stream), params);
+}
+
+namespace {
+// The adapter calls' workspace: a buffer that is outgrown is kept (a captured graph may hold its address).
+int adapter_ws_ensure(jl_ctx* c, size_t need) {
+    if (c->adapter_ws_bytes >= need) return JL_OK;
+    void* p = nullptr;
+    need = std::max(need, 2 * c->adapter_ws_bytes);
+    HIP_TRY(c, H->Malloc(&p, need));
+    if (c->adapter_ws) c->adapter_old[c->adapter_olds++] = c->adapter_ws;
+    c->adapter_ws = p;
+    c->adapter_ws_bytes = need;
+    return JL_OK;
+}
+}  // namespace
+
+int jl_reserve_adapters(jl_ctx* c, int max_tok, int n, int max_rank) {
+    if (!c) return JL_ERR_ARG;
+    if (max_tok <= 0 || n < 1 || n > JL_MAX_GROUP || max_rank <= 0) return fail(c, JL_ERR_ARG, "reserve adapters: %d tokens, %d projections, rank %d", max_tok, n, max_rank);
+    if (max_rank > 512) return JL_DECLINED;
+    HIP_TRY(c, H->SetDevice(c->device));
+    return adapter_ws_ensure(c, (size_t)max_tok * n * max_rank * 4);
+}
+
+int jl_adapter_group_dev(jl_ctx* c, const jl_adapter_group* g, void* stream) {
+    if (!c) return JL_ERR_ARG;
+    if (!g || g->n < 1 || g->n > JL_MAX_GROUP || !g->x || !g->ids || g->k <= 0 || g->ntok <= 0 || g->n_adapter <= 0 || g->rank <= 0)
+        return fail(c, JL_ERR_ARG, "adapter group: bad group");
+    const int wb = plain_bytes(g->type), xb = plain_bytes(g->x_type);
+    if (!wb || !xb || g->k % 32 != 0 || g->rank > 512) return JL_DECLINED;
+    int most = 0;
+    AdapterArgs a;
+    for (int i = 0; i < g->n; i++) {
+        if (!g->out[i] || !g->a[i] || !g->b[i] || g->rows[i] <= 0) return fail(c, JL_ERR_ARG, "adapter group: null operand or no rows");
+        if (!aligned16(g->a[i]) || !aligned16(g->b[i]) || (((uintptr_t)g->out[i] | (uintptr_t)g->base[i]) & 3)) return JL_DECLINED;
+        most = std::max(most, g->rows[i]);
+        a.out[i] = g->out[i]; a.base[i] = g->base[i]; a.a[i] = g->a[i]; a.b[i] = g->b[i]; a.rows[i] = g->rows[i];
+    }
+    if (!aligned16(g->x) || (((uintptr_t)g->ids | (uintptr_t)g->ranks | (uintptr_t)g->scale) & 3) || most > 256 * 65535 || (unsigned)g->ntok > 0xffffffffu / 256)
+        return JL_DECLINED;
+    HIP_TRY(c, H->SetDevice(c->device));
+    int rc = adapter_ws_ensure(c, (size_t)g->ntok * g->n * g->rank * 4);
+    if (rc != JL_OK) return rc;
+    a.ids = g->ids; a.ranks = g->ranks; a.scale = g->scale; a.x = g->x; a.u = (float*)c->adapter_ws;
+    a.n = g->n; a.n_adapter = g->n_adapter; a.rank = g->rank; a.k = g->k; a.ntok = g->ntok;
+    hipStream_t st = pick_stream(c, stream);
+    void* params[] = {&a};
+    Name down, up;
+    down << "jl_adapter_down_" << plain_tag(g->type) << "_" << plain_tag(g->x_type);
+    rc = launch(c, down, (unsigned)g->ntok, (unsigned)(g->rank + 3) / 4, 256, 0, st, params, (unsigned)g->n);
+    if (rc != JL_OK) return rc;
+    up << "jl_adapter_up_" << plain_tag(g->type);
+    return launch(c, up, (unsigned)g->ntok, (unsigned)(most + 255) / 256, 256, (unsigned)g->rank * 4, st, params, (unsigned)g->n);
 }
 
 int jl_dequant_dev(jl_ctx* c, int type, const void* src, float* dst, size_t n, void* stream) {
@@ -2749,6 +2871,31 @@ int jl_moe_route_dev(jl_ctx* c, const float* logits, int rows, int n_expert, int
     void* params[] = {&a};
     // the form with the fewest experts a lane that holds them all (less code for a lone wavefront to fetch)
     const char* name = n_expert <= 128 ? "jl_moe_route_g2" : n_expert <= 256 ? "jl_moe_route_g4" : "jl_moe_route";
+    return launch(c, name, (unsigned)rows, 1, 64, 0, pick_stream(c, stream), params);
+}
+
+int jl_moe_select_dev(jl_ctx* c, const float* logits, int rows, int n_expert, const jl_moe_select* plan, uint32_t* sel,
+                      int sel_stride, float* wt, void* stream) {
+    if (!c) return JL_ERR_ARG;
+    if (!logits || !plan || !sel || !wt || rows <= 0 || n_expert <= 0 || plan->k_used <= 0 || sel_stride < plan->k_used)
+        return fail(c, JL_ERR_ARG, "moe select: bad operand");
+    if (!(std::isfinite(plan->scale))) return fail(c, JL_ERR_ARG, "moe select: scale=%g", (double)plan->scale);
+    const int n_group = plan->n_group <= 1 ? 1 : plan->n_group;
+    if (plan->n_group < 0 || (n_group > 1 && (plan->k_group < 1 || plan->k_group > n_group)))
+        return fail(c, JL_ERR_ARG, "moe select: %d of %d groups", plan->k_group, plan->n_group);
+    if (plan->score != JL_SCORE_SOFTMAX && plan->score != JL_SCORE_SIGMOID) return JL_DECLINED;
+    if (n_expert > 1024 || plan->k_used > 16 || n_group > 64 || n_expert % n_group != 0) return JL_DECLINED;
+    if (n_group > 1 && plan->group_top != 1 && plan->group_top != 2) return JL_DECLINED;
+    if ((unsigned)rows > 0xffffffffu / 64) return JL_DECLINED;   // threads a launch can have
+    if (plan->k_used > (n_group > 1 ? plan->k_group * (n_expert / n_group) : n_expert)) return JL_DECLINED;
+    if (((uintptr_t)logits | (uintptr_t)plan->bias | (uintptr_t)sel | (uintptr_t)wt) & 3) return JL_DECLINED;
+    HIP_TRY(c, H->SetDevice(c->device));
+    MoeSelectArgs a;
+    a.logits = logits; a.bias = plan->bias; a.sel = sel; a.wt = wt; a.n_expert = n_expert; a.k_used = plan->k_used; a.sel_stride = sel_stride;
+    a.sigmoid = plan->score == JL_SCORE_SIGMOID; a.n_group = n_group; a.k_group = plan->k_group; a.group_top = plan->group_top;
+    a.renorm = plan->renorm != 0; a.scale = plan->scale;
+    void* params[] = {&a};
+    const char* name = n_expert <= 128 ? "jl_moe_select_g2" : n_expert <= 256 ? "jl_moe_select_g4" : n_expert <= 512 ? "jl_moe_select_g8" : "jl_moe_select_g16";
     return launch(c, name, (unsigned)rows, 1, 64, 0, pick_stream(c, stream), params);
 }
 

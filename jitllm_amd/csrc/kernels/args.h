@@ -576,3 +576,47 @@ struct PackedMultiArgs {
     float norm_eps;
     double inv_k;        // 1 / k
 };
+
+// Rows normed between two projections (kernels/norm_rows.h): h = resid + alpha * x, y = RMSNorm(h) * w, and y quantized.
+struct NormRowsArgs {
+    const void* x;           // [rows][x_stride] f32 / f16 / bf16
+    const float* resid;      // [rows][resid_stride], or null: h = x
+    float* resid_out;        // null, or where h goes (may be resid)
+    const float* w;          // [n], or null: ones
+    void* y;                 // null, or [rows][y_stride] f32 / f16 / bf16
+    int8_t* q;               // null, or [rows][n] with as [rows][n/32] and s16 [rows][n/16]
+    float* as;
+    float* s16;
+    size_t x_stride, resid_stride, y_stride;   // elements
+    int rows, n, x_type, y_type;
+    int per;                 // activation window / 32
+    int threads;             // of the workgroup (the forms that give a row a whole one)
+    float alpha, eps;
+};
+
+// The router's general form (kernels/moe_select.h).
+struct MoeSelectArgs {
+    const float* logits;     // [rows][n_expert]
+    const float* bias;       // [n_expert] or null
+    uint32_t* sel;           // [rows][sel_stride]
+    float* wt;               // [rows][k_used]
+    int n_expert, k_used, sel_stride, sigmoid;
+    int n_group, k_group, group_top, renorm;
+    float scale;
+};
+
+// Low-rank adapters beside up to four projections that read one x (kernels/adapter.h).
+#define JL_ADAPTER_GROUP 4
+struct AdapterArgs {
+    float* out[JL_ADAPTER_GROUP];          // [ntok][rows]
+    const float* base[JL_ADAPTER_GROUP];   // the same, may be out; null: zeros
+    const void* a[JL_ADAPTER_GROUP];       // [n_adapter][rank][k]
+    const void* b[JL_ADAPTER_GROUP];       // [n_adapter][rows][rank]
+    int rows[JL_ADAPTER_GROUP];
+    const uint32_t* ids;                   // [ntok]
+    const uint32_t* ranks;                 // [n_adapter] or null
+    const float* scale;                    // [n_adapter] or null
+    const void* x;                         // [ntok][k]
+    float* u;                              // [ntok][n][rank] workspace
+    int n, n_adapter, rank, k, ntok;
+};

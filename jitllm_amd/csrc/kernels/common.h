@@ -13,6 +13,9 @@ typedef i32 i32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 // ggml type numbers (the reference's quant.Type, format/quant/types.go:14-55)
+#define JL_F32 0
+#define JL_F16 1
+#define JL_BF16 30
 #define JL_Q8_0 8
 #define JL_Q4_K 12
 #define JL_Q6_K 14

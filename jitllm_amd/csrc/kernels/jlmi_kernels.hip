@@ -2,6 +2,7 @@
 // hipModuleLaunchKernel.  Built with
 //   hipcc --genco --offload-arch=gfx950 -O3 -ffp-contract=off ...
 // Entry points are extern "C" so the host can look them up by name.
+#include "adapter.h"
 #include "common.h"
 #include "dequant.h"
 #include "few_i8.h"
@@ -13,7 +14,9 @@
 #include "moe.h"
 #include "moe_cols.h"
 #include "moe_planes.h"
+#include "moe_select.h"
 #include "mxfp4.h"
+#include "norm_rows.h"
 #include "packed.h"
 #include "quantize.h"
 
@@ -349,6 +352,12 @@ extern "C" __global__ __launch_bounds__(256, 2) void jl_gemm_q4k_w16(GemmW16Args
 extern "C" __global__ __launch_bounds__(64) void jl_moe_route(MoeRouteArgs p) { moe_route_body<16>(p); }
 extern "C" __global__ __launch_bounds__(64) void jl_moe_route_g2(MoeRouteArgs p) { moe_route_body<2>(p); }
 extern "C" __global__ __launch_bounds__(64) void jl_moe_route_g4(MoeRouteArgs p) { moe_route_body<4>(p); }
+#define JL_MOE_SELECT(NAME, NG)                                                             \
+    extern "C" __global__ __launch_bounds__(64) void jl_moe_select_##NAME(MoeSelectArgs p) { \
+        __shared__ i32 keys[64 * NG];                                                       \
+        moe_select_body<NG>(p, keys);                                                       \
+    }
+JL_MOE_SELECT(g2, 2) JL_MOE_SELECT(g4, 4) JL_MOE_SELECT(g8, 8) JL_MOE_SELECT(g16, 16)
 // grid = (token groups, 8 at most, experts, ceil(token groups / 8)), by_expert: (experts, token groups); block = 128; a group is
 // JL_LOGITS_TOK tokens
 extern "C" __global__ __launch_bounds__(128) void jl_moe_logits(MoeLogitsArgs p) {
@@ -669,3 +678,20 @@ extern "C" __global__ __launch_bounds__(64) void jl_probe_wait(const u32x4* __re
     const uint64_t t0 = wall_clock64();
     while (wall_clock64() - t0 < ticks) __builtin_amdgcn_s_sleep(8);
 }
+
+// ------------------------------------------------- around the projections
+// l<lanes>_<groups>: grid = ceil(rows / (256 / lanes)), block = 256; wg_<groups>: grid = rows, block = p.threads
+#define JL_NORM_ROWS(NAME, LPR, NI, WG, BLOCK)                                                                                                      \
+    extern "C" __global__ __launch_bounds__(BLOCK) void jl_norm_rows_##NAME(NormRowsArgs p) { norm_rows_body<LPR, NI, WG, true>(p, (double*)jl_smem); } \
+    extern "C" __global__ __launch_bounds__(BLOCK) void jl_norm_rows_##NAME##_any(NormRowsArgs p) { norm_rows_body<LPR, NI, WG, false>(p, (double*)jl_smem); }
+JL_NORM_ROWS(l16_1, 16, 1, false, 256) JL_NORM_ROWS(l32_1, 32, 1, false, 256) JL_NORM_ROWS(l64_1, 64, 1, false, 256)
+JL_NORM_ROWS(l64_2, 64, 2, false, 256) JL_NORM_ROWS(l64_4, 64, 4, false, 256)
+JL_NORM_ROWS(wg_1, 64, 1, true, 1024) JL_NORM_ROWS(wg_2, 64, 2, true, 1024) JL_NORM_ROWS(wg_4, 64, 4, true, 1024)
+JL_NORM_ROWS(wg_8, 64, 8, true, 1024) JL_NORM_ROWS(wg_16, 64, 16, true, 1024)
+// grid = (tokens, ceil(rank / 4), projections), block = 256; grid = (tokens, ceil(rows / 256), projections), block = 256
+#define JL_ADAPTER(T, TYPE)                                                                                                                   \
+    extern "C" __global__ __launch_bounds__(256) void jl_adapter_down_##T##_f32(AdapterArgs p) { adapter_down_body<TYPE, JL_F32>(p); }        \
+    extern "C" __global__ __launch_bounds__(256) void jl_adapter_down_##T##_f16(AdapterArgs p) { adapter_down_body<TYPE, JL_F16>(p); }        \
+    extern "C" __global__ __launch_bounds__(256) void jl_adapter_down_##T##_bf16(AdapterArgs p) { adapter_down_body<TYPE, JL_BF16>(p); }      \
+    extern "C" __global__ __launch_bounds__(256) void jl_adapter_up_##T(AdapterArgs p) { adapter_up_body<TYPE>(p, (float*)jl_smem); }
+JL_ADAPTER(f32, JL_F32) JL_ADAPTER(f16, JL_F16) JL_ADAPTER(bf16, JL_BF16)

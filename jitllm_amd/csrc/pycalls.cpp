@@ -33,6 +33,9 @@ struct Api {
     decltype(&jl_moe_block_packed_dev) moe_block_packed_dev;
     decltype(&jl_matmul_mxfp4_bf16_dev) matmul_mxfp4_bf16_dev;
     decltype(&jl_matmul_mxfp4_packed_bf16_dev) matmul_mxfp4_packed_bf16_dev;
+    decltype(&jl_norm_rows_dev) norm_rows_dev;
+    decltype(&jl_moe_select_dev) moe_select_dev;
+    decltype(&jl_adapter_group_dev) adapter_group_dev;
 } api;
 PyObject *host_types, *bank_type;                                  // quant.BLOCK, _lib.PackedBank
 PyObject *s_qs, *s_d, *s_sc, *s_row, *s_stride, *s_served;
@@ -105,6 +108,12 @@ bool real(PyObject* o, float* v) {
     if (d == -1.0 && PyErr_Occurred()) return false;
     *v = (float)d;
     return true;
+}
+bool opt_num(PyObject* o, int* v) { return !o || num(o, v); }
+bool size(PyObject* o, size_t* v) {   // absent: as it was
+    if (!o) return true;
+    *v = PyLong_AsSize_t(o);
+    return !PyErr_Occurred();
 }
 // The stream argument: None or an address (an int, or a ctypes pointer).
 bool stream_of(PyObject* o, void** p) {
@@ -306,6 +315,63 @@ PyObject* py_moe_block_dev(SIG) {
     }), "jl_moe_block_dev");
 }
 
+// ---- around the projections
+PyObject* py_norm_rows_dev(SIG) {
+    TAKE("norm_rows_dev", 5, "x", "rows", "n", "w", "eps", "x_type", "x_stride", "resid", "resid_stride", "alpha", "resid_out", "y", "y_type", "y_stride", "q", "a_s",
+         "sum16", "stream");
+    jl_norm_rows g;
+    memset(&g, 0, sizeof g);
+    g.alpha = 1.f;
+    void *x, *w, *resid, *resid_out, *y, *q, *as, *s16, *st;
+    if (!ptr(a[0], &x) || !num(a[1], &g.rows) || !num(a[2], &g.n) || !opt(a[3], &w) || !real(a[4], &g.eps) || !opt_num(a[5], &g.x_type) || !size(a[6], &g.x_stride) ||
+        !opt(a[7], &resid) || !size(a[8], &g.resid_stride) || !real(a[9], &g.alpha) || !opt(a[10], &resid_out) || !opt(a[11], &y) || !opt_num(a[12], &g.y_type) ||
+        !size(a[13], &g.y_stride) || !opt(a[14], &q) || !opt(a[15], &as) || !opt(a[16], &s16) || !stream_of(a[17], &st))
+        return nullptr;
+    g.x = x; g.w = (const float*)w; g.resid = (const float*)resid; g.resid_out = (float*)resid_out; g.y = y;
+    g.q = (int8_t*)q; g.as = (float*)as; g.sum16 = (float*)s16;
+    return ended(self, unlocked([&] { return api.norm_rows_dev(self->ctx, &g, st); }), "jl_norm_rows_dev");
+}
+
+PyObject* py_moe_select_dev(SIG) {
+    TAKE("moe_select_dev", 7, "logits", "rows", "n_expert", "k_used", "sel", "sel_stride", "wt", "score", "bias", "n_group", "k_group", "group_top", "renorm", "scale",
+         "stream");
+    jl_moe_select g = {JL_SCORE_SOFTMAX, nullptr, 1, 1, 1, 0, 1, 1.f};
+    void *logits, *sel, *wt, *bias, *st;
+    int rows, n_expert, sel_stride;
+    if (!ptr(a[0], &logits) || !num(a[1], &rows) || !num(a[2], &n_expert) || !num(a[3], &g.k_used) || !ptr(a[4], &sel) || !num(a[5], &sel_stride) || !ptr(a[6], &wt) ||
+        !opt_num(a[7], &g.score) || !opt(a[8], &bias) || !opt_num(a[9], &g.n_group) || !opt_num(a[10], &g.k_group) || !opt_num(a[11], &g.group_top) ||
+        !real(a[13], &g.scale) || !stream_of(a[14], &st))
+        return nullptr;
+    if (a[12] && (g.renorm = PyObject_IsTrue(a[12])) < 0) return nullptr;
+    g.bias = (const float*)bias;
+    return ended(self, unlocked([&] { return api.moe_select_dev(self->ctx, (const float*)logits, rows, n_expert, &g, (uint32_t*)sel, sel_stride, (float*)wt, st); }),
+                 "jl_moe_select_dev");
+}
+
+PyObject* py_adapter_group_dev(SIG) {
+    TAKE("adapter_group_dev", 12, "outs", "bases", "rows", "a", "b", "t", "n_adapter", "rank", "x", "k", "ids", "ntok", "scale", "ranks", "x_type", "stream");
+    const Py_ssize_t n = PySequence_Size(a[0]);
+    if (n < 0) return nullptr;
+    if (n > JL_MAX_GROUP) {
+        PyErr_Format(PyExc_IndexError, "a group holds up to %d projections", JL_MAX_GROUP);
+        return nullptr;
+    }
+    jl_adapter_group g;
+    memset(&g, 0, sizeof g);
+    g.n = (int)n;
+    void *p, *x, *ids, *scale, *ranks, *st;
+    if (!each(a[0], g.n, [&](int i, PyObject* o) { return ptr(o, &p) && (g.out[i] = (float*)p, true); }) ||
+        (a[1] != Py_None && !each(a[1], g.n, [&](int i, PyObject* o) { return opt(o, &p) && (g.base[i] = (const float*)p, true); })) ||
+        !each(a[2], g.n, [&](int i, PyObject* o) { return num(o, &g.rows[i]); }) ||
+        !each(a[3], g.n, [&](int i, PyObject* o) { return ptr(o, &p) && (g.a[i] = p, true); }) ||
+        !each(a[4], g.n, [&](int i, PyObject* o) { return ptr(o, &p) && (g.b[i] = p, true); }) || !num(a[5], &g.type) || !num(a[6], &g.n_adapter) ||
+        !num(a[7], &g.rank) || !ptr(a[8], &x) || !num(a[9], &g.k) || !ptr(a[10], &ids) || !num(a[11], &g.ntok) || !opt(a[12], &scale) || !opt(a[13], &ranks) ||
+        !opt_num(a[14], &g.x_type) || !stream_of(a[15], &st))
+        return nullptr;
+    g.x = x; g.ids = (const uint32_t*)ids; g.scale = (const float*)scale; g.ranks = (const uint32_t*)ranks;
+    return ended(self, unlocked([&] { return api.adapter_group_dev(self->ctx, &g, st); }), "jl_adapter_group_dev");
+}
+
 // ---- host memory: numpy arrays, checked
 bool is(PyObject* o, int type) {
     return PyArray_Check(o) && PyArray_TYPE((PyArrayObject*)o) == type && PyArray_ISNOTSWAPPED((PyArrayObject*)o);
@@ -393,6 +459,18 @@ PyMethodDef methods[] = {
       "moe_block_dev(resid, t, gate, up, down, router, x, rows, k_used, n_expert, n_ffn, n_embd, sel=None, wt=None, stream=None,\n"
       "down_type=None, router_type=0).  The whole mixture block, router included: resid [rows][n_embd] += mixture output.\n"
       "gate / up / down: banks of GGUF sheets (device addresses), or three packed_bank(...) structures."),
+    M(norm_rows_dev,
+      "norm_rows_dev(x, rows, n, w, eps, x_type=0, x_stride=0, resid=None, resid_stride=0, alpha=1.0, resid_out=None, y=None, y_type=0,\n"
+      "y_stride=0, q=None, a_s=None, sum16=None, stream=None).  h = resid + alpha * x (-> resid_out), y = RMSNorm(h) * w in f32 (type 0),\n"
+      "f16 (1) or bf16 (30), and the quantizer's int8 form of it, over rows; strides in elements (0: n)."),
+    M(moe_select_dev,
+      "moe_select_dev(logits, rows, n_expert, k_used, sel, sel_stride, wt, score=0, bias=None, n_group=1, k_group=1, group_top=1,\n"
+      "renorm=True, scale=1.0, stream=None).  The router in its general form: softmax (0) or sigmoid (1) scores, a bias for the\n"
+      "selection, the k_group best groups, the k_used best experts; places without an expert get the id n_expert and weight 0."),
+    M(adapter_group_dev,
+      "adapter_group_dev(outs, bases, rows, a, b, t, n_adapter, rank, x, k, ids, ntok, scale=None, ranks=None, x_type=0, stream=None).\n"
+      "outs[i][t] = bases[i][t] + scale[ids[t]] * b[i][ids[t]] (a[i][ids[t]] x[t]) for up to four projections that read one x;\n"
+      "bases (or an entry of it) None: zeros."),
     M(MatVec, "MatVec(out, t, w, x, nrows, k).  nn.Device.MatVec: out[0:nrows] = W x over raw GGUF bytes; False = declined."),
     M(MatMul, "MatMul(out, t, w, x, nrows, k, ntok).  JIT.MatMul (/root/reference/engine/nn/matmul.go:27): x [ntok][k] -> out [ntok][nrows]."),
     M(MatVecPacked, "MatVecPacked(out, t, p, x, nrows, k).  JIT.MatVecPacked (/root/reference/engine/nn/packed.go:24);\n"
@@ -416,6 +494,7 @@ PyObject* py_bind(PyObject*, PyObject* args) {
     }
     FN(matvec) FN(matmul) FN(matvec_packed) FN(matmul_packed) FN(matvec_dev) FN(matvec_packed_dev) FN(matvec_group_dev) FN(matmul_dev)
     FN(matmul_packed_dev) FN(layer_ffn_dev) FN(moe_block_dev) FN(moe_block_packed_dev) FN(matmul_mxfp4_bf16_dev) FN(matmul_mxfp4_packed_bf16_dev)
+    FN(norm_rows_dev) FN(moe_select_dev) FN(adapter_group_dev)
 #undef FN
     Py_INCREF(types);
     Py_INCREF(bank);

@@ -140,6 +140,10 @@ class Device(_calls.Calls):
         """Grow every workspace a matmul of this shape would grow, launching nothing."""
         return self._served(self._l.jl_reserve_shape(self._ctx, t, nrows, k, ntok, int(packed)), "jl_reserve_shape")
 
+    def reserve_adapters(self, max_tok, n, max_rank):
+        """Size the workspace of adapter_group_dev for up to max_tok tokens, n projections and rank max_rank."""
+        self._served(self._l.jl_reserve_adapters(self._ctx, max_tok, n, max_rank), "jl_reserve_adapters")
+
     def probe_dev(self, kind, src, nbytes, grid=0, block=0, stream=None):
         """An empty kernel (kind 0) or a kernel that only reads nbytes at src (kind 1)."""
         return self._served(self._l.jl_probe_dev(self._ctx, kind, src, nbytes, grid, block, stream), "jl_probe_dev")

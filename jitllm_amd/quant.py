@@ -4,6 +4,7 @@ The numbers are the ggml_type values a GGUF file carries, the same ones the
 reference's quant.Type uses (/root/reference/format/quant/types.go:14-85).
 """
 
+F32, F16, BF16 = 0, 1, 30     # plain values: normed rows, adapters, router weights
 Q8_0 = 8
 Q4_K = 12
 Q6_K = 14
