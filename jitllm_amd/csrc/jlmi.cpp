@@ -2238,8 +2238,9 @@ int jl_ctx_create(jl_ctx** out, const jl_options* opts) {
         for (const char* any : {"", "_any"}) names.push_back(std::string("jl_norm_rows_") + form + any);
     for (const char* g : {"g2", "g4", "g8", "g16"}) names.push_back(std::string("jl_moe_select_") + g);
     for (const char* t : {"f32", "f16", "bf16"}) {
-        for (const char* xt : {"f32", "f16", "bf16"}) names.push_back(std::string("jl_adapter_down_") + t + "_" + xt);
-        names.push_back(std::string("jl_adapter_up_") + t);
+        for (const char* xt : {"f32", "f16", "bf16"})
+            for (const char* nt : {"_n1", "_n4", "_n8"}) names.push_back(std::string("jl_adapter_down_") + t + "_" + xt + nt);
+        for (const char* form : {"_t1", "_t1_any", "_t4", "_t4_any"}) names.push_back(std::string("jl_adapter_up_") + t + form);
     }
     for (const char* pl : {"", "planes_"})
         for (int nt = 1; nt <= 4; nt++)
@@ -2533,12 +2534,30 @@ int adapter_ws_ensure(jl_ctx* c, size_t need) {
 }
 }  // namespace
 
+namespace {
+// How an adapter call is cut: K slices for as many workgroups as two rounds of the chip hold.
+struct AdapterPlan { int rank_pad, nt, passes, slices; };
+AdapterPlan adapter_plan(const jl_ctx* c, int ntok, int n, int rank, int k, int n_adapter) {
+    AdapterPlan a;
+    a.rank_pad = (rank + 15) / 16 * 16;
+    const int tiles = n * a.rank_pad / 16;
+    a.nt = tiles <= 1 ? 1 : tiles <= 4 ? 4 : 8;
+    a.passes = (tiles + a.nt - 1) / a.nt;
+    const long units = std::max((long)(ntok + 15) / 16, (long)std::min(ntok, n_adapter));
+    a.slices = (int)std::max(1l, std::min({16l, 2l * c->num_cu / (units * a.passes), (long)k / 32 / 8}));
+    return a;
+}
+size_t adapter_ws_bytes(const AdapterPlan& a, int ntok, int n) { return (size_t)a.slices * ntok * n * a.rank_pad * 4; }
+}  // namespace
+
 int jl_reserve_adapters(jl_ctx* c, int max_tok, int n, int max_rank) {
     if (!c) return JL_ERR_ARG;
     if (max_tok <= 0 || n < 1 || n > JL_MAX_GROUP || max_rank <= 0) return fail(c, JL_ERR_ARG, "reserve adapters: %d tokens, %d projections, rank %d", max_tok, n, max_rank);
     if (max_rank > 512) return JL_DECLINED;
     HIP_TRY(c, H->SetDevice(c->device));
-    return adapter_ws_ensure(c, (size_t)max_tok * n * max_rank * 4);
+    // slices * tokens: sixteen slices at most, and more than one only while slices * tokens / 16 is within two rounds of the chip
+    const size_t cols = (size_t)n * ((max_rank + 15) / 16 * 16);
+    return adapter_ws_ensure(c, std::max((size_t)max_tok, std::min((size_t)16 * max_tok, (size_t)32 * c->num_cu)) * cols * 4);
 }
 
 int jl_adapter_group_dev(jl_ctx* c, const jl_adapter_group* g, void* stream) {
@@ -2547,29 +2566,41 @@ int jl_adapter_group_dev(jl_ctx* c, const jl_adapter_group* g, void* stream) {
         return fail(c, JL_ERR_ARG, "adapter group: bad group");
     const int wb = plain_bytes(g->type), xb = plain_bytes(g->x_type);
     if (!wb || !xb || g->k % 32 != 0 || g->rank > 512) return JL_DECLINED;
-    int most = 0;
     AdapterArgs a;
+    long wide = 0;
+    bool vec = true;
     for (int i = 0; i < g->n; i++) {
         if (!g->out[i] || !g->a[i] || !g->b[i] || g->rows[i] <= 0) return fail(c, JL_ERR_ARG, "adapter group: null operand or no rows");
         if (!aligned16(g->a[i]) || !aligned16(g->b[i]) || (((uintptr_t)g->out[i] | (uintptr_t)g->base[i]) & 3)) return JL_DECLINED;
-        most = std::max(most, g->rows[i]);
+        vec = vec && g->rows[i] % 4 == 0 && aligned16(g->out[i]) && aligned16(g->base[i]);
+        wide += g->rows[i];
         a.out[i] = g->out[i]; a.base[i] = g->base[i]; a.a[i] = g->a[i]; a.b[i] = g->b[i]; a.rows[i] = g->rows[i];
     }
-    if (!aligned16(g->x) || (((uintptr_t)g->ids | (uintptr_t)g->ranks | (uintptr_t)g->scale) & 3) || most > 256 * 65535 || (unsigned)g->ntok > 0xffffffffu / 256)
-        return JL_DECLINED;
+    if (!aligned16(g->x) || (((uintptr_t)g->ids | (uintptr_t)g->ranks | (uintptr_t)g->scale) & 3)) return JL_DECLINED;
+    if (g->ntok > 16 * 65535 || wide > 0x1000000) return JL_DECLINED;   // grid of a launch
     HIP_TRY(c, H->SetDevice(c->device));
-    int rc = adapter_ws_ensure(c, (size_t)g->ntok * g->n * g->rank * 4);
+    const AdapterPlan pl = adapter_plan(c, g->ntok, g->n, g->rank, g->k, g->n_adapter);
+    int rc = adapter_ws_ensure(c, adapter_ws_bytes(pl, g->ntok, g->n));
     if (rc != JL_OK) return rc;
     a.ids = g->ids; a.ranks = g->ranks; a.scale = g->scale; a.x = g->x; a.u = (float*)c->adapter_ws;
     a.n = g->n; a.n_adapter = g->n_adapter; a.rank = g->rank; a.k = g->k; a.ntok = g->ntok;
+    a.rank_pad = pl.rank_pad; a.slices = pl.slices; a.passes = pl.passes;
     hipStream_t st = pick_stream(c, stream);
     void* params[] = {&a};
+    // a chunk of 64 tokens has at most 4 + n_adapter tiles
+    const int tok64 = (g->ntok + 63) / 64, most = std::min(g->ntok, 64);
+    const unsigned slots = (unsigned)std::min(most, (most + 15) / 16 + g->n_adapter - 1);
     Name down, up;
-    down << "jl_adapter_down_" << plain_tag(g->type) << "_" << plain_tag(g->x_type);
-    rc = launch(c, down, (unsigned)g->ntok, (unsigned)(g->rank + 3) / 4, 256, 0, st, params, (unsigned)g->n);
+    down << "jl_adapter_down_" << plain_tag(g->type) << "_" << plain_tag(g->x_type) << "_n" << pl.nt;
+    rc = launch(c, down, slots, (unsigned)tok64, 256, 0, st, params, (unsigned)(pl.passes * pl.slices));
     if (rc != JL_OK) return rc;
-    up << "jl_adapter_up_" << plain_tag(g->type);
-    return launch(c, up, (unsigned)g->ntok, (unsigned)(most + 255) / 256, 256, (unsigned)g->rank * 4, st, params, (unsigned)g->n);
+    const bool few = g->ntok <= 16;
+    a.up_waves = wide * ((g->ntok + 63) / 64) >= 512L * c->num_cu ? 8 : 4;
+    unsigned blocks = 0;
+    for (int i = 0; i < g->n; i++) blocks += (unsigned)(g->rows[i] + 64 * a.up_waves - 1) / (64 * a.up_waves);
+    up << "jl_adapter_up_" << plain_tag(g->type) << (few ? "_t1" : "_t4") << (vec ? "" : "_any");
+    const unsigned groups = (unsigned)std::min(few ? std::min(g->ntok, 16) : most, g->n_adapter + 1);
+    return launch(c, up, blocks, groups, 64 * a.up_waves, 0, st, params, (unsigned)(few ? 1 : tok64));
 }
 
 int jl_dequant_dev(jl_ctx* c, int type, const void* src, float* dst, size_t n, void* stream) {

@@ -617,6 +617,9 @@ struct AdapterArgs {
     const uint32_t* ranks;                 // [n_adapter] or null
     const float* scale;                    // [n_adapter] or null
     const void* x;                         // [ntok][k]
-    float* u;                              // [ntok][n][rank] workspace
+    float* u;                              // [slices][ntok][n * rank_pad] workspace
     int n, n_adapter, rank, k, ntok;
+    int rank_pad;                          // rank rounded up to sixteen
+    int slices, passes;                    // K slices and passes over the columns of u (adapter_down)
+    int up_waves;                          // wavefronts a workgroup (adapter_up)
 };

@@ -688,10 +688,24 @@ JL_NORM_ROWS(l16_1, 16, 1, false, 256) JL_NORM_ROWS(l32_1, 32, 1, false, 256) JL
 JL_NORM_ROWS(l64_2, 64, 2, false, 256) JL_NORM_ROWS(l64_4, 64, 4, false, 256)
 JL_NORM_ROWS(wg_1, 64, 1, true, 1024) JL_NORM_ROWS(wg_2, 64, 2, true, 1024) JL_NORM_ROWS(wg_4, 64, 4, true, 1024)
 JL_NORM_ROWS(wg_8, 64, 8, true, 1024) JL_NORM_ROWS(wg_16, 64, 16, true, 1024)
-// grid = (tokens, ceil(rank / 4), projections), block = 256; grid = (tokens, ceil(rows / 256), projections), block = 256
-#define JL_ADAPTER(T, TYPE)                                                                                                                   \
-    extern "C" __global__ __launch_bounds__(256) void jl_adapter_down_##T##_f32(AdapterArgs p) { adapter_down_body<TYPE, JL_F32>(p); }        \
-    extern "C" __global__ __launch_bounds__(256) void jl_adapter_down_##T##_f16(AdapterArgs p) { adapter_down_body<TYPE, JL_F16>(p); }        \
-    extern "C" __global__ __launch_bounds__(256) void jl_adapter_down_##T##_bf16(AdapterArgs p) { adapter_down_body<TYPE, JL_BF16>(p); }      \
-    extern "C" __global__ __launch_bounds__(256) void jl_adapter_up_##T(AdapterArgs p) { adapter_up_body<TYPE>(p, (float*)jl_smem); }
+// grid = (tile slots, chunks of 64 tokens, passes * slices), block = 256
+#define JL_ADAPTER_DOWN(T, TYPE, XT, XTYPE, NT)                                                                    \
+    extern "C" __global__ __launch_bounds__(256) void jl_adapter_down_##T##_##XT##_n##NT(AdapterArgs p) {          \
+        __shared__ f32x4 red[4 * NT * 64];                                                                         \
+        adapter_down_body<TYPE, XTYPE, NT>(p, red);                                                                \
+    }
+// grid = (column blocks, group slots, chunks of 16 TT tokens), block = 64 p.up_waves (8 at most)
+#define JL_ADAPTER_UP(T, TYPE, TT)                                                                                 \
+    extern "C" __global__ __launch_bounds__(512) void jl_adapter_up_##T##_t##TT(AdapterArgs p) {                   \
+        __shared__ __attribute__((aligned(16))) uint8_t s[JL_AD_UP_LDS(TT)];                                       \
+        adapter_up_body<TYPE, TT, true>(p, s);                                                                     \
+    }                                                                                                              \
+    extern "C" __global__ __launch_bounds__(512) void jl_adapter_up_##T##_t##TT##_any(AdapterArgs p) {             \
+        __shared__ __attribute__((aligned(16))) uint8_t s[JL_AD_UP_LDS(TT)];                                       \
+        adapter_up_body<TYPE, TT, false>(p, s);                                                                    \
+    }
+#define JL_ADAPTER_X(T, TYPE, XT, XTYPE) JL_ADAPTER_DOWN(T, TYPE, XT, XTYPE, 1) JL_ADAPTER_DOWN(T, TYPE, XT, XTYPE, 4) JL_ADAPTER_DOWN(T, TYPE, XT, XTYPE, 8)
+#define JL_ADAPTER(T, TYPE)                                                                                        \
+    JL_ADAPTER_X(T, TYPE, f32, JL_F32) JL_ADAPTER_X(T, TYPE, f16, JL_F16) JL_ADAPTER_X(T, TYPE, bf16, JL_BF16)     \
+    JL_ADAPTER_UP(T, TYPE, 1) JL_ADAPTER_UP(T, TYPE, 4)
 JL_ADAPTER(f32, JL_F32) JL_ADAPTER(f16, JL_F16) JL_ADAPTER(bf16, JL_BF16)
