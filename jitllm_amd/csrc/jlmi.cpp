@@ -37,6 +37,7 @@ struct Tuning {
     int xpre = 0;               // decode matvec: 1 / 2 / 4 float4 groups of x a thread loads ahead of its weights
     int q8pair = 0;             // Q8_0 rows: 2 keeps one block a lane-slot (2-byte-aligned loads)
     int packed_rw = 0, packed_block = 0, moe_group = 0, moe_logits = 0;
+    int adapter_form = 0, adapter_slices = 0, adapter_sets = 0;
     int moe_shares = 0;
     int gemm_rows = 0;
     int gemm_form = 0;
@@ -2237,10 +2238,12 @@ int jl_ctx_create(jl_ctx** out, const jl_options* opts) {
     for (const char* form : {"l16_1", "l32_1", "l64_1", "l64_2", "l64_4", "wg_1", "wg_2", "wg_4", "wg_8", "wg_16"})
         for (const char* any : {"", "_any"}) names.push_back(std::string("jl_norm_rows_") + form + any);
     for (const char* g : {"g2", "g4", "g8", "g16"}) names.push_back(std::string("jl_moe_select_") + g);
+    names.push_back("jl_adapter_sum");
     for (const char* t : {"f32", "f16", "bf16"}) {
         for (const char* xt : {"f32", "f16", "bf16"})
-            for (const char* nt : {"_n1", "_n4", "_n8"}) names.push_back(std::string("jl_adapter_down_") + t + "_" + xt + nt);
-        for (const char* form : {"_t1", "_t1_any", "_t4", "_t4_any"}) names.push_back(std::string("jl_adapter_up_") + t + form);
+            for (const char* nt : {"_n1", "_n2"}) names.push_back(std::string("jl_adapter_down_") + t + "_" + xt + nt);
+        for (const char* l : {"_l1", "_l2", "_l4", "_l8"}) names.push_back(std::string("jl_adapter_one_") + t + l);
+        for (const char* form : {"_k1", "_k1_any", "_k2", "_k2_any", "_many", "_many_any"}) names.push_back(std::string("jl_adapter_up_") + t + form);
     }
     for (const char* pl : {"", "planes_"})
         for (int nt = 1; nt <= 4; nt++)
@@ -2411,6 +2414,9 @@ int jl_set_tuning(jl_ctx* c, const char* key, int value) {
     else if (!strcmp(key, "matvec.grid")) c->tune.grid = value;
     else if (!strcmp(key, "packed.rw")) c->tune.packed_rw = value;
     else if (!strcmp(key, "packed.block")) c->tune.packed_block = value;
+    else if (!strcmp(key, "adapter.form")) c->tune.adapter_form = value;
+    else if (!strcmp(key, "adapter.slices")) c->tune.adapter_slices = value;
+    else if (!strcmp(key, "adapter.sets")) c->tune.adapter_sets = value;
     else if (!strcmp(key, "moe.group")) c->tune.moe_group = value;
     else if (!strcmp(key, "moe.logits")) c->tune.moe_logits = value;
     else if (!strcmp(key, "moe.q6k_cols")) (void)value;   // (accepted, without effect)
@@ -2535,19 +2541,22 @@ int adapter_ws_ensure(jl_ctx* c, size_t need) {
 }  // namespace
 
 namespace {
-// How an adapter call is cut: K slices for as many workgroups as two rounds of the chip hold.
+// How adapter_down is cut: a group is 64 tokens' of one adapter; a workgroup takes a group, 4 nt tiles of sixteen rows of A and a slice of K.
+// Slices for two workgroups a CU, as far as the groups are known: there is one for 64 tokens at least, and one for every adapter met.
 struct AdapterPlan { int rank_pad, nt, passes, slices; };
 AdapterPlan adapter_plan(const jl_ctx* c, int ntok, int n, int rank, int k, int n_adapter) {
     AdapterPlan a;
     a.rank_pad = (rank + 15) / 16 * 16;
     const int tiles = n * a.rank_pad / 16;
-    a.nt = tiles <= 1 ? 1 : tiles <= 4 ? 4 : 8;
-    a.passes = (tiles + a.nt - 1) / a.nt;
-    const long units = std::max((long)(ntok + 15) / 16, (long)std::min(ntok, n_adapter));
-    a.slices = (int)std::max(1l, std::min({16l, 2l * c->num_cu / (units * a.passes), (long)k / 32 / 8}));
+    a.nt = tiles <= 4 ? 1 : 2;
+    a.passes = (tiles + 4 * a.nt - 1) / (4 * a.nt);
+    const long units = (long)a.passes * std::max((ntok + 63) / 64, std::min(ntok, n_adapter)), steps = (k + 127) / 128;
+    a.slices = (int)std::max(1l, std::min({16l, steps, c->tune.adapter_slices ? (long)c->tune.adapter_slices : 2l * c->num_cu / units}));
     return a;
 }
-size_t adapter_ws_bytes(const AdapterPlan& a, int ntok, int n) { return (size_t)a.slices * ntok * n * a.rank_pad * 4; }
+// Bytes of the sums of `rows` slices * tokens and of u in bf16 pieces.
+size_t adapter_part_bytes(size_t rows, int n, int rank) { return rows * n * ((rank + 15) / 16 * 16) * 4; }
+size_t adapter_u_bytes(int ntok, int n, int rank) { return (size_t)ntok * n * ((rank + 31) / 32) * 192; }
 }  // namespace
 
 int jl_reserve_adapters(jl_ctx* c, int max_tok, int n, int max_rank) {
@@ -2555,9 +2564,9 @@ int jl_reserve_adapters(jl_ctx* c, int max_tok, int n, int max_rank) {
     if (max_tok <= 0 || n < 1 || n > JL_MAX_GROUP || max_rank <= 0) return fail(c, JL_ERR_ARG, "reserve adapters: %d tokens, %d projections, rank %d", max_tok, n, max_rank);
     if (max_rank > 512) return JL_DECLINED;
     HIP_TRY(c, H->SetDevice(c->device));
-    // slices * tokens: sixteen slices at most, and more than one only while slices * tokens / 16 is within two rounds of the chip
-    const size_t cols = (size_t)n * ((max_rank + 15) / 16 * 16);
-    return adapter_ws_ensure(c, std::max((size_t)max_tok, std::min((size_t)16 * max_tok, (size_t)32 * c->num_cu)) * cols * 4);
+    // slices * tokens: sixteen slices at most, more than one while slices * tokens / 64 is within two workgroups a CU
+    const size_t rows = std::max((size_t)max_tok, std::min((size_t)16 * max_tok, (size_t)128 * c->num_cu));
+    return adapter_ws_ensure(c, adapter_part_bytes(rows, n, max_rank) + adapter_u_bytes(max_tok, n, max_rank));
 }
 
 int jl_adapter_group_dev(jl_ctx* c, const jl_adapter_group* g, void* stream) {
@@ -2579,28 +2588,48 @@ int jl_adapter_group_dev(jl_ctx* c, const jl_adapter_group* g, void* stream) {
     if (!aligned16(g->x) || (((uintptr_t)g->ids | (uintptr_t)g->ranks | (uintptr_t)g->scale) & 3)) return JL_DECLINED;
     if (g->ntok > 16 * 65535 || wide > 0x1000000) return JL_DECLINED;   // grid of a launch
     HIP_TRY(c, H->SetDevice(c->device));
-    const AdapterPlan pl = adapter_plan(c, g->ntok, g->n, g->rank, g->k, g->n_adapter);
-    int rc = adapter_ws_ensure(c, adapter_ws_bytes(pl, g->ntok, g->n));
-    if (rc != JL_OK) return rc;
-    a.ids = g->ids; a.ranks = g->ranks; a.scale = g->scale; a.x = g->x; a.u = (float*)c->adapter_ws;
+    a.ids = g->ids; a.ranks = g->ranks; a.scale = g->scale; a.x = g->x; a.u = nullptr;
     a.n = g->n; a.n_adapter = g->n_adapter; a.rank = g->rank; a.k = g->k; a.ntok = g->ntok;
-    a.rank_pad = pl.rank_pad; a.slices = pl.slices; a.passes = pl.passes;
+    const AdapterPlan pl = adapter_plan(c, g->ntok, g->n, g->rank, g->k, g->n_adapter);
+    a.part = nullptr; a.u = nullptr;
+    a.rank_pad = pl.rank_pad; a.passes = pl.passes; a.slices = pl.slices; a.x_type = g->x_type; a.up_sets = a.one_sets = 1;
     hipStream_t st = pick_stream(c, stream);
     void* params[] = {&a};
-    // a chunk of 64 tokens has at most 4 + n_adapter tiles
-    const int tok64 = (g->ntok + 63) / 64, most = std::min(g->ntok, 64);
-    const unsigned slots = (unsigned)std::min(most, (most + 15) / 16 + g->n_adapter - 1);
-    Name down, up;
-    down << "jl_adapter_down_" << plain_tag(g->type) << "_" << plain_tag(g->x_type) << "_n" << pl.nt;
-    rc = launch(c, down, slots, (unsigned)tok64, 256, 0, st, params, (unsigned)(pl.passes * pl.slices));
+    const char *t = plain_tag(g->type), *xt = plain_tag(g->x_type);
+    const int chunks = (g->ntok + 63) / 64, most = std::min(g->ntok, 64);   // the kernels look at 64 tokens at a time
+    auto blocks = [&](int width) {   // column blocks of all projections
+        unsigned b = 0;
+        for (int i = 0; i < g->n; i++) b += (unsigned)(g->rows[i] + width - 1) / width;
+        return b;
+    };
+    Name name;
+    const long sets = (long)g->ntok * blocks(1024);
+    const bool one = g->rank <= 64 && g->ntok <= 65535 && (c->tune.adapter_form ? c->tune.adapter_form == 1 : g->rank <= 16 && sets <= c->num_cu);
+    if (one) {
+        const int l = g->rank <= 8 ? 1 : g->rank <= 16 ? 2 : g->rank <= 32 ? 4 : 8;
+        name << "jl_adapter_one_" << t << "_l" << l;
+        return launch(c, name, blocks(1024 * a.one_sets), (unsigned)g->ntok, 1024, 0, st, params);
+    }
+    const size_t part = adapter_part_bytes((size_t)a.slices * g->ntok, g->n, g->rank);
+    int rc = adapter_ws_ensure(c, part + adapter_u_bytes(g->ntok, g->n, g->rank));
     if (rc != JL_OK) return rc;
-    const bool few = g->ntok <= 16;
-    a.up_waves = wide * ((g->ntok + 63) / 64) >= 512L * c->num_cu ? 8 : 4;
-    unsigned blocks = 0;
-    for (int i = 0; i < g->n; i++) blocks += (unsigned)(g->rows[i] + 64 * a.up_waves - 1) / (64 * a.up_waves);
-    up << "jl_adapter_up_" << plain_tag(g->type) << (few ? "_t1" : "_t4") << (vec ? "" : "_any");
-    const unsigned groups = (unsigned)std::min(few ? std::min(g->ntok, 16) : most, g->n_adapter + 1);
-    return launch(c, up, blocks, groups, 64 * a.up_waves, 0, st, params, (unsigned)(few ? 1 : tok64));
+    a.part = (float*)c->adapter_ws;
+    a.u = (uint16_t*)((char*)c->adapter_ws + part);
+    name << "jl_adapter_down_" << t << "_" << xt << "_n" << pl.nt;
+    rc = launch(c, name, (unsigned)std::min(most, g->n_adapter), (unsigned)chunks, 256, 0, st, params, (unsigned)(a.passes * a.slices));
+    if (rc != JL_OK) return rc;
+    const double added = (double)blocks(256) * g->ntok * a.slices * g->rank * 4;   // bytes that adapter_up would add up
+    if (c->tune.adapter_form ? c->tune.adapter_form == 3 : added > 30e6) {
+        const size_t octs = (size_t)g->ntok * g->n * ((a.rank_pad + 31) / 32) * 4;
+        rc = launch(c, "jl_adapter_sum", (unsigned)((octs + 255) / 256), 1, 256, 0, st, params);
+        if (rc != JL_OK) return rc;
+        a.slices = 0;
+    }
+    Name up;
+    up << "jl_adapter_up_" << t << (g->rank <= 32 ? "_k1" : g->rank <= 64 ? "_k2" : "_many") << (vec ? "" : "_any");
+    a.up_sets = c->tune.adapter_sets ? c->tune.adapter_sets : (long)blocks(256) * chunks >= 6 * c->num_cu ? 2 : 1;
+    const unsigned groups = g->ntok >= 1024 ? 1 : (unsigned)std::min(most, g->n_adapter + 1);
+    return launch(c, up, blocks(256 * a.up_sets), groups, 256, 0, st, params, (unsigned)chunks);
 }
 
 int jl_dequant_dev(jl_ctx* c, int type, const void* src, float* dst, size_t n, void* stream) {

@@ -2,16 +2,19 @@
 //   out_i[t] = base_i[t] + scale[a] * B_i[a] (A_i[a] x[t]),     A_i [n_adapter][rank][k], B_i [n_adapter][rows_i][rank]
 // for up to four projections that read one x.  A token whose id no adapter has, or whose adapter has rank 0, gets base alone.
 //
-// Two kernels on the bf16 matrix cores: adapter_down makes u = scale * A x for tiles of sixteen tokens of one adapter, adapter_up adds
-// B u to base.  Both take 64 (16) consecutive tokens and find for themselves which of them share an adapter (a ballot per adapter met), so
-// nothing is sorted beforehand; a token meets its own adapter only, so no number of another's can reach it.
+// On the bf16 matrix cores: adapter_down makes sums of u = A x for the tokens of an adapter and a slice of K, adapter_up adds B u to base (where
+// many column blocks would each add the slices up, adapter_sum does it first); for few tokens of a small rank adapter_one does everything
+// in one launch, by dot products in f32.  A workgroup looks at 64 consecutive tokens and finds for itself which of them share an adapter (a ballot
+// per adapter met), so nothing is sorted beforehand; a token meets its own adapter only, so no number of another's can reach it.
 //
 // Products are exact: an f32 value is three bf16 values (8 mantissa bits each, cut off, not rounded), an f16 value two, and every
 // piece of one operand meets every piece of the other in the f32 accumulator -- one matrix instruction for bf16 x bf16, three for f32 x
 // against bf16 adapters, nine for f32 x f32.  What rounds is the f32 sum, as in a dot product in f32.  (An infinity cut into pieces
 // leaves a NaN: it was going to be no finite number.)
 //
-// adapter_up is bound by base and out, adapter_down by x (many tokens) or the adapters (few).
+// What decides the layout of the work (measured on MI355X): sixteen rows of 64 bytes a load, as the matrix instruction's operands and results lie, run
+// at two thirds of the rate of rows of 256 bytes and more, so x, base and out are moved by rows and change places in LDS; and a CU draws about 35
+// bytes a ns from the L2s whatever its wavefronts ask for, so an adapter's A is spread over as many workgroups as there are.
 #pragma once
 #include "args.h"
 #include "common.h"
@@ -93,231 +96,521 @@ template <int PA, int PB> __device__ __forceinline__ f32x4 ad_mfma(const u32x4 (
     return acc;
 }
 
-// A lane's token of the chunk [first, first + size): its adapter, n_adapter where it has none; 0xFFFFFFFF: no token.
-__device__ __forceinline__ u32 ad_id(const AdapterArgs& p, int first, int size) {
-    const int lane = threadIdx.x & 63, tok = first + lane;
-    if (lane >= size || tok >= p.ntok) return 0xFFFFFFFFu;
+// A lane's token of the 64 from `first` on: its adapter, n_adapter where it has none; 0xFFFFFFFF: no token.
+__device__ __forceinline__ u32 ad_id(const AdapterArgs& p, int first) {
+    const int tok = first + (threadIdx.x & 63);
+    if (tok >= p.ntok) return 0xFFFFFFFFu;
     u32 id = min(p.ids[tok], (u32)p.n_adapter);
     if (p.ranks && id < (u32)p.n_adapter && p.ranks[id] == 0) id = (u32)p.n_adapter;
     return id;
 }
-__device__ __forceinline__ int ad_rank(const AdapterArgs& p, u32 id) { return p.ranks ? (int)min(p.ranks[id], (u32)p.rank) : p.rank; }
+__device__ __forceinline__ int ad_rank(const AdapterArgs& p, u32 id) {
+    return id >= (u32)p.n_adapter ? 0 : p.ranks ? (int)min(p.ranks[id], (u32)p.rank) : p.rank;
+}
+// Four consecutive elements as f32.
+template <int T> struct AdQuad {
+    u32x2 w;
+    __device__ __forceinline__ void load(const void* p, size_t at) { w = *(const u32x2*)((const uint16_t*)p + at); }
+    __device__ __forceinline__ float value(int i) const {
+        const uint16_t h = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+        return T == JL_F16 ? half_bits_to_f32(h) : __uint_as_float((u32)h << 16);
+    }
+};
+template <> struct AdQuad<JL_F32> {
+    f32x4 w;
+    __device__ __forceinline__ void load(const void* p, size_t at) { w = *(const f32x4*)((const float*)p + at); }
+    __device__ __forceinline__ float value(int i) const { return w[i]; }
+};
 
-// ---------------------------------------------------------------- u = scale * A x
-// grid = (tile slots of a chunk of 64 tokens, chunks, column passes * K slices), block = 256, LDS = 4 NT KB.
-// A tile is up to sixteen tokens of one adapter; workgroup (slot, chunk) takes the chunk's tiles slot, slot + gridDim.x, ...  The four
-// wavefronts cut the workgroup's slice of K in four and add their sums through LDS; NT tiles of sixteen columns (rows of A, all
-// projections' side by side, each rounded up to sixteen) a pass.  u is [K slices][ntok][n * rank_pad].
-template <int T, int XT, int NT>
-__device__ __forceinline__ void adapter_down_body(const AdapterArgs& p, f32x4* red) {
-    constexpr int PW = AdType<T>::pieces, PX = AdType<XT>::pieces;
-    constexpr int UN = NT * sizeof(AdType<T>) <= 16 ? 8 : NT * sizeof(AdType<T>) <= 64 ? 2 : 1;   // K steps asked for at a time
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int chunk = blockIdx.y * 64, pass = blockIdx.z % p.passes, slice = blockIdx.z / p.passes;
-    const int rp = p.rank_pad, ncol = p.n * rp, tiles = ncol / 16;
-    const u32 id = ad_id(p, chunk, 64);
-    const int steps = p.k / 32, part = slice * 4 + wave, parts = p.slices * 4;
-    const int lo = (int)((long)steps * part / parts), hi = (int)((long)steps * (part + 1) / parts);
-
-    int seen = 0, want = blockIdx.x;
-    uint64_t rest = __ballot(id < (u32)p.n_adapter);
-    while (rest) {   // uniform, and the same in every wavefront
-        const int lead = __builtin_ctzll(rest);
-        const u32 a = (u32)__builtin_amdgcn_readlane((i32)id, lead);
-        uint64_t of = __ballot(id == a);
-        const int all = __builtin_popcountll(of), nt = (all + 15) / 16;
-        if (want >= seen + nt) {
-            seen += nt;
+// The groups of the 64 tokens from `first` on, one adapter's (or, with `limit` one higher, none's) tokens each, in the order in which they
+// come; every gridDim-th is a workgroup's.  Uniform.
+struct AdGroups {
+    uint64_t rest;
+    int at;
+    __device__ __forceinline__ AdGroups(u32 id, u32 limit) : rest(__ballot(id < limit)), at(0) {}
+    // the next of the groups slot, slot + slots, ...: its adapter and which of the 64 lanes' tokens are of it
+    __device__ __forceinline__ bool next(u32 id, int slot, int slots, u32& a, uint64_t& of) {
+        while (rest) {
+            a = (u32)__builtin_amdgcn_readlane((i32)id, __builtin_ctzll(rest));
+            of = __ballot(id == a);
             rest &= ~of;
-            continue;
+            if (at++ % slots == slot) return true;
         }
-        const int sub = want - seen, count = min(16, all - 16 * sub);
-        for (int i = 0; i < 16 * sub; i++) of &= of - 1;
-        int tok = chunk + __builtin_ctzll(of);   // the lane's token, lane % 16 of the tile; the first where there are fewer
-        for (int i = 0; i < count; i++) {
-            if ((lane & 15) == i) tok = chunk + __builtin_ctzll(of);
-            of &= of - 1;
-        }
-        const int rank = ad_rank(p, a);
-        const size_t xat = (size_t)tok * p.k + 8 * (lane >> 4);
+        return false;
+    }
+};
+// The group's tokens, in order, to toks (every wavefront writes the same).
+__device__ __forceinline__ void ad_tokens(uint64_t of, int first, int* toks) {
+    const int lane = threadIdx.x & 63;
+    if ((of >> lane) & 1) toks[__builtin_popcountll(of & ((1ull << lane) - 1))] = first + lane;
+}
+
+// ---------------------------------------------------------------- sums of A x
+// grid = (group slots of 64 tokens, ntok / 64, passes * slices), block = 256.  A workgroup takes a group's up to 64 tokens (four tiles), NT column
+// tiles a wavefront (sixteen rows of A each; all projections' side by side, a rank rounded up to sixteen) and a slice of K, 128 at a time: x by
+// rows of 512 bytes through registers, cut into pieces on the way to LDS, where all four wavefronts read it; A's fragments straight from
+// memory, each once a workgroup.  Writes part [slices][ntok][n * rank_pad].
+// LDS: [pieces][64 tokens][136] bf16 (a row's 272 bytes put sixteen rows' reads on different banks).
+#define JL_AD_DOWN_K 128
+#define JL_AD_DOWN_ROW 136
+template <int T, int XT, int NT>
+__device__ __forceinline__ void adapter_down_body(const AdapterArgs& p, uint16_t* sx, int* toks) {
+    constexpr int PW = AdType<T>::pieces, PX = AdType<XT>::pieces, ROW = JL_AD_DOWN_ROW;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, first = blockIdx.y * 64;
+    const int pass = blockIdx.z % p.passes, slice = blockIdx.z / p.passes;
+    const int ctiles = p.rank_pad / 16, all = p.n * ctiles, c0 = (pass * 4 + wave) * NT;
+    const int steps = (p.k + JL_AD_DOWN_K - 1) / JL_AD_DOWN_K;
+    const int lo = steps * slice / p.slices, hi = steps * (slice + 1) / p.slices;
+    const u32 id = ad_id(p, first);
+    AdGroups groups(id, (u32)p.n_adapter);
+    u32 a;
+    uint64_t of;
+    while (groups.next(id, blockIdx.x, gridDim.x, a, of)) {
+        const int count = __builtin_popcountll(of), nt = (count + 15) / 16, rank = ad_rank(p, a);
+        ad_tokens(of, first, toks);
+        __syncthreads();
         const void* wp[NT];
         size_t wat[NT];
 #pragma unroll
         for (int t = 0; t < NT; t++) {
-            const int c = min(pass * NT + t, tiles - 1), i = c * 16 / rp, r = min(c * 16 % rp + (lane & 15), rank - 1);
+            const int c = min(c0 + t, all - 1), i = c / ctiles, r = min((c - i * ctiles) * 16 + (lane & 15), rank - 1);
             wp[t] = p.a[i];
             wat[t] = ((size_t)a * p.rank + r) * p.k + 8 * (lane >> 4);
         }
-        f32x4 acc[NT];
+        // a thread's rows of x: token 8 i + tid / 32 of the group, four elements from 4 (tid % 32) on
+        size_t xat[8];
 #pragma unroll
-        for (int t = 0; t < NT; t++) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-        auto group = [&](int s, auto un) {
-            constexpr int U = decltype(un)::value;
-            AdType<XT> x[U];
-            AdType<T> w[U][NT];
+        for (int i = 0; i < 8; i++) xat[i] = (size_t)toks[min(8 * i + tid / 32, count - 1)] * p.k + 4 * (tid & 31);
+        AdQuad<XT> x[8];
+        AdType<T> w[4][NT];
+        auto load_x = [&](int s) {
+            const int k0 = s * JL_AD_DOWN_K;
+            if (k0 + 4 * (tid & 31) >= p.k) return;
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                x[u].load(p.x, xat + 32 * (size_t)(s + u));
+            for (int i = 0; i < 8; i++)
+                if (i < 2 * nt) x[i].load(p.x, xat[i] + k0);
+        };
+        auto load_w = [&](int s) {
+            const int k0 = s * JL_AD_DOWN_K;
 #pragma unroll
-                for (int t = 0; t < NT; t++) w[u][t].load(wp[t], wat[t] + 32 * (size_t)(s + u));
-            }
+            for (int q = 0; q < 4; q++)
+                if (k0 + 32 * q < p.k) {
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                u32x4 xp[PX];
-                ad_pieces<XT>(x[u], xp);
+                    for (int t = 0; t < NT; t++)
+                        if (c0 + t < all) w[q][t].load(wp[t], wat[t] + k0 + 32 * q);
+                }
+        };
+        f32x4 acc[4][NT];
 #pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    u32x4 wq[PW];
-                    ad_pieces<T>(w[u][t], wq);
-                    acc[t] = ad_mfma<PW, PX>(wq, xp, acc[t]);
+        for (int m = 0; m < 4; m++)
+#pragma unroll
+            for (int t = 0; t < NT; t++) acc[m][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (lo < hi) {
+            load_x(lo);
+            load_w(lo);
+        }
+        for (int s = lo; s < hi; s++) {
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (i < 2 * nt) {
+                    float v[4];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) v[j] = x[i].value(j);
+#pragma unroll
+                    for (int n = 0; n < PX; n++) {
+                        u32 b[4];
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            b[j] = __float_as_uint(v[j]);
+                            if (n + 1 < PX) v[j] -= __uint_as_float(b[j] & 0xFFFF0000u);
+                        }
+                        *(u32x2*)(sx + (n * 64 + 8 * i + tid / 32) * ROW + 4 * (tid & 31)) =
+                            u32x2{__builtin_amdgcn_perm(b[1], b[0], 0x07060302), __builtin_amdgcn_perm(b[3], b[2], 0x07060302)};
+                    }
+                }
+            __syncthreads();
+            if (s + 1 < hi) load_x(s + 1);
+            const int nq = min(4, (p.k - s * JL_AD_DOWN_K) / 32);
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                if (q >= nq || c0 >= all) continue;
+                u32x4 wq[NT][PW];
+#pragma unroll
+                for (int t = 0; t < NT; t++) ad_pieces<T>(w[q][t], wq[t]);
+#pragma unroll
+                for (int m = 0; m < 4; m++) {
+                    if (m >= nt) continue;
+                    u32x4 xq[PX];
+#pragma unroll
+                    for (int n = 0; n < PX; n++) xq[n] = *(const u32x4*)(sx + (n * 64 + 16 * m + (lane & 15)) * ROW + 32 * q + 8 * (lane >> 4));
+#pragma unroll
+                    for (int t = 0; t < NT; t++) acc[m][t] = ad_mfma<PW, PX>(wq[t], xq, acc[m][t]);
                 }
             }
-        };
-        int s = lo;
-        for (; s + UN <= hi; s += UN) group(s, GemmIntC<UN>{});
-        if constexpr (UN > 1)
-            for (; s < hi; s++) group(s, GemmIntC<1>{});
-#pragma unroll
-        for (int t = 0; t < NT; t++) red[(wave * NT + t) * 64 + lane] = acc[t];
-        __syncthreads();
-        const float g = p.scale ? p.scale[a] : 1.f;
-        for (int t = wave; t < NT; t += 4) {
-            const int c = pass * NT + t;
-            if (c >= tiles) break;
-            f32x4 v = red[t * 64 + lane];
-#pragma unroll
-            for (int w = 1; w < 4; w++) v += red[(w * NT + t) * 64 + lane];
-            const int r = c * 16 % rp + 4 * (lane >> 4);
-#pragma unroll
-            for (int i = 0; i < 4; i++) v[i] = r + i < rank ? g * v[i] : 0.f;
-            if ((lane & 15) < count) *(f32x4*)(p.u + ((size_t)slice * p.ntok + tok) * ncol + c * 16 + 4 * (lane >> 4)) = v;
+            if (s + 1 < hi) load_w(s + 1);
+            __syncthreads();
         }
-        __syncthreads();
-        want += gridDim.x;
+#pragma unroll
+        for (int m = 0; m < 4; m++) {
+            if (16 * m + (lane & 15) >= count) continue;
+            float* u = p.part + ((size_t)slice * p.ntok + toks[16 * m + (lane & 15)]) * all * 16 + 4 * (lane >> 4);
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+                if (c0 + t < all) *(f32x4*)(u + (c0 + t) * 16) = acc[m][t];
+        }
+        __syncthreads();   // (toks is the next group's)
     }
 }
 
-// ---------------------------------------------------------------- out = base + B u
-// grid = (column blocks of all projections, group slots of a chunk of 16 TT tokens, chunks), block = 64 p.up_waves, a wavefront 64 columns
-// (rows of B).  A group is the chunk's tokens of one adapter (or of none), up to TT tiles of sixteen; B's fragments meet all of them.
-// u's fragments, its K slices added, lie in LDS as bf16 pieces, a rank of 128 at a time.
-// VEC: rows of out and base on 16-byte boundaries.
-#define JL_AD_UP_LDS(TT) ((TT) * 4 * 3 * 1024 + (TT) * 16 * 4)
-template <int T, int TT, bool VEC>
-__device__ __forceinline__ void adapter_up_body(const AdapterArgs& p, uint8_t* smem) {
-    constexpr int PW = AdType<T>::pieces;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, threads = 64 * p.up_waves;
-    const int chunk = blockIdx.z * 16 * TT;
-    int pi = 0, cb = blockIdx.x;   // projection, column block in it
-    while (pi + 1 < p.n && cb >= (p.rows[pi] + threads - 1) / threads) {
-        cb -= (p.rows[pi] + threads - 1) / threads;
-        pi++;
+// Eight of a token's u, of projection pi from r on: the slices added up, times the adapter's scale, 0 from its rank on, as bf16 pieces.
+__device__ __forceinline__ void ad_sum_u(const AdapterArgs& p, int tok, int pi, int r, float scale, int rank, u32x4 (&o)[3]) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = 0.f;
+    if (r < p.rank_pad) {
+        const int ncol = p.n * p.rank_pad;
+        const float* u = p.part + (size_t)tok * ncol + pi * p.rank_pad + r;
+        const size_t step = (size_t)p.ntok * ncol;
+        for (int s = 0; s < p.slices; s += 4) {   // four slices on their way at a time
+            f32x4 lo[4], hi[4];
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const float* at = u + step * min(s + q, p.slices - 1);
+                lo[q] = *(const f32x4*)at;
+                hi[q] = *(const f32x4*)(at + 4);
+            }
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+                if (s + q < p.slices) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) { v[i] += lo[q][i]; v[4 + i] += hi[q][i]; }
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = r + i < rank ? scale * v[i] : 0.f;
     }
-    const int rows = p.rows[pi], col0 = cb * threads + wave * 64;
+    ad_split<3>(v, o);
+}
+// part -> u [ntok][n][K steps of 32][3 pieces][32] bf16.  grid = ceil(ntok * n * K steps * 4 / 256), block = 256: a thread eight of a row.
+__device__ __forceinline__ void adapter_sum_body(const AdapterArgs& p) {
+    const int ks = (p.rank_pad + 31) / 32;
+    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    const int oct = (int)(i % (ks * 4)), pi = (int)(i / (ks * 4) % p.n);
+    const size_t tok = i / ((size_t)ks * 4 * p.n);
+    if (tok >= (size_t)p.ntok) return;
+    const u32 id = p.ids[tok];
+    if (id >= (u32)p.n_adapter) return;   // (nobody reads u of a token without an adapter)
+    u32x4 o[3];
+    ad_sum_u(p, (int)tok, pi, 8 * oct, p.scale ? p.scale[id] : 1.f, ad_rank(p, id), o);
+    uint16_t* u = p.u + ((tok * p.n + pi) * ks + oct / 4) * 96 + oct % 4 * 8;
+#pragma unroll
+    for (int n = 0; n < 3; n++) *(u32x4*)(u + 32 * n) = o[n];
+}
+
+// ---------------------------------------------------------------- out = base + B u
+// A fragment of B: eight columns of row `col` of the adapter's sheet from r on, zeros from its rank on.
+template <int T>
+__device__ __forceinline__ void ad_load_b(AdType<T>& w, const AdapterArgs& p, int pi, u32 a, int col, int r, int rank) {
+    w.load_some(p.b[pi], ((size_t)a * p.rows[pi] + col) * p.rank + min(r, rank), min(max(rank - r, 0), 8));
+}
+// The projection of a column block and the block's number in it; width: columns a block.
+__device__ __forceinline__ int ad_projection(const AdapterArgs& p, int& block, int width) {
+    int i = 0;
+    while (i + 1 < p.n && block >= (p.rows[i] + width - 1) / width) {
+        block -= (p.rows[i] + width - 1) / width;
+        i++;
+    }
+    return i;
+}
+
+// grid = (column blocks of all projections, group slots of 64 tokens, ntok / 64), block = 256, a wavefront 64 columns (rows of B) a set of
+// 256, p.up_sets sets.  u's fragments of the group's (up to four) tiles lie in LDS, KS K steps of 32 at a time; B's stay in registers and meet
+// tile after tile.  A tile's sums change places in LDS and meet base by rows of 256 bytes, asked for a tile ahead.
+// KS = 1: ranks up to 32, 2: up to 64.  MANY: any rank, KS steps at a time; the four tiles' sums stay in registers and base is read at the end.
+// VEC: rows of out and base on 16-byte boundaries.
+// LDS: frag [4 tiles][KS][3][64] x 16 bytes, move [4 wavefronts][16][68] floats, toks [64].
+#define JL_AD_MOVE 68
+template <int T, int KS, bool MANY, bool VEC>
+__device__ __forceinline__ void adapter_up_body(const AdapterArgs& p, u32x4* frag, float* move, int* toks) {
+    constexpr int PW = AdType<T>::pieces;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, first = blockIdx.z * 64;
+    int block = blockIdx.x;
+    const int pi = ad_projection(p, block, 256 * p.up_sets);
+    const int rows = p.rows[pi], ksteps = (p.rank_pad + 31) / 32;
     const float* base = p.base[pi];
     float* out = p.out[pi];
-    const int rp = p.rank_pad, ncol = p.n * rp;
-    u32x4* frag = (u32x4*)smem;                                   // [ks][tile][piece][lane]
-    int* toks = (int*)(smem + TT * 4 * 3 * 1024);
-    const u32 id = ad_id(p, chunk, 16 * TT);
-
-    int at = 0;
-    uint64_t rest = __ballot(id != 0xFFFFFFFFu);
-    while (rest) {   // uniform, and the same in every wavefront
-        const int lead = __builtin_ctzll(rest);
-        const u32 a = (u32)__builtin_amdgcn_readlane((i32)id, lead);
-        const uint64_t of = __ballot(id == a);
-        rest &= ~of;
-        if (at++ % (int)gridDim.y != (int)blockIdx.y) continue;
-        const int count = __builtin_popcountll(of), nt = (count + 15) / 16;
+    move += wave * 16 * JL_AD_MOVE;
+    const u32 id = ad_id(p, first);
+    AdGroups groups(id, (u32)p.n_adapter + 1);
+    u32 a;
+    uint64_t of;
+    while (groups.next(id, blockIdx.y, gridDim.y, a, of)) {
         const bool none = a >= (u32)p.n_adapter;
         if (none && base == out) continue;
-        if (wave == 0 && id == a) toks[__builtin_popcountll(of & ((1ull << lane) - 1))] = chunk + lane;
+        const int count = __builtin_popcountll(of), nt = (count + 15) / 16, rank = ad_rank(p, a);
+        const float scale = none || !p.scale ? 1.f : p.scale[a];
+        ad_tokens(of, first, toks);
         __syncthreads();
-        // base, asked for ahead of everything
-        f32x4 bs[TT][4], acc[TT][4];
-        size_t oat[TT];
-        bool live[TT];
+        // by rows: token 4 i + lane / 16 of a tile, four columns from 4 (lane % 16) on
+        f32x4 bs[4];
+        size_t oat[4];
+        auto load_base = [&](int tt, int col) {
+            const int c = col + 4 * (lane & 15);
 #pragma unroll
-        for (int tt = 0; tt < TT; tt++) {
-            const int m = 16 * tt + (lane & 15);
-            live[tt] = m < count;
-            oat[tt] = (size_t)toks[min(m, count - 1)] * rows;
-#pragma unroll
-            for (int c = 0; c < 4; c++) {
-                const int col = col0 + 16 * c + 4 * (lane >> 4);
-                bs[tt][c] = acc[tt][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-                if (tt < nt && base) {
+            for (int i = 0; i < 4; i++) {
+                oat[i] = (size_t)toks[min(16 * tt + 4 * i + (lane >> 4), count - 1)] * rows + c;
+                bs[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if (base) {
                     if (VEC) {
-                        if (col < rows) bs[tt][c] = *(const f32x4*)(base + oat[tt] + col);
+                        if (c < rows) bs[i] = *(const f32x4*)(base + oat[i]);
                     } else {
 #pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            if (col + i < rows) bs[tt][c][i] = base[oat[tt] + col + i];
+                        for (int e = 0; e < 4; e++)
+                            if (c + e < rows) bs[i][e] = base[oat[i] + e];
                     }
                 }
             }
-        }
-        const int rank = none ? 0 : ad_rank(p, a);
-        for (int r0 = 0; r0 < rank; r0 += 128) {
-            const int nk = min(4, (rank - r0 + 31) / 32);
-            for (int f = wave; f < nk * nt; f += p.up_waves) {
-                const int ks = f / nt, tt = f % nt, m = 16 * tt + (lane & 15), r = r0 + 32 * ks + 8 * (lane >> 4);
-                float v[8];
+        };
+        auto finish = [&](int tt, int col, f32x4 (&acc)[4], const f32x4 (&b0)[4], const size_t (&o0)[4]) {
+            f32x4 v[4];
+            if (none) {
 #pragma unroll
-                for (int i = 0; i < 8; i++) v[i] = 0.f;
-                if (m < count && r < rp) {
-                    const float* u = p.u + (size_t)toks[m] * ncol + pi * rp + r;
-                    for (int s = 0; s < p.slices; s++, u += (size_t)p.ntok * ncol) {
-                        const f32x4 lo = *(const f32x4*)u, hi = *(const f32x4*)(u + 4);
+                for (int i = 0; i < 4; i++) v[i] = b0[i];
+            } else {
 #pragma unroll
-                        for (int i = 0; i < 4; i++) { v[i] += lo[i]; v[4 + i] += hi[i]; }
-                    }
-                }
-                u32x4 o[3];
-                ad_split<3>(v, o);
+                for (int c = 0; c < 4; c++) *(f32x4*)(move + (lane & 15) * JL_AD_MOVE + 16 * c + 4 * (lane >> 4)) = acc[c];
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (a wavefront's own LDS)
 #pragma unroll
-                for (int n = 0; n < 3; n++) frag[((ks * TT + tt) * 3 + n) * 64 + lane] = o[n];
+                for (int i = 0; i < 4; i++) v[i] = *(const f32x4*)(move + (4 * i + (lane >> 4)) * JL_AD_MOVE + 4 * (lane & 15));
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                if (base)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) v[i] = b0[i] + v[i];
             }
-            __syncthreads();
-            for (int ks = 0; ks < nk; ks++) {
-                const int r = r0 + 32 * ks + 8 * (lane >> 4);
-                u32x4 wq[4][PW];
+            const int c = col + 4 * (lane & 15);
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    const int col = min(col0 + 16 * c + (lane & 15), rows - 1);
-                    AdType<T> w;
-                    w.load_some(p.b[pi], ((size_t)a * rows + col) * p.rank + min(r, rank), min(max(rank - r, 0), 8));
-                    ad_pieces<T>(w, wq[c]);
-                }
-#pragma unroll
-                for (int tt = 0; tt < TT; tt++) {
-                    if (tt >= nt) continue;
-                    u32x4 uq[3];
-#pragma unroll
-                    for (int n = 0; n < 3; n++) uq[n] = frag[((ks * TT + tt) * 3 + n) * 64 + lane];
-#pragma unroll
-                    for (int c = 0; c < 4; c++) acc[tt][c] = ad_mfma<PW, 3>(wq[c], uq, acc[tt][c]);
-                }
-            }
-            __syncthreads();
-        }
-#pragma unroll
-        for (int tt = 0; tt < TT; tt++) {
-            if (tt >= nt || !live[tt]) continue;
-#pragma unroll
-            for (int c = 0; c < 4; c++) {
-                const int col = col0 + 16 * c + 4 * (lane >> 4);
-                const f32x4 v = none ? bs[tt][c] : base ? bs[tt][c] + acc[tt][c] : acc[tt][c];
+            for (int i = 0; i < 4; i++) {
+                if (16 * tt + 4 * i + (lane >> 4) >= count) continue;
                 if (VEC) {
-                    if (col < rows) *(f32x4*)(out + oat[tt] + col) = v;
+                    if (c < rows) *(f32x4*)(out + o0[i]) = v[i];
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        if (col + i < rows) out[oat[tt] + col + i] = v[i];
+                    for (int e = 0; e < 4; e++)
+                        if (c + e < rows) out[o0[i] + e] = v[i][e];
+                }
+            }
+        };
+        auto stage = [&](int s0) {   // u's fragments of K steps [s0, s0 + KS)
+            for (int f = wave; f < nt * KS; f += 4) {
+                const int tt = f / KS, s = s0 + f % KS, m = 16 * tt + (lane & 15);
+                u32x4 o[3];
+                const int tok = toks[min(m, count - 1)];
+                if (p.slices) {
+                    ad_sum_u(p, tok, pi, 32 * s + 8 * (lane >> 4), scale, rank, o);
+                } else {
+                    const uint16_t* u = p.u + (((size_t)tok * p.n + pi) * ksteps + min(s, ksteps - 1)) * 96 + 8 * (lane >> 4);
+#pragma unroll
+                    for (int n = 0; n < 3; n++) o[n] = *(const u32x4*)(u + 32 * n);
+                }
+#pragma unroll
+                for (int n = 0; n < 3; n++) frag[((tt * KS + f % KS) * 3 + n) * 64 + lane] = o[n];
+            }
+        };
+        auto load_b = [&](int s0, int col, u32x4 (&wq)[KS][4][PW]) {
+#pragma unroll
+            for (int s = 0; s < KS; s++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    AdType<T> w;
+                    ad_load_b<T>(w, p, pi, a, min(col + 16 * c + (lane & 15), rows - 1), 32 * (s0 + s) + 8 * (lane >> 4), rank);
+                    ad_pieces<T>(w, wq[s][c]);
+                }
+        };
+        auto multiply = [&](int tt, const u32x4 (&wq)[KS][4][PW], f32x4 (&acc)[4]) {
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+                u32x4 uq[3];
+#pragma unroll
+                for (int n = 0; n < 3; n++) uq[n] = frag[((tt * KS + s) * 3 + n) * 64 + lane];
+#pragma unroll
+                for (int c = 0; c < 4; c++) acc[c] = ad_mfma<PW, 3>(wq[s][c], uq, acc[c]);
+            }
+        };
+        int col = block * 256 * p.up_sets + wave * 64;
+        if constexpr (!MANY) {
+            if (col < rows) load_base(0, col);
+            if (!none) stage(0);
+            __syncthreads();
+            for (int set = 0; set < p.up_sets && col < rows; set++, col += 256) {
+                u32x4 wq[KS][4][PW];
+                if (!none) load_b(0, col, wq);
+                for (int tt = 0; tt < nt; tt++) {
+                    f32x4 acc[4], b0[4];
+                    size_t o0[4];
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+                        b0[c] = bs[c];
+                        o0[c] = oat[c];
+                    }
+                    if (tt + 1 < nt) load_base(tt + 1, col);
+                    else if (set + 1 < p.up_sets && col + 256 < rows) load_base(0, col + 256);
+                    if (!none) multiply(tt, wq, acc);
+                    finish(tt, col, acc, b0, o0);
+                }
+            }
+        } else {
+            for (int set = 0; set < p.up_sets; set++, col += 256) {   // (every wavefront takes part in the staging)
+                f32x4 acc[4][4];
+#pragma unroll
+                for (int tt = 0; tt < 4; tt++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) acc[tt][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if (!none)
+                    for (int s0 = 0; 32 * s0 < rank; s0 += KS) {
+                        stage(s0);
+                        __syncthreads();
+                        if (col < rows) {
+                            u32x4 wq[KS][4][PW];
+                            load_b(s0, col, wq);
+#pragma unroll
+                            for (int tt = 0; tt < 4; tt++)
+                                if (tt < nt) multiply(tt, wq, acc[tt]);
+                        }
+                        __syncthreads();
+                    }
+                if (col < rows) {
+#pragma unroll
+                    for (int tt = 0; tt < 4; tt++)
+                        if (tt < nt) {
+                            load_base(tt, col);
+                            finish(tt, col, acc[tt], bs, oat);
+                        }
                 }
             }
         }
-        __syncthreads();   // (toks is the next group's)
+        __syncthreads();   // (toks and frag are the next group's)
+    }
+}
+
+// ---------------------------------------------------------------- both, few tokens
+// One launch: a workgroup makes u of one token for one projection by dot products -- its sixteen wavefronts cut K (and the rows of A where
+// K is short) among them -- and then a block of columns of out.  Every column block makes u anew: A and x come from L2 then, which costs less than a
+// second launch.  What counts here is the number of trips to memory one after the other: the adapter's id, then base, B, A and x together
+// (a rank up to sixteen), then out.
+// L lanes a column: eight elements of a row of B each (rank <= 8 L); a wavefront's 64 columns are L loads of 64 / L rows, whole lines.
+// grid = (column blocks of all projections, ntok), block = 1024; a column block is 1024 p.one_sets columns.
+// LDS: part [16][8 L] and u [8 L] floats.
+#define JL_AD_ONE_LDS(L) (17 * 8 * (L))
+template <int N> __device__ __forceinline__ float ad_lane_sum(float v) {   // over N consecutive lanes; each has it
+    if (N >= 2) v += dpp_f32<JL_DPP_QUAD_XOR1, 0xf>(v);
+    if (N >= 4) v += dpp_f32<JL_DPP_QUAD_XOR2, 0xf>(v);
+    if (N >= 8) v += dpp_f32<JL_DPP_ROW_HALF_MIRROR, 0xf>(v);
+    return v;
+}
+template <int T, int L>
+__device__ __forceinline__ void adapter_one_body(const AdapterArgs& p, float* lds) {
+    constexpr int R = 8 * L, RB = R < 16 ? R : 16;   // rows of A asked for at a time
+    constexpr bool AHEAD = L * sizeof(AdType<T>) <= 64;   // B asked for ahead of A: while it fits the registers
+    float* part = lds;
+    float* us = lds + 16 * R;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tok = blockIdx.y;
+    int block = blockIdx.x;
+    const int width = 1024 * p.one_sets, pi = ad_projection(p, block, width);
+    const int rows = p.rows[pi], k = p.k;
+    const float* base = p.base[pi];
+    float* out = p.out[pi];
+    const u32 id = p.ids[tok];
+    const int rank = id >= (u32)p.n_adapter ? 0 : ad_rank(p, id);   // uniform
+    const size_t orow = (size_t)tok * rows;
+    // the lane's column of a set and, in load j, of B: 64 / L rows a load, lane / L of them
+    const int mine = lane % L * (64 / L) + lane / L, col0 = block * width + wave * 64;
+    if (rank == 0) {
+        if (base == out) return;
+        for (int s = 0, col = col0 + mine; s < p.one_sets; s++, col += 1024)
+            if (col < rows) out[orow + col] = base ? base[orow + col] : 0.f;
+        return;
+    }
+    AdType<T> b[L];
+    const int r0 = 8 * (lane % L);
+    auto load_b = [&](int col) {
+#pragma unroll
+        for (int j = 0; j < L; j++)
+            b[j].load_some(p.b[pi], ((size_t)id * rows + min(col + j * (64 / L) + lane / L, rows - 1)) * p.rank + min(r0, rank), min(max(rank - r0, 0), 8));
+    };
+    float bs = base && col0 + mine < rows ? base[orow + col0 + mine] : 0.f;
+    if (AHEAD) load_b(col0);
+
+    // u: wavefront = (piece of K modulo pieces, rows modulo 16 / pieces); a piece is 256 elements, four a lane
+    const int np = (k + 255) / 256;
+    const int pieces = np > 8 ? 16 : np > 4 ? 8 : np > 2 ? 4 : np;   // a power of two
+    const int piece = wave & (pieces - 1), step = 16 / pieces, first = wave / pieces;
+    for (int r = first; r < rank; r += RB * step) {
+        float sum[RB];
+#pragma unroll
+        for (int j = 0; j < RB; j++) sum[j] = 0.f;
+        for (int q = piece; q < np; q += pieces) {
+            const int e = q * 256 + 4 * lane;
+            const size_t xat = (size_t)tok * k + min(e, k - 4);
+            float x[4];
+            if (p.x_type == JL_F32) {
+                AdQuad<JL_F32> v;
+                v.load(p.x, xat);
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[i] = v.value(i);
+            } else if (p.x_type == JL_F16) {
+                AdQuad<JL_F16> v;
+                v.load(p.x, xat);
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[i] = v.value(i);
+            } else {
+                AdQuad<JL_BF16> v;
+                v.load(p.x, xat);
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[i] = v.value(i);
+            }
+            AdQuad<T> w[RB];
+#pragma unroll
+            for (int j = 0; j < RB; j++) w[j].load(p.a[pi], ((size_t)id * p.rank + min(r + j * step, rank - 1)) * k + min(e, k - 4));
+            if (e < k) {
+#pragma unroll
+                for (int j = 0; j < RB; j++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) sum[j] = __builtin_fmaf(w[j].value(i), x[i], sum[j]);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < RB; j++) {
+            const float v = wave_sum_to_lane63(sum[j]);
+            if (lane == 63 && r + j * step < rank) part[piece * R + r + j * step] = v;
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x < R) {
+        float v = 0.f;
+        if ((int)threadIdx.x < rank)
+            for (int q = 0; q < pieces; q++) v += part[q * R + threadIdx.x];
+        us[threadIdx.x] = (p.scale ? p.scale[id] : 1.f) * v;   // (0 from the rank on, as B's elements read there)
+        if ((int)threadIdx.x >= rank) us[threadIdx.x] = 0.f;
+    }
+    __syncthreads();
+    float u[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) u[i] = us[r0 + i];
+    for (int s = 0; s < p.one_sets; s++) {
+        const int col = col0 + 1024 * s;
+        if (col >= rows) break;   // uniform a wavefront
+        if (s || !AHEAD) load_b(col);
+        if (s) bs = base && col + mine < rows ? base[orow + col + mine] : 0.f;
+        float d = 0.f;
+#pragma unroll
+        for (int j = 0; j < L; j++) {
+            float v = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) v = __builtin_fmaf(b[j].value(i), u[i], v);
+            v = ad_lane_sum<L>(v);
+            if (lane % L == j) d = v;
+        }
+        if (col + mine < rows) out[orow + col + mine] = base ? bs + d : d;
     }
 }

@@ -617,9 +617,11 @@ struct AdapterArgs {
     const uint32_t* ranks;                 // [n_adapter] or null
     const float* scale;                    // [n_adapter] or null
     const void* x;                         // [ntok][k]
-    float* u;                              // [slices][ntok][n * rank_pad] workspace
+    float* part;                           // workspace: sums over a slice of K each, [slices][ntok][n * rank_pad]
+    uint16_t* u;                           // workspace: u as three bf16 pieces, [ntok][n][K steps of 32][3][32]
     int n, n_adapter, rank, k, ntok;
     int rank_pad;                          // rank rounded up to sixteen
-    int slices, passes;                    // K slices and passes over the columns of u (adapter_down)
-    int up_waves;                          // wavefronts a workgroup (adapter_up)
+    int x_type;                            // (adapter_one)
+    int passes, slices;                    // of adapter_down; slices 0 in adapter_up: u has been made
+    int up_sets, one_sets;                 // sets of 256 (adapter_one: 1024) columns a workgroup
 };

@@ -688,24 +688,32 @@ JL_NORM_ROWS(l16_1, 16, 1, false, 256) JL_NORM_ROWS(l32_1, 32, 1, false, 256) JL
 JL_NORM_ROWS(l64_2, 64, 2, false, 256) JL_NORM_ROWS(l64_4, 64, 4, false, 256)
 JL_NORM_ROWS(wg_1, 64, 1, true, 1024) JL_NORM_ROWS(wg_2, 64, 2, true, 1024) JL_NORM_ROWS(wg_4, 64, 4, true, 1024)
 JL_NORM_ROWS(wg_8, 64, 8, true, 1024) JL_NORM_ROWS(wg_16, 64, 16, true, 1024)
-// grid = (tile slots, chunks of 64 tokens, passes * slices), block = 256
-#define JL_ADAPTER_DOWN(T, TYPE, XT, XTYPE, NT)                                                                    \
-    extern "C" __global__ __launch_bounds__(256) void jl_adapter_down_##T##_##XT##_n##NT(AdapterArgs p) {          \
-        __shared__ f32x4 red[4 * NT * 64];                                                                         \
-        adapter_down_body<TYPE, XTYPE, NT>(p, red);                                                                \
+// grid = (group slots, ntok / 64, passes * slices), block = 256
+#define JL_ADAPTER_DOWN(T, TYPE, XT, XTYPE, NT)                                                                              \
+    extern "C" __global__ __launch_bounds__(256) void jl_adapter_down_##T##_##XT##_n##NT(AdapterArgs p) {                    \
+        __shared__ __attribute__((aligned(16))) uint16_t sx[AdType<XTYPE>::pieces * 64 * JL_AD_DOWN_ROW];                    \
+        __shared__ int toks[64];                                                                                             \
+        adapter_down_body<TYPE, XTYPE, NT>(p, sx, toks);                                                                     \
     }
-// grid = (column blocks, group slots, chunks of 16 TT tokens), block = 64 p.up_waves (8 at most)
-#define JL_ADAPTER_UP(T, TYPE, TT)                                                                                 \
-    extern "C" __global__ __launch_bounds__(512) void jl_adapter_up_##T##_t##TT(AdapterArgs p) {                   \
-        __shared__ __attribute__((aligned(16))) uint8_t s[JL_AD_UP_LDS(TT)];                                       \
-        adapter_up_body<TYPE, TT, true>(p, s);                                                                     \
-    }                                                                                                              \
-    extern "C" __global__ __launch_bounds__(512) void jl_adapter_up_##T##_t##TT##_any(AdapterArgs p) {             \
-        __shared__ __attribute__((aligned(16))) uint8_t s[JL_AD_UP_LDS(TT)];                                       \
-        adapter_up_body<TYPE, TT, false>(p, s);                                                                    \
+extern "C" __global__ __launch_bounds__(256) void jl_adapter_sum(AdapterArgs p) { adapter_sum_body(p); }
+// grid = (column blocks, ntok), block = 1024
+#define JL_ADAPTER_ONE(T, TYPE, L)                                                                                           \
+    extern "C" __global__ __launch_bounds__(1024) void jl_adapter_one_##T##_l##L(AdapterArgs p) {                            \
+        __shared__ float s[JL_AD_ONE_LDS(L)];                                                                                \
+        adapter_one_body<TYPE, L>(p, s);                                                                                     \
     }
-#define JL_ADAPTER_X(T, TYPE, XT, XTYPE) JL_ADAPTER_DOWN(T, TYPE, XT, XTYPE, 1) JL_ADAPTER_DOWN(T, TYPE, XT, XTYPE, 4) JL_ADAPTER_DOWN(T, TYPE, XT, XTYPE, 8)
-#define JL_ADAPTER(T, TYPE)                                                                                        \
-    JL_ADAPTER_X(T, TYPE, f32, JL_F32) JL_ADAPTER_X(T, TYPE, f16, JL_F16) JL_ADAPTER_X(T, TYPE, bf16, JL_BF16)     \
-    JL_ADAPTER_UP(T, TYPE, 1) JL_ADAPTER_UP(T, TYPE, 4)
+// grid = (column blocks, group slots, ntok / 64), block = 256
+#define JL_ADAPTER_UP_V(T, TYPE, NAME, KS, MANY, VEC)                                                                        \
+    extern "C" __global__ __launch_bounds__(256) void jl_adapter_up_##T##_##NAME(AdapterArgs p) {                            \
+        __shared__ u32x4 frag[4 * KS * 3 * 64];                                                                              \
+        __shared__ __attribute__((aligned(16))) float move[4 * 16 * JL_AD_MOVE];                                             \
+        __shared__ int toks[64];                                                                                             \
+        adapter_up_body<TYPE, KS, MANY, VEC>(p, frag, move, toks);                                                           \
+    }
+#define JL_ADAPTER_UP(T, TYPE, NAME, KS, MANY) JL_ADAPTER_UP_V(T, TYPE, NAME, KS, MANY, true) JL_ADAPTER_UP_V(T, TYPE, NAME##_any, KS, MANY, false)
+#define JL_ADAPTER_X(T, TYPE, XT, XTYPE) JL_ADAPTER_DOWN(T, TYPE, XT, XTYPE, 1) JL_ADAPTER_DOWN(T, TYPE, XT, XTYPE, 2)
+#define JL_ADAPTER(T, TYPE)                                                                                                  \
+    JL_ADAPTER_X(T, TYPE, f32, JL_F32) JL_ADAPTER_X(T, TYPE, f16, JL_F16) JL_ADAPTER_X(T, TYPE, bf16, JL_BF16)               \
+    JL_ADAPTER_ONE(T, TYPE, 1) JL_ADAPTER_ONE(T, TYPE, 2) JL_ADAPTER_ONE(T, TYPE, 4) JL_ADAPTER_ONE(T, TYPE, 8)              \
+    JL_ADAPTER_UP(T, TYPE, k1, 1, false) JL_ADAPTER_UP(T, TYPE, k2, 2, false) JL_ADAPTER_UP(T, TYPE, many, 1, true)
 JL_ADAPTER(f32, JL_F32) JL_ADAPTER(f16, JL_F16) JL_ADAPTER(bf16, JL_BF16)
