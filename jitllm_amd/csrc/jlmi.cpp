@@ -2242,7 +2242,8 @@ int jl_ctx_create(jl_ctx** out, const jl_options* opts) {
     for (const char* t : {"f32", "f16", "bf16"}) {
         for (const char* xt : {"f32", "f16", "bf16"})
             for (const char* nt : {"_n1", "_n2"}) names.push_back(std::string("jl_adapter_down_") + t + "_" + xt + nt);
-        for (const char* l : {"_l1", "_l2", "_l4", "_l8"}) names.push_back(std::string("jl_adapter_one_") + t + l);
+        for (const char* l : {"_l1", "_l2", "_l4", "_l8"}) for (const char* form : {"one_", "cols_"}) names.push_back(std::string("jl_adapter_") + form + t + l);
+        names.push_back(std::string("jl_adapter_dots_") + t);
         for (const char* form : {"_k1", "_k1_any", "_k2", "_k2_any", "_many", "_many_any"}) names.push_back(std::string("jl_adapter_up_") + t + form);
     }
     for (const char* pl : {"", "planes_"})
@@ -2592,7 +2593,7 @@ int jl_adapter_group_dev(jl_ctx* c, const jl_adapter_group* g, void* stream) {
     a.n = g->n; a.n_adapter = g->n_adapter; a.rank = g->rank; a.k = g->k; a.ntok = g->ntok;
     const AdapterPlan pl = adapter_plan(c, g->ntok, g->n, g->rank, g->k, g->n_adapter);
     a.part = nullptr; a.u = nullptr;
-    a.rank_pad = pl.rank_pad; a.passes = pl.passes; a.slices = pl.slices; a.x_type = g->x_type; a.up_sets = a.one_sets = 1;
+    a.rank_pad = pl.rank_pad; a.passes = pl.passes; a.slices = pl.slices; a.x_type = g->x_type; a.up_sets = 1;
     hipStream_t st = pick_stream(c, stream);
     void* params[] = {&a};
     const char *t = plain_tag(g->type), *xt = plain_tag(g->x_type);
@@ -2604,11 +2605,25 @@ int jl_adapter_group_dev(jl_ctx* c, const jl_adapter_group* g, void* stream) {
     };
     Name name;
     const long sets = (long)g->ntok * blocks(1024);
-    const bool one = g->rank <= 64 && g->ntok <= 65535 && (c->tune.adapter_form ? c->tune.adapter_form == 1 : g->rank <= 16 && sets <= c->num_cu);
-    if (one) {
-        const int l = g->rank <= 8 ? 1 : g->rank <= 16 ? 2 : g->rank <= 32 ? 4 : 8;
+    const int l = g->rank <= 8 ? 1 : g->rank <= 16 ? 2 : g->rank <= 32 ? 4 : 8;   // lanes a column
+    const bool dots = g->rank <= 64 && g->ntok <= 65535;
+    const int form = c->tune.adapter_form ? c->tune.adapter_form : dots && g->rank <= 16 && sets <= c->num_cu ? 1 : dots && g->ntok <= 16 ? 2 : 0;
+    if (dots && form == 1) {
         name << "jl_adapter_one_" << t << "_l" << l;
-        return launch(c, name, blocks(1024 * a.one_sets), (unsigned)g->ntok, 1024, 0, st, params);
+        return launch(c, name, blocks(1024), (unsigned)g->ntok, 1024, 0, st, params);
+    }
+    if (dots && form == 2) {
+        a.slices = std::min(16, (g->k + 1023) / 1024);
+        int rc = adapter_ws_ensure(c, adapter_part_bytes((size_t)a.slices * g->ntok, g->n, g->rank));
+        if (rc != JL_OK) return rc;
+        a.part = (float*)c->adapter_ws;
+        name << "jl_adapter_dots_" << t;
+        rc = launch(c, name, (unsigned)a.slices, (unsigned)g->ntok, 256, 0, st, params, (unsigned)(g->n * a.rank_pad / 16));
+        if (rc != JL_OK) return rc;
+        a.up_sets = c->tune.adapter_sets ? c->tune.adapter_sets : 1;
+        Name cols;
+        cols << "jl_adapter_cols_" << t << "_l" << l;
+        return launch(c, cols, blocks(256 * a.up_sets), (unsigned)g->ntok, 256, 0, st, params);
     }
     const size_t part = adapter_part_bytes((size_t)a.slices * g->ntok, g->n, g->rank);
     int rc = adapter_ws_ensure(c, part + adapter_u_bytes(g->ntok, g->n, g->rank));
@@ -2619,7 +2634,7 @@ int jl_adapter_group_dev(jl_ctx* c, const jl_adapter_group* g, void* stream) {
     rc = launch(c, name, (unsigned)std::min(most, g->n_adapter), (unsigned)chunks, 256, 0, st, params, (unsigned)(a.passes * a.slices));
     if (rc != JL_OK) return rc;
     const double added = (double)blocks(256) * g->ntok * a.slices * g->rank * 4;   // bytes that adapter_up would add up
-    if (c->tune.adapter_form ? c->tune.adapter_form == 3 : added > 30e6) {
+    if (c->tune.adapter_form ? c->tune.adapter_form == 4 : added > 30e6) {
         const size_t octs = (size_t)g->ntok * g->n * ((a.rank_pad + 31) / 32) * 4;
         rc = launch(c, "jl_adapter_sum", (unsigned)((octs + 255) / 256), 1, 256, 0, st, params);
         if (rc != JL_OK) return rc;

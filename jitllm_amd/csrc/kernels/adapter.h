@@ -3,8 +3,7 @@
 // for up to four projections that read one x.  A token whose id no adapter has, or whose adapter has rank 0, gets base alone.
 //
 // On the bf16 matrix cores: adapter_down makes sums of u = A x for the tokens of an adapter and a slice of K, adapter_up adds B u to base (where
-// many column blocks would each add the slices up, adapter_sum does it first); for few tokens of a small rank adapter_one does everything
-// in one launch, by dot products in f32.  A workgroup looks at 64 consecutive tokens and finds for itself which of them share an adapter (a ballot
+// many column blocks would each add the slices up, adapter_sum does it first).  A workgroup looks at 64 consecutive tokens and finds for itself which of them share an adapter (a ballot
 // per adapter met), so nothing is sorted beforehand; a token meets its own adapter only, so no number of another's can reach it.
 //
 // Products are exact: an f32 value is three bf16 values (8 mantissa bits each, cut off, not rounded), an f16 value two, and every
@@ -160,7 +159,7 @@ __device__ __forceinline__ void adapter_down_body(const AdapterArgs& p, uint16_t
     const int pass = blockIdx.z % p.passes, slice = blockIdx.z / p.passes;
     const int ctiles = p.rank_pad / 16, all = p.n * ctiles, c0 = (pass * 4 + wave) * NT;
     const int steps = (p.k + JL_AD_DOWN_K - 1) / JL_AD_DOWN_K;
-    const int lo = steps * slice / p.slices, hi = steps * (slice + 1) / p.slices;
+    const int lo = steps * slice / p.slices, hi = steps * (slice + 1) / p.slices;   // (slices <= steps)
     const u32 id = ad_id(p, first);
     AdGroups groups(id, (u32)p.n_adapter);
     u32 a;
@@ -177,42 +176,36 @@ __device__ __forceinline__ void adapter_down_body(const AdapterArgs& p, uint16_t
             wp[t] = p.a[i];
             wat[t] = ((size_t)a * p.rank + r) * p.k + 8 * (lane >> 4);
         }
-        // a thread's rows of x: token 8 i + tid / 32 of the group, four elements from 4 (tid % 32) on
-        size_t xat[8];
+        auto run = [&](auto tiles) {   // (of the group, rounded up to one or four: no branch between the matrix instructions)
+            constexpr int MT = decltype(tiles)::value;
+            // a thread's rows of x: token 8 i + tid / 32 of the group, four elements from 4 (tid % 32) on
+            size_t xat[2 * MT];
 #pragma unroll
-        for (int i = 0; i < 8; i++) xat[i] = (size_t)toks[min(8 * i + tid / 32, count - 1)] * p.k + 4 * (tid & 31);
-        AdQuad<XT> x[8];
-        AdType<T> w[4][NT];
-        auto load_x = [&](int s) {
-            const int k0 = s * JL_AD_DOWN_K;
-            if (k0 + 4 * (tid & 31) >= p.k) return;
+            for (int i = 0; i < 2 * MT; i++) xat[i] = (size_t)toks[min(8 * i + tid / 32, count - 1)] * p.k;
+            AdQuad<XT> x[2 * MT];
+            AdType<T> w[4][NT];
+            // (past the end of K: its last elements, which meet nothing)
+            auto load_x = [&](int s) {
+                const int e = min(s * JL_AD_DOWN_K + 4 * (tid & 31), p.k - 4);
 #pragma unroll
-            for (int i = 0; i < 8; i++)
-                if (i < 2 * nt) x[i].load(p.x, xat[i] + k0);
-        };
-        auto load_w = [&](int s) {
-            const int k0 = s * JL_AD_DOWN_K;
+                for (int i = 0; i < 2 * MT; i++) x[i].load(p.x, xat[i] + e);
+            };
+            auto load_w = [&](int s, int q) {
+                const int e = min(s * JL_AD_DOWN_K + 32 * q, p.k - 32);
 #pragma unroll
-            for (int q = 0; q < 4; q++)
-                if (k0 + 32 * q < p.k) {
+                for (int t = 0; t < NT; t++) w[q][t].load(wp[t], wat[t] + e);
+            };
+            f32x4 acc[MT][NT];
 #pragma unroll
-                    for (int t = 0; t < NT; t++)
-                        if (c0 + t < all) w[q][t].load(wp[t], wat[t] + k0 + 32 * q);
-                }
-        };
-        f32x4 acc[4][NT];
+            for (int m = 0; m < MT; m++)
 #pragma unroll
-        for (int m = 0; m < 4; m++)
-#pragma unroll
-            for (int t = 0; t < NT; t++) acc[m][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (lo < hi) {
+                for (int t = 0; t < NT; t++) acc[m][t] = f32x4{0.f, 0.f, 0.f, 0.f};
             load_x(lo);
-            load_w(lo);
-        }
-        for (int s = lo; s < hi; s++) {
 #pragma unroll
-            for (int i = 0; i < 8; i++)
-                if (i < 2 * nt) {
+            for (int q = 0; q < 4; q++) load_w(lo, q);
+            for (int s = lo; s < hi; s++) {
+#pragma unroll
+                for (int i = 0; i < 2 * MT; i++) {
                     float v[4];
 #pragma unroll
                     for (int j = 0; j < 4; j++) v[j] = x[i].value(j);
@@ -228,36 +221,50 @@ __device__ __forceinline__ void adapter_down_body(const AdapterArgs& p, uint16_t
                             u32x2{__builtin_amdgcn_perm(b[1], b[0], 0x07060302), __builtin_amdgcn_perm(b[3], b[2], 0x07060302)};
                     }
                 }
-            __syncthreads();
-            if (s + 1 < hi) load_x(s + 1);
-            const int nq = min(4, (p.k - s * JL_AD_DOWN_K) / 32);
+                lds_barrier();
+                const int next = min(s + 1, hi - 1), nq = min(4, (p.k - s * JL_AD_DOWN_K) / 32);
+                load_x(next);
+                if (c0 < all) {
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                if (q >= nq || c0 >= all) continue;
-                u32x4 wq[NT][PW];
+                    for (int q = 0; q < 4; q++) {
+                        if (q < nq) {
+                            u32x4 xq[MT][PX], wq[NT][PW];
 #pragma unroll
-                for (int t = 0; t < NT; t++) ad_pieces<T>(w[q][t], wq[t]);
+                            for (int m = 0; m < MT; m++)
 #pragma unroll
-                for (int m = 0; m < 4; m++) {
-                    if (m >= nt) continue;
-                    u32x4 xq[PX];
+                                for (int n = 0; n < PX; n++) xq[m][n] = *(const u32x4*)(sx + (n * 64 + 16 * m + (lane & 15)) * ROW + 32 * q + 8 * (lane >> 4));
 #pragma unroll
-                    for (int n = 0; n < PX; n++) xq[n] = *(const u32x4*)(sx + (n * 64 + 16 * m + (lane & 15)) * ROW + 32 * q + 8 * (lane >> 4));
+                            for (int t = 0; t < NT; t++) ad_pieces<T>(w[q][t], wq[t]);
+                            load_w(next, q);
+                            // the smallest products first; a piece's products of all tiles side by side
 #pragma unroll
-                    for (int t = 0; t < NT; t++) acc[m][t] = ad_mfma<PW, PX>(wq[t], xq, acc[m][t]);
+                            for (int o = PW + PX - 2; o >= 0; o--)
+#pragma unroll
+                                for (int i = 0; i < PW; i++)
+                                    if (o - i >= 0 && o - i < PX) {
+#pragma unroll
+                                        for (int m = 0; m < MT; m++)
+#pragma unroll
+                                            for (int t = 0; t < NT; t++)
+                                                acc[m][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(ad_bf16x8, wq[t][i]),
+                                                                                                    __builtin_bit_cast(ad_bf16x8, xq[m][o - i]), acc[m][t], 0, 0, 0);
+                                    }
+                        }
+                    }
                 }
+                lds_barrier();
             }
-            if (s + 1 < hi) load_w(s + 1);
-            __syncthreads();
-        }
 #pragma unroll
-        for (int m = 0; m < 4; m++) {
-            if (16 * m + (lane & 15) >= count) continue;
-            float* u = p.part + ((size_t)slice * p.ntok + toks[16 * m + (lane & 15)]) * all * 16 + 4 * (lane >> 4);
+            for (int m = 0; m < MT; m++) {
+                if (16 * m + (lane & 15) >= count) continue;
+                float* u = p.part + ((size_t)slice * p.ntok + toks[16 * m + (lane & 15)]) * all * 16 + 4 * (lane >> 4);
 #pragma unroll
-            for (int t = 0; t < NT; t++)
-                if (c0 + t < all) *(f32x4*)(u + (c0 + t) * 16) = acc[m][t];
-        }
+                for (int t = 0; t < NT; t++)
+                    if (c0 + t < all) *(f32x4*)(u + (c0 + t) * 16) = acc[m][t];
+            }
+        };
+        if (nt > 1) run(GemmIntC<4>{});
+        else run(GemmIntC<1>{});
         __syncthreads();   // (toks is the next group's)
     }
 }
@@ -493,115 +500,83 @@ __device__ __forceinline__ void adapter_up_body(const AdapterArgs& p, u32x4* fra
     }
 }
 
-// ---------------------------------------------------------------- both, few tokens
-// One launch: a workgroup makes u of one token for one projection by dot products -- its sixteen wavefronts cut K (and the rows of A where
-// K is short) among them -- and then a block of columns of out.  Every column block makes u anew: A and x come from L2 then, which costs less than a
-// second launch.  What counts here is the number of trips to memory one after the other: the adapter's id, then base, B, A and x together
-// (a rank up to sixteen), then out.
-// L lanes a column: eight elements of a row of B each (rank <= 8 L); a wavefront's 64 columns are L loads of 64 / L rows, whole lines.
-// grid = (column blocks of all projections, ntok), block = 1024; a column block is 1024 p.one_sets columns.
-// LDS: part [16][8 L] and u [8 L] floats.
-#define JL_AD_ONE_LDS(L) (17 * 8 * (L))
+// ---------------------------------------------------------------- few tokens: dot products in f32
+// Sums over the wavefront of RB values a lane; lane l has those of rows 4 i + l % 4 in s[i].  Half of the values leave a lane with each of the
+// first two steps: 52 instructions for sixteen rows, where a sum at a time would take 96 (and those were a third of the kernels' time).
+template <int RB> __device__ __forceinline__ void ad_wave_rows(float (&s)[RB]) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int i = 0; i < RB / 2; i++) {
+        const float keep = lane & 1 ? s[2 * i + 1] : s[2 * i], give = lane & 1 ? s[2 * i] : s[2 * i + 1];
+        s[i] = keep + dpp_f32<JL_DPP_QUAD_XOR1, 0xf>(give);
+    }
+#pragma unroll
+    for (int i = 0; i < RB / 4; i++) {
+        const float keep = lane & 2 ? s[2 * i + 1] : s[2 * i], give = lane & 2 ? s[2 * i] : s[2 * i + 1];
+        float v = keep + dpp_f32<JL_DPP_QUAD_XOR2, 0xf>(give);
+        v += dpp_f32<0x124, 0xf>(v);   // rotations by four and eight lanes of sixteen
+        v += dpp_f32<0x128, 0xf>(v);
+        auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+        auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        s[i] = __uint_as_float(h[0]) + __uint_as_float(h[1]);
+    }
+}
+// Dot products of RB rows of A (row, row + step, ..., the last again past `rank`) with a token's x over the pieces q, q + pieces, ... of 256
+// elements of K, four a lane.
+template <int T, int RB> __device__ __forceinline__ void ad_rows(const AdapterArgs& p, int pi, u32 id, int rank, size_t xrow, int row, int step, int q, int pieces, float (&sum)[RB]) {
+    const int lane = threadIdx.x & 63, k = p.k;
+#pragma unroll
+    for (int j = 0; j < RB; j++) sum[j] = 0.f;
+    for (; q * 256 < k; q += pieces) {
+        const int e = q * 256 + 4 * lane, at = min(e, k - 4);
+        AdQuad<T> w[RB];
+#pragma unroll
+        for (int j = 0; j < RB; j++) w[j].load(p.a[pi], ((size_t)id * p.rank + min(row + j * step, rank - 1)) * k + at);
+        float x[4];
+        if (p.x_type == JL_F32) {
+            AdQuad<JL_F32> v;
+            v.load(p.x, xrow + at);
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[i] = v.value(i);
+        } else {
+            AdQuad<JL_BF16> v;
+            v.load(p.x, xrow + at);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint16_t h = (uint16_t)(v.w[i / 2] >> (16 * (i & 1)));
+                x[i] = p.x_type == JL_F16 ? half_bits_to_f32(h) : __uint_as_float((u32)h << 16);
+            }
+        }
+        if (e < k) {
+#pragma unroll
+            for (int j = 0; j < RB; j++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) sum[j] = __builtin_fmaf(w[j].value(i), x[i], sum[j]);
+        }
+    }
+}
+// Columns of out.  L lanes a column: eight elements of a row of B each (rank <= 8 L); a wavefront's 64 columns are L loads of 64 / L rows, whole
+// lines, and lane l ends up with column l % L * (64 / L) + l / L.
 template <int N> __device__ __forceinline__ float ad_lane_sum(float v) {   // over N consecutive lanes; each has it
     if (N >= 2) v += dpp_f32<JL_DPP_QUAD_XOR1, 0xf>(v);
     if (N >= 4) v += dpp_f32<JL_DPP_QUAD_XOR2, 0xf>(v);
     if (N >= 8) v += dpp_f32<JL_DPP_ROW_HALF_MIRROR, 0xf>(v);
     return v;
 }
-template <int T, int L>
-__device__ __forceinline__ void adapter_one_body(const AdapterArgs& p, float* lds) {
-    constexpr int R = 8 * L, RB = R < 16 ? R : 16;   // rows of A asked for at a time
-    constexpr bool AHEAD = L * sizeof(AdType<T>) <= 64;   // B asked for ahead of A: while it fits the registers
-    float* part = lds;
-    float* us = lds + 16 * R;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tok = blockIdx.y;
-    int block = blockIdx.x;
-    const int width = 1024 * p.one_sets, pi = ad_projection(p, block, width);
-    const int rows = p.rows[pi], k = p.k;
-    const float* base = p.base[pi];
-    float* out = p.out[pi];
-    const u32 id = p.ids[tok];
-    const int rank = id >= (u32)p.n_adapter ? 0 : ad_rank(p, id);   // uniform
-    const size_t orow = (size_t)tok * rows;
-    // the lane's column of a set and, in load j, of B: 64 / L rows a load, lane / L of them
-    const int mine = lane % L * (64 / L) + lane / L, col0 = block * width + wave * 64;
-    if (rank == 0) {
-        if (base == out) return;
-        for (int s = 0, col = col0 + mine; s < p.one_sets; s++, col += 1024)
-            if (col < rows) out[orow + col] = base ? base[orow + col] : 0.f;
-        return;
-    }
+template <int T, int L> struct AdColumns {
     AdType<T> b[L];
-    const int r0 = 8 * (lane % L);
-    auto load_b = [&](int col) {
+    float base;
+    __device__ __forceinline__ void load(const AdapterArgs& p, int pi, u32 id, int rank, size_t orow, int col, bool with_b, bool with_base) {
+        const int lane = threadIdx.x & 63, rows = p.rows[pi], r0 = 8 * (lane % L), mine = col + lane % L * (64 / L) + lane / L;
+        if (with_base) base = p.base[pi] && mine < rows ? p.base[pi][orow + mine] : 0.f;
+        if (with_b)
 #pragma unroll
-        for (int j = 0; j < L; j++)
-            b[j].load_some(p.b[pi], ((size_t)id * rows + min(col + j * (64 / L) + lane / L, rows - 1)) * p.rank + min(r0, rank), min(max(rank - r0, 0), 8));
-    };
-    float bs = base && col0 + mine < rows ? base[orow + col0 + mine] : 0.f;
-    if (AHEAD) load_b(col0);
-
-    // u: wavefront = (piece of K modulo pieces, rows modulo 16 / pieces); a piece is 256 elements, four a lane
-    const int np = (k + 255) / 256;
-    const int pieces = np > 8 ? 16 : np > 4 ? 8 : np > 2 ? 4 : np;   // a power of two
-    const int piece = wave & (pieces - 1), step = 16 / pieces, first = wave / pieces;
-    for (int r = first; r < rank; r += RB * step) {
-        float sum[RB];
-#pragma unroll
-        for (int j = 0; j < RB; j++) sum[j] = 0.f;
-        for (int q = piece; q < np; q += pieces) {
-            const int e = q * 256 + 4 * lane;
-            const size_t xat = (size_t)tok * k + min(e, k - 4);
-            float x[4];
-            if (p.x_type == JL_F32) {
-                AdQuad<JL_F32> v;
-                v.load(p.x, xat);
-#pragma unroll
-                for (int i = 0; i < 4; i++) x[i] = v.value(i);
-            } else if (p.x_type == JL_F16) {
-                AdQuad<JL_F16> v;
-                v.load(p.x, xat);
-#pragma unroll
-                for (int i = 0; i < 4; i++) x[i] = v.value(i);
-            } else {
-                AdQuad<JL_BF16> v;
-                v.load(p.x, xat);
-#pragma unroll
-                for (int i = 0; i < 4; i++) x[i] = v.value(i);
-            }
-            AdQuad<T> w[RB];
-#pragma unroll
-            for (int j = 0; j < RB; j++) w[j].load(p.a[pi], ((size_t)id * p.rank + min(r + j * step, rank - 1)) * k + min(e, k - 4));
-            if (e < k) {
-#pragma unroll
-                for (int j = 0; j < RB; j++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) sum[j] = __builtin_fmaf(w[j].value(i), x[i], sum[j]);
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < RB; j++) {
-            const float v = wave_sum_to_lane63(sum[j]);
-            if (lane == 63 && r + j * step < rank) part[piece * R + r + j * step] = v;
-        }
+            for (int j = 0; j < L; j++)
+                b[j].load_some(p.b[pi], ((size_t)id * rows + min(col + j * (64 / L) + lane / L, rows - 1)) * p.rank + min(r0, rank), min(max(rank - r0, 0), 8));
     }
-    __syncthreads();
-    if (threadIdx.x < R) {
-        float v = 0.f;
-        if ((int)threadIdx.x < rank)
-            for (int q = 0; q < pieces; q++) v += part[q * R + threadIdx.x];
-        us[threadIdx.x] = (p.scale ? p.scale[id] : 1.f) * v;   // (0 from the rank on, as B's elements read there)
-        if ((int)threadIdx.x >= rank) us[threadIdx.x] = 0.f;
-    }
-    __syncthreads();
-    float u[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) u[i] = us[r0 + i];
-    for (int s = 0; s < p.one_sets; s++) {
-        const int col = col0 + 1024 * s;
-        if (col >= rows) break;   // uniform a wavefront
-        if (s || !AHEAD) load_b(col);
-        if (s) bs = base && col + mine < rows ? base[orow + col + mine] : 0.f;
+    __device__ __forceinline__ void finish(const AdapterArgs& p, int pi, size_t orow, int col, const float (&u)[8]) {
+        const int lane = threadIdx.x & 63, mine = col + lane % L * (64 / L) + lane / L;
         float d = 0.f;
 #pragma unroll
         for (int j = 0; j < L; j++) {
@@ -611,6 +586,124 @@ __device__ __forceinline__ void adapter_one_body(const AdapterArgs& p, float* ld
             v = ad_lane_sum<L>(v);
             if (lane % L == j) d = v;
         }
-        if (col + mine < rows) out[orow + col + mine] = base ? bs + d : d;
+        if (mine < p.rows[pi]) p.out[pi][orow + mine] = p.base[pi] ? base + d : d;
+    }
+};
+// base (zeros without one) to the columns of a token without an adapter: those of a workgroup of `threads` from col on, `sets` times.
+__device__ __forceinline__ void ad_copy(const AdapterArgs& p, int pi, size_t orow, int col, int threads, int sets) {
+    const float* base = p.base[pi];
+    if (base == p.out[pi]) return;
+    for (int s = 0; s < sets; s++, col += threads)
+        if (col < p.rows[pi]) p.out[pi][orow + col] = base ? base[orow + col] : 0.f;
+}
+
+// One launch: a workgroup makes u of one token for one projection -- its sixteen wavefronts cut K (and the rows of A where K is short) among
+// them -- and then a block of 1024 columns of out.  Every column block makes u anew: A and x come from L2 then, which costs less than a second
+// launch while the rank is small (4096 x 4096, one token: rank 8 4.9 us, 16 6.5, 32 10.3; the two launches below 7 to 8).  What counts here is the
+// number of trips to memory one after the other: the adapter's id, then base, B, A and x together, then out.
+// grid = (column blocks of all projections, ntok), block = 1024.  LDS: part [16][8 L] and u [8 L] floats.
+#define JL_AD_ONE_LDS(L) (17 * 8 * (L))
+template <int T, int L>
+__device__ __forceinline__ void adapter_one_body(const AdapterArgs& p, float* lds) {
+    constexpr int R = 8 * L, RB = R < 16 ? R : 16;   // rows of A asked for at a time
+    constexpr bool AHEAD = L * sizeof(AdType<T>) <= 64;   // B asked for ahead of A: while it fits the registers
+    float* part = lds;
+    float* us = lds + 16 * R;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tok = blockIdx.y;
+    int block = blockIdx.x;
+    const int pi = ad_projection(p, block, 1024);
+    const u32 id = p.ids[tok];
+    const int rank = id >= (u32)p.n_adapter ? 0 : ad_rank(p, id);   // uniform
+    const size_t orow = (size_t)tok * p.rows[pi];
+    if (rank == 0) return ad_copy(p, pi, orow, block * 1024 + (int)threadIdx.x, 1024, 1);
+    const int col = block * 1024 + wave * 64;
+    const bool here = col < p.rows[pi];
+    AdColumns<T, L> c;
+    if (here) c.load(p, pi, id, rank, orow, col, AHEAD, true);
+    // wavefront = (piece of K modulo pieces, rows modulo 16 / pieces)
+    const int np = (p.k + 255) / 256, pieces = np > 8 ? 16 : np > 4 ? 8 : np > 2 ? 4 : np;   // a power of two
+    const int piece = wave & (pieces - 1), step = 16 / pieces;
+    for (int r = wave / pieces; r < rank; r += RB * step) {
+        float sum[RB];
+        ad_rows<T, RB>(p, pi, id, rank, (size_t)tok * p.k, r, step, piece, pieces, sum);
+        ad_wave_rows<RB>(sum);
+#pragma unroll
+        for (int i = 0; i < RB / 4; i++) {
+            const int row = r + (4 * i + lane) * step;
+            if (lane < 4 && row < rank) part[piece * R + row] = sum[i];
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x < R) {
+        float v = 0.f;
+        if ((int)threadIdx.x < rank) {
+            for (int q = 0; q < pieces; q++) v += part[q * R + threadIdx.x];
+            v *= p.scale ? p.scale[id] : 1.f;
+        }
+        us[threadIdx.x] = v;
+    }
+    __syncthreads();
+    if (!here) return;
+    float u[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) u[i] = us[8 * (lane % L) + i];
+    if (!AHEAD) c.load(p, pi, id, rank, orow, col, true, false);
+    c.finish(p, pi, orow, col, u);
+}
+
+// Two launches.  Sums of A x of a token: grid = (slices of 1024 elements of K modulo p.slices, ntok, projections * ceil(rank / 16)), block = 256, a
+// wavefront sixteen rows of A over 256 elements; part as adapter_down's.
+template <int T> __device__ __forceinline__ void adapter_dots_body(const AdapterArgs& p, float* lds) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tok = blockIdx.y, ctiles = p.rank_pad / 16;
+    const int pi = blockIdx.z / ctiles, r = blockIdx.z % ctiles * 16;
+    const u32 id = p.ids[tok];
+    const int rank = id >= (u32)p.n_adapter ? 0 : ad_rank(p, id);   // uniform
+    if (r >= rank) return;   // (adapter_cols reads no u from the rank on)
+    float sum[16];
+    ad_rows<T, 16>(p, pi, id, rank, (size_t)tok * p.k, r, 1, (int)blockIdx.x * 4 + wave, p.slices * 4, sum);
+    ad_wave_rows<16>(sum);
+    if (lane < 4)
+#pragma unroll
+        for (int i = 0; i < 4; i++) lds[wave * 16 + 4 * i + lane] = sum[i];
+    __syncthreads();
+    if (threadIdx.x < 16)
+        p.part[((size_t)blockIdx.x * p.ntok + tok) * p.n * p.rank_pad + pi * p.rank_pad + r + threadIdx.x] =
+            lds[threadIdx.x] + lds[16 + threadIdx.x] + (lds[32 + threadIdx.x] + lds[48 + threadIdx.x]);
+}
+// Columns of out from it: grid = (blocks of 256 p.up_sets columns of all projections, ntok), block = 256, LDS = 8 L floats.
+template <int T, int L> __device__ __forceinline__ void adapter_cols_body(const AdapterArgs& p, float* us) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tok = blockIdx.y;
+    int block = blockIdx.x;
+    const int pi = ad_projection(p, block, 256 * p.up_sets);
+    const int ncol = p.n * p.rank_pad;
+    float v[16];
+    if (threadIdx.x < 8 * L) {   // (asked for before the id is known; past the rank's padding, and past what adapter_dots wrote: not used)
+        const float* at = p.part + (size_t)tok * ncol + pi * p.rank_pad + min((int)threadIdx.x, p.rank_pad - 1);
+#pragma unroll
+        for (int s = 0; s < 16; s++) v[s] = s < p.slices ? at[(size_t)s * p.ntok * ncol] : 0.f;
+    }
+    const u32 id = p.ids[tok];
+    const int rank = id >= (u32)p.n_adapter ? 0 : ad_rank(p, id);   // uniform
+    const size_t orow = (size_t)tok * p.rows[pi];
+    if (rank == 0) return ad_copy(p, pi, orow, block * 256 * p.up_sets + (int)threadIdx.x, 256, p.up_sets);
+    int col = block * 256 * p.up_sets + wave * 64;
+    AdColumns<T, L> c;
+    if (col < p.rows[pi]) c.load(p, pi, id, rank, orow, col, true, true);
+    if (threadIdx.x < 8 * L) {
+        float t = 0.f;
+        if ((int)threadIdx.x < rank) {
+#pragma unroll
+            for (int s = 0; s < 16; s++) t += v[s];
+            t *= p.scale ? p.scale[id] : 1.f;
+        }
+        us[threadIdx.x] = t;
+    }
+    __syncthreads();
+    float u[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) u[i] = us[8 * (lane % L) + i];
+    for (int s = 0; s < p.up_sets && col < p.rows[pi]; s++, col += 256) {
+        if (s) c.load(p, pi, id, rank, orow, col, true, true);
+        c.finish(p, pi, orow, col, u);
     }
 }

@@ -621,7 +621,7 @@ struct AdapterArgs {
     uint16_t* u;                           // workspace: u as three bf16 pieces, [ntok][n][K steps of 32][3][32]
     int n, n_adapter, rank, k, ntok;
     int rank_pad;                          // rank rounded up to sixteen
-    int x_type;                            // (adapter_one)
+    int x_type;                            // (the dot products)
     int passes, slices;                    // of adapter_down; slices 0 in adapter_up: u has been made
-    int up_sets, one_sets;                 // sets of 256 (adapter_one: 1024) columns a workgroup
+    int up_sets;                           // sets of 256 columns a workgroup
 };

@@ -696,11 +696,21 @@ JL_NORM_ROWS(wg_8, 64, 8, true, 1024) JL_NORM_ROWS(wg_16, 64, 16, true, 1024)
         adapter_down_body<TYPE, XTYPE, NT>(p, sx, toks);                                                                     \
     }
 extern "C" __global__ __launch_bounds__(256) void jl_adapter_sum(AdapterArgs p) { adapter_sum_body(p); }
-// grid = (column blocks, ntok), block = 1024
+// grid = (column blocks, ntok), block = 1024; _cols 256
 #define JL_ADAPTER_ONE(T, TYPE, L)                                                                                           \
     extern "C" __global__ __launch_bounds__(1024) void jl_adapter_one_##T##_l##L(AdapterArgs p) {                            \
         __shared__ float s[JL_AD_ONE_LDS(L)];                                                                                \
         adapter_one_body<TYPE, L>(p, s);                                                                                     \
+    }                                                                                                                        \
+    extern "C" __global__ __launch_bounds__(256) void jl_adapter_cols_##T##_l##L(AdapterArgs p) {                            \
+        __shared__ float s[8 * L];                                                                                           \
+        adapter_cols_body<TYPE, L>(p, s);                                                                                    \
+    }
+// grid = (slices, ntok, projections * ceil(rank / 16)), block = 256
+#define JL_ADAPTER_DOTS(T, TYPE)                                                                                             \
+    extern "C" __global__ __launch_bounds__(256) void jl_adapter_dots_##T(AdapterArgs p) {                                   \
+        __shared__ float s[64];                                                                                              \
+        adapter_dots_body<TYPE>(p, s);                                                                                       \
     }
 // grid = (column blocks, group slots, ntok / 64), block = 256
 #define JL_ADAPTER_UP_V(T, TYPE, NAME, KS, MANY, VEC)                                                                        \
@@ -714,6 +724,6 @@ extern "C" __global__ __launch_bounds__(256) void jl_adapter_sum(AdapterArgs p) 
 #define JL_ADAPTER_X(T, TYPE, XT, XTYPE) JL_ADAPTER_DOWN(T, TYPE, XT, XTYPE, 1) JL_ADAPTER_DOWN(T, TYPE, XT, XTYPE, 2)
 #define JL_ADAPTER(T, TYPE)                                                                                                  \
     JL_ADAPTER_X(T, TYPE, f32, JL_F32) JL_ADAPTER_X(T, TYPE, f16, JL_F16) JL_ADAPTER_X(T, TYPE, bf16, JL_BF16)               \
-    JL_ADAPTER_ONE(T, TYPE, 1) JL_ADAPTER_ONE(T, TYPE, 2) JL_ADAPTER_ONE(T, TYPE, 4) JL_ADAPTER_ONE(T, TYPE, 8)              \
+    JL_ADAPTER_DOTS(T, TYPE) JL_ADAPTER_ONE(T, TYPE, 1) JL_ADAPTER_ONE(T, TYPE, 2) JL_ADAPTER_ONE(T, TYPE, 4) JL_ADAPTER_ONE(T, TYPE, 8) \
     JL_ADAPTER_UP(T, TYPE, k1, 1, false) JL_ADAPTER_UP(T, TYPE, k2, 2, false) JL_ADAPTER_UP(T, TYPE, many, 1, true)
 JL_ADAPTER(f32, JL_F32) JL_ADAPTER(f16, JL_F16) JL_ADAPTER(bf16, JL_BF16)
