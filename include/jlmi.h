@@ -375,9 +375,10 @@ int jl_matvec_packed_group(jl_ctx *ctx, int n, float *const *outs, const int *ty
  * (JL_TYPE_F32, _F16, _BF16); x [ntok][k] of x_type (the same three).  ranks, when given, holds each adapter's own rank (more
  * than `rank` counts as `rank`): rows of A and columns of B from there on are not used.  scale null: ones.  A token whose id is
  * n_adapter or more has no adapter and gets base alone, as does one whose adapter has rank 0.  ids, ranks and scale are device
- * memory, read by the kernels.  Products and sums are f32 whatever the types.  k % 32 == 0, rank <= 512; a, b and x 16-byte
- * aligned.  The workspace (ntok * n * rank floats at most) is the context's, grown on demand; a buffer that is outgrown lives until the
- * context goes, so a captured graph that holds its address stays valid.  jl_reserve_adapters sizes it ahead of time.
+ * memory, read by the kernels.  Products and sums are f32 whatever the types.  k % 32 == 0, rank <= 512, n_adapter <= 8192; a, b and x 16-byte
+ * aligned.  Few tokens take one or two launches of dot products, more of them the matrix cores (on exact pieces of the operands);
+ * a token's result does not depend on the other tokens of the call, but by their number on the last bits.  The workspace (jl_reserve_adapters) is
+ * the context's, grown on demand; a buffer that is outgrown lives until the context goes, so a captured graph that holds its address stays valid.
  * No counterpart in the reference. */
 typedef struct jl_adapter_group {
     int n;

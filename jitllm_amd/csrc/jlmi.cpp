@@ -2239,6 +2239,7 @@ int jl_ctx_create(jl_ctx** out, const jl_options* opts) {
         for (const char* any : {"", "_any"}) names.push_back(std::string("jl_norm_rows_") + form + any);
     for (const char* g : {"g2", "g4", "g8", "g16"}) names.push_back(std::string("jl_moe_select_") + g);
     names.push_back("jl_adapter_sum");
+    names.push_back("jl_adapter_group");
     for (const char* t : {"f32", "f16", "bf16"}) {
         for (const char* xt : {"f32", "f16", "bf16"})
             for (const char* nt : {"_n1", "_n2"}) names.push_back(std::string("jl_adapter_down_") + t + "_" + xt + nt);
@@ -2542,22 +2543,25 @@ int adapter_ws_ensure(jl_ctx* c, size_t need) {
 }  // namespace
 
 namespace {
-// How adapter_down is cut: a group is 64 tokens' of one adapter; a workgroup takes a group, 4 nt tiles of sixteen rows of A and a slice of K.
-// Slices for two workgroups a CU, as far as the groups are known: there is one for 64 tokens at least, and one for every adapter met.
-struct AdapterPlan { int rank_pad, nt, passes, slices; };
+constexpr int kMaxAdapters = 8192;   // counters of the grouping in LDS
+// How the matrix-core form is cut: a tile is up to 64 tokens of one adapter; a workgroup of adapter_down takes a tile, 4 nt tiles of sixteen rows of A
+// and a slice of K.  Slices for two workgroups a CU, as far as the tiles are known: there is one for 64 tokens at least, and one for every adapter met.
+struct AdapterPlan { int rank_pad, nt, passes, slices, max_tiles; };
 AdapterPlan adapter_plan(const jl_ctx* c, int ntok, int n, int rank, int k, int n_adapter) {
     AdapterPlan a;
     a.rank_pad = (rank + 15) / 16 * 16;
     const int tiles = n * a.rank_pad / 16;
     a.nt = tiles <= 4 ? 1 : 2;
     a.passes = (tiles + 4 * a.nt - 1) / (4 * a.nt);
+    a.max_tiles = ntok / 64 + std::min(n_adapter + 1, ntok);
     const long units = (long)a.passes * std::max((ntok + 63) / 64, std::min(ntok, n_adapter)), steps = (k + 127) / 128;
     a.slices = (int)std::max(1l, std::min({16l, steps, c->tune.adapter_slices ? (long)c->tune.adapter_slices : 2l * c->num_cu / units}));
     return a;
 }
-// Bytes of the sums of `rows` slices * tokens and of u in bf16 pieces.
+// Bytes of the sums of `rows` slices * tokens, of u in bf16 pieces, and of the lists of tokens and tiles.
 size_t adapter_part_bytes(size_t rows, int n, int rank) { return rows * n * ((rank + 15) / 16 * 16) * 4; }
 size_t adapter_u_bytes(int ntok, int n, int rank) { return (size_t)ntok * n * ((rank + 31) / 32) * 192; }
+size_t adapter_list_bytes(int ntok, int n_adapter) { return ((size_t)ntok / 64 + std::min(n_adapter + 1, ntok)) * 16 + (size_t)ntok * 4; }
 }  // namespace
 
 int jl_reserve_adapters(jl_ctx* c, int max_tok, int n, int max_rank) {
@@ -2567,7 +2571,7 @@ int jl_reserve_adapters(jl_ctx* c, int max_tok, int n, int max_rank) {
     HIP_TRY(c, H->SetDevice(c->device));
     // slices * tokens: sixteen slices at most, more than one while slices * tokens / 64 is within two workgroups a CU
     const size_t rows = std::max((size_t)max_tok, std::min((size_t)16 * max_tok, (size_t)128 * c->num_cu));
-    return adapter_ws_ensure(c, adapter_part_bytes(rows, n, max_rank) + adapter_u_bytes(max_tok, n, max_rank));
+    return adapter_ws_ensure(c, adapter_part_bytes(rows, n, max_rank) + adapter_u_bytes(max_tok, n, max_rank) + adapter_list_bytes(max_tok, kMaxAdapters));
 }
 
 int jl_adapter_group_dev(jl_ctx* c, const jl_adapter_group* g, void* stream) {
@@ -2575,7 +2579,7 @@ int jl_adapter_group_dev(jl_ctx* c, const jl_adapter_group* g, void* stream) {
     if (!g || g->n < 1 || g->n > JL_MAX_GROUP || !g->x || !g->ids || g->k <= 0 || g->ntok <= 0 || g->n_adapter <= 0 || g->rank <= 0)
         return fail(c, JL_ERR_ARG, "adapter group: bad group");
     const int wb = plain_bytes(g->type), xb = plain_bytes(g->x_type);
-    if (!wb || !xb || g->k % 32 != 0 || g->rank > 512) return JL_DECLINED;
+    if (!wb || !xb || g->k % 32 != 0 || g->rank > 512 || g->n_adapter > kMaxAdapters) return JL_DECLINED;
     AdapterArgs a;
     long wide = 0;
     bool vec = true;
@@ -2592,12 +2596,12 @@ int jl_adapter_group_dev(jl_ctx* c, const jl_adapter_group* g, void* stream) {
     a.ids = g->ids; a.ranks = g->ranks; a.scale = g->scale; a.x = g->x; a.u = nullptr;
     a.n = g->n; a.n_adapter = g->n_adapter; a.rank = g->rank; a.k = g->k; a.ntok = g->ntok;
     const AdapterPlan pl = adapter_plan(c, g->ntok, g->n, g->rank, g->k, g->n_adapter);
-    a.part = nullptr; a.u = nullptr;
+    a.part = nullptr; a.u = nullptr; a.perm = a.tiles = nullptr;
+    a.max_tiles = pl.max_tiles;
     a.rank_pad = pl.rank_pad; a.passes = pl.passes; a.slices = pl.slices; a.x_type = g->x_type; a.up_sets = 1;
     hipStream_t st = pick_stream(c, stream);
     void* params[] = {&a};
     const char *t = plain_tag(g->type), *xt = plain_tag(g->x_type);
-    const int chunks = (g->ntok + 63) / 64, most = std::min(g->ntok, 64);   // the kernels look at 64 tokens at a time
     auto blocks = [&](int width) {   // column blocks of all projections
         unsigned b = 0;
         for (int i = 0; i < g->n; i++) b += (unsigned)(g->rows[i] + width - 1) / width;
@@ -2607,7 +2611,14 @@ int jl_adapter_group_dev(jl_ctx* c, const jl_adapter_group* g, void* stream) {
     const long sets = (long)g->ntok * blocks(1024);
     const int l = g->rank <= 8 ? 1 : g->rank <= 16 ? 2 : g->rank <= 32 ? 4 : 8;   // lanes a column
     const bool dots = g->rank <= 64 && g->ntok <= 65535;
-    const int form = c->tune.adapter_form ? c->tune.adapter_form : dots && g->rank <= 16 && sets <= c->num_cu ? 1 : dots && g->ntok <= 16 ? 2 : 0;
+    // Which form, by what each is estimated to take (us; fitted to 16-bit adapters beside 4096 to 28672 rows of k = 4096, 32 to 2048 tokens, 1 to 64
+    // adapters, within a quarter of the times there).  Dot products read A and B for every token, the matrix cores for every tile:
+    //   128 tokens of 8 adapters, rank 16 beside 4096: 8.7 against 21 us; rank 64 beside 2 x 14336: 40 against 33;
+    //   512 tokens of 8, rank 16: 17 and 26, rank 64: 38 and 30; of 64 adapters, rank 64: 43 and 44; 2048 tokens of 64, rank 16: 60 and 52.
+    const double wide_d = (double)wide, nk = (double)g->n * g->k, bytes = g->rank * (nk + wide_d) * wb;
+    const double dots_us = 6 + g->ntok * (0.61e-7 * wb * g->rank * nk + wide_d * (3.1e-6 + 3.4e-8 * wb * g->rank));
+    const double mm_us = 17 + g->ntok * (1.7e-6 * g->k + 1.6e-6 * wide_d + 2.5e-9 * bytes) + std::max((g->ntok + 63) / 64, std::min(g->ntok, g->n_adapter)) * bytes / 3.7e6;
+    const int form = c->tune.adapter_form ? c->tune.adapter_form : !dots ? 0 : g->rank <= 16 && sets <= c->num_cu ? 1 : dots_us <= mm_us ? 2 : 0;
     if (dots && form == 1) {
         name << "jl_adapter_one_" << t << "_l" << l;
         return launch(c, name, blocks(1024), (unsigned)g->ntok, 1024, 0, st, params);
@@ -2620,31 +2631,38 @@ int jl_adapter_group_dev(jl_ctx* c, const jl_adapter_group* g, void* stream) {
         name << "jl_adapter_dots_" << t;
         rc = launch(c, name, (unsigned)a.slices, (unsigned)g->ntok, 256, 0, st, params, (unsigned)(g->n * a.rank_pad / 16));
         if (rc != JL_OK) return rc;
-        a.up_sets = c->tune.adapter_sets ? c->tune.adapter_sets : 1;
+        // (columns a workgroup: fewer and longer ones where there are many; us by 256 / 512 / 1024: 128 tokens rank 16 beside 4096 rows 8.7 / 8.6 / 9.5,
+        // 6144 13.3 / 11.6 / 12.1, 28672 28 / 22 / 20)
+        const long wgs = (long)g->ntok * blocks(256);
+        a.up_sets = c->tune.adapter_sets ? c->tune.adapter_sets : wgs <= 8l * c->num_cu ? 1 : wgs <= 24l * c->num_cu ? 2 : 4;
         Name cols;
         cols << "jl_adapter_cols_" << t << "_l" << l;
         return launch(c, cols, blocks(256 * a.up_sets), (unsigned)g->ntok, 256, 0, st, params);
     }
-    const size_t part = adapter_part_bytes((size_t)a.slices * g->ntok, g->n, g->rank);
-    int rc = adapter_ws_ensure(c, part + adapter_u_bytes(g->ntok, g->n, g->rank));
+    const size_t part = adapter_part_bytes((size_t)a.slices * g->ntok, g->n, g->rank), ub = adapter_u_bytes(g->ntok, g->n, g->rank);   // (multiples of 64)
+    int rc = adapter_ws_ensure(c, part + ub + adapter_list_bytes(g->ntok, g->n_adapter));
     if (rc != JL_OK) return rc;
-    a.part = (float*)c->adapter_ws;
-    a.u = (uint16_t*)((char*)c->adapter_ws + part);
+    char* ws = (char*)c->adapter_ws;
+    a.part = (float*)ws;
+    a.u = (uint16_t*)(ws + part);
+    a.tiles = (uint32_t*)(ws + part + ub);
+    a.perm = a.tiles + (size_t)a.max_tiles * 4;
+    rc = launch(c, "jl_adapter_group", 1, 1, 1024, (unsigned)(g->n_adapter + 33) * 4, st, params);
+    if (rc != JL_OK) return rc;
     name << "jl_adapter_down_" << t << "_" << xt << "_n" << pl.nt;
-    rc = launch(c, name, (unsigned)std::min(most, g->n_adapter), (unsigned)chunks, 256, 0, st, params, (unsigned)(a.passes * a.slices));
+    rc = launch(c, name, (unsigned)a.max_tiles, 1, 256, 0, st, params, (unsigned)(a.passes * a.slices));
     if (rc != JL_OK) return rc;
     const double added = (double)blocks(256) * g->ntok * a.slices * g->rank * 4;   // bytes that adapter_up would add up
-    if (c->tune.adapter_form ? c->tune.adapter_form == 4 : added > 30e6) {
-        const size_t octs = (size_t)g->ntok * g->n * ((a.rank_pad + 31) / 32) * 4;
-        rc = launch(c, "jl_adapter_sum", (unsigned)((octs + 255) / 256), 1, 256, 0, st, params);
+    if (form == 4 || (form != 3 && added > 30e6)) {
+        const size_t quads = (size_t)g->ntok * g->n * ((a.rank_pad + 31) / 32) * 8;
+        rc = launch(c, "jl_adapter_sum", (unsigned)((quads + 255) / 256), 1, 256, 0, st, params);
         if (rc != JL_OK) return rc;
         a.slices = 0;
     }
     Name up;
     up << "jl_adapter_up_" << t << (g->rank <= 32 ? "_k1" : g->rank <= 64 ? "_k2" : "_many") << (vec ? "" : "_any");
-    a.up_sets = c->tune.adapter_sets ? c->tune.adapter_sets : (long)blocks(256) * chunks >= 6 * c->num_cu ? 2 : 1;
-    const unsigned groups = g->ntok >= 1024 ? 1 : (unsigned)std::min(most, g->n_adapter + 1);
-    return launch(c, up, blocks(256 * a.up_sets), groups, 256, 0, st, params, (unsigned)chunks);
+    a.up_sets = c->tune.adapter_sets ? c->tune.adapter_sets : (long)blocks(256) * (g->ntok / 64) >= 6 * c->num_cu ? 2 : 1;
+    return launch(c, up, blocks(256 * a.up_sets), (unsigned)a.max_tiles, 256, 0, st, params);
 }
 
 int jl_dequant_dev(jl_ctx* c, int type, const void* src, float* dst, size_t n, void* stream) {

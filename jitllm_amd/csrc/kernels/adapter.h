@@ -2,9 +2,10 @@
 //   out_i[t] = base_i[t] + scale[a] * B_i[a] (A_i[a] x[t]),     A_i [n_adapter][rank][k], B_i [n_adapter][rows_i][rank]
 // for up to four projections that read one x.  A token whose id no adapter has, or whose adapter has rank 0, gets base alone.
 //
-// On the bf16 matrix cores: adapter_down makes sums of u = A x for the tokens of an adapter and a slice of K, adapter_up adds B u to base (where
-// many column blocks would each add the slices up, adapter_sum does it first).  A workgroup looks at 64 consecutive tokens and finds for itself which of them share an adapter (a ballot
-// per adapter met), so nothing is sorted beforehand; a token meets its own adapter only, so no number of another's can reach it.
+// Many tokens: adapter_group puts the tokens of an adapter side by side; then on the bf16 matrix cores, for tiles of up to 64 of them, adapter_down
+// makes sums of u = A x over slices of K and adapter_up adds B u to base (where many column blocks would each add the slices up, adapter_sum does
+// it first).  Few tokens, or few of each adapter: dot products in f32, in two launches or one (the end of this file).  A token meets its own adapter
+// only, so no number of another's can reach it.
 //
 // Products are exact: an f32 value is three bf16 values (8 mantissa bits each, cut off, not rounded), an f16 value two, and every
 // piece of one operand meets every piece of the other in the f32 accumulator -- one matrix instruction for bf16 x bf16, three for f32 x
@@ -12,8 +13,8 @@
 // leaves a NaN: it was going to be no finite number.)
 //
 // What decides the layout of the work (measured on MI355X): sixteen rows of 64 bytes a load, as the matrix instruction's operands and results lie, run
-// at two thirds of the rate of rows of 256 bytes and more, so x, base and out are moved by rows and change places in LDS; and a CU draws about 35
-// bytes a ns from the L2s whatever its wavefronts ask for, so an adapter's A is spread over as many workgroups as there are.
+// at two thirds of the rate of rows of 256 bytes, so x, base and out are moved by rows and change places in LDS; and with few tokens a call is
+// trips to memory one after the other, so everything whose address is known is asked for at once.
 #pragma once
 #include "args.h"
 #include "common.h"
@@ -95,17 +96,8 @@ template <int PA, int PB> __device__ __forceinline__ f32x4 ad_mfma(const u32x4 (
     return acc;
 }
 
-// A lane's token of the 64 from `first` on: its adapter, n_adapter where it has none; 0xFFFFFFFF: no token.
-__device__ __forceinline__ u32 ad_id(const AdapterArgs& p, int first) {
-    const int tok = first + (threadIdx.x & 63);
-    if (tok >= p.ntok) return 0xFFFFFFFFu;
-    u32 id = min(p.ids[tok], (u32)p.n_adapter);
-    if (p.ranks && id < (u32)p.n_adapter && p.ranks[id] == 0) id = (u32)p.n_adapter;
-    return id;
-}
-__device__ __forceinline__ int ad_rank(const AdapterArgs& p, u32 id) {
-    return id >= (u32)p.n_adapter ? 0 : p.ranks ? (int)min(p.ranks[id], (u32)p.rank) : p.rank;
-}
+__device__ __forceinline__ int ad_rank(const AdapterArgs& p, u32 id) { return p.ranks ? (int)min(p.ranks[id], (u32)p.rank) : p.rank; }
+
 // Four consecutive elements as f32.
 template <int T> struct AdQuad {
     u32x2 w;
@@ -121,31 +113,105 @@ template <> struct AdQuad<JL_F32> {
     __device__ __forceinline__ float value(int i) const { return w[i]; }
 };
 
-// The groups of the 64 tokens from `first` on, one adapter's (or, with `limit` one higher, none's) tokens each, in the order in which they
-// come; every gridDim-th is a workgroup's.  Uniform.
-struct AdGroups {
-    uint64_t rest;
-    int at;
-    __device__ __forceinline__ AdGroups(u32 id, u32 limit) : rest(__ballot(id < limit)), at(0) {}
-    // the next of the groups slot, slot + slots, ...: its adapter and which of the 64 lanes' tokens are of it
-    __device__ __forceinline__ bool next(u32 id, int slot, int slots, u32& a, uint64_t& of) {
-        while (rest) {
-            a = (u32)__builtin_amdgcn_readlane((i32)id, __builtin_ctzll(rest));
-            of = __ballot(id == a);
-            rest &= ~of;
-            if (at++ % slots == slot) return true;
+// ---------------------------------------------------------------- tokens by adapter
+// perm: the tokens, those of an adapter side by side (those without one last); tiles: {adapter, first place in perm, tokens} of pieces of up to
+// 64 of them, n_adapter for those without one, 0 tokens behind the last.  The order inside an adapter is whatever the LDS additions make
+// it: no result depends on what else is in a token's tile.  One workgroup of 1024; LDS: n_adapter + 1 counters, 16 totals.
+__device__ __forceinline__ void adapter_group_body(const AdapterArgs& p, u32* count) {
+    const int tid = threadIdx.x, kinds = p.n_adapter + 1, lane = tid & 63, wave = tid >> 6;
+    u32* tot = count + kinds;
+    auto kind = [&](int t) {
+        const u32 id = min(p.ids[t], (u32)p.n_adapter);
+        return p.ranks && id < (u32)p.n_adapter && p.ranks[id] == 0 ? (u32)p.n_adapter : id;
+    };
+    u32 mine[4];   // of the first 4096 tokens; later ones are read again
+#pragma unroll
+    for (int i = 0; i < 4; i++) mine[i] = tid + 1024 * i < p.ntok ? kind(tid + 1024 * i) : 0;
+    for (int i = tid; i < kinds; i += 1024) count[i] = 0;
+    __syncthreads();
+    // a token's place among its kind's so far; one addition for a wavefront whose tokens are all of a kind (a prompt's), which LDS would take one by one
+    auto take = [&](u32 k, bool live) {
+        const uint64_t on = __ballot(live);
+        const u32 first = (u32)__builtin_amdgcn_readfirstlane((i32)k);
+        if (on == ~0ull && __ballot(k == first) == ~0ull) {
+            u32 at = 0;
+            if (lane == 0) at = atomicAdd(&count[first], 64u);
+            return (u32)__builtin_amdgcn_readfirstlane((i32)at) + lane;
         }
-        return false;
+        return live ? atomicAdd(&count[k], 1u) : 0u;
+    };
+#pragma unroll
+    for (int i = 0; i < 4; i++) (void)take(mine[i], tid + 1024 * i < p.ntok);
+    for (int t0 = 4096; t0 < p.ntok; t0 += 1024) (void)take(t0 + tid < p.ntok ? kind(t0 + tid) : 0, t0 + tid < p.ntok);
+    __syncthreads();
+    // places and tiles before a thread's run of kinds
+    const int per = (kinds + 1023) / 1024, lo = min(tid * per, kinds), hi = min(lo + per, kinds);
+    u32 np = 0, nt = 0;
+    for (int i = lo; i < hi; i++) {
+        np += count[i];
+        nt += (count[i] + 63) / 64;
+    }
+    u32 sp = np, st = nt;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const u32 a = __shfl_up(sp, off, 64), b = __shfl_up(st, off, 64);
+        if (lane >= off) {
+            sp += a;
+            st += b;
+        }
+    }
+    if (lane == 63) {
+        tot[wave] = sp;
+        tot[16 + wave] = st;
+    }
+    __syncthreads();
+    for (int w = 0; w < wave; w++) {
+        sp += tot[w];
+        st += tot[16 + w];
+    }
+    u32 all = 0;
+    for (int w = 0; w < 16; w++) all += tot[16 + w];
+    u32 place = sp - np, tile = st - nt;
+    for (int i = lo; i < hi; i++) {
+        const u32 n = count[i];
+        for (u32 t = 0; t < n; t += 64) ((u32x4*)p.tiles)[tile++] = u32x4{(u32)i, place + t, min(64u, n - t), 0};
+        count[i] = place;
+        place += n;
+    }
+    for (u32 t = all + tid; t < (u32)p.max_tiles; t += 1024) ((u32x4*)p.tiles)[t] = u32x4{(u32)p.n_adapter, 0, 0, 0};
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const bool live = tid + 1024 * i < p.ntok;
+        const u32 at = take(mine[i], live);
+        if (live) p.perm[at] = tid + 1024 * i;
+    }
+    for (int t0 = 4096; t0 < p.ntok; t0 += 1024) {
+        const bool live = t0 + tid < p.ntok;
+        const u32 at = take(live ? kind(t0 + tid) : 0, live);
+        if (live) p.perm[at] = t0 + tid;
+    }
+}
+struct AdTile {
+    u32 a;
+    int count, nt, rank;
+    bool none;
+    // toks: the tile's tokens, in LDS behind the next barrier.  False: no such tile.
+    __device__ __forceinline__ bool of(const AdapterArgs& p, int tile, int* toks) {
+        const u32x4 t = ((const u32x4*)p.tiles)[tile];
+        count = (int)t.z;
+        if (count == 0) return false;
+        a = t.x;
+        none = a >= (u32)p.n_adapter;
+        nt = (count + 15) / 16;
+        rank = none ? 0 : ad_rank(p, a);
+        if (threadIdx.x < 64 && (int)threadIdx.x < count) toks[threadIdx.x] = p.perm[t.y + threadIdx.x];
+        return true;
     }
 };
-// The group's tokens, in order, to toks (every wavefront writes the same).
-__device__ __forceinline__ void ad_tokens(uint64_t of, int first, int* toks) {
-    const int lane = threadIdx.x & 63;
-    if ((of >> lane) & 1) toks[__builtin_popcountll(of & ((1ull << lane) - 1))] = first + lane;
-}
 
 // ---------------------------------------------------------------- sums of A x
-// grid = (group slots of 64 tokens, ntok / 64, passes * slices), block = 256.  A workgroup takes a group's up to 64 tokens (four tiles), NT column
+// grid = (tiles, 1, passes * slices), block = 256.  A workgroup takes a tile's up to 64 tokens (four of sixteen), NT column
 // tiles a wavefront (sixteen rows of A each; all projections' side by side, a rank rounded up to sixteen) and a slice of K, 128 at a time: x by
 // rows of 512 bytes through registers, cut into pieces on the way to LDS, where all four wavefronts read it; A's fragments straight from
 // memory, each once a workgroup.  Writes part [slices][ntok][n * rank_pad].
@@ -155,19 +221,17 @@ __device__ __forceinline__ void ad_tokens(uint64_t of, int first, int* toks) {
 template <int T, int XT, int NT>
 __device__ __forceinline__ void adapter_down_body(const AdapterArgs& p, uint16_t* sx, int* toks) {
     constexpr int PW = AdType<T>::pieces, PX = AdType<XT>::pieces, ROW = JL_AD_DOWN_ROW;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, first = blockIdx.y * 64;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int pass = blockIdx.z % p.passes, slice = blockIdx.z / p.passes;
     const int ctiles = p.rank_pad / 16, all = p.n * ctiles, c0 = (pass * 4 + wave) * NT;
     const int steps = (p.k + JL_AD_DOWN_K - 1) / JL_AD_DOWN_K;
     const int lo = steps * slice / p.slices, hi = steps * (slice + 1) / p.slices;   // (slices <= steps)
-    const u32 id = ad_id(p, first);
-    AdGroups groups(id, (u32)p.n_adapter);
-    u32 a;
-    uint64_t of;
-    while (groups.next(id, blockIdx.x, gridDim.x, a, of)) {
-        const int count = __builtin_popcountll(of), nt = (count + 15) / 16, rank = ad_rank(p, a);
-        ad_tokens(of, first, toks);
-        __syncthreads();
+    AdTile tile;
+    if (!tile.of(p, blockIdx.x, toks) || tile.none) return;
+    const u32 a = tile.a;
+    const int count = tile.count, rank = tile.rank;
+    __syncthreads();
+    {
         const void* wp[NT];
         size_t wat[NT];
 #pragma unroll
@@ -263,9 +327,8 @@ __device__ __forceinline__ void adapter_down_body(const AdapterArgs& p, uint16_t
                     if (c0 + t < all) *(f32x4*)(u + (c0 + t) * 16) = acc[m][t];
             }
         };
-        if (nt > 1) run(GemmIntC<4>{});
+        if (tile.nt > 1) run(GemmIntC<4>{});
         else run(GemmIntC<1>{});
-        __syncthreads();   // (toks is the next group's)
     }
 }
 
@@ -298,20 +361,37 @@ __device__ __forceinline__ void ad_sum_u(const AdapterArgs& p, int tok, int pi, 
     }
     ad_split<3>(v, o);
 }
-// part -> u [ntok][n][K steps of 32][3 pieces][32] bf16.  grid = ceil(ntok * n * K steps * 4 / 256), block = 256: a thread eight of a row.
+// part -> u [ntok][n][K steps of 32][3 pieces][32] bf16.  grid = ceil(ntok * n * K steps * 8 / 256), block = 256: a thread four of a row, all slices on
+// their way at a time.
 __device__ __forceinline__ void adapter_sum_body(const AdapterArgs& p) {
-    const int ks = (p.rank_pad + 31) / 32;
+    const int ks = (p.rank_pad + 31) / 32, ncol = p.n * p.rank_pad;
     const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
-    const int oct = (int)(i % (ks * 4)), pi = (int)(i / (ks * 4) % p.n);
-    const size_t tok = i / ((size_t)ks * 4 * p.n);
+    const int quad = (int)(i % (ks * 8)), pi = (int)(i / (ks * 8) % p.n), r = 4 * quad;
+    const size_t tok = i / ((size_t)ks * 8 * p.n);
     if (tok >= (size_t)p.ntok) return;
+    const float* at = p.part + tok * ncol + pi * p.rank_pad + min(r, p.rank_pad - 4);
+    f32x4 v[16];
+#pragma unroll
+    for (int s = 0; s < 16; s++) v[s] = s < p.slices ? *(const f32x4*)(at + (size_t)s * p.ntok * ncol) : f32x4{0.f, 0.f, 0.f, 0.f};
     const u32 id = p.ids[tok];
     if (id >= (u32)p.n_adapter) return;   // (nobody reads u of a token without an adapter)
-    u32x4 o[3];
-    ad_sum_u(p, (int)tok, pi, 8 * oct, p.scale ? p.scale[id] : 1.f, ad_rank(p, id), o);
-    uint16_t* u = p.u + ((tok * p.n + pi) * ks + oct / 4) * 96 + oct % 4 * 8;
+    const int rank = ad_rank(p, id);
+    const float scale = p.scale ? p.scale[id] : 1.f;
 #pragma unroll
-    for (int n = 0; n < 3; n++) *(u32x4*)(u + 32 * n) = o[n];
+    for (int s = 1; s < 16; s++) v[0] += v[s];
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[0][e] = r + e < rank ? scale * v[0][e] : 0.f;
+    uint16_t* u = p.u + ((tok * p.n + pi) * ks + quad / 8) * 96 + quad % 8 * 4;
+#pragma unroll
+    for (int n = 0; n < 3; n++) {
+        u32 b[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            b[e] = __float_as_uint(v[0][e]);
+            v[0][e] -= __uint_as_float(b[e] & 0xFFFF0000u);
+        }
+        *(u32x2*)(u + 32 * n) = u32x2{__builtin_amdgcn_perm(b[1], b[0], 0x07060302), __builtin_amdgcn_perm(b[3], b[2], 0x07060302)};
+    }
 }
 
 // ---------------------------------------------------------------- out = base + B u
@@ -330,9 +410,9 @@ __device__ __forceinline__ int ad_projection(const AdapterArgs& p, int& block, i
     return i;
 }
 
-// grid = (column blocks of all projections, group slots of 64 tokens, ntok / 64), block = 256, a wavefront 64 columns (rows of B) a set of
-// 256, p.up_sets sets.  u's fragments of the group's (up to four) tiles lie in LDS, KS K steps of 32 at a time; B's stay in registers and meet
-// tile after tile.  A tile's sums change places in LDS and meet base by rows of 256 bytes, asked for a tile ahead.
+// grid = (column blocks of all projections, tiles), block = 256, a wavefront 64 columns (rows of B) a set of
+// 256, p.up_sets sets.  u's fragments of the tile's (up to four) sixteens lie in LDS, KS K steps of 32 at a time; B's stay in registers and meet
+// one after the other.  A tile's sums change places in LDS and meet base by rows of 256 bytes, asked for a tile ahead.
 // KS = 1: ranks up to 32, 2: up to 64.  MANY: any rank, KS steps at a time; the four tiles' sums stay in registers and base is read at the end.
 // VEC: rows of out and base on 16-byte boundaries.
 // LDS: frag [4 tiles][KS][3][64] x 16 bytes, move [4 wavefronts][16][68] floats, toks [64].
@@ -340,23 +420,20 @@ __device__ __forceinline__ int ad_projection(const AdapterArgs& p, int& block, i
 template <int T, int KS, bool MANY, bool VEC>
 __device__ __forceinline__ void adapter_up_body(const AdapterArgs& p, u32x4* frag, float* move, int* toks) {
     constexpr int PW = AdType<T>::pieces;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, first = blockIdx.z * 64;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int block = blockIdx.x;
     const int pi = ad_projection(p, block, 256 * p.up_sets);
     const int rows = p.rows[pi], ksteps = (p.rank_pad + 31) / 32;
     const float* base = p.base[pi];
     float* out = p.out[pi];
     move += wave * 16 * JL_AD_MOVE;
-    const u32 id = ad_id(p, first);
-    AdGroups groups(id, (u32)p.n_adapter + 1);
-    u32 a;
-    uint64_t of;
-    while (groups.next(id, blockIdx.y, gridDim.y, a, of)) {
-        const bool none = a >= (u32)p.n_adapter;
-        if (none && base == out) continue;
-        const int count = __builtin_popcountll(of), nt = (count + 15) / 16, rank = ad_rank(p, a);
+    AdTile tile;
+    if (!tile.of(p, blockIdx.y, toks) || (tile.none && base == out)) return;
+    {
+        const bool none = tile.none;
+        const u32 a = tile.a;
+        const int count = tile.count, nt = tile.nt, rank = tile.rank;
         const float scale = none || !p.scale ? 1.f : p.scale[a];
-        ad_tokens(of, first, toks);
         __syncthreads();
         // by rows: token 4 i + lane / 16 of a tile, four columns from 4 (lane % 16) on
         f32x4 bs[4];
@@ -496,7 +573,6 @@ __device__ __forceinline__ void adapter_up_body(const AdapterArgs& p, u32x4* fra
                 }
             }
         }
-        __syncthreads();   // (toks and frag are the next group's)
     }
 }
 
@@ -567,26 +643,32 @@ template <int N> __device__ __forceinline__ float ad_lane_sum(float v) {   // ov
 template <int T, int L> struct AdColumns {
     AdType<T> b[L];
     float base;
-    __device__ __forceinline__ void load(const AdapterArgs& p, int pi, u32 id, int rank, size_t orow, int col, bool with_b, bool with_base) {
+    // (B by the bank's rank: the adapter's own is known later)
+    __device__ __forceinline__ void load(const AdapterArgs& p, int pi, u32 id, size_t orow, int col, bool with_b, bool with_base) {
         const int lane = threadIdx.x & 63, rows = p.rows[pi], r0 = 8 * (lane % L), mine = col + lane % L * (64 / L) + lane / L;
         if (with_base) base = p.base[pi] && mine < rows ? p.base[pi][orow + mine] : 0.f;
         if (with_b)
 #pragma unroll
             for (int j = 0; j < L; j++)
-                b[j].load_some(p.b[pi], ((size_t)id * rows + min(col + j * (64 / L) + lane / L, rows - 1)) * p.rank + min(r0, rank), min(max(rank - r0, 0), 8));
+                b[j].load_some(p.b[pi], ((size_t)id * rows + min(col + j * (64 / L) + lane / L, rows - 1)) * p.rank + min(r0, p.rank), min(max(p.rank - r0, 0), 8));
     }
-    __device__ __forceinline__ void finish(const AdapterArgs& p, int pi, size_t orow, int col, const float (&u)[8]) {
-        const int lane = threadIdx.x & 63, mine = col + lane % L * (64 / L) + lane / L;
+    __device__ __forceinline__ void finish(const AdapterArgs& p, int pi, size_t orow, int col, int rank, const float (&u)[8]) {
+        const int lane = threadIdx.x & 63, mine = col + lane % L * (64 / L) + lane / L, left = rank - 8 * (lane % L);
         float d = 0.f;
 #pragma unroll
         for (int j = 0; j < L; j++) {
             float v = 0.f;
+            if (p.ranks) {   // columns of B from the adapter's rank on may hold anything
 #pragma unroll
-            for (int i = 0; i < 8; i++) v = __builtin_fmaf(b[j].value(i), u[i], v);
+                for (int i = 0; i < 8; i++) v = __builtin_fmaf(i < left ? b[j].value(i) : 0.f, u[i], v);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) v = __builtin_fmaf(b[j].value(i), u[i], v);
+            }
             v = ad_lane_sum<L>(v);
             if (lane % L == j) d = v;
         }
-        if (mine < p.rows[pi]) p.out[pi][orow + mine] = p.base[pi] ? base + d : d;
+        if (mine < p.rows[pi]) p.out[pi][orow + mine] = !p.base[pi] ? d : rank ? base + d : base;
     }
 };
 // base (zeros without one) to the columns of a token without an adapter: those of a workgroup of `threads` from col on, `sets` times.
@@ -613,24 +695,24 @@ __device__ __forceinline__ void adapter_one_body(const AdapterArgs& p, float* ld
     int block = blockIdx.x;
     const int pi = ad_projection(p, block, 1024);
     const u32 id = p.ids[tok];
-    const int rank = id >= (u32)p.n_adapter ? 0 : ad_rank(p, id);   // uniform
     const size_t orow = (size_t)tok * p.rows[pi];
-    if (rank == 0) return ad_copy(p, pi, orow, block * 1024 + (int)threadIdx.x, 1024, 1);
+    if (id >= (u32)p.n_adapter) return ad_copy(p, pi, orow, block * 1024 + (int)threadIdx.x, 1024, 1);   // uniform
+    const int rank = ad_rank(p, id);
     const int col = block * 1024 + wave * 64;
     const bool here = col < p.rows[pi];
     AdColumns<T, L> c;
-    if (here) c.load(p, pi, id, rank, orow, col, AHEAD, true);
+    if (here) c.load(p, pi, id, orow, col, AHEAD, true);
     // wavefront = (piece of K modulo pieces, rows modulo 16 / pieces)
     const int np = (p.k + 255) / 256, pieces = np > 8 ? 16 : np > 4 ? 8 : np > 2 ? 4 : np;   // a power of two
     const int piece = wave & (pieces - 1), step = 16 / pieces;
-    for (int r = wave / pieces; r < rank; r += RB * step) {
+    for (int r = wave / pieces; r < p.rank; r += RB * step) {
         float sum[RB];
-        ad_rows<T, RB>(p, pi, id, rank, (size_t)tok * p.k, r, step, piece, pieces, sum);
+        ad_rows<T, RB>(p, pi, id, p.rank, (size_t)tok * p.k, r, step, piece, pieces, sum);
         ad_wave_rows<RB>(sum);
 #pragma unroll
         for (int i = 0; i < RB / 4; i++) {
             const int row = r + (4 * i + lane) * step;
-            if (lane < 4 && row < rank) part[piece * R + row] = sum[i];
+            if (lane < 4 && row < p.rank) part[piece * R + row] = sum[i];
         }
     }
     __syncthreads();
@@ -647,8 +729,8 @@ __device__ __forceinline__ void adapter_one_body(const AdapterArgs& p, float* ld
     float u[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) u[i] = us[8 * (lane % L) + i];
-    if (!AHEAD) c.load(p, pi, id, rank, orow, col, true, false);
-    c.finish(p, pi, orow, col, u);
+    if (!AHEAD) c.load(p, pi, id, orow, col, true, false);
+    c.finish(p, pi, orow, col, rank, u);
 }
 
 // Two launches.  Sums of A x of a token: grid = (slices of 1024 elements of K modulo p.slices, ntok, projections * ceil(rank / 16)), block = 256, a
@@ -657,10 +739,11 @@ template <int T> __device__ __forceinline__ void adapter_dots_body(const Adapter
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tok = blockIdx.y, ctiles = p.rank_pad / 16;
     const int pi = blockIdx.z / ctiles, r = blockIdx.z % ctiles * 16;
     const u32 id = p.ids[tok];
-    const int rank = id >= (u32)p.n_adapter ? 0 : ad_rank(p, id);   // uniform
-    if (r >= rank) return;   // (adapter_cols reads no u from the rank on)
+    if (id >= (u32)p.n_adapter) return;
+    // (the first tile does not wait for the adapter's own rank: adapter_cols uses no u from there on)
+    if (r && r >= ad_rank(p, id)) return;   // uniform
     float sum[16];
-    ad_rows<T, 16>(p, pi, id, rank, (size_t)tok * p.k, r, 1, (int)blockIdx.x * 4 + wave, p.slices * 4, sum);
+    ad_rows<T, 16>(p, pi, id, p.rank, (size_t)tok * p.k, r, 1, (int)blockIdx.x * 4 + wave, p.slices * 4, sum);
     ad_wave_rows<16>(sum);
     if (lane < 4)
 #pragma unroll
@@ -683,12 +766,12 @@ template <int T, int L> __device__ __forceinline__ void adapter_cols_body(const 
         for (int s = 0; s < 16; s++) v[s] = s < p.slices ? at[(size_t)s * p.ntok * ncol] : 0.f;
     }
     const u32 id = p.ids[tok];
-    const int rank = id >= (u32)p.n_adapter ? 0 : ad_rank(p, id);   // uniform
     const size_t orow = (size_t)tok * p.rows[pi];
-    if (rank == 0) return ad_copy(p, pi, orow, block * 256 * p.up_sets + (int)threadIdx.x, 256, p.up_sets);
+    if (id >= (u32)p.n_adapter) return ad_copy(p, pi, orow, block * 256 * p.up_sets + (int)threadIdx.x, 256, p.up_sets);   // uniform
+    const int rank = ad_rank(p, id);
     int col = block * 256 * p.up_sets + wave * 64;
     AdColumns<T, L> c;
-    if (col < p.rows[pi]) c.load(p, pi, id, rank, orow, col, true, true);
+    if (col < p.rows[pi]) c.load(p, pi, id, orow, col, true, true);
     if (threadIdx.x < 8 * L) {
         float t = 0.f;
         if ((int)threadIdx.x < rank) {
@@ -703,7 +786,7 @@ template <int T, int L> __device__ __forceinline__ void adapter_cols_body(const 
 #pragma unroll
     for (int i = 0; i < 8; i++) u[i] = us[8 * (lane % L) + i];
     for (int s = 0; s < p.up_sets && col < p.rows[pi]; s++, col += 256) {
-        if (s) c.load(p, pi, id, rank, orow, col, true, true);
-        c.finish(p, pi, orow, col, u);
+        if (s) c.load(p, pi, id, orow, col, true, true);
+        c.finish(p, pi, orow, col, rank, u);
     }
 }

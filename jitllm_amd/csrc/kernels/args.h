@@ -619,6 +619,9 @@ struct AdapterArgs {
     const void* x;                         // [ntok][k]
     float* part;                           // workspace: sums over a slice of K each, [slices][ntok][n * rank_pad]
     uint16_t* u;                           // workspace: u as three bf16 pieces, [ntok][n][K steps of 32][3][32]
+    uint32_t* perm;                        // workspace: tokens by adapter [ntok]
+    uint32_t* tiles;                       // workspace: adapter, first place in perm, tokens, 0 [max_tiles][4]
+    int max_tiles;
     int n, n_adapter, rank, k, ntok;
     int rank_pad;                          // rank rounded up to sixteen
     int x_type;                            // (the dot products)

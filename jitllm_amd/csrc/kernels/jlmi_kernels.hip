@@ -688,7 +688,9 @@ JL_NORM_ROWS(l16_1, 16, 1, false, 256) JL_NORM_ROWS(l32_1, 32, 1, false, 256) JL
 JL_NORM_ROWS(l64_2, 64, 2, false, 256) JL_NORM_ROWS(l64_4, 64, 4, false, 256)
 JL_NORM_ROWS(wg_1, 64, 1, true, 1024) JL_NORM_ROWS(wg_2, 64, 2, true, 1024) JL_NORM_ROWS(wg_4, 64, 4, true, 1024)
 JL_NORM_ROWS(wg_8, 64, 8, true, 1024) JL_NORM_ROWS(wg_16, 64, 16, true, 1024)
-// grid = (group slots, ntok / 64, passes * slices), block = 256
+// grid = 1, block = 1024, LDS = (n_adapter + 33) words
+extern "C" __global__ __launch_bounds__(1024) void jl_adapter_group(AdapterArgs p) { adapter_group_body(p, (u32*)jl_smem); }
+// grid = (tiles, 1, passes * slices), block = 256
 #define JL_ADAPTER_DOWN(T, TYPE, XT, XTYPE, NT)                                                                              \
     extern "C" __global__ __launch_bounds__(256) void jl_adapter_down_##T##_##XT##_n##NT(AdapterArgs p) {                    \
         __shared__ __attribute__((aligned(16))) uint16_t sx[AdType<XTYPE>::pieces * 64 * JL_AD_DOWN_ROW];                    \
@@ -712,7 +714,7 @@ extern "C" __global__ __launch_bounds__(256) void jl_adapter_sum(AdapterArgs p) 
         __shared__ float s[64];                                                                                              \
         adapter_dots_body<TYPE>(p, s);                                                                                       \
     }
-// grid = (column blocks, group slots, ntok / 64), block = 256
+// grid = (column blocks, tiles), block = 256
 #define JL_ADAPTER_UP_V(T, TYPE, NAME, KS, MANY, VEC)                                                                        \
     extern "C" __global__ __launch_bounds__(256) void jl_adapter_up_##T##_##NAME(AdapterArgs p) {                            \
         __shared__ u32x4 frag[4 * KS * 3 * 64];                                                                              \

@@ -121,6 +121,7 @@ ADAPT = dict(outs=[P], bases=[P], rows=[40], a=[P], b=[P], t=quant.F16, n_adapte
     (dict(x_type=quant.MXFP4), False),
     (dict(k=48), False),
     (dict(rank=513), False),
+    (dict(n_adapter=8193), False),
     (dict(a=[P + 8]), False),
     (dict(x=P + 4), False),
     (dict(outs=[P + 2]), False),
