@@ -37,7 +37,7 @@ struct Tuning {
     int xpre = 0;               // decode matvec: 1 / 2 / 4 float4 groups of x a thread loads ahead of its weights
     int q8pair = 0;             // Q8_0 rows: 2 keeps one block a lane-slot (2-byte-aligned loads)
     int packed_rw = 0, packed_block = 0, moe_group = 0, moe_logits = 0;
-    int adapter_form = 0, adapter_slices = 0, adapter_sets = 0;
+    int moe_select = 0, adapter_form = 0, adapter_slices = 0, adapter_sets = 0;
     int moe_shares = 0;
     int gemm_rows = 0;
     int gemm_form = 0;
@@ -2237,13 +2237,14 @@ int jl_ctx_create(jl_ctx** out, const jl_options* opts) {
     names.push_back("jl_few_prep");
     for (const char* form : {"l16_1", "l32_1", "l64_1", "l64_2", "l64_4", "wg_1", "wg_2", "wg_4", "wg_8", "wg_16"})
         for (const char* any : {"", "_any"}) names.push_back(std::string("jl_norm_rows_") + form + any);
-    for (const char* g : {"g2", "g4", "g8", "g16"}) names.push_back(std::string("jl_moe_select_") + g);
+    for (const char* g : {"g1", "g2", "g3", "g4", "g3p", "g4p", "g6p", "g8p", "g12p", "g16p"}) names.push_back(std::string("jl_moe_select_") + g);
     names.push_back("jl_adapter_sum");
     names.push_back("jl_adapter_group");
     for (const char* t : {"f32", "f16", "bf16"}) {
         for (const char* xt : {"f32", "f16", "bf16"})
             for (const char* nt : {"_n1", "_n2"}) names.push_back(std::string("jl_adapter_down_") + t + "_" + xt + nt);
-        for (const char* l : {"_l1", "_l2", "_l4", "_l8"}) for (const char* form : {"one_", "cols_"}) names.push_back(std::string("jl_adapter_") + form + t + l);
+        for (const char* l : {"_l1", "_l2", "_l4", "_l8"}) names.push_back(std::string("jl_adapter_cols_") + t + l);
+        for (const char* l : {"_l1", "_l2"}) names.push_back(std::string("jl_adapter_one_") + t + l);
         names.push_back(std::string("jl_adapter_dots_") + t);
         for (const char* form : {"_k1", "_k1_any", "_k2", "_k2_any", "_many", "_many_any"}) names.push_back(std::string("jl_adapter_up_") + t + form);
     }
@@ -2416,6 +2417,7 @@ int jl_set_tuning(jl_ctx* c, const char* key, int value) {
     else if (!strcmp(key, "matvec.grid")) c->tune.grid = value;
     else if (!strcmp(key, "packed.rw")) c->tune.packed_rw = value;
     else if (!strcmp(key, "packed.block")) c->tune.packed_block = value;
+    else if (!strcmp(key, "moe.select")) c->tune.moe_select = value;
     else if (!strcmp(key, "adapter.form")) c->tune.adapter_form = value;
     else if (!strcmp(key, "adapter.slices")) c->tune.adapter_slices = value;
     else if (!strcmp(key, "adapter.sets")) c->tune.adapter_sets = value;
@@ -2619,11 +2621,11 @@ int jl_adapter_group_dev(jl_ctx* c, const jl_adapter_group* g, void* stream) {
     const double dots_us = 6 + g->ntok * (0.61e-7 * wb * g->rank * nk + wide_d * (3.1e-6 + 3.4e-8 * wb * g->rank));
     const double mm_us = 17 + g->ntok * (1.7e-6 * g->k + 1.6e-6 * wide_d + 2.5e-9 * bytes) + std::max((g->ntok + 63) / 64, std::min(g->ntok, g->n_adapter)) * bytes / 3.7e6;
     const int form = c->tune.adapter_form ? c->tune.adapter_form : !dots ? 0 : g->rank <= 16 && sets <= c->num_cu ? 1 : dots_us <= mm_us ? 2 : 0;
-    if (dots && form == 1) {
+    if (dots && form == 1 && g->rank <= 16) {
         name << "jl_adapter_one_" << t << "_l" << l;
         return launch(c, name, blocks(1024), (unsigned)g->ntok, 1024, 0, st, params);
     }
-    if (dots && form == 2) {
+    if (dots && (form == 1 || form == 2)) {
         a.slices = std::min(16, (g->k + 1023) / 1024);
         int rc = adapter_ws_ensure(c, adapter_part_bytes((size_t)a.slices * g->ntok, g->n, g->rank));
         if (rc != JL_OK) return rc;
@@ -2987,9 +2989,21 @@ int jl_moe_select_dev(jl_ctx* c, const float* logits, int rows, int n_expert, co
     a.logits = logits; a.bias = plan->bias; a.sel = sel; a.wt = wt; a.n_expert = n_expert; a.k_used = plan->k_used; a.sel_stride = sel_stride;
     a.sigmoid = plan->score == JL_SCORE_SIGMOID; a.n_group = n_group; a.k_group = plan->k_group; a.group_top = plan->group_top;
     a.renorm = plan->renorm != 0; a.scale = plan->scale;
+    // experts a lane: the fewest of the forms there are (a lane's every expert costs its arithmetic and a place in its sorted list)
+    int ng = (n_expert + 63) / 64;
+    while (ng != 1 && ng != 2 && ng != 3 && ng != 4 && ng != 6 && ng != 8 && ng != 12 && ng != 16) ng++;
+    const int vw = ng % 4 == 0 ? 4 : ng % 2 == 0 ? 2 : 1;
+    a.wide = n_expert % vw == 0 && (((uintptr_t)logits | (uintptr_t)plan->bias) & (4 * vw - 1)) == 0;
+    a.rows = rows; a.inv_size = (1 << 20) / (n_expert / n_group) + 1;
+    a.waves = rows >= 4 * c->num_cu ? 4 : 1;   // (a row a workgroup while there are few: they then lie on as many CUs)
     void* params[] = {&a};
-    const char* name = n_expert <= 128 ? "jl_moe_select_g2" : n_expert <= 256 ? "jl_moe_select_g4" : n_expert <= 512 ? "jl_moe_select_g8" : "jl_moe_select_g16";
-    return launch(c, name, (unsigned)rows, 1, 64, 0, pick_stream(c, stream), params);
+    Name name;
+    // Packed keys or whole ones: a round over packed keys is shorter, whole keys have no last step through LDS.  us, packed / whole, top 8:
+    // 128 experts 3.5 / 3.1 (one row), 11.7 / 11.2 (16384); 256 3.5 / 3.5, 777 rows 4.6 / 4.1, 2048 5.2 / 4.7, 16384 14.7 / 16.3; 384 3.9 / 4.1,
+    // 2048 rows 5.9 / 5.6, 16384 18.9 / 21.7; 512 4.1 / 4.5, 22.0 / 25.8.
+    const bool packed = ng > 4 || (ng > 2 && (c->tune.moe_select ? c->tune.moe_select == 1 : rows >= 16 * c->num_cu));
+    name << "jl_moe_select_g" << ng << (packed ? "p" : "");
+    return launch(c, name, (unsigned)((rows + a.waves - 1) / a.waves), 1, 64u * a.waves, 0, pick_stream(c, stream), params);
 }
 
 int jl_moe_logits_dev(jl_ctx* c, float* logits, int wtype, const void* w, const float* x, int n_expert, int k,

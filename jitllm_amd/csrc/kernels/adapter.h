@@ -687,8 +687,7 @@ __device__ __forceinline__ void ad_copy(const AdapterArgs& p, int pi, size_t oro
 #define JL_AD_ONE_LDS(L) (17 * 8 * (L))
 template <int T, int L>
 __device__ __forceinline__ void adapter_one_body(const AdapterArgs& p, float* lds) {
-    constexpr int R = 8 * L, RB = R < 16 ? R : 16;   // rows of A asked for at a time
-    constexpr bool AHEAD = L * sizeof(AdType<T>) <= 64;   // B asked for ahead of A: while it fits the registers
+    constexpr int R = 8 * L, RB = R < 16 || T == JL_F32 ? 8 : 16;   // rows of A asked for at a time, as many as the registers hold beside B
     float* part = lds;
     float* us = lds + 16 * R;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tok = blockIdx.y;
@@ -701,7 +700,7 @@ __device__ __forceinline__ void adapter_one_body(const AdapterArgs& p, float* ld
     const int col = block * 1024 + wave * 64;
     const bool here = col < p.rows[pi];
     AdColumns<T, L> c;
-    if (here) c.load(p, pi, id, orow, col, AHEAD, true);
+    if (here) c.load(p, pi, id, orow, col, true, true);
     // wavefront = (piece of K modulo pieces, rows modulo 16 / pieces)
     const int np = (p.k + 255) / 256, pieces = np > 8 ? 16 : np > 4 ? 8 : np > 2 ? 4 : np;   // a power of two
     const int piece = wave & (pieces - 1), step = 16 / pieces;
@@ -729,7 +728,6 @@ __device__ __forceinline__ void adapter_one_body(const AdapterArgs& p, float* ld
     float u[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) u[i] = us[8 * (lane % L) + i];
-    if (!AHEAD) c.load(p, pi, id, orow, col, true, false);
     c.finish(p, pi, orow, col, rank, u);
 }
 

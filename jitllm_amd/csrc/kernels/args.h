@@ -602,6 +602,9 @@ struct MoeSelectArgs {
     float* wt;               // [rows][k_used]
     int n_expert, k_used, sel_stride, sigmoid;
     int n_group, k_group, group_top, renorm;
+    int rows, waves;         // wavefronts (rows) a workgroup
+    int wide;                // rows and bias keep 8- (16-) byte alignment
+    int inv_size;            // 2^20 / (experts a group) + 1: e / size = e * inv_size >> 20 for e < 1024
     float scale;
 };
 

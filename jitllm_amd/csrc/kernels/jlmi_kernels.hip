@@ -352,12 +352,17 @@ extern "C" __global__ __launch_bounds__(256, 2) void jl_gemm_q4k_w16(GemmW16Args
 extern "C" __global__ __launch_bounds__(64) void jl_moe_route(MoeRouteArgs p) { moe_route_body<16>(p); }
 extern "C" __global__ __launch_bounds__(64) void jl_moe_route_g2(MoeRouteArgs p) { moe_route_body<2>(p); }
 extern "C" __global__ __launch_bounds__(64) void jl_moe_route_g4(MoeRouteArgs p) { moe_route_body<4>(p); }
-#define JL_MOE_SELECT(NAME, NG)                                                             \
-    extern "C" __global__ __launch_bounds__(64) void jl_moe_select_##NAME(MoeSelectArgs p) { \
-        __shared__ i32 keys[64 * NG];                                                       \
-        moe_select_body<NG>(p, keys);                                                       \
+// grid = ceil(rows / p.waves), block = 64 p.waves (4 at most)
+#define JL_MOE_SELECT(NAME, NG, PACKED)                                                                \
+    extern "C" __global__ __launch_bounds__(256) void jl_moe_select_##NAME(MoeSelectArgs p) {         \
+        __shared__ __attribute__((aligned(16))) u32 keys[4][64 * NG];                                  \
+        __shared__ __attribute__((aligned(16))) float scores[4][PACKED ? 64 * NG : 1];                 \
+        const int wave = threadIdx.x >> 6;                                                             \
+        const size_t row = (size_t)blockIdx.x * p.waves + wave;                                        \
+        if (row < (size_t)p.rows) moe_select_body<NG, PACKED>(p, row, keys[wave], scores[wave]);       \
     }
-JL_MOE_SELECT(g2, 2) JL_MOE_SELECT(g4, 4) JL_MOE_SELECT(g8, 8) JL_MOE_SELECT(g16, 16)
+JL_MOE_SELECT(g1, 1, false) JL_MOE_SELECT(g2, 2, false) JL_MOE_SELECT(g3, 3, false) JL_MOE_SELECT(g4, 4, false)
+JL_MOE_SELECT(g3p, 3, true) JL_MOE_SELECT(g4p, 4, true) JL_MOE_SELECT(g6p, 6, true) JL_MOE_SELECT(g8p, 8, true) JL_MOE_SELECT(g12p, 12, true) JL_MOE_SELECT(g16p, 16, true)
 // grid = (token groups, 8 at most, experts, ceil(token groups / 8)), by_expert: (experts, token groups); block = 128; a group is
 // JL_LOGITS_TOK tokens
 extern "C" __global__ __launch_bounds__(128) void jl_moe_logits(MoeLogitsArgs p) {
@@ -698,12 +703,14 @@ extern "C" __global__ __launch_bounds__(1024) void jl_adapter_group(AdapterArgs 
         adapter_down_body<TYPE, XTYPE, NT>(p, sx, toks);                                                                     \
     }
 extern "C" __global__ __launch_bounds__(256) void jl_adapter_sum(AdapterArgs p) { adapter_sum_body(p); }
-// grid = (column blocks, ntok), block = 1024; _cols 256
+// grid = (column blocks, ntok), block = 1024; ranks up to 16
 #define JL_ADAPTER_ONE(T, TYPE, L)                                                                                           \
     extern "C" __global__ __launch_bounds__(1024) void jl_adapter_one_##T##_l##L(AdapterArgs p) {                            \
         __shared__ float s[JL_AD_ONE_LDS(L)];                                                                                \
         adapter_one_body<TYPE, L>(p, s);                                                                                     \
-    }                                                                                                                        \
+    }
+// grid = (column blocks, ntok), block = 256
+#define JL_ADAPTER_COLS(T, TYPE, L)                                                                                          \
     extern "C" __global__ __launch_bounds__(256) void jl_adapter_cols_##T##_l##L(AdapterArgs p) {                            \
         __shared__ float s[8 * L];                                                                                           \
         adapter_cols_body<TYPE, L>(p, s);                                                                                    \
@@ -726,6 +733,7 @@ extern "C" __global__ __launch_bounds__(256) void jl_adapter_sum(AdapterArgs p) 
 #define JL_ADAPTER_X(T, TYPE, XT, XTYPE) JL_ADAPTER_DOWN(T, TYPE, XT, XTYPE, 1) JL_ADAPTER_DOWN(T, TYPE, XT, XTYPE, 2)
 #define JL_ADAPTER(T, TYPE)                                                                                                  \
     JL_ADAPTER_X(T, TYPE, f32, JL_F32) JL_ADAPTER_X(T, TYPE, f16, JL_F16) JL_ADAPTER_X(T, TYPE, bf16, JL_BF16)               \
-    JL_ADAPTER_DOTS(T, TYPE) JL_ADAPTER_ONE(T, TYPE, 1) JL_ADAPTER_ONE(T, TYPE, 2) JL_ADAPTER_ONE(T, TYPE, 4) JL_ADAPTER_ONE(T, TYPE, 8) \
+    JL_ADAPTER_ONE(T, TYPE, 1) JL_ADAPTER_ONE(T, TYPE, 2) JL_ADAPTER_DOTS(T, TYPE)                                           \
+    JL_ADAPTER_COLS(T, TYPE, 1) JL_ADAPTER_COLS(T, TYPE, 2) JL_ADAPTER_COLS(T, TYPE, 4) JL_ADAPTER_COLS(T, TYPE, 8)          \
     JL_ADAPTER_UP(T, TYPE, k1, 1, false) JL_ADAPTER_UP(T, TYPE, k2, 2, false) JL_ADAPTER_UP(T, TYPE, many, 1, true)
 JL_ADAPTER(f32, JL_F32) JL_ADAPTER(f16, JL_F16) JL_ADAPTER(bf16, JL_BF16)

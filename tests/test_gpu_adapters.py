@@ -94,20 +94,40 @@ SHAPES = [(1, 32, [1], 1, 1), (1, 4096, [4096], 16, 3), (2, 64, [17], 3, 2), (3,
           (513, 256, [100], 257, 2), (40, 128, [96], 512, 3), (1000, 288, [144, 160], 24, 9)]
 
 
+@pytest.fixture(params=["chosen", "one", "dots", "matrix", "matrix+sum"])
+def form(dev, request):
+    """Every form of the call beside the one it chooses ("adapter.form"; one that has no kernel for a rank is not taken)."""
+    dev.set_tuning(adapter__form={"chosen": 0, "one": 1, "dots": 2, "matrix": 3, "matrix+sum": 4}[request.param])
+    yield
+    dev.set_tuning(adapter__form=0)
+
+
 @pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("ntok, k, rows, rank, n_adapter", SHAPES)
-def test_whole_numbers_are_exact(dev, ntok, k, rows, rank, n_adapter, t):
+def test_whole_numbers_are_exact(dev, form, ntok, k, rows, rank, n_adapter, t):
     c = Case(ntok + rank, ntok, k, rows, rank, n_adapter, t=t, whole=True)
     assert c.call(dev)
     dev.synchronize()
     c.check(exact=True)
 
 
+@pytest.mark.parametrize("slices", [1, 3, 16])
+@pytest.mark.parametrize("sets", [1, 2, 4])
+def test_cuts_of_the_work(dev, form, slices, sets):
+    dev.set_tuning(adapter__slices=slices, adapter__sets=sets)
+    for ntok, k, rows, rank in ((5, 1120, [700], 40), (130, 2080, [513, 1030], 12)):
+        c = Case(slices + sets, ntok, k, rows, rank, 3, whole=True, ranks=[rank, 3, 5])
+        assert c.call(dev)
+        dev.synchronize()
+        c.check(exact=True)
+    dev.set_tuning(adapter__slices=0, adapter__sets=0)
+
+
 @pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("xt", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("ntok, k, rows, rank, n_adapter", [(1, 4096, [2048], 16, 3), (9, 2880, [720, 100], 20, 2), (48, 1024, [1000], 64, 8), (200, 1536, [1031], 40, 3),
                                                             (700, 512, [512, 256], 64, 2)])
-def test_types(dev, ntok, k, rows, rank, n_adapter, xt, t):
+def test_types(dev, form, ntok, k, rows, rank, n_adapter, xt, t):
     c = Case(7 * ntok + k, ntok, k, rows, rank, n_adapter, t=t, xt=xt)
     assert c.call(dev)
     dev.synchronize()
@@ -116,7 +136,7 @@ def test_types(dev, ntok, k, rows, rank, n_adapter, xt, t):
 
 @pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("ntok", [1, 12, 90, 400])
-def test_ranks_of_their_own(dev, ntok, t):
+def test_ranks_of_their_own(dev, form, ntok, t):
     """Each adapter its rank, none among them, more than the bank's among them; what the banks hold past it is not used."""
     ranks = [0, 1, 5, 16, 23, 24, 1000, 7]
     c = Case(ntok, ntok, 320, [200, 72], 24, 8, t=t, ranks=ranks, whole=True)
@@ -135,7 +155,7 @@ def test_ranks_of_their_own(dev, ntok, t):
 
 
 @pytest.mark.parametrize("ntok", [3, 64, 500])
-def test_no_number_stays_with_its_tokens(dev, ntok):
+def test_no_number_stays_with_its_tokens(dev, form, ntok):
     """An adapter of NaN and infinity, and a token of NaN: no other token sees them."""
     c = Case(ntok, ntok, 256, [130], 16, 3, whole=True, ids=np.arange(ntok) % 4)
     for v in (c.d["a"][0], c.d["b"][0]):
@@ -155,7 +175,7 @@ def test_no_number_stays_with_its_tokens(dev, ntok):
 
 
 @pytest.mark.parametrize("ntok", [1, 20, 300])
-def test_in_place_without_base_and_without_scale(dev, ntok):
+def test_in_place_without_base_and_without_scale(dev, form, ntok):
     c = Case(ntok, ntok, 512, [192, 48], 16, 4, whole=True)
     assert c.call(dev, in_place=True)
     dev.synchronize()
@@ -168,7 +188,7 @@ def test_in_place_without_base_and_without_scale(dev, ntok):
 
 @pytest.mark.parametrize("order", ["one", "none", "sorted", "runs", "each its own", "past the last", "blocks"])
 @pytest.mark.parametrize("ntok", [6, 64, 380])
-def test_orders_of_the_tokens(dev, ntok, order):
+def test_orders_of_the_tokens(dev, form, ntok, order):
     na = ntok if order == "each its own" else 5
     rng = np.random.default_rng(ntok)
     ids = {"one": np.full(ntok, 3), "none": np.full(ntok, 0xFFFFFFFF), "sorted": np.sort(rng.integers(0, 6, ntok)),
@@ -181,7 +201,7 @@ def test_orders_of_the_tokens(dev, ntok, order):
     c.check(exact=True)
 
 
-def test_a_call_after_a_larger_one(dev):
+def test_a_call_after_a_larger_one(dev, form):
     """The workspace holds what an earlier call left: nothing of it is read."""
     for ntok, rank, na in ((600, 96, 3), (20, 8, 2), (3, 64, 1), (250, 33, 4)):
         c = Case(ntok, ntok, 256, [90, 130], rank, na, whole=True, ranks=None if rank != 33 else [0, 33, 4, 9])
@@ -190,8 +210,8 @@ def test_a_call_after_a_larger_one(dev):
         c.check(exact=True)
 
 
-@pytest.mark.parametrize("ntok, rank", [(1, 16), (24, 16), (24, 64), (300, 64)])
-def test_captured_and_replayed(dev, ntok, rank):
+@pytest.mark.parametrize("ntok, rank", [(1, 16), (24, 16), (24, 64), (300, 64), (5000, 16)])
+def test_captured_and_replayed(dev, form, ntok, rank):
     """Two graphs of one context, their calls replayed in turn between eager calls and after the workspace has grown."""
     st = Stream()
     dev.reserve_adapters(ntok, 2, rank)
@@ -228,7 +248,7 @@ def test_reserved_calls_allocate_nothing(dev):
     c.check(exact=True)
 
 
-def test_same_bits_every_time(dev):
+def test_same_bits_every_time(dev, form):
     for ntok in (5, 64, 400):
         c = Case(ntok, ntok, 1024, [300], 32, 3)
         assert c.call(dev)

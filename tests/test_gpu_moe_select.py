@@ -69,9 +69,17 @@ def check(dev, logits, k, **kw):
 SIZES = [1, 2, 3, 7, 16, 33, 64, 65, 100, 128, 129, 160, 255, 256, 257, 384, 512, 513, 777, 1000, 1024]
 
 
+@pytest.fixture(params=["chosen", "packed", "whole"])
+def form(dev, request):
+    """The kernel's two ways to select, beside the one it chooses ("moe.select")."""
+    dev.set_tuning(moe__select={"chosen": 0, "packed": 1, "whole": 2}[request.param])
+    yield
+    dev.set_tuning(moe__select=0)
+
+
 @pytest.mark.parametrize("score", [0, 1])
 @pytest.mark.parametrize("n", SIZES)
-def test_sizes(dev, n, score):
+def test_sizes(dev, form, n, score):
     rng = np.random.default_rng(n)
     for k in sorted({1, min(2, n), min(8, n), min(13, n), min(16, n)}):
         logits = rng.standard_normal((9, n)).astype(np.float32)
@@ -83,7 +91,7 @@ def test_sizes(dev, n, score):
 @pytest.mark.parametrize("top", [1, 2])
 @pytest.mark.parametrize("n, n_group, k_group, k", [(256, 8, 4, 8), (8, 8, 3, 3), (16, 8, 2, 4), (160, 8, 3, 6), (64, 64, 16, 16), (1024, 64, 5, 16), (384, 4, 1, 10),
                                                     (1000, 2, 1, 16), (63, 7, 7, 9), (66, 2, 1, 5), (1024, 2, 2, 8), (128, 16, 1, 8), (256, 4, 2, 8), (12, 3, 2, 8)])
-def test_groups(dev, n, n_group, k_group, k, top, score):
+def test_groups(dev, form, n, n_group, k_group, k, top, score):
     rng = np.random.default_rng(n + n_group + k)
     logits, bias = rng.standard_normal((17, n)).astype(np.float32), (0.2 * rng.standard_normal(n)).astype(np.float32)
     check(dev, logits, k, score=score, bias=bias, n_group=n_group, k_group=k_group, top=top, scale=1.5)
@@ -94,7 +102,7 @@ def test_groups(dev, n, n_group, k_group, k, top, score):
 
 @pytest.mark.parametrize("score", [0, 1])
 @pytest.mark.parametrize("n, groups", [(40, 1), (256, 8), (600, 1)])
-def test_ties_go_to_the_lowest_index(dev, n, groups, score):
+def test_ties_go_to_the_lowest_index(dev, form, n, groups, score):
     rng = np.random.default_rng(n)
     logits = rng.integers(-1, 2, (33, n)).astype(np.float32)
     kw = dict(score=score, n_group=groups, k_group=max(1, groups // 2), top=2 if groups > 1 else 1)
@@ -107,7 +115,7 @@ def test_ties_go_to_the_lowest_index(dev, n, groups, score):
     check(dev, np.full((4, n), -120.0, np.float32), 8, bias=bias, **kw)  # choices of either zero
 
 
-def test_masks(dev):
+def test_masks(dev, form):
     """Experts out of service by logit or bias, fewer than are wanted, none at all; the type's lowest value is a number."""
     n, k = 70, 8
     rng = np.random.default_rng(3)
@@ -132,6 +140,20 @@ def test_masks(dev):
         assert np.all(sel[r] == n) and np.all(wt[r] == 0)
     sel, wt = run(dev, logits, k, score=1)
     assert sel[6, 0] == 7 and wt[6, 0] > 0 and 9 not in sel[7] and np.all(wt[7] > 0)
+
+
+@pytest.mark.parametrize("n", [200, 384, 1024])
+def test_choices_that_share_their_high_bits(dev, form, n):
+    """Choices a few steps of f32 apart, in any order: packed keys (22 bits) cannot tell them, whole ones do.  A handful of them
+    among others, then more than the 64 that are put in order, the whole row."""
+    rng = np.random.default_rng(n)
+    for close in (2, 5, 30, 63, 64, 65, 100, n):
+        logits = (rng.standard_normal((6, n)) - 3).astype(np.float32)
+        for row in logits:
+            at = rng.permutation(n)[: min(close, n)]
+            row[at] = np.float32(1.0) + rng.integers(0, 40, len(at)).astype(np.float32) * np.float32(2.0 ** -23)
+        check(dev, logits, 8, score=1)
+        check(dev, logits, 16, score=0, bias=np.zeros(n, np.float32))
 
 
 def test_softmax_without_bias_is_the_router(dev):
