@@ -2571,7 +2571,7 @@ int jl_reserve_adapters(jl_ctx* c, int max_tok, int n, int max_rank) {
     if (max_tok <= 0 || n < 1 || n > JL_MAX_GROUP || max_rank <= 0) return fail(c, JL_ERR_ARG, "reserve adapters: %d tokens, %d projections, rank %d", max_tok, n, max_rank);
     if (max_rank > 512) return JL_DECLINED;
     HIP_TRY(c, H->SetDevice(c->device));
-    // slices * tokens: sixteen slices at most, more than one while slices * tokens / 64 is within two workgroups a CU
+    // slices * tokens: sixteen slices at most, more than one while slices * tokens / 64 is within two workgroups a CU (both forms' bound)
     const size_t rows = std::max((size_t)max_tok, std::min((size_t)16 * max_tok, (size_t)128 * c->num_cu));
     return adapter_ws_ensure(c, adapter_part_bytes(rows, n, max_rank) + adapter_u_bytes(max_tok, n, max_rank) + adapter_list_bytes(max_tok, kMaxAdapters));
 }
@@ -2626,7 +2626,8 @@ int jl_adapter_group_dev(jl_ctx* c, const jl_adapter_group* g, void* stream) {
         return launch(c, name, blocks(1024), (unsigned)g->ntok, 1024, 0, st, params);
     }
     if (dots && (form == 1 || form == 2)) {
-        a.slices = std::min(16, (g->k + 1023) / 1024);
+        // (slices * tokens as far as jl_reserve_adapters has room for them: a workgroup goes on to the next slice where there are fewer)
+        a.slices = std::max(1, std::min({16, (g->k + 1023) / 1024, 128 * c->num_cu / g->ntok}));
         int rc = adapter_ws_ensure(c, adapter_part_bytes((size_t)a.slices * g->ntok, g->n, g->rank));
         if (rc != JL_OK) return rc;
         a.part = (float*)c->adapter_ws;

@@ -248,6 +248,26 @@ def test_reserved_calls_allocate_nothing(dev):
     c.check(exact=True)
 
 
+@pytest.mark.parametrize("which", [2, 3])
+def test_a_reservation_covers_every_cut_of_the_work(dev, which):
+    """3000 tokens of sixteen slices each would be more sums than are reserved for 3000 tokens."""
+    from jitllm_amd.device import Device
+    c = Case(6, 3000, 16384, [64], 64, 2, t="bf16", xt="bf16", whole=True)
+    own = Device(0)
+    try:
+        own.set_tuning(adapter__form=which)
+        own.reserve_adapters(3000, 1, 64)
+        assert Case(7, 3, 64, [8], 4, 1).call(own)
+        own.synchronize()
+        before = mem_info()[0]
+        assert c.call(own)
+        own.synchronize()
+        assert mem_info()[0] == before
+        c.check(exact=True)
+    finally:
+        own.close()
+
+
 def test_same_bits_every_time(dev, form):
     for ntok in (5, 64, 400):
         c = Case(ntok, ntok, 1024, [300], 32, 3)
