@@ -2548,6 +2548,7 @@ namespace {
 constexpr int kMaxAdapters = 8192;   // counters of the grouping in LDS
 // How the matrix-core form is cut: a tile is up to 64 tokens of one adapter; a workgroup of adapter_down takes a tile, 4 nt tiles of sixteen rows of A
 // and a slice of K.  Slices for two workgroups a CU, as far as the tiles are known: there is one for 64 tokens at least, and one for every adapter met.
+// (us by 1 / 2 / 4 / 8 / 16 slices, 8 adapters, k = 4096: 256 tokens rank 16 beside 4096 98 / 59 / 39 / 30 / 25, 2048 tokens rank 64 131 / 83 / 60 / 51 / 50.)
 struct AdapterPlan { int rank_pad, nt, passes, slices, max_tiles; };
 AdapterPlan adapter_plan(const jl_ctx* c, int ntok, int n, int rank, int k, int n_adapter) {
     AdapterPlan a;
@@ -2620,7 +2621,11 @@ int jl_adapter_group_dev(jl_ctx* c, const jl_adapter_group* g, void* stream) {
     const double wide_d = (double)wide, nk = (double)g->n * g->k, bytes = g->rank * (nk + wide_d) * wb;
     const double dots_us = 6 + g->ntok * (0.61e-7 * wb * g->rank * nk + wide_d * (3.1e-6 + 3.4e-8 * wb * g->rank));
     const double mm_us = 17 + g->ntok * (1.7e-6 * g->k + 1.6e-6 * wide_d + 2.5e-9 * bytes) + std::max((g->ntok + 63) / 64, std::min(g->ntok, g->n_adapter)) * bytes / 3.7e6;
-    const int form = c->tune.adapter_form ? c->tune.adapter_form : !dots ? 0 : g->rank <= 16 && sets <= c->num_cu ? 1 : dots_us <= mm_us ? 2 : 0;
+    // One launch or two of dot products: every column block makes u anew, which is little while tokens and ranks are few.  us, one / two, beside 4096
+    // rows: rank 8, 1 token 4.6 / 6.5, 64 (as many workgroups as CUs) 5.2 / 7.0, 64 of q, k and v (half as many again) 8.0 / 8.9; rank 16, 1 token
+    // 6.1 / 6.8, 16 (a quarter) 6.5 / 6.8, 16 of q, k and v 7.3 / 7.2, 64 8.0 / 7.3.
+    const bool once = g->rank <= 16 && sets <= (g->rank <= 8 ? 3l * c->num_cu / 2 : c->num_cu / 4);
+    const int form = c->tune.adapter_form ? c->tune.adapter_form : !dots ? 0 : once ? 1 : dots_us <= mm_us ? 2 : 0;
     if (dots && form == 1 && g->rank <= 16) {
         name << "jl_adapter_one_" << t << "_l" << l;
         return launch(c, name, blocks(1024), (unsigned)g->ntok, 1024, 0, st, params);
@@ -2655,8 +2660,11 @@ int jl_adapter_group_dev(jl_ctx* c, const jl_adapter_group* g, void* stream) {
     name << "jl_adapter_down_" << t << "_" << xt << "_n" << pl.nt;
     rc = launch(c, name, (unsigned)a.max_tiles, 1, 256, 0, st, params, (unsigned)(a.passes * a.slices));
     if (rc != JL_OK) return rc;
-    const double added = (double)blocks(256) * g->ntok * a.slices * g->rank * 4;   // bytes that adapter_up would add up
-    if (form == 4 || (form != 3 && added > 30e6)) {
+    // The slices added up first, a launch of its own, or by every column block: bytes that adapter_up would read for it.  us, by adapter_up / first
+    // (bytes): 512 tokens rank 16 beside 4096 26.4 / 26.7 (8 MB), 1024 30.1 / 29.7 (17), 256 rank 64 32.7 / 27.9 (17), 256 rank 16 beside 2 x 14336
+    // 32.8 / 31.1 (29), 512 rank 64 beside 4096 35.2 / 30.3 (34), 2048 rank 64 beside 2 x 14336 187 / 150 (940).
+    const double added = (double)blocks(256) * g->ntok * a.slices * g->rank * 4;
+    if (form == 4 || (form != 3 && added > 12e6)) {
         const size_t quads = (size_t)g->ntok * g->n * ((a.rank_pad + 31) / 32) * 8;
         rc = launch(c, "jl_adapter_sum", (unsigned)((quads + 255) / 256), 1, 256, 0, st, params);
         if (rc != JL_OK) return rc;
@@ -2664,8 +2672,7 @@ int jl_adapter_group_dev(jl_ctx* c, const jl_adapter_group* g, void* stream) {
     }
     Name up;
     up << "jl_adapter_up_" << t << (g->rank <= 32 ? "_k1" : g->rank <= 64 ? "_k2" : "_many") << (vec ? "" : "_any");
-    a.up_sets = c->tune.adapter_sets ? c->tune.adapter_sets : (long)blocks(256) * (g->ntok / 64) >= 6 * c->num_cu ? 2 : 1;
-    return launch(c, up, blocks(256 * a.up_sets), (unsigned)a.max_tiles, 256, 0, st, params);
+    return launch(c, up, blocks(256), (unsigned)a.max_tiles, 256, 0, st, params);
 }
 
 int jl_dequant_dev(jl_ctx* c, int type, const void* src, float* dst, size_t n, void* stream) {

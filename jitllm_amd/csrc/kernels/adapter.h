@@ -410,8 +410,8 @@ __device__ __forceinline__ int ad_projection(const AdapterArgs& p, int& block, i
     return i;
 }
 
-// grid = (column blocks of all projections, tiles), block = 256, a wavefront 64 columns (rows of B) a set of
-// 256, p.up_sets sets.  u's fragments of the tile's (up to four) sixteens lie in LDS, KS K steps of 32 at a time; B's stay in registers and meet
+// grid = (blocks of 256 columns of all projections, tiles), block = 256, a wavefront 64 columns (rows of B; two such sets a workgroup
+// were slower everywhere: 2048 tokens rank 64 beside 2 x 14336 149.8 against 143.8 us, beside 4096 57 against 50).  u's fragments of the tile's (up to four) sixteens lie in LDS, KS K steps of 32 at a time; B's stay in registers and meet
 // one after the other.  A tile's sums change places in LDS and meet base by rows of 256 bytes, asked for a tile ahead.
 // KS = 1: ranks up to 32, 2: up to 64.  MANY: any rank, KS steps at a time; the four tiles' sums stay in registers and base is read at the end.
 // VEC: rows of out and base on 16-byte boundaries.
@@ -422,7 +422,7 @@ __device__ __forceinline__ void adapter_up_body(const AdapterArgs& p, u32x4* fra
     constexpr int PW = AdType<T>::pieces;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int block = blockIdx.x;
-    const int pi = ad_projection(p, block, 256 * p.up_sets);
+    const int pi = ad_projection(p, block, 256);
     const int rows = p.rows[pi], ksteps = (p.rank_pad + 31) / 32;
     const float* base = p.base[pi];
     float* out = p.out[pi];
@@ -520,57 +520,53 @@ __device__ __forceinline__ void adapter_up_body(const AdapterArgs& p, u32x4* fra
                 for (int c = 0; c < 4; c++) acc[c] = ad_mfma<PW, 3>(wq[s][c], uq, acc[c]);
             }
         };
-        int col = block * 256 * p.up_sets + wave * 64;
+        const int col = block * 256 + wave * 64;
         if constexpr (!MANY) {
             if (col < rows) load_base(0, col);
             if (!none) stage(0);
             __syncthreads();
-            for (int set = 0; set < p.up_sets && col < rows; set++, col += 256) {
-                u32x4 wq[KS][4][PW];
-                if (!none) load_b(0, col, wq);
-                for (int tt = 0; tt < nt; tt++) {
-                    f32x4 acc[4], b0[4];
-                    size_t o0[4];
+            if (col >= rows) return;
+            u32x4 wq[KS][4][PW];
+            if (!none) load_b(0, col, wq);
+            for (int tt = 0; tt < nt; tt++) {
+                f32x4 acc[4], b0[4];
+                size_t o0[4];
 #pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
-                        b0[c] = bs[c];
-                        o0[c] = oat[c];
-                    }
-                    if (tt + 1 < nt) load_base(tt + 1, col);
-                    else if (set + 1 < p.up_sets && col + 256 < rows) load_base(0, col + 256);
-                    if (!none) multiply(tt, wq, acc);
-                    finish(tt, col, acc, b0, o0);
+                for (int c = 0; c < 4; c++) {
+                    acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    b0[c] = bs[c];
+                    o0[c] = oat[c];
                 }
+                if (tt + 1 < nt) load_base(tt + 1, col);
+                if (!none) multiply(tt, wq, acc);
+                finish(tt, col, acc, b0, o0);
             }
-        } else {
-            for (int set = 0; set < p.up_sets; set++, col += 256) {   // (every wavefront takes part in the staging)
-                f32x4 acc[4][4];
+        } else {   // (every wavefront takes part in the staging)
+            f32x4 acc[4][4];
+#pragma unroll
+            for (int tt = 0; tt < 4; tt++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) acc[tt][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (!none)
+                for (int s0 = 0; 32 * s0 < rank; s0 += KS) {
+                    stage(s0);
+                    __syncthreads();
+                    if (col < rows) {
+                        u32x4 wq[KS][4][PW];
+                        load_b(s0, col, wq);
+#pragma unroll
+                        for (int tt = 0; tt < 4; tt++)
+                            if (tt < nt) multiply(tt, wq, acc[tt]);
+                    }
+                    __syncthreads();
+                }
+            if (col < rows) {
 #pragma unroll
                 for (int tt = 0; tt < 4; tt++)
-#pragma unroll
-                    for (int c = 0; c < 4; c++) acc[tt][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-                if (!none)
-                    for (int s0 = 0; 32 * s0 < rank; s0 += KS) {
-                        stage(s0);
-                        __syncthreads();
-                        if (col < rows) {
-                            u32x4 wq[KS][4][PW];
-                            load_b(s0, col, wq);
-#pragma unroll
-                            for (int tt = 0; tt < 4; tt++)
-                                if (tt < nt) multiply(tt, wq, acc[tt]);
-                        }
-                        __syncthreads();
+                    if (tt < nt) {
+                        load_base(tt, col);
+                        finish(tt, col, acc[tt], bs, oat);
                     }
-                if (col < rows) {
-#pragma unroll
-                    for (int tt = 0; tt < 4; tt++)
-                        if (tt < nt) {
-                            load_base(tt, col);
-                            finish(tt, col, acc[tt], bs, oat);
-                        }
-                }
             }
         }
     }
@@ -681,7 +677,7 @@ __device__ __forceinline__ void ad_copy(const AdapterArgs& p, int pi, size_t oro
 
 // One launch: a workgroup makes u of one token for one projection -- its sixteen wavefronts cut K (and the rows of A where K is short) among
 // them -- and then a block of 1024 columns of out.  Every column block makes u anew: A and x come from L2 then, which costs less than a second
-// launch while the rank is small (4096 x 4096, one token: rank 8 4.9 us, 16 6.5, 32 10.3; the two launches below 7 to 8).  What counts here is the
+// launch while the rank is small (4096 x 4096, one token: rank 8 4.6 us, 16 6.1; the two launches below 6.5 and 6.8).  What counts here is the
 // number of trips to memory one after the other: the adapter's id, then base, B, A and x together, then out.
 // grid = (column blocks of all projections, ntok), block = 1024.  LDS: part [16][8 L] and u [8 L] floats.
 #define JL_AD_ONE_LDS(L) (17 * 8 * (L))

@@ -629,5 +629,5 @@ struct AdapterArgs {
     int rank_pad;                          // rank rounded up to sixteen
     int x_type;                            // (the dot products)
     int passes, slices;                    // of adapter_down; slices 0 in adapter_up: u has been made
-    int up_sets;                           // sets of 256 columns a workgroup
+    int up_sets;                           // sets of 256 columns a workgroup of adapter_cols
 };
