@@ -21,22 +21,33 @@
 
 typedef __bf16 ad_bf16x8 __attribute__((ext_vector_type(8)));
 struct __attribute__((packed, aligned(2))) ad_u32x4_a2 { u32x4 v; };
+struct __attribute__((packed, aligned(2))) ad_u32x2_a2 { u32x2 v; };
+struct __attribute__((packed, aligned(2))) ad_u32_a2 { u32 v; };
 struct __attribute__((packed, aligned(4))) ad_f32x4_a4 { f32x4 v; };
+struct __attribute__((packed, aligned(4))) ad_u32x2_a4 { u32x2 v; };
 
 template <int T> struct AdType {   // 16-bit: a fragment's eight values as they lie
     static constexpr int pieces = T == JL_F16 ? 2 : 1;
     u32x4 w;
     __device__ __forceinline__ void load(const void* p, size_t at) { w = ((const ad_u32x4_a2*)((const uint16_t*)p + at))->v; }
-    // the first `left` of the eight (the others are not touched and read 0)
+    // The first `left` of the eight: a four, a two and a one of them, as far as they are there.  place() puts them where they belong, zeros behind them;
+    // it is apart from the loads so that nothing waits for one of them before all are on their way.
     __device__ __forceinline__ void load_some(const void* p, size_t at, int left) {
         if (left >= 8) return load(p, at);
+        const uint16_t* h = (const uint16_t*)p + at;
         w = u32x4{0, 0, 0, 0};
-        for (int i = 0; i < left; i++) {
-            const u32 h = ((const uint16_t*)p)[at + i];
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (i / 2 == j) w[j] |= h << (16 * (i & 1));
+        if (left & 4) {
+            const u32x2 four = ((const ad_u32x2_a2*)h)->v;
+            w[0] = four.x;
+            w[1] = four.y;
         }
+        if (left & 2) w[2] = ((const ad_u32_a2*)(h + (left & 4)))->v;
+        if (left & 1) w[3] = h[left & 6];
+    }
+    __device__ __forceinline__ void place(int left) {
+        if (left >= 8) return;
+        const u32 hi = left & 4 ? ~0u : 0u, next = left & 2 ? ~0u : 0u, a = w[2] | (w[3] & ~next), b = w[3] & next;   // (bits: no index into registers)
+        w = u32x4{w[0] | (a & ~hi), w[1] | (b & ~hi), a & hi, b & hi};
     }
     __device__ __forceinline__ float value(int i) const {
         const uint16_t h = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
@@ -52,8 +63,25 @@ template <> struct AdType<JL_F32> {
     }
     __device__ __forceinline__ void load_some(const void* p, size_t at, int left) {
         if (left >= 8) return load(p, at);
+        const float* f = (const float*)p + at;
+        w[0] = w[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (left & 4) w[0] = ((const ad_f32x4_a4*)f)->v;
+        if (left & 2) {
+            const u32x2 two = ((const ad_u32x2_a4*)(f + (left & 4)))->v;
+            w[1][0] = __uint_as_float(two.x);
+            w[1][1] = __uint_as_float(two.y);
+        }
+        if (left & 1) w[1][2] = f[left & 6];
+    }
+    __device__ __forceinline__ void place(int left) {
+        if (left >= 8) return;
+        const u32 hi = left & 4 ? ~0u : 0u, next = left & 2 ? ~0u : 0u, one = __float_as_uint(w[1][2]);
+        const u32 r[3] = {__float_as_uint(w[1][0]) | (one & ~next), __float_as_uint(w[1][1]), one & next};
 #pragma unroll
-        for (int i = 0; i < 8; i++) w[i / 4][i & 3] = i < left ? ((const float*)p)[at + i] : 0.f;
+        for (int i = 0; i < 3; i++) {
+            w[0][i] = __uint_as_float(__float_as_uint(w[0][i]) | (r[i] & ~hi));
+            w[1][i] = __uint_as_float(r[i] & hi);
+        }
     }
     __device__ __forceinline__ float value(int i) const { return w[i / 4][i & 3]; }
 };
@@ -398,7 +426,7 @@ __device__ __forceinline__ void adapter_sum_body(const AdapterArgs& p) {
 // A fragment of B: eight columns of row `col` of the adapter's sheet from r on, zeros from its rank on.
 template <int T>
 __device__ __forceinline__ void ad_load_b(AdType<T>& w, const AdapterArgs& p, int pi, u32 a, int col, int r, int rank) {
-    w.load_some(p.b[pi], ((size_t)a * p.rows[pi] + col) * p.rank + min(r, rank), min(max(rank - r, 0), 8));
+    w.load_some(p.b[pi], ((size_t)a * p.rows[pi] + col) * p.rank + min(r, rank), min(max(rank - r, 0), 8));   // (place() it)
 }
 // The projection of a column block and the block's number in it; width: columns a block.
 __device__ __forceinline__ int ad_projection(const AdapterArgs& p, int& block, int width) {
@@ -501,13 +529,17 @@ __device__ __forceinline__ void adapter_up_body(const AdapterArgs& p, u32x4* fra
             }
         };
         auto load_b = [&](int s0, int col, u32x4 (&wq)[KS][4][PW]) {
+            AdType<T> w[KS][4];
+#pragma unroll
+            for (int s = 0; s < KS; s++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) ad_load_b<T>(w[s][c], p, pi, a, min(col + 16 * c + (lane & 15), rows - 1), 32 * (s0 + s) + 8 * (lane >> 4), rank);
 #pragma unroll
             for (int s = 0; s < KS; s++)
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
-                    AdType<T> w;
-                    ad_load_b<T>(w, p, pi, a, min(col + 16 * c + (lane & 15), rows - 1), 32 * (s0 + s) + 8 * (lane >> 4), rank);
-                    ad_pieces<T>(w, wq[s][c]);
+                    w[s][c].place(max(rank - 32 * (s0 + s) - 8 * (lane >> 4), 0));
+                    ad_pieces<T>(w[s][c], wq[s][c]);
                 }
         };
         auto multiply = [&](int tt, const u32x4 (&wq)[KS][4][PW], f32x4 (&acc)[4]) {
@@ -629,34 +661,52 @@ template <int T, int RB> __device__ __forceinline__ void ad_rows(const AdapterAr
     }
 }
 // Columns of out.  L lanes a column: eight elements of a row of B each (rank <= 8 L); a wavefront's 64 columns are L loads of 64 / L rows, whole
-// lines, and lane l ends up with column l % L * (64 / L) + l / L.
+// lines, and lane l ends up with column l % L * (64 / L) + l / L.  A row's last eight elements start where they end with the row, also where the
+// lane before has the first of them: those meet zeros (ad_first says how many).
+template <int L> __device__ __forceinline__ int ad_first(int r0, int bank_rank) { return L == 1 ? 0 : max(r0 - (bank_rank - 8), 0); }   // (L > 1: rank > 8)
 template <int N> __device__ __forceinline__ float ad_lane_sum(float v) {   // over N consecutive lanes; each has it
     if (N >= 2) v += dpp_f32<JL_DPP_QUAD_XOR1, 0xf>(v);
     if (N >= 4) v += dpp_f32<JL_DPP_QUAD_XOR2, 0xf>(v);
     if (N >= 8) v += dpp_f32<JL_DPP_ROW_HALF_MIRROR, 0xf>(v);
     return v;
 }
+// A lane's eight of u, which lie in LDS.
+template <int L> __device__ __forceinline__ void ad_take_u(const AdapterArgs& p, const float* us, float (&u)[8]) {
+    const int r0 = 8 * ((threadIdx.x & 63) % L);
+    if (L == 1 || p.rank % 8 == 0) {   // uniform; 16-byte reads
+#pragma unroll
+        for (int i = 0; i < 8; i++) u[i] = us[r0 + i];
+    } else {
+        const int first = ad_first<L>(r0, p.rank);
+#pragma unroll
+        for (int i = 0; i < 8; i++) u[i] = i < first ? 0.f : us[r0 - first + i];
+    }
+}
 template <int T, int L> struct AdColumns {
     AdType<T> b[L];
     float base;
     // (B by the bank's rank: the adapter's own is known later)
     __device__ __forceinline__ void load(const AdapterArgs& p, int pi, u32 id, size_t orow, int col, bool with_b, bool with_base) {
-        const int lane = threadIdx.x & 63, rows = p.rows[pi], r0 = 8 * (lane % L), mine = col + lane % L * (64 / L) + lane / L;
+        const int lane = threadIdx.x & 63, rows = p.rows[pi], r0 = 8 * (lane % L), r = r0 - ad_first<L>(r0, p.rank), mine = col + lane % L * (64 / L) + lane / L;
         if (with_base) base = p.base[pi] && mine < rows ? p.base[pi][orow + mine] : 0.f;
         if (with_b)
 #pragma unroll
-            for (int j = 0; j < L; j++)
-                b[j].load_some(p.b[pi], ((size_t)id * rows + min(col + j * (64 / L) + lane / L, rows - 1)) * p.rank + min(r0, p.rank), min(max(p.rank - r0, 0), 8));
+            for (int j = 0; j < L; j++) {
+                const size_t at = ((size_t)id * rows + min(col + j * (64 / L) + lane / L, rows - 1)) * p.rank + r;
+                if (L > 1) b[j].load(p.b[pi], at);
+                else b[j].load_some(p.b[pi], at, p.rank);   // (uniform)
+            }
     }
     __device__ __forceinline__ void finish(const AdapterArgs& p, int pi, size_t orow, int col, int rank, const float (&u)[8]) {
-        const int lane = threadIdx.x & 63, mine = col + lane % L * (64 / L) + lane / L, left = rank - 8 * (lane % L);
+        const int lane = threadIdx.x & 63, r0 = 8 * (lane % L), first = ad_first<L>(r0, p.rank), mine = col + lane % L * (64 / L) + lane / L, left = rank - r0 + first;
         float d = 0.f;
 #pragma unroll
         for (int j = 0; j < L; j++) {
             float v = 0.f;
-            if (p.ranks) {   // columns of B from the adapter's rank on may hold anything
+            if (L == 1) b[j].place(p.rank);
+            if (p.ranks || (L > 1 && p.rank != 8 * L)) {   // columns of B from the adapter's rank on may hold anything
 #pragma unroll
-                for (int i = 0; i < 8; i++) v = __builtin_fmaf(i < left ? b[j].value(i) : 0.f, u[i], v);
+                for (int i = 0; i < 8; i++) v = __builtin_fmaf(i >= first && i < left ? b[j].value(i) : 0.f, u[i], v);
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; i++) v = __builtin_fmaf(b[j].value(i), u[i], v);
@@ -722,8 +772,7 @@ __device__ __forceinline__ void adapter_one_body(const AdapterArgs& p, float* ld
     __syncthreads();
     if (!here) return;
     float u[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) u[i] = us[8 * (lane % L) + i];
+    ad_take_u<L>(p, us, u);
     c.finish(p, pi, orow, col, rank, u);
 }
 
@@ -777,8 +826,7 @@ template <int T, int L> __device__ __forceinline__ void adapter_cols_body(const 
     }
     __syncthreads();
     float u[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) u[i] = us[8 * (lane % L) + i];
+    ad_take_u<L>(p, us, u);
     for (int s = 0; s < p.up_sets && col < p.rows[pi]; s++, col += 256) {
         if (s) c.load(p, pi, id, orow, col, true, true);
         c.finish(p, pi, orow, col, rank, u);

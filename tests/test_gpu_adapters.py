@@ -238,6 +238,23 @@ def test_captured_and_replayed(dev, form, ntok, rank):
     st.destroy()
 
 
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rank", [3, 8, 11, 16, 20, 24, 33, 61, 100])
+def test_an_infinity_stays_in_its_column(dev, form, rank, t):
+    """Wherever it stands in a row of B, also where rows are read in pieces that overlap; other columns and adapters are as without it."""
+    c = Case(rank, 6, 64, [70], rank, 2, t=t, whole=True, ids=[0, 1, 0, 2, 1, 0], scale=False)
+    h = c.d["b"][0].get()
+    cols = [0, 31, 69]
+    for i, col in enumerate(cols):
+        h[1, col, [0, rank // 2, rank - 1][i]] = stored(np.float32([np.inf]), t)[0]
+    c.d["b"][0].put(h)
+    assert c.call(dev)
+    dev.synchronize()
+    got, hit = c.d["out"][0].get()[:-1], np.zeros((6, 70), bool)
+    hit[np.ix_([1, 4], cols)] = True
+    assert np.all(~np.isfinite(got[hit])) and np.array_equal(got[~hit], c.want[0].astype(np.float32)[~hit])
+
+
 def test_reserved_calls_allocate_nothing(dev):
     dev.reserve_adapters(700, 3, 80)
     c = Case(5, 700, 128, [64, 64, 64], 80, 2, whole=True)
