@@ -2235,7 +2235,7 @@ int jl_ctx_create(jl_ctx** out, const jl_options* opts) {
     std::vector<std::string> names = {"jl_quantize_act", "jl_dequant", "jl_matvec_q4k_r1_pq", "jl_matvec_q4k_r1_pq_res", "jl_matvec_q8_0_r1_pq", "jl_matvec_q8_0_r1_pq_res", "jl_matvec_q6k_r1_pq", "jl_matvec_q6k_r1_pq_res", "jl_matvec_q8_0p_r1_pq", "jl_matvec_q8_0p_r1_pq_res", "jl_matvec_q4k_r1_res", "jl_matvec_q4k_r1_x4_res", "jl_matvec_q8_0_r1_res", "jl_matvec_q8_0_r1_x4_res", "jl_matvec_q6k_r1_res", "jl_matvec_q6k_r1_x4_res", "jl_matvec_q8_0p_r1_res", "jl_matvec_q8_0p_r1_x4_res", "jl_matvec_q8_0p_r1", "jl_matvec_q8_0p_r2", "jl_matvec_q8_0p_r4", "jl_gemm_prep_q4k", "jl_gemm_prep_q4k_w16", "jl_gemm_q4k_r64", "jl_gemm_q4k_r128", "jl_gemm_q4k_wide", "jl_gemm_prep_q4k_fold", "jl_gemm_q4k_fold_wide", "jl_gemm_q4k_fold_wide4", "jl_gemm_q4k_k2", "jl_gemm_q4k_k2_planes", "jl_gemm_prep_q4k_planes", "jl_gemm_q4k_r64_planes", "jl_gemm_q4k_wide_planes", "jl_gemm_w16_prep_q4k", "jl_gemm_q4k_w16", "jl_gemm_q4k_few32", "jl_moe_route", "jl_moe_route_g2", "jl_moe_route_g4", "jl_moe_logits", "jl_moe_logits_e2", "jl_moe_logits_e2_f16", "jl_moe_logits_e4", "jl_moe_logits_e4_f16", "jl_moe_logits_e8", "jl_moe_logits_e8_f16", "jl_moe_group", "jl_moe_group2", "jl_moe_quant", "jl_moe_matvec_planes_q4k", "jl_moe_combine", "jl_moe_worklist", "jl_moe_gemm_prep", "jl_moe_gemm_prep_planes", "jl_moe_gemm_q4k", "jl_moe_g16_prep", "jl_moe_g16_prep_planes", "jl_moe_g16_c1", "jl_moe_g16_c2", "jl_moe_g16_c3", "jl_moe_g16_f1", "jl_moe_g16_f2", "jl_moe_g16_f3", "jl_moe_g16_g1", "jl_moe_g16_g2", "jl_moe_g16_g3", "jl_moe_g16_d1", "jl_moe_g16_d2", "jl_moe_g16_d3", "jl_moe_g16p_c1", "jl_moe_g16p_c2", "jl_moe_g16p_c3", "jl_moe_g16p_f1", "jl_moe_g16p_f2", "jl_moe_g16p_f3", "jl_moe_g16p_g1", "jl_moe_g16p_g2", "jl_moe_g16p_g3", "jl_moe_g16p_d1", "jl_moe_g16p_d2", "jl_moe_g16p_d3", "jl_moe_gemm_r64", "jl_moe_gemm_r64_planes", "jl_mxfp4_prep", "jl_mxfp4_prep_few", "jl_mxfp4_few_t1", "jl_mxfp4_few_t2", "jl_mxfp4_few_t3", "jl_mxfp4_few_t4", "jl_mxfp4_few_planes_t1", "jl_mxfp4_few_planes_t2", "jl_mxfp4_few_planes_t3", "jl_mxfp4_few_planes_t4", "jl_mxfp4_few_c3", "jl_mxfp4_few_c4", "jl_mxfp4_few_planes_c3", "jl_mxfp4_few_planes_c4", "jl_mxfp4_gemm", "jl_mxfp4_gemm_r96", "jl_mxfp4_matvec", "jl_mxfp4_matvec1_b1", "jl_mxfp4_matvec1_b2", "jl_mxfp4_matvec1_b3", "jl_mxfp4_scaled_prep", "jl_mxfp4_scaled_gemm", "jl_mxfp4_planes_prep", "jl_mxfp4_planes_gemm", "jl_mxfp4_planes_gemm_r96", "jl_mxfp4_matvec_planes_r64", "jl_mxfp4_matvec_planes_r32", "jl_mxfp4_matvec_planes_r16", "jl_unpack_mxfp4", "jl_sum_parts", "jl_silu_mul", "jl_add_rows", "jl_host_in", "jl_host_done", "jl_q4k_fold_range", "jl_probe_read", "jl_probe_empty", "jl_probe_wait", "jl_probe_mfma", "jl_probe_mfma_v5",
                                       "jl_pack_weights", "jl_unpack_q4k", "jl_unpack_q6k", "jl_unpack_q8_0"};
     names.push_back("jl_few_prep");
-    for (const char* form : {"l16_1", "l32_1", "l64_1", "l64_2", "l64_4", "wg_1", "wg_2", "wg_4", "wg_8", "wg_16"})
+    for (const char* form : {"l16_1", "l32_1", "l64_1", "wg_1", "wg_2", "wg_4", "wg_8", "wg_16"})
         for (const char* any : {"", "_any"}) names.push_back(std::string("jl_norm_rows_") + form + any);
     for (const char* g : {"g1", "g2", "g3", "g4", "g3p", "g4p", "g6p", "g8p", "g12p", "g16p"}) names.push_back(std::string("jl_moe_select_") + g);
     names.push_back("jl_adapter_sum");
@@ -2509,14 +2509,20 @@ int jl_norm_rows_dev(jl_ctx* c, const jl_norm_rows* g, void* stream) {
     Name name;
     name << "jl_norm_rows_";
     unsigned grid, block = 256, lds = 0;
-    if (quads <= 256) {   // a wavefront a row, or a part of one
+    // Up to 256 elements a wavefront a row, or a part of one; longer rows a workgroup each.  us with the residual and int8, a wavefront's form / a workgroup: 4096
+    // rows of 64 2.6 / 3.7, 128 3.5 / 3.9, 256 4.7 / 4.5; 512 7.4 / 6.9, 1024 12.2 / 11.8 and one row of 1024 3.7 / 2.5.
+    if (quads <= 64) {
         const int lanes = quads <= 16 ? 16 : quads <= 32 ? 32 : 64;
-        name << "l" << lanes << "_" << (quads <= 64 ? 1 : quads <= 128 ? 2 : 4);
+        name << "l" << lanes << "_1";
         grid = (unsigned)(((long)g->rows + 256 / lanes - 1) / (256 / lanes));
-    } else {              // a workgroup a row
+    } else {
+        // Groups of four a thread: threads enough to have a row's loads on their way at once while a CU has one row, about 512 of them where rows follow
+        // each other on a CU.  us by 1 / 2 / 4 / 8 groups, int8: one row of 4096 3.3 / 3.3 / 4.2 / 6.2, 7168 - / 4.4 / 4.8 / 6.2, 14336 - / - / 6.4 / 7.4;
+        // 4096 rows of 2048 21.5 / 22.6 / 25.5 / 24.5, 4096 42.3 / 33.6 / 37.8 / 40.9, 7168 - / 79 / 81 / 82, 14336 - / - / 173 / 161.
+        const int most = g->rows > c->num_cu ? 512 : 896;
         int ni = 1;
-        while (quads > 1024 * ni) ni *= 2;
-        if (g->rows > c->num_cu && ni < 4) ni = 4;
+        while (quads > most * ni && ni < 8) ni *= 2;
+        if (quads > 1024 * ni) ni = 16;
         block = (unsigned)((quads + 64 * ni - 1) / (64 * ni) * 64);
         name << "wg_" << ni;
         grid = (unsigned)g->rows;

@@ -690,7 +690,6 @@ extern "C" __global__ __launch_bounds__(64) void jl_probe_wait(const u32x4* __re
     extern "C" __global__ __launch_bounds__(BLOCK) void jl_norm_rows_##NAME(NormRowsArgs p) { norm_rows_body<LPR, NI, WG, true>(p, (double*)jl_smem); } \
     extern "C" __global__ __launch_bounds__(BLOCK) void jl_norm_rows_##NAME##_any(NormRowsArgs p) { norm_rows_body<LPR, NI, WG, false>(p, (double*)jl_smem); }
 JL_NORM_ROWS(l16_1, 16, 1, false, 256) JL_NORM_ROWS(l32_1, 32, 1, false, 256) JL_NORM_ROWS(l64_1, 64, 1, false, 256)
-JL_NORM_ROWS(l64_2, 64, 2, false, 256) JL_NORM_ROWS(l64_4, 64, 4, false, 256)
 JL_NORM_ROWS(wg_1, 64, 1, true, 1024) JL_NORM_ROWS(wg_2, 64, 2, true, 1024) JL_NORM_ROWS(wg_4, 64, 4, true, 1024)
 JL_NORM_ROWS(wg_8, 64, 8, true, 1024) JL_NORM_ROWS(wg_16, 64, 16, true, 1024)
 // grid = 1, block = 1024, LDS = (n_adapter + 33) words

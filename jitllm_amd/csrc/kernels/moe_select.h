@@ -10,21 +10,22 @@
 //   weight = s / (sum of the taken s in their order + 1e-20), or s; times scale
 //
 // One wavefront a row, NG experts a lane side by side.  With many rows the kernel is bound by its vector instructions, not by
-// its bytes (16384 rows of 384 experts: 24.6 us in the first form, a chain of wave maxima over 32-bit keys and the library's f64
+// its bytes (16384 rows of 384 experts: 18.6 us, 22.4 in the first form, a chain of wave maxima over 32-bit keys and the library's f64
 // exponential and division; 25 MB would take 5.5), with one row by their latency.  So:
 //   * the f64 exponential is eighteen instructions (an f64 multiply-add costs what an f32 one does here) and the quotient a
 //     reciprocal refined in three multiply-adds: either is off by under 2^-50, where the narrowing to f32 keeps 2^-24;
 //   * the selection goes by packed keys, the 22 high bits of c's order over the expert's index, which a lane sorts once and then only
 //     shifts: a round is a wave maximum of the lanes' heads.  Packed keys that differ in their high bits are in c's order; where two
-//     of them do not -- one row in ten -- what was taken is put in order by its whole keys, and where more than 64 experts are that near to
-//     one another (scores that are all one value) the row takes whole keys from the start.
+//     of them do not -- one row in ten of sigmoid scores, one in three hundred of softmax ones -- what was taken is put in order by its
+//     whole keys, and where more than 64 experts are that near to one another (scores that are all one value) the row takes whole keys
+//     from the start.
 #pragma once
 #include "args.h"
 #include "common.h"
 #include "moe.h"
 
-// e^x for |x| <= 800 (0 and infinity past f64's range), to 2^-51 or so: x = n ln2 + r with |r| <= ln2 / 2, the exponential's series in r up to r^12 / 12! (the next term is under
-// 2^-52), times 2^n.
+// e^x for |x| <= 800 (0 and infinity past f64's range), to 2^-51 or so: x = n ln2 + r with |r| <= ln2 / 2, the exponential's series in r
+// up to r^12 / 12! (the next term is under 2^-52), times 2^n.
 __device__ __forceinline__ double select_exp(double x) {
     const double n = __builtin_rint(x * 1.4426950408889634074);
     double r = __builtin_fma(-n, 0x1.62e42fefa39efp-1, x);   // ln2 in two parts

@@ -7,7 +7,8 @@
 //   y = f32(f64(h) * f64(w) * inv)              than the f32 it is narrowed to, so y does not depend on the order of the sum
 //   q, as, sum16 = the quantizer of y           (quantize.h: bit for bit jl_quantize_act_dev over y)
 //
-// A row is read once, kept in registers across the sum, and written once: the kernel is bound by its bytes.
+// A row is read once, kept in registers across the sum, and written once: the kernel is bound by its bytes.  With the residual and int8 4096 rows of 7168 take
+// 82 us (387 MB, 4.7 TB/s), of 14336 161 (775 MB, 4.8), 512 of 4096 7.8 (28 MB; one round of workgroups, its ramp and tail); one row of 4096 2.7 in f32, near the launch.
 #pragma once
 #include "args.h"
 #include "common.h"
@@ -95,15 +96,18 @@ __device__ __forceinline__ void norm_rows_body(const NormRowsArgs& p, double* pa
     const size_t row = WG ? blockIdx.x : (size_t)blockIdx.x * (256 / LPR) + tid / LPR;
     const bool here = WG || row < (size_t)p.rows;
     const int n = p.n;
-    f32x4 h[NI], w[NI];
+    // w after the sum: beside h it does not fit the registers of 1024 threads (with it one row of 14336 took 20 us in this form, now one of 65536 does)
+    constexpr bool LATE = NI > 8;
+    f32x4 h[NI], w[LATE ? 1 : NI];
 #pragma unroll
     for (int i = 0; i < NI; i++) {
         const int e = 4 * (lane + nthr * i);
         const bool live = here && e < n;
-        h[i] = w[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        h[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (!LATE) w[LATE ? 0 : i] = h[i];
         if (live) {
             h[i] = norm_load<VEC>(p.x, row * p.x_stride + e, p.x_type, n - e);
-            w[i] = p.w ? norm_load<VEC>(p.w, e, JL_F32, n - e) : f32x4{1.f, 1.f, 1.f, 1.f};
+            if (!LATE) w[LATE ? 0 : i] = p.w ? norm_load<VEC>(p.w, e, JL_F32, n - e) : f32x4{1.f, 1.f, 1.f, 1.f};
             if (p.resid) {
                 const f32x4 r = norm_load<VEC>(p.resid, row * p.resid_stride + e, JL_F32, n - e);
                 h[i] = r + p.alpha * h[i];
@@ -130,9 +134,10 @@ __device__ __forceinline__ void norm_rows_body(const NormRowsArgs& p, double* pa
     for (int i = 0; i < NI; i++) {
         const int e = 4 * (lane + nthr * i);
         const bool live = here && e < n;
-        f32x4 y;
+        f32x4 y, g = w[LATE ? 0 : i];
+        if (LATE) g = live && p.w ? norm_load<VEC>(p.w, e, JL_F32, n - e) : f32x4{1.f, 1.f, 1.f, 1.f};
 #pragma unroll
-        for (int j = 0; j < 4; j++) y[j] = (float)((double)h[i][j] * (double)w[i][j] * inv);
+        for (int j = 0; j < 4; j++) y[j] = (float)((double)h[i][j] * (double)g[j] * inv);
         if (live && p.resid_out) norm_store<VEC>(p.resid_out, row * p.resid_stride + e, JL_F32, n - e, h[i]);
         if (live && p.y) norm_store<VEC>(p.y, row * p.y_stride + e, p.y_type, n - e, y);
         if (p.q) {
