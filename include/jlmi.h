@@ -374,7 +374,8 @@ int jl_matvec_packed_group(jl_ctx *ctx, int n, float *const *outs, const int *ty
  *     out[i][t] = base[i][t] + scale[a] * B_i[a] (A_i[a] x[t])
  * for n <= JL_MAX_GROUP projections that read one x (a block's q, k and v; its gate and up; one projection) -- base[i] is what
  * jl_matmul_dev, jl_matvec_group_dev or their packed and MXFP4 forms made of the shared weights, [ntok][rows[i]] f32; it may be
- * out[i] (added in place), and null stands for zeros.  a[i] [n_adapter][rank][k] and b[i] [n_adapter][rows[i]][rank] of `type`
+ * out[i] (added in place), and null stands for zeros; otherwise no output overlaps another operand, another
+ * output among them.  a[i] [n_adapter][rank][k] and b[i] [n_adapter][rows[i]][rank] of `type`
  * (JL_TYPE_F32, _F16, _BF16); x [ntok][k] of x_type (the same three).  ranks, when given, holds each adapter's own rank (more
  * than `rank` counts as `rank`): rows of A and columns of B from there on are not used.  scale null: ones.  A token whose id is
  * n_adapter or more has no adapter and gets base alone, as does one whose adapter has rank 0.  ids, ranks and scale are device

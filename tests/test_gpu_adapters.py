@@ -285,6 +285,17 @@ def test_a_reservation_covers_every_cut_of_the_work(dev, which):
         own.close()
 
 
+@pytest.mark.parametrize("which", [0, 3])
+@pytest.mark.parametrize("ntok, n_adapter, rank", [(5000, 8192, 3), (70000, 5, 4), (4097, 1, 40)])
+def test_many_tokens_and_many_adapters(dev, which, ntok, n_adapter, rank):
+    dev.set_tuning(adapter__form=which)
+    c = Case(ntok, ntok, 32, [12], rank, n_adapter, whole=True)
+    assert c.call(dev)
+    dev.synchronize()
+    dev.set_tuning(adapter__form=0)
+    c.check(exact=True)
+
+
 def test_same_bits_every_time(dev, form):
     for ntok in (5, 64, 400):
         c = Case(ntok, ntok, 1024, [300], 32, 3)

@@ -134,6 +134,11 @@ def test_int8_form_is_the_quantizers(dev, window, rows, n):
     dev.SetActWindow(32)
 
 
+@pytest.mark.parametrize("rows, n", [(300, 288), (300, 512), (300, 2048), (2, 7168), (300, 7168), (300, 14336), (3, 32768), (2, 32800), (300, 40000), (1, 65536)])
+def test_int8_form_over_the_sizes_of_a_workgroup(dev, rows, n):
+    test_int8_form_is_the_quantizers(dev, 256, rows, n)
+
+
 def test_in_place(dev):
     """resid_out over resid and y over x: as with buffers of their own."""
     rows, n = 37, 2880
