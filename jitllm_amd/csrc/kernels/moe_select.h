@@ -123,7 +123,7 @@ __device__ __forceinline__ void moe_select_body(const MoeSelectArgs& p, size_t r
         double sum = 0.0, ex[NG];
 #pragma unroll
         for (int i = 0; i < NG; i++) {
-            ex[i] = select_exp((double)fmaxf(v[i], mx - 800.f) - (double)mx);   // (e^-800 is 0 here)
+            ex[i] = select_exp(fmax((double)v[i] - (double)mx, -800.0));   // (e^-800 is 0 here; in f32 mx - 800 is mx from 2^34 on)
             sum += ex[i];
         }
         const double inv = select_rcp(fine ? route_wave_sum(sum) : 1.0);
