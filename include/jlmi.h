@@ -601,7 +601,7 @@ int jl_moe_route_dev(jl_ctx *ctx, const float *logits, int rows, int n_expert, i
  *     s = softmax over all experts (JL_SCORE_SOFTMAX) or 1 / (1 + e^-l) (JL_SCORE_SIGMOID), in f64, narrowed to f32
  *     c = s + bias[e]                                (f32; bias null: c = s): what the selection goes by, never the weight
  *     n_group > 1: expert e is of group e / (n_expert / n_group); a group is worth its best c (group_top 1) or the sum of its
- *         two best (2; a missing second adds nothing), and only the k_group best groups' experts are selected from
+ *         two best (2, in f32; a missing second adds nothing), and only the k_group best groups' experts are selected from
  *     the k_used largest c by (c descending, index ascending); groups likewise
  *     weight = s / (sum of the selected s in selection order + 1e-20) where renorm is not 0, else s; times scale
  * An expert whose logit is -infinity, or whose c is -infinity (a bias of -infinity takes it out of service) or no number, is

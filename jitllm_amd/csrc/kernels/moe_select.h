@@ -159,7 +159,7 @@ __device__ __forceinline__ void moe_select_body(const MoeSelectArgs& p, size_t r
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
         u32 g = a;
-        if (p.group_top > 1 && b) g = select_key(select_value(a) + select_value(b) + 0.0f);
+        if (p.group_top > 1 && b) g = max(select_key(select_value(a) + select_value(b) + 0.0f), 1u);   // (a sum of -inf is the last, not no group)
         const int per = whole ? lpg : 1;
         for (int r = 0; r < p.k_group; r++) {
             const u32 best = select_wave_max(g);

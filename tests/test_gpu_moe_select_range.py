@@ -42,3 +42,23 @@ def test_softmax_of_large_logits_by_rows(dev, form, rows):  # noqa: F811
     logits = np.tile(np.float32([0.0, 2e10]), (rows, 1))
     check(dev, logits, 1)
     check(dev, logits, 2, renorm=False)
+
+
+@pytest.mark.parametrize("score", [0, 1])
+@pytest.mark.parametrize("n, n_group, k_group, k", [(16, 4, 2, 6), (256, 8, 4, 8), (256, 8, 8, 16), (63, 7, 3, 9), (160, 8, 3, 16), (384, 4, 2, 8), (1000, 10, 4, 16)])
+def test_groups_whose_two_best_pass_the_range(dev, form, n, n_group, k_group, k, score):  # noqa: F811
+    """The sum of a group's two best choices is -infinity where a bias is the type's lowest value: such a group is the last that is kept,
+    its experts can still be taken.  Sums of +infinity are the first, the lowest of them."""
+    rng = np.random.default_rng(n + k_group)
+    logits, size = rng.standard_normal((7, n)).astype(np.float32), n // n_group
+    low = np.zeros((4, n_group, size), np.float32)
+    low[0] = LOWEST                                         # every group
+    low[1, 1:] = LOWEST                                     # all but the first
+    low[2, : n_group - 1] = LOWEST                          # all but the last
+    low[2, 0] = -np.inf                                     # (and the first out of service)
+    low[3, n_group // 2:] = -LOWEST
+    low[3, 0] = LOWEST
+    with np.errstate(over="ignore"):
+        for bias in low.reshape(4, n):
+            check(dev, logits, k, score=score, bias=bias, n_group=n_group, k_group=k_group, top=2, scale=0.5)
+            check(dev, logits, k, score=score, bias=bias, n_group=n_group, k_group=k_group, top=1, renorm=False)
