@@ -2553,8 +2553,10 @@ int adapter_ws_ensure(jl_ctx* c, size_t need) {
 namespace {
 constexpr int kMaxAdapters = 8192;   // counters of the grouping in LDS
 // How the matrix-core form is cut: a tile is up to 64 tokens of one adapter; a workgroup of adapter_down takes a tile, 4 nt tiles of sixteen rows of A
-// and a slice of K.  Slices for two workgroups a CU, as far as the tiles are known: there is one for 64 tokens at least, and one for every adapter met.
-// (us by 1 / 2 / 4 / 8 / 16 slices, 8 adapters, k = 4096: 256 tokens rank 16 beside 4096 98 / 59 / 39 / 30 / 25, 2048 tokens rank 64 131 / 83 / 60 / 51 / 50.)
+// and a slice of K.  Slices for two workgroups a CU.  How many tiles there are the device finds out: one for 64 tokens at least, and one for every adapter of
+// the bank at most; the geometric mean of the two is taken, so that neither a bank that lies idle nor requests that each bring their own are taken for the other.
+// (us by 1 / 2 / 4 / 8 / 16 slices, k = 4096: 8 adapters, 256 tokens rank 16 beside 4096 98 / 59 / 39 / 30 / 25, 2048 tokens rank 64 131 / 83 / 60 / 51 / 50;
+// 512 adapters, 2048 tokens rank 64 beside 4096, two of them met 108 / 70 / 54 / 46 / 43, all met 169 / 185 / 168 / 179 / 188.)
 struct AdapterPlan { int rank_pad, nt, passes, slices, max_tiles; };
 AdapterPlan adapter_plan(const jl_ctx* c, int ntok, int n, int rank, int k, int n_adapter) {
     AdapterPlan a;
@@ -2563,7 +2565,8 @@ AdapterPlan adapter_plan(const jl_ctx* c, int ntok, int n, int rank, int k, int 
     a.nt = tiles <= 4 ? 1 : 2;
     a.passes = (tiles + 4 * a.nt - 1) / (4 * a.nt);
     a.max_tiles = ntok / 64 + std::min(n_adapter + 1, ntok);
-    const long units = (long)a.passes * std::max((ntok + 63) / 64, std::min(ntok, n_adapter)), steps = (k + 127) / 128;
+    const int least = (ntok + 63) / 64, most = std::max(least, std::min(ntok, n_adapter));
+    const long units = (long)(a.passes * std::sqrt((double)least * most)), steps = (k + 127) / 128;
     a.slices = (int)std::max(1l, std::min({16l, steps, c->tune.adapter_slices ? (long)c->tune.adapter_slices : 2l * c->num_cu / units}));
     return a;
 }
@@ -2605,7 +2608,7 @@ int jl_adapter_group_dev(jl_ctx* c, const jl_adapter_group* g, void* stream) {
     a.ids = g->ids; a.ranks = g->ranks; a.scale = g->scale; a.x = g->x; a.u = nullptr;
     a.n = g->n; a.n_adapter = g->n_adapter; a.rank = g->rank; a.k = g->k; a.ntok = g->ntok;
     const AdapterPlan pl = adapter_plan(c, g->ntok, g->n, g->rank, g->k, g->n_adapter);
-    a.part = nullptr; a.u = nullptr; a.perm = a.tiles = nullptr;
+    a.part = nullptr; a.perm = a.tiles = nullptr;
     a.max_tiles = pl.max_tiles;
     a.rank_pad = pl.rank_pad; a.passes = pl.passes; a.slices = pl.slices; a.x_type = g->x_type; a.up_sets = 1;
     hipStream_t st = pick_stream(c, stream);
@@ -2620,18 +2623,26 @@ int jl_adapter_group_dev(jl_ctx* c, const jl_adapter_group* g, void* stream) {
     const long sets = (long)g->ntok * blocks(1024);
     const int l = g->rank <= 8 ? 1 : g->rank <= 16 ? 2 : g->rank <= 32 ? 4 : 8;   // lanes a column
     const bool dots = g->rank <= 64 && g->ntok <= 65535;
-    // Which form, by what each is estimated to take (us; fitted to 16-bit adapters beside 4096 to 28672 rows of k = 4096, 32 to 2048 tokens, 1 to 64
-    // adapters, within a quarter of the times there).  Dot products read A and B for every token, the matrix cores for every tile:
+    // Which form, by what each is estimated to take.  Dot products read A and B for every token, the matrix cores for every tile:
     //   128 tokens of 8 adapters, rank 16 beside 4096: 8.7 against 21 us; rank 64 beside 2 x 14336: 40 against 33;
-    //   512 tokens of 8, rank 16: 17 and 26, rank 64: 38 and 30; of 64 adapters, rank 64: 43 and 44; 2048 tokens of 64, rank 16: 60 and 52.
-    const double wide_d = (double)wide, nk = (double)g->n * g->k, bytes = g->rank * (nk + wide_d) * wb;
-    const double dots_us = 6 + g->ntok * (0.61e-7 * wb * g->rank * nk + wide_d * (3.1e-6 + 3.4e-8 * wb * g->rank));
-    const double mm_us = 17 + g->ntok * (1.7e-6 * g->k + 1.6e-6 * wide_d + 2.5e-9 * bytes) + std::max((g->ntok + 63) / 64, std::min(g->ntok, g->n_adapter)) * bytes / 3.7e6;
+    //   512 tokens of 8, rank 16: 17 and 26, rank 64: 38 and 30; of 64 adapters, rank 64: 43 and 44; 2048 tokens of 64, rank 16: 60 and 52;
+    //   1024 tokens, rank 64 beside 2 x 14336, a bank of 512: four of them met 270 and 101, all of them 717 and 607.
+    // us for `met` adapters among the tokens: workgroups and bytes of the two launches against bytes of the tiles, their workgroups and those of the tiles
+    // that there could have been.  Fitted to 2956 calls (8 to 4096 tokens, banks of 1 to 1024, one to all of them met, ranks 3 to 64, every type), nine
+    // in ten within 30 %.  How many are met the ids say, on the device: the call takes the form that is off by the smaller factor over both ends, one adapter and all of them.
+    const double wide_d = (double)wide, nk = (double)g->n * g->k, bytes = g->rank * (nk + wide_d) * wb, columns = blocks(256), nt = g->ntok;
+    const double dot_wgs = (double)g->n * (pl.rank_pad / 16) * std::min(16, (g->k + 1023) / 1024);
+    const auto dots_us = [&](double met) { return 6.4 + nt * (4.8e-8 * wb * g->rank * wide_d + 2.2e-3 * dot_wgs + 4.1e-4 * columns) + 9.5e-8 * met * bytes; };
+    const auto mm_us = [&](double met) {
+        return 15 + wb + nt * (1.42e-6 * g->k + 1.39e-6 * wide_d + 1.8e-9 * bytes) + (nt / 64 + met) * (1.67e-7 * bytes + 1.6e-3 * columns) + 2.9e-4 * pl.max_tiles * columns;
+    };
+    const int most = std::min(g->ntok, g->n_adapter);
+    const bool fewer = dots_us(1) * dots_us(most) <= 1.1 * mm_us(1) * mm_us(most);   // (1.1: what is about equal stays with two launches)
     // One launch or two of dot products: every column block makes u anew, which is little while tokens and ranks are few.  us, one / two, beside 4096
     // rows: rank 8, 1 token 4.6 / 6.5, 64 (as many workgroups as CUs) 5.2 / 7.0, 64 of q, k and v (half as many again) 8.0 / 8.9; rank 16, 1 token
     // 6.1 / 6.8, 16 (a quarter) 6.5 / 6.8, 16 of q, k and v 7.3 / 7.2, 64 8.0 / 7.3.
     const bool once = g->rank <= 16 && sets <= (g->rank <= 8 ? 3l * c->num_cu / 2 : c->num_cu / 4);
-    const int form = c->tune.adapter_form ? c->tune.adapter_form : !dots ? 0 : once ? 1 : dots_us <= mm_us ? 2 : 0;
+    const int form = c->tune.adapter_form ? c->tune.adapter_form : !dots ? 0 : once ? 1 : fewer ? 2 : 0;
     if (dots && form == 1 && g->rank <= 16) {
         name << "jl_adapter_one_" << t << "_l" << l;
         return launch(c, name, blocks(1024), (unsigned)g->ntok, 1024, 0, st, params);
