@@ -114,7 +114,7 @@ int jl_synchronize(jl_ctx *ctx);
  * "moe.chunk" (form 3: super-blocks a step, 1-3),
  * "moe.select" (jl_moe_select_dev, 129 to 256 experts: 1 packed keys, 2 whole ones), "adapter.form" (1 one launch of dot products, ranks up to
  * 16; 2 two launches, up to 64; 3 / 4 the matrix cores without / with a launch that adds the slices of K up), "adapter.slices" (of K) and
- * "adapter.sets" (sets of 256 columns a workgroup of the two launches),
+ * "adapter.sets" (sets of 256 columns a workgroup of the two launches, 1 to 4),
  * "moe.group" / "moe.logits" / "moe.waves" / "moe.lpr" (forms of the mixture block's other kernels; "moe.logits": expert
  * rows a workgroup, and 16 / 32 more for token groups / expert rows side by side),
  * "mxfp4.split" (K slices of the MXFP4 GEMM), "mxfp4.rows" (96 or 128 rows a tile; 1: the

@@ -2659,7 +2659,7 @@ int jl_adapter_group_dev(jl_ctx* c, const jl_adapter_group* g, void* stream) {
         // (columns a workgroup: fewer and longer ones where there are many; us by 256 / 512 / 1024: 128 tokens rank 16 beside 4096 rows 8.7 / 8.6 / 9.5,
         // 6144 13.3 / 11.6 / 12.1, 28672 28 / 22 / 20)
         const long wgs = (long)g->ntok * blocks(256);
-        a.up_sets = c->tune.adapter_sets ? c->tune.adapter_sets : wgs <= 8l * c->num_cu ? 1 : wgs <= 24l * c->num_cu ? 2 : 4;
+        a.up_sets = c->tune.adapter_sets ? std::clamp(c->tune.adapter_sets, 1, 4) : wgs <= 8l * c->num_cu ? 1 : wgs <= 24l * c->num_cu ? 2 : 4;
         Name cols;
         cols << "jl_adapter_cols_" << t << "_l" << l;
         return launch(c, cols, blocks(256 * a.up_sets), (unsigned)g->ntok, 256, 0, st, params);
