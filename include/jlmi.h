@@ -381,7 +381,9 @@ int jl_matvec_packed_group(jl_ctx *ctx, int n, float *const *outs, const int *ty
  * n_adapter or more has no adapter and gets base alone, as does one whose adapter has rank 0.  ids, ranks and scale are device
  * memory, read by the kernels.  Products and sums are f32 whatever the types.  k % 32 == 0, rank <= 512, n_adapter <= 8192; a, b and x 16-byte
  * aligned.  Few tokens take one or two launches of dot products, more of them the matrix cores (on exact pieces of the operands);
- * a token's result does not depend on the other tokens of the call, but by their number on the last bits.  The workspace (jl_reserve_adapters) is
+ * a token's result does not depend on the other tokens of the call, but by their number on the last bits -- and on these two: a result that is
+ * no finite number (an infinity in x, A or B, or a sum past f32) is the infinity from dot products and may be a NaN from the matrix cores, which
+ * also keep no bits of an f32 value, A x among them, that lie below 2^-133 (all 24 from 2^-110 on).  ntok <= 1048560, the projections' rows 2^24 together.  The workspace (jl_reserve_adapters) is
  * the context's, grown on demand; a buffer that is outgrown lives until the context goes, so a captured graph that holds its address stays valid.
  * No counterpart in the reference. */
 typedef struct jl_adapter_group {

@@ -10,7 +10,8 @@
 // Products are exact: an f32 value is three bf16 values (8 mantissa bits each, cut off, not rounded), an f16 value two, and every
 // piece of one operand meets every piece of the other in the f32 accumulator -- one matrix instruction for bf16 x bf16, three for f32 x
 // against bf16 adapters, nine for f32 x f32.  What rounds is the f32 sum, as in a dot product in f32.  (An infinity cut into pieces
-// leaves a NaN: it was going to be no finite number.)
+// leaves a NaN, as does one that meets a zero piece: it was going to be no finite number.  A bf16 value ends at 2^-133: what an f32 value has below that is lost,
+// from 2^-110 on nothing.)
 //
 // What decides the layout of the work (measured on MI355X): sixteen rows of 64 bytes a load, as the matrix instruction's operands and results lie, run
 // at two thirds of the rate of rows of 256 bytes, so x, base and out are moved by rows and change places in LDS; and with few tokens a call is
