@@ -177,9 +177,10 @@ int jl_forget(jl_ctx *ctx, const void *p, size_t n);
 /* Threads.  The host-pointer entry points (no _dev in the name) may be called from any
  * thread: each holds the context's lock for its whole synchronous run.  The *_dev entry
  * points take no lock and share the context's workspaces (activation fragments, K-split
- * slabs, the mixture block's lists, the flag word of jl_pack_weights_dev and
- * jl_fold_admit_dev): a context's *_dev calls are made by one thread at a time, on one stream
- * at a time, as the reference's tier makes its device calls (jit/gpu/tier/tier.go:2831-2843);
+ * slabs, the mixture block's lists, the adapters' sums and lists, the flag word of
+ * jl_pack_weights_dev and jl_fold_admit_dev): a context's *_dev calls are made by one thread
+ * at a time, on one stream at a time -- replays of graphs that hold such calls among them: two
+ * of a context's, or one and a call, do not run at the same time --, as the reference's tier makes its device calls (jit/gpu/tier/tier.go:2831-2843);
  * give each thread that launches concurrently a context of its own.
  *
  * The lock the host-pointer entry points hold for their whole synchronous run (the

@@ -145,7 +145,7 @@ template <> struct AdQuad<JL_F32> {
 // ---------------------------------------------------------------- tokens by adapter
 // perm: the tokens, those of an adapter side by side (those without one last); tiles: {adapter, first place in perm, tokens} of pieces of up to
 // 64 of them, n_adapter for those without one, 0 tokens behind the last.  The order inside an adapter is whatever the LDS additions make
-// it: no result depends on what else is in a token's tile.  One workgroup of 1024; LDS: n_adapter + 1 counters, 16 totals.
+// it: no result depends on what else is in a token's tile.  One workgroup of 1024; LDS: n_adapter + 1 counters, 32 totals.
 __device__ __forceinline__ void adapter_group_body(const AdapterArgs& p, u32* count) {
     const int tid = threadIdx.x, kinds = p.n_adapter + 1, lane = tid & 63, wave = tid >> 6;
     u32* tot = count + kinds;
@@ -687,16 +687,15 @@ template <int T, int L> struct AdColumns {
     AdType<T> b[L];
     float base;
     // (B by the bank's rank: the adapter's own is known later)
-    __device__ __forceinline__ void load(const AdapterArgs& p, int pi, u32 id, size_t orow, int col, bool with_b, bool with_base) {
+    __device__ __forceinline__ void load(const AdapterArgs& p, int pi, u32 id, size_t orow, int col) {
         const int lane = threadIdx.x & 63, rows = p.rows[pi], r0 = 8 * (lane % L), r = r0 - ad_first<L>(r0, p.rank), mine = col + lane % L * (64 / L) + lane / L;
-        if (with_base) base = p.base[pi] && mine < rows ? p.base[pi][orow + mine] : 0.f;
-        if (with_b)
+        base = p.base[pi] && mine < rows ? p.base[pi][orow + mine] : 0.f;
 #pragma unroll
-            for (int j = 0; j < L; j++) {
-                const size_t at = ((size_t)id * rows + min(col + j * (64 / L) + lane / L, rows - 1)) * p.rank + r;
-                if (L > 1) b[j].load(p.b[pi], at);
-                else b[j].load_some(p.b[pi], at, p.rank);   // (uniform)
-            }
+        for (int j = 0; j < L; j++) {
+            const size_t at = ((size_t)id * rows + min(col + j * (64 / L) + lane / L, rows - 1)) * p.rank + r;
+            if (L > 1) b[j].load(p.b[pi], at);
+            else b[j].load_some(p.b[pi], at, p.rank);   // (uniform)
+        }
     }
     __device__ __forceinline__ void finish(const AdapterArgs& p, int pi, size_t orow, int col, int rank, const float (&u)[8]) {
         const int lane = threadIdx.x & 63, r0 = 8 * (lane % L), first = ad_first<L>(r0, p.rank), mine = col + lane % L * (64 / L) + lane / L, left = rank - r0 + first;
@@ -747,7 +746,7 @@ __device__ __forceinline__ void adapter_one_body(const AdapterArgs& p, float* ld
     const int col = block * 1024 + wave * 64;
     const bool here = col < p.rows[pi];
     AdColumns<T, L> c;
-    if (here) c.load(p, pi, id, orow, col, true, true);
+    if (here) c.load(p, pi, id, orow, col);
     // wavefront = (piece of K modulo pieces, rows modulo 16 / pieces)
     const int np = (p.k + 255) / 256, pieces = np > 8 ? 16 : np > 4 ? 8 : np > 2 ? 4 : np;   // a power of two
     const int piece = wave & (pieces - 1), step = 16 / pieces;
@@ -815,7 +814,7 @@ template <int T, int L> __device__ __forceinline__ void adapter_cols_body(const 
     const int rank = ad_rank(p, id);
     int col = block * 256 * p.up_sets + wave * 64;
     AdColumns<T, L> c;
-    if (col < p.rows[pi]) c.load(p, pi, id, orow, col, true, true);
+    if (col < p.rows[pi]) c.load(p, pi, id, orow, col);
     if (threadIdx.x < 8 * L) {
         float t = 0.f;
         if ((int)threadIdx.x < rank) {
@@ -829,7 +828,7 @@ template <int T, int L> __device__ __forceinline__ void adapter_cols_body(const 
     float u[8];
     ad_take_u<L>(p, us, u);
     for (int s = 0; s < p.up_sets && col < p.rows[pi]; s++, col += 256) {
-        if (s) c.load(p, pi, id, orow, col, true, true);
+        if (s) c.load(p, pi, id, orow, col);
         c.finish(p, pi, orow, col, rank, u);
     }
 }

@@ -8,7 +8,7 @@
 //   q, as, sum16 = the quantizer of y           (quantize.h: bit for bit jl_quantize_act_dev over y)
 //
 // A row is read once, kept in registers across the sum, and written once: the kernel is bound by its bytes.  With the residual and int8 4096 rows of 7168 take
-// 82 us (387 MB, 4.7 TB/s), of 14336 161 (775 MB, 4.8), 512 of 4096 7.8 (28 MB; one round of workgroups, its ramp and tail); one row of 4096 2.7 in f32, near the launch.
+// 82 us (393 MB, 4.8 TB/s), of 14336 161 (785 MB, 4.9), 512 of 4096 7.8 (28 MB; one round of workgroups, its ramp and tail); one row of 4096 2.7 in f32, near the launch.
 #pragma once
 #include "args.h"
 #include "common.h"
