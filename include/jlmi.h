@@ -610,7 +610,7 @@ int jl_moe_route_dev(jl_ctx *ctx, const float *logits, int rows, int n_expert, i
  * An expert whose logit is -infinity, or whose c is -infinity (a bias of -infinity takes it out of service) or no number, is
  * never selected; a softmax row that holds a NaN or +infinity has no numbers and selects nothing.  A row with fewer experts to
  * select than k_used has the id n_expert and weight 0 in the places left over -- an id no expert has, which
- * jl_moe_ffn_dev and the grouping leave out.  Fills sel [rows][sel_stride] (first k_used of each row) and wt [rows][k_used].
+ * jl_moe_ffn_dev and the grouping leave out (jl_moe_combine_dev by their pos, see there).  Fills sel [rows][sel_stride] (first k_used of each row) and wt [rows][k_used].
  * n_expert <= 1024, k_used <= 16, n_group <= 64 and a divisor of n_expert, k_used <= k_group * (n_expert / n_group);
  * n_group 0 or 1: no groups. */
 #define JL_SCORE_SOFTMAX 0
@@ -652,7 +652,9 @@ int jl_moe_matvec_dev(jl_ctx *ctx, float *out0, float *out1, int type, const voi
 
 /* kernels.ExpertCombineGrouped (jit/gpu/kernels/moegroup.go:38-68) with the host path's
  * order (engine/model/moe.go:127-134, :752-759): resid[r] += sum of wt[r][s] *
- * y[pos[r*k_used+s]] over the row's experts in ascending expert id. */
+ * y[pos[r*k_used+s]] over the row's experts in ascending expert id.  A pair whose pos is 0xFFFFFFFF
+ * adds nothing: where a selection may hold ids that no expert has (jl_moe_select_dev's empty places), fill pos with it
+ * before jl_moe_group_dev, which writes no pos of theirs. */
 int jl_moe_combine_dev(jl_ctx *ctx, float *resid, const float *y, const float *wt,
                        const uint32_t *sel, int sel_stride, const uint32_t *pos, int rows,
                        int k_used, int n_embd, void *stream);

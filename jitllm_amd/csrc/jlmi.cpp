@@ -3140,7 +3140,7 @@ int moe_combine_launch(jl_ctx* c, float* resid, const float* y, const float* wt,
 }
 }  // namespace
 
-// (how many experts there are is not known here: every id counts)
+// (how many experts there are is not known here: every id counts that has a column)
 int jl_moe_combine_dev(jl_ctx* c, float* resid, const float* y, const float* wt, const uint32_t* sel,
                        int sel_stride, const uint32_t* pos, int rows, int k_used, int n_embd, void* stream) {
     if (!c) return JL_ERR_ARG;

@@ -417,7 +417,7 @@ struct MoeCombineArgs {
     const float* y;         // [ncols][n_embd]
     const float* wt;        // [rows][k_used]
     const uint32_t* sel;    // [rows][sel_stride]
-    const uint32_t* pos;    // [rows*k_used]; not read for an id that no expert has
+    const uint32_t* pos;    // [rows*k_used]; not used for an id that no expert has; 0xFFFFFFFF: no column
     int sel_stride, k_used, n_embd;
     uint32_t last_id;       // ids past this one are no expert's and add nothing
 };

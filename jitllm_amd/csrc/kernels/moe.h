@@ -1370,10 +1370,12 @@ __device__ __forceinline__ void moe_combine_body(const MoeCombineArgs& args) {
     f32x4* res = as_global((f32x4*)(p.resid + (size_t)r * p.n_embd));
     const f32x4* y4 = as_global((const f32x4*)p.y);
     const int slot = min(lane, ku - 1);
-    const i32 mine = (i32)as_global(p.sel)[(size_t)r * p.sel_stride + slot];
+    const i32 id = (i32)as_global(p.sel)[(size_t)r * p.sel_stride + slot];
     const float wt = as_global(p.wt)[(size_t)r * ku + slot];
     const i32 at = (i32)as_global(p.pos)[(size_t)r * ku + slot];
-    const int have = (int)__builtin_popcountll(__ballot(lane < ku && (u32)mine <= p.last_id));   // (the other ids' ranks are behind these)
+    const bool column = at != -1;   // (a pair without one is ranked last)
+    const i32 mine = column ? id : -1;
+    const int have = (int)__builtin_popcountll(__ballot(lane < ku && column && (u32)mine <= p.last_id));   // (the other ids' ranks are behind these)
     f32x4 acc = res[nc];
     int rank = 0;   // a stable rank: equal ids (not a valid routing) keep their slot order
     for (int j = 0; j < ku; j++) {
