@@ -47,6 +47,7 @@ extern "C" {
 #define JL_TYPE_Q8_0 8
 #define JL_TYPE_Q4_K 12
 #define JL_TYPE_Q6_K 14
+#define JL_TYPE_I8 24   /* rows of a cache: 8-bit values, one f32 scale a row */
 #define JL_TYPE_BF16 30 /* normed rows and adapters */
 #define JL_TYPE_MXFP4 39
 
@@ -177,7 +178,7 @@ int jl_forget(jl_ctx *ctx, const void *p, size_t n);
 /* Threads.  The host-pointer entry points (no _dev in the name) may be called from any
  * thread: each holds the context's lock for its whole synchronous run.  The *_dev entry
  * points take no lock and share the context's workspaces (activation fragments, K-split
- * slabs, the mixture block's lists, the adapters' sums and lists, the flag word of
+ * slabs, the mixture block's lists, the adapters' sums and lists, the attention's partial sums, the flag word of
  * jl_pack_weights_dev and jl_fold_admit_dev): a context's *_dev calls are made by one thread
  * at a time, on one stream at a time -- replays of graphs that hold such calls among them: two
  * of a context's, or one and a call, do not run at the same time --, as the reference's tier makes its device calls (jit/gpu/tier/tier.go:2831-2843);
@@ -579,6 +580,100 @@ int jl_matmul_mxfp4_bf16_dev(jl_ctx *ctx, float *out, const void *w, const uint1
 int jl_matmul_mxfp4_packed_bf16_dev(jl_ctx *ctx, float *out, const uint32_t *qs, const uint32_t *d,
                                     int row, int stride, const uint16_t *x, int nrows, int k,
                                     int ntok, void *stream);
+
+/* ---- between a block's projections, and behind the last one (device pointers) ---------------------------------------- */
+
+/* A paged cache of keys and values.  Rows of d elements of `type`: JL_TYPE_F16, JL_TYPE_BF16, or JL_TYPE_I8 with one f32 scale a row.  k and v are pools of
+ * n_page pages of page_size positions (a power of two, 16 or more; one page a sequence makes a contiguous cache):
+ *     row of page p, head h, place s:   p * page_stride + h * head_stride + s * row_stride    elements from k (v) on
+ *     its scale:                        k_scale[(p * n_kv + h) * page_size + s]
+ * (strides 0: back to back, [n_page][n_kv][page_size][d]; other orders by their strides, e.g. row_stride n_kv * d, head_stride d).  Position i of sequence s
+ * lies on page table[s * table_stride + i / page_size], in place i modulo page_size; table is device memory, n_seq rows of table_pages entries
+ * (table_stride 0: table_pages).  An entry of n_page or more is no page: what lies there is written nowhere, read as zeros, and seen by no one.
+ * d a multiple of 16 up to 256; strides multiples of 16; k, v and the scales 16-byte aligned; table_pages * page_size up to 2^31.  Offsets are 64 bits wide.
+ * The structure is read by the call and not kept.  (The reference's tier pages its cache likewise, jit/gpu/tier; the layout here is its own.) */
+typedef struct jl_kv_cache {
+    int type;
+    int n_kv, d;
+    int page_size, n_page;
+    void *k, *v;
+    float *k_scale, *v_scale;
+    size_t page_stride, head_stride, row_stride;
+    const uint32_t *table;
+    int n_seq, table_pages, table_stride;
+} jl_kv_cache;
+
+/* Rows of ntok tokens into the cache (jl_kv_write_dev), or back from it (jl_kv_read_dev): token t is position pos[t] of sequence seq[t] (seq null: of sequence t).
+ * k and v [ntok][stride] of `type` (JL_TYPE_F32, _F16, _BF16), a token's n_kv rows back to back, strides in elements (0: n_kv * d); one of the two may be null.
+ * 16-bit rows: values rounded to nearest even.  8-bit rows: the activation quantizer's arithmetic with the row as its window, d = amax / 127,
+ * round-half-away(x * (1 / d)), read back as f32(q * d); a row that is not finite reads as NaN, one of nothing above 2^-121 as zeros.  A token whose sequence is n_seq or
+ * more, whose position lies behind the table's pages or on no page, is not written, and reads as zeros.  Tokens of one call have places of their own (of two with
+ * one place either's bytes may stay); what else the pages hold is left as it was.  seq and pos are device memory. */
+typedef struct jl_kv_rows {
+    int ntok;
+    void *k, *v;
+    int type;
+    size_t k_stride, v_stride;
+    const uint32_t *seq, *pos;
+} jl_kv_rows;
+int jl_kv_write_dev(jl_ctx *ctx, const jl_kv_cache *cache, const jl_kv_rows *rows, void *stream);
+int jl_kv_read_dev(jl_ctx *ctx, const jl_kv_cache *cache, const jl_kv_rows *rows, void *stream);
+
+/* Attention of ntok new tokens over the cache, which holds their own keys and values already.  Token t of sequence seq[t] (null: t) sees the positions from
+ * max(0, len[t] - window) (window 0: from 0) to len[t] - 1, so one call serves a decode batch (a token a sequence), drafted tokens, prompts (len = position + 1),
+ * and an encoder's states (every token the same len).  Query head h reads key head h / (n_head / n_kv):
+ *     s_p = scale * (q . k_p)            softcap > 0: softcap * tanh(s_p / softcap)
+ *     out = sum_p e^(s_p) v_p / (sum_p e^(s_p) + e^(sink[h]))        sink null: without it
+ *     lse = ln of that denominator                                   lse null: not wanted
+ * q [ntok][q_stride] of q_type, out [ntok][out_stride] of out_type (JL_TYPE_F32, _F16, _BF16; strides in elements, 0: n_head * d), lse [ntok][n_head] f32.
+ * A token that sees nothing (len 0, no such sequence, no pages) has zeros, lse -infinity or its sink.  len counts at most the table's positions.  Sums are f32, and q and the weights
+ * keep 22 bits or more (16 of the weights over a bf16 cache where out is 16 bits wide); a token's result does not depend on the other tokens of the call but in the last bits, by
+ * where the cache was cut among the workgroups.  Infinities and NaNs in rows that a token does not see change nothing of its result.
+ * Tokens of one sequence share the reads of its rows where they follow each other.  q 16-byte aligned, its stride a multiple of 16 bytes; n_head a multiple of n_kv.  out overlaps no
+ * other operand.  Two launches; the workspace (jl_reserve_attend) is the context's, of one size for a row width whatever the tokens, and a buffer that is outgrown
+ * lives until the context goes, so a captured graph that holds its address stays valid.  The reference's attention is another part of its device seam
+ * (engine/nn/device.go:1096-1176). */
+typedef struct jl_attend {
+    int ntok, n_head;
+    const void *q;
+    int q_type;
+    size_t q_stride;
+    void *out;
+    int out_type;
+    size_t out_stride;
+    const uint32_t *seq, *len;
+    float scale;
+    int window;
+    float softcap;
+    const float *sink;
+    float *lse;
+} jl_attend;
+int jl_attend_dev(jl_ctx *ctx, const jl_kv_cache *cache, const jl_attend *g, void *stream);
+/* Sizes the workspace for jl_attend_dev calls over rows of up to max_d elements. */
+int jl_reserve_attend(jl_ctx *ctx, int max_d);
+
+/* A token a row of logits [rows][stride] of `type` (JL_TYPE_F32, _F16, _BF16; stride 0: n), by a given number u[row] in [0, 1).  With the row's temperature T and
+ *     w_i = e^((x_i - max) / T)          order: x descending, on a tie the lower index first
+ *     kept = the shortest of: the first top_k (0: all); the shortest beginning of the order whose sum of w reaches top_p of that of the first top_k (1 or more:
+ *            all); those with w >= min_p (0: all); one at least
+ *     token = the first kept i, by index, for which the sum of the kept w up to i exceeds u times the sum of all kept
+ *     prob = its w over that sum        (null: not wanted)
+ * T of 0 or less, or no number: the largest, the first of several.  An infinity is larger than the rest and shares with its equals; -infinity and NaN are never
+ * taken; a row without anything else gets the token n and prob 0.  u of 1 or more, or no number: the last kept.  w is f64's to 2^-44, sums are exact in 64 bits whole numbers, so a
+ * row's token does not depend on the call it is in.  temperature (null: ones), top_k, top_p, min_p (null: off) and u are device memory, [rows].
+ * n up to 524288, rows up to 1048576. */
+typedef struct jl_sample {
+    int rows, n;
+    const void *logits;
+    int type;
+    size_t stride;
+    const float *temperature;
+    const uint32_t *top_k;
+    const float *top_p, *min_p, *u;
+    uint32_t *token;
+    float *prob;
+} jl_sample;
+int jl_sample_dev(jl_ctx *ctx, const jl_sample *g, void *stream);
 
 /* ---- mixture of experts (device pointers) ----------------------------- */
 

@@ -83,6 +83,34 @@ class AdapterGroup(C.Structure):
                 ("k", C.c_int), ("ids", C.c_void_p), ("ntok", C.c_int)]
 
 
+class KvCache(C.Structure):
+    """jl_kv_cache."""
+    _fields_ = [("type", C.c_int), ("n_kv", C.c_int), ("d", C.c_int), ("page_size", C.c_int), ("n_page", C.c_int), ("k", C.c_void_p),
+                ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p), ("page_stride", C.c_size_t),
+                ("head_stride", C.c_size_t), ("row_stride", C.c_size_t), ("table", C.c_void_p), ("n_seq", C.c_int),
+                ("table_pages", C.c_int), ("table_stride", C.c_int)]
+
+
+class KvRows(C.Structure):
+    """jl_kv_rows."""
+    _fields_ = [("ntok", C.c_int), ("k", C.c_void_p), ("v", C.c_void_p), ("type", C.c_int), ("k_stride", C.c_size_t),
+                ("v_stride", C.c_size_t), ("seq", C.c_void_p), ("pos", C.c_void_p)]
+
+
+class Attend(C.Structure):
+    """jl_attend."""
+    _fields_ = [("ntok", C.c_int), ("n_head", C.c_int), ("q", C.c_void_p), ("q_type", C.c_int), ("q_stride", C.c_size_t),
+                ("out", C.c_void_p), ("out_type", C.c_int), ("out_stride", C.c_size_t), ("seq", C.c_void_p), ("len", C.c_void_p),
+                ("scale", C.c_float), ("window", C.c_int), ("softcap", C.c_float), ("sink", C.c_void_p), ("lse", C.c_void_p)]
+
+
+class Sample(C.Structure):
+    """jl_sample."""
+    _fields_ = [("rows", C.c_int), ("n", C.c_int), ("logits", C.c_void_p), ("type", C.c_int), ("stride", C.c_size_t),
+                ("temperature", C.c_void_p), ("top_k", C.c_void_p), ("top_p", C.c_void_p), ("min_p", C.c_void_p), ("u", C.c_void_p),
+                ("token", C.c_void_p), ("prob", C.c_void_p)]
+
+
 SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 
 # name -> (restype, argtypes); every symbol include/jlmi.h declares
@@ -147,6 +175,11 @@ SIGNATURES = {
     "jl_moe_select_dev": (_int, [_vp, _vp, _int, _int, C.POINTER(MoeSelect), _vp, _int, _vp, _vp]),
     "jl_adapter_group_dev": (_int, [_vp, C.POINTER(AdapterGroup), _vp]),
     "jl_reserve_adapters": (_int, [_vp, _int, _int, _int]),
+    "jl_kv_write_dev": (_int, [_vp, C.POINTER(KvCache), C.POINTER(KvRows), _vp]),
+    "jl_kv_read_dev": (_int, [_vp, C.POINTER(KvCache), C.POINTER(KvRows), _vp]),
+    "jl_attend_dev": (_int, [_vp, C.POINTER(KvCache), C.POINTER(Attend), _vp]),
+    "jl_reserve_attend": (_int, [_vp, _int]),
+    "jl_sample_dev": (_int, [_vp, C.POINTER(Sample), _vp]),
     "jl_moe_group_dev": (_int, [_vp, _vp, _int, _int, _int, _int, _vp, _vp, _vp, _vp]),
     "jl_moe_matvec_dev": (_int, [_vp, _vp, _vp, _int, _vp, _vp, _vp, _vp, _vp, _vp, _int, _int, _int, _int, _vp]),
     "jl_moe_matvec_packed_dev": (_int, [_vp, _vp, _vp, _int, C.POINTER(PackedBank), C.POINTER(PackedBank), _vp, _vp, _vp,
@@ -180,6 +213,6 @@ def load():
         for name, (res, args) in SIGNATURES.items():
             fn = getattr(lib, name)
             fn.restype, fn.argtypes = res, args
-        _calls.bind({n: C.cast(getattr(lib, n), C.c_void_p).value for n in SIGNATURES}, quant.BLOCK, PackedBank)
+        _calls.bind({n: C.cast(getattr(lib, n), C.c_void_p).value for n in SIGNATURES}, quant.BLOCK, PackedBank, KvCache)
         _lib = lib
     return _lib

@@ -213,6 +213,12 @@ struct jl_ctx {
     void* adapter_old[64] = {};   // (each at least twice the one before)
     int adapter_olds = 0;
 
+    // partial sums of an attention call whose sequences several workgroups share, and the buffers it outgrew (as the adapters')
+    void* attend_ws = nullptr;
+    size_t attend_ws_bytes = 0;
+    void* attend_old[64] = {};
+    int attend_olds = 0;
+
     // host-pointer seam state
     std::map<const void*, Resident> resident;
     void* stage_x = nullptr;    // device
@@ -2238,6 +2244,13 @@ int jl_ctx_create(jl_ctx** out, const jl_options* opts) {
     for (const char* form : {"l16_1", "l32_1", "l64_1", "wg_1", "wg_2", "wg_4", "wg_8", "wg_16"})
         for (const char* any : {"", "_any"}) names.push_back(std::string("jl_norm_rows_") + form + any);
     for (const char* g : {"g1", "g2", "g3", "g4", "g3p", "g4p", "g6p", "g8p", "g12p", "g16p"}) names.push_back(std::string("jl_moe_select_") + g);
+    for (const char* n : {"jl_kv_write", "jl_kv_read", "jl_sample"}) names.push_back(n);
+    for (const char* form : {"d64_n1", "d64_n2", "d128_n1", "d128_n2", "d256_n1"}) names.push_back(std::string("jl_attend_join_") + form);
+    for (const char* t : {"f16", "i8", "bf16"})
+        for (const char* d : {"_d64", "_d128", "_d256"})
+            for (const char* q : {"_q1", strcmp(t, "bf16") ? "_q2" : "_q3"})
+                for (const char* nt : {"_n1", "_n2"})
+                    if (strcmp(d, "_d256") || !strcmp(nt, "_n1")) names.push_back(std::string("jl_attend_") + t + d + q + nt);
     names.push_back("jl_adapter_sum");
     names.push_back("jl_adapter_group");
     for (const char* t : {"f32", "f16", "bf16"}) {
@@ -2376,6 +2389,8 @@ void jl_ctx_destroy(jl_ctx* c) {
     if (c->moe_route_ws) (void)H->Free(c->moe_route_ws);
     if (c->adapter_ws) (void)H->Free(c->adapter_ws);
     for (int i = 0; i < c->adapter_olds; i++) (void)H->Free(c->adapter_old[i]);
+    if (c->attend_ws) (void)H->Free(c->attend_ws);
+    for (int i = 0; i < c->attend_olds; i++) (void)H->Free(c->attend_old[i]);
     for (auto& kv : c->layers)
         if (kv.second.mem) (void)H->Free(kv.second.mem);
     if (c->one_group) (void)H->Free(c->one_group);
@@ -2537,17 +2552,19 @@ int jl_norm_rows_dev(jl_ctx* c, const jl_norm_rows* g, void* stream) {
 }
 
 namespace {
-// The adapter calls' workspace: a buffer that is outgrown is kept (a captured graph may hold its address).
-int adapter_ws_ensure(jl_ctx* c, size_t need) {
-    if (c->adapter_ws_bytes >= need) return JL_OK;
+// A workspace whose outgrown buffers are kept (a captured graph may hold their address).
+int kept_ws_ensure(jl_ctx* c, void** ws, size_t* have, void** old, int* olds, size_t need) {
+    if (*have >= need) return JL_OK;
     void* p = nullptr;
-    need = std::max(need, 2 * c->adapter_ws_bytes);
+    need = std::max(need, 2 * *have);
     HIP_TRY(c, H->Malloc(&p, need));
-    if (c->adapter_ws) c->adapter_old[c->adapter_olds++] = c->adapter_ws;
-    c->adapter_ws = p;
-    c->adapter_ws_bytes = need;
+    if (*ws) old[(*olds)++] = *ws;
+    *ws = p;
+    *have = need;
     return JL_OK;
 }
+int adapter_ws_ensure(jl_ctx* c, size_t need) { return kept_ws_ensure(c, &c->adapter_ws, &c->adapter_ws_bytes, c->adapter_old, &c->adapter_olds, need); }
+int attend_ws_ensure(jl_ctx* c, size_t need) { return kept_ws_ensure(c, &c->attend_ws, &c->attend_ws_bytes, c->attend_old, &c->attend_olds, need); }
 }  // namespace
 
 namespace {
@@ -3029,6 +3046,147 @@ int jl_moe_select_dev(jl_ctx* c, const float* logits, int rows, int n_expert, co
     const bool packed = ng > 4 || (ng > 2 && (c->tune.moe_select ? c->tune.moe_select == 1 : rows >= 16 * c->num_cu));
     name << "jl_moe_select_g" << ng << (packed ? "p" : "");
     return launch(c, name, (unsigned)((rows + a.waves - 1) / a.waves), 1, 64u * a.waves, 0, pick_stream(c, stream), params);
+}
+
+/* ------------------------------------------------ a paged cache, attention over it, sampling */
+
+namespace {
+// The cache as the kernels take it: JL_OK, JL_DECLINED or an error.
+int kv_view(jl_ctx* c, const jl_kv_cache* g, const char* what, KvArgs* a) {
+    if (!g) return fail(c, JL_ERR_ARG, "%s: no cache", what);
+    if (g->n_kv <= 0 || g->d <= 0 || g->page_size <= 0 || g->n_page <= 0 || g->n_seq <= 0 || g->table_pages <= 0)
+        return fail(c, JL_ERR_ARG, "%s: a cache of %d heads of %d, %d pages of %d, %d sequences of %d pages", what, g->n_kv, g->d, g->n_page, g->page_size,
+                    g->n_seq, g->table_pages);
+    if (!g->k || !g->v || !g->table) return fail(c, JL_ERR_ARG, "%s: null cache", what);
+    const bool i8 = g->type == JL_TYPE_I8;
+    if (i8 && (!g->k_scale || !g->v_scale)) return fail(c, JL_ERR_ARG, "%s: an 8-bit cache has scales", what);
+    if (g->table_stride && g->table_stride < g->table_pages) return fail(c, JL_ERR_ARG, "%s: table_stride is shorter than a sequence's pages", what);
+    if ((!i8 && g->type != JL_TYPE_F16 && g->type != JL_TYPE_BF16) || g->d % 16 != 0 || g->d > 256) return JL_DECLINED;
+    if (g->page_size < 16 || (g->page_size & (g->page_size - 1))) return JL_DECLINED;
+    if ((unsigned long long)g->table_pages * (unsigned)g->page_size > 1ull << 31) return JL_DECLINED;
+    a->shift = __builtin_ctz((unsigned)g->page_size);
+    a->row_stride = g->row_stride ? g->row_stride : (size_t)g->d;
+    a->head_stride = g->head_stride ? g->head_stride : a->row_stride * g->page_size;
+    a->page_stride = g->page_stride ? g->page_stride : a->head_stride * g->n_kv;
+    if (a->row_stride < (size_t)g->d || a->head_stride < (size_t)g->d || a->page_stride < (size_t)g->d)
+        return fail(c, JL_ERR_ARG, "%s: a stride is shorter than a row", what);
+    if ((a->row_stride | a->head_stride | a->page_stride) & 15) return JL_DECLINED;
+    if (!aligned16(g->k) || !aligned16(g->v) || !aligned16(g->k_scale) || !aligned16(g->v_scale) || ((uintptr_t)g->table & 3)) return JL_DECLINED;
+    a->k = g->k; a->v = g->v; a->k_scale = g->k_scale; a->v_scale = g->v_scale; a->table = g->table;
+    a->type = g->type; a->n_kv = g->n_kv; a->d = g->d;
+    a->n_page = (uint32_t)g->n_page; a->n_seq = (uint32_t)g->n_seq; a->table_pages = (uint32_t)g->table_pages;
+    a->table_stride = (uint32_t)(g->table_stride ? g->table_stride : g->table_pages);
+    return JL_OK;
+}
+
+int kv_rows(jl_ctx* c, const jl_kv_cache* cache, const jl_kv_rows* g, void* stream, bool write) {
+    const char* const what = write ? "kv write" : "kv read";
+    if (!c) return JL_ERR_ARG;
+    KvRowsArgs a;
+    if (!g || g->ntok <= 0 || !g->pos || (!g->k && !g->v)) return fail(c, JL_ERR_ARG, "%s: bad operand", what);
+    int rc = kv_view(c, cache, what, &a.c);
+    if (rc != JL_OK) return rc;
+    const size_t n = (size_t)cache->n_kv * cache->d;
+    a.k_stride = g->k_stride ? g->k_stride : n;
+    a.v_stride = g->v_stride ? g->v_stride : n;
+    if (a.k_stride < n || a.v_stride < n) return fail(c, JL_ERR_ARG, "%s: a stride is shorter than a token", what);
+    const int b = plain_bytes(g->type);
+    if (!b) return JL_DECLINED;
+    if ((((uintptr_t)g->k | (uintptr_t)g->v) & (b - 1)) || (((uintptr_t)g->seq | (uintptr_t)g->pos) & 3)) return JL_DECLINED;
+    a.vec = aligned16(g->k) && aligned16(g->v) && (a.k_stride * b) % 16 == 0 && (a.v_stride * b) % 16 == 0;
+    a.k = g->k; a.v = g->v; a.seq = g->seq; a.pos = g->pos; a.ntok = g->ntok; a.type = g->type;
+    a.lanes = cache->d <= 64 ? 8 : cache->d <= 128 ? 16 : 32;
+    const unsigned long long rows = (unsigned long long)g->ntok * cache->n_kv, groups = (rows + 256 / a.lanes - 1) / (256 / a.lanes);
+    if (groups * 256 > 0xffffffffull) return JL_DECLINED;   // threads a launch can have
+    HIP_TRY(c, H->SetDevice(c->device));
+    void* params[] = {&a};
+    return launch(c, write ? "jl_kv_write" : "jl_kv_read", (unsigned)groups, 2, 256, 0, pick_stream(c, stream), params);
+}
+}  // namespace
+
+int jl_kv_write_dev(jl_ctx* c, const jl_kv_cache* cache, const jl_kv_rows* g, void* stream) { return kv_rows(c, cache, g, stream, true); }
+int jl_kv_read_dev(jl_ctx* c, const jl_kv_cache* cache, const jl_kv_rows* g, void* stream) { return kv_rows(c, cache, g, stream, false); }
+
+namespace {
+// Workgroups of an attention call: what the chip holds at once (their registers allow two of four wavefronts a CU, one for rows above 128).
+int attend_wgs(const jl_ctx* c, int d) { return (d > 128 ? 1 : 2) * c->num_cu; }
+size_t attend_part_bytes(const jl_ctx* c, int d) {   // two units a workgroup, of up to two tiles of sixteen columns
+    const int row = d <= 64 ? 64 : d <= 128 ? 128 : 256;
+    return (size_t)attend_wgs(c, d) * 2 * (d > 128 ? 16 : 32) * (row + 2) * 4;
+}
+}  // namespace
+
+int jl_reserve_attend(jl_ctx* c, int max_d) {
+    if (!c) return JL_ERR_ARG;
+    if (max_d <= 0) return fail(c, JL_ERR_ARG, "reserve attend: rows of %d", max_d);
+    if (max_d > 256) return JL_DECLINED;
+    HIP_TRY(c, H->SetDevice(c->device));
+    return attend_ws_ensure(c, std::max(attend_part_bytes(c, std::min(max_d, 128)), attend_part_bytes(c, max_d)));
+}
+
+int jl_attend_dev(jl_ctx* c, const jl_kv_cache* cache, const jl_attend* g, void* stream) {
+    if (!c) return JL_ERR_ARG;
+    AttendArgs a;
+    if (!g || !g->q || !g->out || !g->len || g->ntok <= 0 || g->n_head <= 0) return fail(c, JL_ERR_ARG, "attend: bad operand");
+    int rc = kv_view(c, cache, "attend", &a.c);
+    if (rc != JL_OK) return rc;
+    if (!std::isfinite(g->scale) || !(g->softcap >= 0.f) || !std::isfinite(g->softcap) || g->window < 0)
+        return fail(c, JL_ERR_ARG, "attend: scale=%g softcap=%g window=%d", (double)g->scale, (double)g->softcap, g->window);
+    const size_t n = (size_t)g->n_head * cache->d;
+    a.q_stride = g->q_stride ? g->q_stride : n;
+    a.out_stride = g->out_stride ? g->out_stride : n;
+    if (a.q_stride < n || a.out_stride < n) return fail(c, JL_ERR_ARG, "attend: a stride is shorter than a token");
+    const int qb = plain_bytes(g->q_type), ob = plain_bytes(g->out_type);
+    if (!qb || !ob || g->n_head % cache->n_kv != 0) return JL_DECLINED;
+    if (!aligned16(g->q) || (a.q_stride * qb) % 16 != 0 || ((uintptr_t)g->out & (ob - 1))) return JL_DECLINED;
+    if (((uintptr_t)g->len | (uintptr_t)g->seq | (uintptr_t)g->sink | (uintptr_t)g->lse) & 3) return JL_DECLINED;
+    a.q = g->q; a.out = g->out; a.seq = g->seq; a.len = g->len; a.sink = g->sink; a.lse = g->lse;
+    a.ntok = g->ntok; a.n_head = g->n_head; a.group = g->n_head / cache->n_kv; a.q_type = g->q_type; a.out_type = g->out_type;
+    a.window = g->window; a.scale = g->scale; a.cap = g->softcap;
+    a.out_vec = ((uintptr_t)g->out & (4 * ob - 1)) == 0 && a.out_stride % 4 == 0;
+    const int row = cache->d <= 64 ? 64 : cache->d <= 128 ? 128 : 256;
+    // Columns: a token's heads that share a key head, and with more tokens than sequences those of as many of a sequence's tokens as there are on average.
+    const int most = std::max(1, g->ntok / cache->n_seq);
+    const int nt = row < 256 && (long)a.group * most > 16 ? 2 : 1;
+    a.per = std::clamp(16 * nt / a.group, 1, most);
+    a.units = (g->ntok + a.per - 1) / a.per;
+    a.blocks = a.per > 1 ? 1 : (a.group + 16 * nt - 1) / (16 * nt);
+    // No more workgroups than there can be chunks of 128 positions.
+    const unsigned long long chunks = (unsigned long long)g->ntok * cache->n_kv * a.blocks * (((unsigned long long)cache->table_pages * cache->page_size + 127) / 128 + 1);
+    a.wgs = (int)std::min<unsigned long long>(attend_wgs(c, cache->d), chunks);
+    HIP_TRY(c, H->SetDevice(c->device));
+    rc = attend_ws_ensure(c, attend_part_bytes(c, cache->d));
+    if (rc != JL_OK) return rc;
+    a.part = (float*)c->attend_ws;
+    const bool bf = cache->type == JL_TYPE_BF16;
+    const int pieces = bf ? (g->q_type == JL_TYPE_BF16 ? 1 : 3) : g->q_type == JL_TYPE_F32 ? 2 : 1;
+    Name name, join;
+    name << "jl_attend_" << (bf ? "bf16" : cache->type == JL_TYPE_F16 ? "f16" : "i8") << "_d" << row << "_q" << pieces << "_n" << nt;
+    join << "jl_attend_join_d" << row << "_n" << nt;
+    void* params[] = {&a};
+    const hipStream_t st = pick_stream(c, stream);
+    rc = launch(c, name, (unsigned)a.wgs, 1, 256, 0, st, params);
+    return rc == JL_OK ? launch(c, join, (unsigned)a.wgs, 1, 256, 0, st, params) : rc;
+}
+
+int jl_sample_dev(jl_ctx* c, const jl_sample* g, void* stream) {
+    if (!c) return JL_ERR_ARG;
+    if (!g || !g->logits || !g->u || !g->token || g->rows <= 0 || g->n <= 0) return fail(c, JL_ERR_ARG, "sample: bad operand");
+    SampleArgs a;
+    a.stride = g->stride ? g->stride : (size_t)g->n;
+    if (a.stride < (size_t)g->n) return fail(c, JL_ERR_ARG, "sample: a stride is shorter than a row");
+    const int b = plain_bytes(g->type);
+    if (!b || g->n > 524288) return JL_DECLINED;   // sums of 2^19 weights of up to 2^44
+    if (((uintptr_t)g->logits & (b - 1)) ||
+        (((uintptr_t)g->temperature | (uintptr_t)g->top_k | (uintptr_t)g->top_p | (uintptr_t)g->min_p | (uintptr_t)g->u | (uintptr_t)g->token | (uintptr_t)g->prob) & 3))
+        return JL_DECLINED;
+    if (g->rows > 1 << 20) return JL_DECLINED;
+    a.logits = g->logits; a.temperature = g->temperature; a.top_k = g->top_k; a.top_p = g->top_p; a.min_p = g->min_p; a.u = g->u; a.token = g->token;
+    a.prob = g->prob; a.rows = g->rows; a.n = g->n; a.type = g->type;
+    a.vec = ((uintptr_t)g->logits & (4 * b - 1)) == 0 && a.stride % 4 == 0;
+    HIP_TRY(c, H->SetDevice(c->device));
+    void* params[] = {&a};
+    return launch(c, "jl_sample", (unsigned)g->rows, 1, 1024, 0, pick_stream(c, stream), params);
 }
 
 int jl_moe_logits_dev(jl_ctx* c, float* logits, int wtype, const void* w, const float* x, int n_expert, int k,

@@ -631,3 +631,62 @@ struct AdapterArgs {
     int passes, slices;                    // of adapter_down; slices 0 in adapter_up: u has been made
     int up_sets;                           // sets of 256 columns a workgroup of adapter_cols
 };
+
+// A paged cache of keys and values (kernels/kv_cache.h, kernels/attend.h): rows of d elements, [page][head][position in the page].
+struct KvArgs {
+    void* k;
+    void* v;
+    float* k_scale;          // 8-bit rows: [n_page][n_kv][page size], else null
+    float* v_scale;
+    const uint32_t* table;   // [n_seq][table_stride] pages of each sequence, table_pages of them
+    size_t page_stride, head_stride, row_stride;   // elements
+    int type, n_kv, d, shift;                      // page size = 1 << shift
+    uint32_t n_page, n_seq, table_stride, table_pages;
+};
+
+// Rows written into the cache, or read back from it.
+struct KvRowsArgs {
+    KvArgs c;
+    void* k;                 // [ntok][k_stride], a token's heads back to back; null: not these
+    void* v;
+    const uint32_t* seq;     // [ntok], or null: token t is of sequence t
+    const uint32_t* pos;     // [ntok]
+    size_t k_stride, v_stride;   // elements
+    int ntok, type, vec;     // vec: rows on 16-byte boundaries
+    int lanes;               // a row's, 8 elements each: 8, 16 or 32
+};
+
+// Attention of new tokens over the cache (kernels/attend.h).
+struct AttendArgs {
+    KvArgs c;
+    const void* q;           // [ntok][q_stride], a token's heads back to back
+    void* out;
+    const uint32_t* seq;     // [ntok], or null: token t is of sequence t
+    const uint32_t* len;     // [ntok]
+    const float* sink;       // [n_head] or null
+    float* lse;              // [ntok][n_head] or null
+    float* part;             // workspace: [2 wgs][columns][row + 2], see attend.h
+    size_t q_stride, out_stride;   // elements
+    int ntok, n_head, group, q_type, out_type;
+    int per;                 // tokens a unit
+    int units;               // ceil(ntok / per)
+    int blocks;              // column blocks a unit (one where per > 1)
+    int wgs;
+    int window;
+    int out_vec;             // out's rows on 16-byte boundaries
+    float scale, cap;
+};
+
+// A token a row of logits (kernels/sample.h).
+struct SampleArgs {
+    const void* logits;      // [rows][stride]
+    const float* temperature;
+    const uint32_t* top_k;
+    const float* top_p;
+    const float* min_p;
+    const float* u;
+    uint32_t* token;
+    float* prob;
+    size_t stride;
+    int rows, n, type, vec;  // vec: rows on 16-byte boundaries
+};

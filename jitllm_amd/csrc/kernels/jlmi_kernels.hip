@@ -736,3 +736,6 @@ extern "C" __global__ __launch_bounds__(256) void jl_adapter_sum(AdapterArgs p) 
     JL_ADAPTER_COLS(T, TYPE, 1) JL_ADAPTER_COLS(T, TYPE, 2) JL_ADAPTER_COLS(T, TYPE, 4) JL_ADAPTER_COLS(T, TYPE, 8)          \
     JL_ADAPTER_UP(T, TYPE, k1, 1, false) JL_ADAPTER_UP(T, TYPE, k2, 2, false) JL_ADAPTER_UP(T, TYPE, many, 1, true)
 JL_ADAPTER(f32, JL_F32) JL_ADAPTER(f16, JL_F16) JL_ADAPTER(bf16, JL_BF16)
+
+// ------------------------------------------------- a cache, attention over it, sampling
+#include "step_kernels.h"

@@ -36,8 +36,12 @@ struct Api {
     decltype(&jl_norm_rows_dev) norm_rows_dev;
     decltype(&jl_moe_select_dev) moe_select_dev;
     decltype(&jl_adapter_group_dev) adapter_group_dev;
+    decltype(&jl_kv_write_dev) kv_write_dev;
+    decltype(&jl_kv_read_dev) kv_read_dev;
+    decltype(&jl_attend_dev) attend_dev;
+    decltype(&jl_sample_dev) sample_dev;
 } api;
-PyObject *host_types, *bank_type;                                  // quant.BLOCK, _lib.PackedBank
+PyObject *host_types, *bank_type, *cache_type;                     // quant.BLOCK, _lib.PackedBank, _lib.KvCache
 PyObject *s_qs, *s_d, *s_sc, *s_row, *s_stride, *s_served;
 
 struct Calls {
@@ -372,6 +376,67 @@ PyObject* py_adapter_group_dev(SIG) {
     return ended(self, unlocked([&] { return api.adapter_group_dev(self->ctx, &g, st); }), "jl_adapter_group_dev");
 }
 
+// ---- a cache, attention over it, sampling
+// The jl_kv_cache that a kv_cache(...) structure holds.
+bool cache_of(PyObject* o, jl_kv_cache* c) {
+    if ((PyObject*)Py_TYPE(o) != cache_type) {
+        PyErr_SetString(PyExc_TypeError, "a cache is what kv_cache(...) returns");
+        return false;
+    }
+    Py_buffer b;
+    if (PyObject_GetBuffer(o, &b, PyBUF_SIMPLE)) return false;
+    const bool ok = b.len == (Py_ssize_t)sizeof *c;
+    if (ok) memcpy(c, b.buf, sizeof *c);
+    else PyErr_SetString(PyExc_TypeError, "a cache structure of another size");
+    PyBuffer_Release(&b);
+    return ok;
+}
+
+PyObject* kv_rows(SIG, const char* name, decltype(&jl_kv_write_dev) f, const char* what) {
+    static const char* const names[] = {"cache", "k", "v", "type", "pos", "ntok", "seq", "k_stride", "v_stride", "stream"};
+    PyObject* a[10];
+    if (!take(name, names, 6, 10, av, an, kw, a)) return nullptr;
+    jl_kv_cache c;
+    jl_kv_rows g;
+    memset(&g, 0, sizeof g);
+    void *pos, *seq, *st;
+    if (!cache_of(a[0], &c) || !opt(a[1], &g.k) || !opt(a[2], &g.v) || !num(a[3], &g.type) || !opt(a[4], &pos) || !num(a[5], &g.ntok) || !opt(a[6], &seq) ||
+        !size(a[7], &g.k_stride) || !size(a[8], &g.v_stride) || !stream_of(a[9], &st))
+        return nullptr;
+    g.pos = (const uint32_t*)pos; g.seq = (const uint32_t*)seq;
+    return ended(self, unlocked([&] { return f(self->ctx, &c, &g, st); }), what);
+}
+PyObject* py_kv_write_dev(SIG) { return kv_rows(self, av, an, kw, "kv_write_dev", api.kv_write_dev, "jl_kv_write_dev"); }
+PyObject* py_kv_read_dev(SIG) { return kv_rows(self, av, an, kw, "kv_read_dev", api.kv_read_dev, "jl_kv_read_dev"); }
+
+PyObject* py_attend_dev(SIG) {
+    TAKE("attend_dev", 7, "cache", "out", "q", "n_head", "len", "ntok", "scale", "seq", "q_type", "out_type", "q_stride", "out_stride", "window", "softcap", "sink", "lse",
+         "stream");
+    jl_kv_cache c;
+    jl_attend g;
+    memset(&g, 0, sizeof g);
+    void *q, *len, *seq, *sink, *lse, *st;
+    if (!cache_of(a[0], &c) || !ptr(a[1], &g.out) || !ptr(a[2], &q) || !num(a[3], &g.n_head) || !ptr(a[4], &len) || !num(a[5], &g.ntok) || !real(a[6], &g.scale) ||
+        !opt(a[7], &seq) || !opt_num(a[8], &g.q_type) || !opt_num(a[9], &g.out_type) || !size(a[10], &g.q_stride) || !size(a[11], &g.out_stride) ||
+        !opt_num(a[12], &g.window) || !real(a[13], &g.softcap) || !opt(a[14], &sink) || !opt(a[15], &lse) || !stream_of(a[16], &st))
+        return nullptr;
+    g.q = q; g.len = (const uint32_t*)len; g.seq = (const uint32_t*)seq; g.sink = (const float*)sink; g.lse = (float*)lse;
+    return ended(self, unlocked([&] { return api.attend_dev(self->ctx, &c, &g, st); }), "jl_attend_dev");
+}
+
+PyObject* py_sample_dev(SIG) {
+    TAKE("sample_dev", 5, "logits", "rows", "n", "u", "token", "type", "stride", "temperature", "top_k", "top_p", "min_p", "prob", "stream");
+    jl_sample g;
+    memset(&g, 0, sizeof g);
+    void *logits, *u, *token, *t, *k, *p, *m, *prob, *st;
+    if (!ptr(a[0], &logits) || !num(a[1], &g.rows) || !num(a[2], &g.n) || !ptr(a[3], &u) || !ptr(a[4], &token) || !opt_num(a[5], &g.type) || !size(a[6], &g.stride) ||
+        !opt(a[7], &t) || !opt(a[8], &k) || !opt(a[9], &p) || !opt(a[10], &m) || !opt(a[11], &prob) || !stream_of(a[12], &st))
+        return nullptr;
+    g.logits = logits; g.u = (const float*)u; g.token = (uint32_t*)token; g.temperature = (const float*)t; g.top_k = (const uint32_t*)k; g.top_p = (const float*)p;
+    g.min_p = (const float*)m; g.prob = (float*)prob;
+    return ended(self, unlocked([&] { return api.sample_dev(self->ctx, &g, st); }), "jl_sample_dev");
+}
+
 // ---- host memory: numpy arrays, checked
 bool is(PyObject* o, int type) {
     return PyArray_Check(o) && PyArray_TYPE((PyArrayObject*)o) == type && PyArray_ISNOTSWAPPED((PyArrayObject*)o);
@@ -471,6 +536,17 @@ PyMethodDef methods[] = {
       "adapter_group_dev(outs, bases, rows, a, b, t, n_adapter, rank, x, k, ids, ntok, scale=None, ranks=None, x_type=0, stream=None).\n"
       "outs[i][t] = bases[i][t] + scale[ids[t]] * b[i][ids[t]] (a[i][ids[t]] x[t]) for up to four projections that read one x;\n"
       "bases (or an entry of it) None: zeros."),
+    M(kv_write_dev,
+      "kv_write_dev(cache, k, v, type, pos, ntok, seq=None, k_stride=0, v_stride=0, stream=None).  Rows of ntok tokens, [ntok][n_kv][d] in\n"
+      "f32 (type 0), f16 (1) or bf16 (30), to positions pos of sequences seq (None: token t to sequence t) of a kv_cache(...); k or v None: not these."),
+    M(kv_read_dev, "kv_read_dev(cache, k, v, type, pos, ntok, seq=None, k_stride=0, v_stride=0, stream=None): the same rows back."),
+    M(attend_dev,
+      "attend_dev(cache, out, q, n_head, len, ntok, scale, seq=None, q_type=0, out_type=0, q_stride=0, out_stride=0, window=0, softcap=0.0,\n"
+      "sink=None, lse=None, stream=None).  Attention of tokens q [ntok][n_head][d] over a kv_cache(...): token t of sequence seq[t]\n"
+      "(None: t) sees its positions below len[t], the last `window` of them (0: all)."),
+    M(sample_dev,
+      "sample_dev(logits, rows, n, u, token, type=0, stride=0, temperature=None, top_k=None, top_p=None, min_p=None, prob=None,\n"
+      "stream=None).  A token a row by the row's settings (device arrays; None: off) and its number u in [0, 1)."),
     M(MatVec, "MatVec(out, t, w, x, nrows, k).  nn.Device.MatVec: out[0:nrows] = W x over raw GGUF bytes; False = declined."),
     M(MatMul, "MatMul(out, t, w, x, nrows, k, ntok).  JIT.MatMul (/root/reference/engine/nn/matmul.go:27): x [ntok][k] -> out [ntok][nrows]."),
     M(MatVecPacked, "MatVecPacked(out, t, p, x, nrows, k).  JIT.MatVecPacked (/root/reference/engine/nn/packed.go:24);\n"
@@ -480,10 +556,10 @@ PyMethodDef methods[] = {
 
 PyTypeObject calls_type = {PyVarObject_HEAD_INIT(nullptr, 0)};
 
-// bind(addresses by name of the C ABI, the block types host calls serve, the packed bank structure)
+// bind(addresses by name of the C ABI, the block types host calls serve, the packed bank and the cache structure)
 PyObject* py_bind(PyObject*, PyObject* args) {
-    PyObject *fns, *types, *bank;
-    if (!PyArg_ParseTuple(args, "O!OO", &PyDict_Type, &fns, &types, &bank)) return nullptr;
+    PyObject *fns, *types, *bank, *cache;
+    if (!PyArg_ParseTuple(args, "O!OOO", &PyDict_Type, &fns, &types, &bank, &cache)) return nullptr;
 #define FN(field)                                                                     \
     {                                                                                 \
         PyObject* o = PyDict_GetItemString(fns, "jl_" #field);                        \
@@ -494,12 +570,14 @@ PyObject* py_bind(PyObject*, PyObject* args) {
     }
     FN(matvec) FN(matmul) FN(matvec_packed) FN(matmul_packed) FN(matvec_dev) FN(matvec_packed_dev) FN(matvec_group_dev) FN(matmul_dev)
     FN(matmul_packed_dev) FN(layer_ffn_dev) FN(moe_block_dev) FN(moe_block_packed_dev) FN(matmul_mxfp4_bf16_dev) FN(matmul_mxfp4_packed_bf16_dev)
-    FN(norm_rows_dev) FN(moe_select_dev) FN(adapter_group_dev)
+    FN(norm_rows_dev) FN(moe_select_dev) FN(adapter_group_dev) FN(kv_write_dev) FN(kv_read_dev) FN(attend_dev) FN(sample_dev)
 #undef FN
     Py_INCREF(types);
     Py_INCREF(bank);
     Py_XSETREF(host_types, types);
     Py_XSETREF(bank_type, bank);
+    Py_INCREF(cache);
+    Py_XSETREF(cache_type, cache);
     Py_RETURN_NONE;
 }
 

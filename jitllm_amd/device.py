@@ -144,6 +144,18 @@ class Device(_calls.Calls):
         """Size the workspace of adapter_group_dev for up to max_tok tokens, n projections and rank max_rank."""
         self._served(self._l.jl_reserve_adapters(self._ctx, max_tok, n, max_rank), "jl_reserve_adapters")
 
+    def reserve_attend(self, max_d):
+        """Size the workspace of attend_dev for rows of up to max_d elements."""
+        self._served(self._l.jl_reserve_attend(self._ctx, max_d), "jl_reserve_attend")
+
+    @staticmethod
+    def kv_cache(t, n_kv, d, page_size, n_page, k, v, table, n_seq, table_pages, k_scale=None, v_scale=None, page_stride=0,
+                 head_stride=0, row_stride=0, table_stride=0):
+        """jl_kv_cache: pools of pages and the sequences' page table (device addresses), for kv_write_dev, kv_read_dev and attend_dev."""
+        return _lib.KvCache(int(t), int(n_kv), int(d), int(page_size), int(n_page), _ptr(k), _ptr(v), _opt(k_scale), _opt(v_scale),
+                            int(page_stride), int(head_stride), int(row_stride), _ptr(table), int(n_seq), int(table_pages),
+                            int(table_stride))
+
     def probe_dev(self, kind, src, nbytes, grid=0, block=0, stream=None):
         """An empty kernel (kind 0) or a kernel that only reads nbytes at src (kind 1)."""
         return self._served(self._l.jl_probe_dev(self._ctx, kind, src, nbytes, grid, block, stream), "jl_probe_dev")

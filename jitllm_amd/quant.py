@@ -5,6 +5,7 @@ reference's quant.Type uses (/root/reference/format/quant/types.go:14-85).
 """
 
 F32, F16, BF16 = 0, 1, 30     # plain values: normed rows, adapters, router weights
+I8 = 24                       # rows of a cache, one f32 scale each
 Q8_0 = 8
 Q4_K = 12
 Q6_K = 14
