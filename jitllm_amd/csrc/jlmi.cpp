@@ -123,6 +123,9 @@ struct Name {
     operator const char*() const { return s; }
 };
 
+// Whether jl_attend_many_* of rows of `row` and `pieces` of q has a form of two column tiles a wavefront (q's pieces and the sums fit its registers).
+bool attend_two_tiles(int row, int pieces) { return pieces == 1 ? row < 256 : pieces == 2 && row == 64; }
+
 struct Resident {
     void* dev = nullptr;
     size_t bytes = 0;
@@ -2245,12 +2248,14 @@ int jl_ctx_create(jl_ctx** out, const jl_options* opts) {
         for (const char* any : {"", "_any"}) names.push_back(std::string("jl_norm_rows_") + form + any);
     for (const char* g : {"g1", "g2", "g3", "g4", "g3p", "g4p", "g6p", "g8p", "g12p", "g16p"}) names.push_back(std::string("jl_moe_select_") + g);
     for (const char* n : {"jl_kv_write", "jl_kv_read", "jl_sample"}) names.push_back(n);
-    for (const char* form : {"d64_n1", "d64_n2", "d128_n1", "d128_n2", "d256_n1"}) names.push_back(std::string("jl_attend_join_") + form);
+    for (const char* d : {"64", "128", "256"}) names.push_back(std::string("jl_attend_join_d") + d);
     for (const char* t : {"f16", "i8", "bf16"})
         for (const char* d : {"_d64", "_d128", "_d256"})
-            for (const char* q : {"_q1", strcmp(t, "bf16") ? "_q2" : "_q3"})
-                for (const char* nt : {"_n1", "_n2"})
-                    if (strcmp(d, "_d256") || !strcmp(nt, "_n1")) names.push_back(std::string("jl_attend_") + t + d + q + nt);
+            for (const char* q : {"_q1", strcmp(t, "bf16") ? "_q2" : "_q3"}) {
+                for (const char* m : {"", "_m"}) names.push_back(std::string("jl_attend_one_") + t + d + q + m);
+                names.push_back(std::string("jl_attend_many_") + t + d + q + "_n1");
+                if (attend_two_tiles(atoi(d + 2), atoi(q + 2))) names.push_back(std::string("jl_attend_many_") + t + d + q + "_n2");
+            }
     names.push_back("jl_adapter_sum");
     names.push_back("jl_adapter_group");
     for (const char* t : {"f32", "f16", "bf16"}) {
@@ -3070,7 +3075,7 @@ int kv_view(jl_ctx* c, const jl_kv_cache* g, const char* what, KvArgs* a) {
     a->page_stride = g->page_stride ? g->page_stride : a->head_stride * g->n_kv;
     if (a->row_stride < (size_t)g->d || a->head_stride < (size_t)g->d || a->page_stride < (size_t)g->d)
         return fail(c, JL_ERR_ARG, "%s: a stride is shorter than a row", what);
-    if ((a->row_stride | a->head_stride | a->page_stride) & 15) return JL_DECLINED;
+    if (((a->row_stride | a->head_stride | a->page_stride) & 15) || a->row_stride >= 1u << 25) return JL_DECLINED;   // (sixteen rows: 32-bit offsets)
     if (!aligned16(g->k) || !aligned16(g->v) || !aligned16(g->k_scale) || !aligned16(g->v_scale) || ((uintptr_t)g->table & 3)) return JL_DECLINED;
     a->k = g->k; a->v = g->v; a->k_scale = g->k_scale; a->v_scale = g->v_scale; a->table = g->table;
     a->type = g->type; a->n_kv = g->n_kv; a->d = g->d;
@@ -3108,12 +3113,10 @@ int jl_kv_write_dev(jl_ctx* c, const jl_kv_cache* cache, const jl_kv_rows* g, vo
 int jl_kv_read_dev(jl_ctx* c, const jl_kv_cache* cache, const jl_kv_rows* g, void* stream) { return kv_rows(c, cache, g, stream, false); }
 
 namespace {
-// Workgroups of an attention call: what the chip holds at once (their registers allow two of four wavefronts a CU, one for rows above 128).
+// Workgroups of an attention call: what the chip holds at once (two of four wavefronts a CU, by registers and LDS; one for rows above 128).
 int attend_wgs(const jl_ctx* c, int d) { return (d > 128 ? 1 : 2) * c->num_cu; }
-size_t attend_part_bytes(const jl_ctx* c, int d) {   // two units a workgroup, of up to two tiles of sixteen columns
-    const int row = d <= 64 ? 64 : d <= 128 ? 128 : 256;
-    return (size_t)attend_wgs(c, d) * 2 * (d > 128 ? 16 : 32) * (row + 2) * 4;
-}
+int attend_row(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
+size_t attend_part_bytes(int wgs, int d, int cols) { return (size_t)wgs * (2 * (size_t)cols * (attend_row(d) + 2) * 4 + 32); }   // (AtJoin: 32 bytes)
 }  // namespace
 
 int jl_reserve_attend(jl_ctx* c, int max_d) {
@@ -3121,7 +3124,7 @@ int jl_reserve_attend(jl_ctx* c, int max_d) {
     if (max_d <= 0) return fail(c, JL_ERR_ARG, "reserve attend: rows of %d", max_d);
     if (max_d > 256) return JL_DECLINED;
     HIP_TRY(c, H->SetDevice(c->device));
-    return attend_ws_ensure(c, std::max(attend_part_bytes(c, std::min(max_d, 128)), attend_part_bytes(c, max_d)));
+    return attend_ws_ensure(c, attend_part_bytes(attend_wgs(c, 128), std::min(max_d, 128), 128));   // (rows above 128: half the workgroups, half the columns)
 }
 
 int jl_attend_dev(jl_ctx* c, const jl_kv_cache* cache, const jl_attend* g, void* stream) {
@@ -3144,29 +3147,39 @@ int jl_attend_dev(jl_ctx* c, const jl_kv_cache* cache, const jl_attend* g, void*
     a.ntok = g->ntok; a.n_head = g->n_head; a.group = g->n_head / cache->n_kv; a.q_type = g->q_type; a.out_type = g->out_type;
     a.window = g->window; a.scale = g->scale; a.cap = g->softcap;
     a.out_vec = ((uintptr_t)g->out & (4 * ob - 1)) == 0 && a.out_stride % 4 == 0;
-    const int row = cache->d <= 64 ? 64 : cache->d <= 128 ? 128 : 256;
-    // Columns: a token's heads that share a key head, and with more tokens than sequences those of as many of a sequence's tokens as there are on average.
-    const int most = std::max(1, g->ntok / cache->n_seq);
-    const int nt = row < 256 && (long)a.group * most > 16 ? 2 : 1;
-    a.per = std::clamp(16 * nt / a.group, 1, most);
+    const int row = attend_row(cache->d);
+    // Columns: a token's heads that share a key head, and with more tokens than sequences those of as many of a sequence's tokens as there are on average.  Up to
+    // sixteen of them take the form whose wavefronts share the positions, more the one whose wavefronts share the columns.
+    const int most = std::max(1, g->seq ? g->ntok / cache->n_seq : 1);
+    const bool one = most == 1 || (long)a.group * most <= 16;
+    const bool bf = cache->type == JL_TYPE_BF16;
+    // q in one piece where the cache's type holds it; over bf16 three pieces of the weights go with three of q, for a result of 32 bits
+    const int pieces = bf ? (g->q_type == JL_TYPE_BF16 && g->out_type != JL_TYPE_F32 ? 1 : 3) : g->q_type == JL_TYPE_F32 ? 2 : 1;
+    const int nt = one ? 0 : attend_two_tiles(row, pieces) && (long)a.group * most > 64 ? 2 : 1;
+    a.part_cols = one ? 16 : 64 * nt;
+    a.per = std::clamp(a.part_cols / a.group, 1, most);
     a.units = (g->ntok + a.per - 1) / a.per;
-    a.blocks = a.per > 1 ? 1 : (a.group + 16 * nt - 1) / (16 * nt);
+    a.blocks = a.per > 1 ? 1 : (a.group + a.part_cols - 1) / a.part_cols;
+    a.inv_group = 65536 / a.group + 1;
     // No more workgroups than there can be chunks of 128 positions.
-    const unsigned long long chunks = (unsigned long long)g->ntok * cache->n_kv * a.blocks * (((unsigned long long)cache->table_pages * cache->page_size + 127) / 128 + 1);
-    a.wgs = (int)std::min<unsigned long long>(attend_wgs(c, cache->d), chunks);
+    const unsigned long long per_head = ((unsigned long long)cache->table_pages * cache->page_size + 127) / 128 + 1, planes = (unsigned long long)cache->n_kv * a.blocks;
+    a.wgs = (int)std::min<unsigned long long>(attend_wgs(c, cache->d), g->ntok * planes * per_head);
+    a.whole = !one && a.units * planes >= (unsigned)a.wgs;
+    if (a.units * planes > 0xffffffffull / 256) return JL_DECLINED;   // threads a launch can have
     HIP_TRY(c, H->SetDevice(c->device));
-    rc = attend_ws_ensure(c, attend_part_bytes(c, cache->d));
+    rc = a.whole ? JL_OK : attend_ws_ensure(c, attend_part_bytes(a.wgs, cache->d, a.part_cols));
     if (rc != JL_OK) return rc;
     a.part = (float*)c->attend_ws;
-    const bool bf = cache->type == JL_TYPE_BF16;
-    const int pieces = bf ? (g->q_type == JL_TYPE_BF16 ? 1 : 3) : g->q_type == JL_TYPE_F32 ? 2 : 1;
     Name name, join;
-    name << "jl_attend_" << (bf ? "bf16" : cache->type == JL_TYPE_F16 ? "f16" : "i8") << "_d" << row << "_q" << pieces << "_n" << nt;
-    join << "jl_attend_join_d" << row << "_n" << nt;
+    name << "jl_attend_" << (one ? "one_" : "many_") << (bf ? "bf16" : cache->type == JL_TYPE_F16 ? "f16" : "i8") << "_d" << row << "_q" << pieces;
+    if (!one) name << "_n" << nt;
+    else if (a.per > 1) name << "_m";
+    join << "jl_attend_join_d" << row;
     void* params[] = {&a};
     const hipStream_t st = pick_stream(c, stream);
-    rc = launch(c, name, (unsigned)a.wgs, 1, 256, 0, st, params);
-    return rc == JL_OK ? launch(c, join, (unsigned)a.wgs, 1, 256, 0, st, params) : rc;
+    rc = launch(c, name, a.whole ? (unsigned)(a.units * planes) : (unsigned)a.wgs, 1, 256, 0, st, params);
+    if (rc != JL_OK || a.whole) return rc;
+    return launch(c, join, (unsigned)a.wgs, (unsigned)std::min(4, (std::min(a.part_cols, a.group * a.per) + 3) / 4), 256, 0, st, params);
 }
 
 int jl_sample_dev(jl_ctx* c, const jl_sample* g, void* stream) {

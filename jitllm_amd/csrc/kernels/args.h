@@ -665,13 +665,16 @@ struct AttendArgs {
     const uint32_t* len;     // [ntok]
     const float* sink;       // [n_head] or null
     float* lse;              // [ntok][n_head] or null
-    float* part;             // workspace: [2 wgs][columns][row + 2], see attend.h
+    float* part;             // workspace, see attend.h
     size_t q_stride, out_stride;   // elements
     int ntok, n_head, group, q_type, out_type;
     int per;                 // tokens a unit
     int units;               // ceil(ntok / per)
-    int blocks;              // column blocks a unit (one where per > 1)
-    int wgs;
+    int blocks;              // column blocks of a token (one where per > 1)
+    int part_cols;           // columns a block
+    int inv_group;           // 2^16 / group + 1
+    int wgs;                 // workgroups, or their shares of the chunks
+    int whole;               // a unit a workgroup (attend_many)
     int window;
     int out_vec;             // out's rows on 16-byte boundaries
     float scale, cap;

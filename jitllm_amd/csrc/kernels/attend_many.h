@@ -1,0 +1,406 @@
+// Many new tokens over a cache -- prompts, long drafts: more than sixteen columns a unit (attend.h).
+//
+// Each of a workgroup's four wavefronts has NT tiles of sixteen columns; the rows of 64 positions at a time go through LDS, as the fragments the matrix instruction
+// takes (a fragment a kilobyte, a lane's sixteen bytes behind the next lane's: no bank is met twice), so rows are read once for 64 NT columns, and 8-bit values
+// turned into f16 once.  Two wavefronts bring the values, two the keys, of the next 64 positions while all four multiply: one barrier a step.  A wavefront keeps its
+// columns' sums to the end, so nothing is exchanged.  What bounds it is the vector unit: about 120 instructions a tile of columns and 32 positions around the
+// exponentials, beside 24 matrix instructions (16 cycles each) with q in one piece.
+#pragma once
+#include "attend.h"
+
+template <int DP> constexpr int at_stage_words() { return (4 * (DP / 32) + 2 * (DP / 16)) * 256; }   // 64 positions' fragments
+
+// lds: words [2][at_stage_words], then [2] of scales: keys' [64], values' [64]; then [2] of marks [4], and one mark of the span.
+template <int TYPE, int DP, int QP, int PP, int NT>
+__device__ __forceinline__ void attend_many_body(const AttendArgs& p, u32x4* lds, uint64_t* find) {
+    constexpr bool BF = TYPE == JL_BF16, I8 = TYPE == JL_I8;
+    constexpr int C = DP / 16, KC = DP / 32, B = I8 ? 1 : 2, VB = C * B;
+    constexpr int KL = I8 ? KC / 2 : KC, VW = (VB + 3) / 4;
+    constexpr int STAGE = at_stage_words<DP>() / 4;       // in 16-byte pieces
+    constexpr float OFF = BF ? 0.f : JL_AT_OFF;
+    const float inf = __builtin_inff();
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    float* const scales = (float*)(lds + 2 * STAGE);      // [2][128]
+    u32* const marks = (u32*)(scales + 2 * 128);          // [2][4]: tiles on no page, values that are no number, of each half
+
+    AtWork job;
+    u32 unit_end = 0, w = 0;
+    AtJoin join = {0, 0, 0, 0, 0, {0, 0, 0}};
+    if (p.whole) {   // (the last units, which see most of a prompt, first; a key head's on one L2)
+        const u32 planes = (u32)p.c.n_kv * (u32)p.blocks, b = blockIdx.x, i = b / planes, unit = (u32)p.units - 1 - i;
+        job.plane = b - i * planes;
+        job.off = 0;
+        job.first = 0;
+        job.end = ~0ull;
+        unit_end = min((unit + 1) * (u32)p.per, (u32)p.ntok);
+        job.span = at_span<true>(p, unit * (u32)p.per);
+    } else {
+        w = at_group_of(blockIdx.x, (u32)p.wgs);
+        if (!at_work<true>(p, w, find, job)) {
+            if (threadIdx.x == 0) at_join_of<DP>(p)[w] = join;
+            return;
+        }
+    }
+    const u32 row_bytes = (u32)p.c.row_stride * B;
+    const size_t head_bytes = p.c.head_stride * B, page_bytes = p.c.page_stride * B;
+    const u32 in_page = (1u << p.c.shift) - 1;
+    const int half = wave & 1;
+    const bool brings_keys = wave >= 2;
+    // a lane's bytes of a tile's rows, for what its wavefront brings
+    u32 ko[KL];
+#pragma unroll
+    for (int c = 0; c < KL; c++) {
+        const int d = I8 ? 64 * c + 16 * g : 32 * c + 8 * g;
+        ko[c] = d < p.c.d ? n * row_bytes + (u32)d * B : JL_AT_NOWHERE;
+    }
+    const u32 vo = C * n < p.c.d ? 4 * g * row_bytes + (u32)n * VB : JL_AT_NOWHERE;
+
+    for (uint64_t at = job.first; at < job.end;) {
+        const AtSpan span = job.span;
+        const u32 lo = span.lo, hi = span.hi, plane = job.plane, c0 = job.off;
+        const u32 n_chunks = at_chunks(lo, hi), left = (u32)min((uint64_t)(n_chunks - c0), job.end - at);
+        const u32 kv = p.blocks > 1 ? plane / (u32)p.blocks : plane;
+        // steps of 64 positions, from the chunk's first on, up to the last that any token sees
+        const u32 s0 = max(2 * (lo / JL_AT_CHUNK + c0), lo / 64), s1 = min(2 * (lo / JL_AT_CHUNK + c0 + left), (hi + 63) / 64);
+        const u32* const pages = p.c.table + (size_t)span.seq * p.c.table_stride;
+        const char* const from = (const char*)(brings_keys ? p.c.k : p.c.v) + kv * head_bytes;
+        const float* const from_scales = brings_keys ? p.c.k_scale : p.c.v_scale;
+
+        // A value that is no number, in a place that only some of the tokens see, would reach the others as 0 * NaN: such a span is passed over
+        // again, a token at a time, with zeros for what that token does not see.
+        u32 only = ~0u, zlo = lo, zhi = hi;       // the token; what is not zeros
+
+        u32 pg = 0, page[2];
+        auto look = [&](u32 s) {
+            const u32 at0 = (s + (lane >> 1)) * 64 + half * 32 + 16 * (lane & 1);
+            pg = s + (lane >> 1) < s1 && at0 < hi && at0 + 16 > lo ? pages[at0 >> p.c.shift] : ~0u;
+        };
+        u32 st[8 * (VW > KL ? VW : KL)];
+        float sc = 0.f;
+        static_assert(2 * KL * 4 <= 8 * (VW > KL ? VW : KL), "the keys' registers");
+        auto ask = [&](u32 s) {
+            if (((s - s0) & 31) == 0) look(s);
+            const u32 p0 = s * 64 + half * 32;
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                page[i] = (u32)__builtin_amdgcn_readlane((i32)pg, (int)(2 * ((s - s0) & 31) + i));
+                const u32 slot = (p0 + 16 * i) & in_page, held = page[i] < p.c.n_page ? page[i] : 0u;
+                const at_rsrc rs = at_buffer(from + held * page_bytes + (size_t)slot * row_bytes);
+                if (brings_keys) {
+#pragma unroll
+                    for (int c = 0; c < KL; c++) {
+                        const u32x4 y = __builtin_amdgcn_raw_buffer_load_b128(rs, ko[c], 0, 0);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) st[(i * KL + c) * 4 + e] = y[e];
+                    }
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        if constexpr (VW == 1) st[4 * i + r] = __builtin_amdgcn_raw_buffer_load_b32(rs, vo, r * row_bytes, 0);
+                        else if constexpr (VW == 2) {
+                            const u32x2 y = __builtin_amdgcn_raw_buffer_load_b64(rs, vo, r * row_bytes, 0);
+                            st[(4 * i + r) * 2] = y.x; st[(4 * i + r) * 2 + 1] = y.y;
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < VW; e += 4) {
+                                const u32x4 y = __builtin_amdgcn_raw_buffer_load_b128(rs, vo + 4 * e, r * row_bytes, 0);
+#pragma unroll
+                                for (int f = 0; f < 4; f++) st[(4 * i + r) * VW + e + f] = y[f];
+                            }
+                        }
+                    }
+                }
+                if constexpr (I8)
+                    if ((lane >> 4) == i) sc = from_scales[((((size_t)held * p.c.n_kv + kv) << p.c.shift) + slot) + n];
+            }
+        };
+        auto put = [&](u32 s) {
+            u32x4* const to = lds + (s & 1) * STAGE;
+            const u32 p0 = s * 64 + half * 32;
+            const bool none = max(page[0], page[1]) >= p.c.n_page;
+            if (brings_keys) {
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+#pragma unroll
+                    for (int c = 0; c < KC; c++) {
+                        u32x4 y;
+                        if constexpr (I8) {   // bytes b to f16: 0x6400 | (b + 128) is 1152 + b
+#pragma unroll
+                            for (int j = 0; j < 4; j++) {
+                                const u32 t2 = __builtin_amdgcn_perm(0u, st[(i * KL + c / 2) * 4 + 2 * (c % 2) + j / 2], j % 2 ? 0x0c030c02u : 0x0c010c00u) ^ 0x64806480u;
+                                y[j] = __builtin_bit_cast(u32, __builtin_bit_cast(f16x2, t2) - f16x2{(_Float16)1152, (_Float16)1152});
+                            }
+                        } else {
+                            y = u32x4{st[(i * KL + c) * 4], st[(i * KL + c) * 4 + 1], st[(i * KL + c) * 4 + 2], st[(i * KL + c) * 4 + 3]};
+                        }
+                        to[((2 * half + i) * KC + c) * 64 + lane] = y;
+                    }
+                if (lane == 0) marks[(s & 1) * 4 + half] = (page[0] >= p.c.n_page ? 1u : 0u) | (page[1] >= p.c.n_page ? 2u : 0u);
+                if constexpr (I8)
+                    if (lane < 32) scales[(s & 1) * 128 + half * 32 + lane] = sc;
+            } else {
+                if (none || p0 < zlo || p0 + 32 > zhi) {   // zeros for what no token sees: what lies there may be no number
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const u32 at0 = p0 + 16 * (j / 4) + 4 * g + j % 4;
+                        const bool seen = page[j / 4] < p.c.n_page && at0 >= zlo && at0 < zhi;
+#pragma unroll
+                        for (int e = 0; e < VW; e++) st[j * VW + e] = seen ? st[j * VW + e] : 0u;
+                    }
+                    const u32 at0 = p0 + (lane & 31);
+                    if (!(page[(lane >> 4) & 1] < p.c.n_page && at0 >= zlo && at0 < zhi)) sc = 0.f;
+                }
+                if (!I8 && only == ~0u && span.t1 - span.t0 > 1 && (p0 < span.lo_all || p0 + 32 > span.hi_all)) {
+                    u16x2 big = {0, 0};
+#pragma unroll
+                    for (int j = 0; j < 8 * VW; j++) big = __builtin_elementwise_max(big, __builtin_bit_cast(u16x2, st[j] & 0x7fff7fffu));
+                    if (max(big.x, big.y) >= (BF ? 0x7f80 : 0x7c00)) marks[8] = 1;
+                }
+#pragma unroll
+                for (int j = 0; j < C; j++) {
+                    u32x4 vt;
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        if constexpr (I8) {
+                            const u32 b = j % 4;
+                            const u32 t2 = __builtin_amdgcn_perm(st[(2 * r + 1) * VW + j / 4], st[2 * r * VW + j / 4], 0x0c000c00u | b | (4 + b) << 16) ^ 0x64806480u;
+                            vt[r] = __builtin_bit_cast(u32, __builtin_bit_cast(f16x2, t2) - f16x2{(_Float16)1152, (_Float16)1152});
+                        } else {
+                            vt[r] = __builtin_amdgcn_perm(st[(2 * r + 1) * VW + j / 2], st[2 * r * VW + j / 2], j % 2 ? 0x07060302u : 0x05040100u);
+                        }
+                    }
+                    to[(4 * KC + half * C + j) * 64 + lane] = vt;
+                }
+                if constexpr (I8)
+                    if (lane < 32) scales[(s & 1) * 128 + 64 + half * 32 + lane] = sc;
+            }
+        };
+        // the columns
+        u32 tok[NT], head[NT], clo[NT], chi[NT], wlo = ~0u, whi = 0;
+        bool live[NT];
+        u32x4 qf[NT][QP][KC];
+        float qs[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            live[nt] = at_column(p, span.t0, span.t1, plane, (u32)(wave * NT + nt) * 16 + n, tok[nt], head[nt]);
+            u32 q0;
+            at_sees(p, tok[nt], q0, clo[nt], chi[nt]);
+            if (!live[nt]) clo[nt] = chi[nt] = 0;
+            wlo = min(wlo, live[nt] ? clo[nt] : ~0u);
+            whi = max(whi, chi[nt]);
+            float x[KC][8], most = 0.f;
+#pragma unroll
+            for (int c = 0; c < KC; c++) {
+                const int d = I8 ? 64 * (c / 2) + 16 * g + 8 * (c % 2) : 32 * c + 8 * g;
+                f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
+                if (live[nt] && d < p.c.d) kv_load8(p.q, tok[nt] * p.q_stride + (size_t)head[nt] * p.c.d + d, p.q_type, true, a, b);
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    x[c][j] = a[j];
+                    x[c][j + 4] = b[j];
+                    most = fmaxf(most, fmaxf(fabsf(a[j]), fabsf(b[j])));
+                }
+            }
+            int e = 0;
+            if (!BF) {   // into f16's range: the column's largest to [2^14, 2^15)
+                most = at_max4(most);
+                e = most > 0.f && most < inf ? 15 - __builtin_amdgcn_frexp_expf(most) : 0;
+            }
+            qs[nt] = __builtin_amdgcn_ldexpf(fabsf(p.scale), -e);   // (a negative scale's sign goes to q: the largest score is the largest product)
+            qs[nt] = p.cap == 0.f ? qs[nt] * JL_AT_LOG2E : qs[nt] / p.cap;
+            const u32 sign = __float_as_uint(p.scale) & 0x80000000u;
+#pragma unroll
+            for (int c = 0; c < KC; c++) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[c][j] = __uint_as_float(__float_as_uint(BF ? x[c][j] : __builtin_amdgcn_ldexpf(x[c][j], e)) ^ sign);
+#pragma unroll
+                for (int k = 0; k < QP; k++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) qf[nt][k][c][j] = at_piece<BF>(x[c][2 * j], x[c][2 * j + 1]);
+            }
+        }
+        u32 wlo_all = 0, whi_all = ~0u;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            wlo_all = max(wlo_all, live[nt] ? clo[nt] : 0u);
+            whi_all = min(whi_all, live[nt] ? chi[nt] : ~0u);
+        }
+#pragma unroll
+        for (int d = 1; d < 16; d *= 2) {
+            wlo = min(wlo, (u32)__shfl_xor((int)wlo, d, 64)); whi = max(whi, (u32)__shfl_xor((int)whi, d, 64));
+            wlo_all = max(wlo_all, (u32)__shfl_xor((int)wlo_all, d, 64)); whi_all = min(whi_all, (u32)__shfl_xor((int)whi_all, d, 64));
+        }
+        wlo = at_uni(wlo); whi = at_uni(whi); wlo_all = at_uni(wlo_all); whi_all = at_uni(whi_all);
+
+        for (;;) {
+        f32x4 acc[NT][C];
+        float m[NT], l[NT];
+        int ve = -200;          // 8-bit rows: acc is times 2^-ve
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            m[nt] = -inf;
+            l[nt] = 0.f;
+#pragma unroll
+            for (int j = 0; j < C; j++) acc[nt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+
+        if (s0 < s1) ask(s0);
+        __syncthreads();        // (the pass before has read its last stage)
+        if (threadIdx.x == 0) marks[8] = 0;
+        __syncthreads();
+        if (s0 < s1) put(s0);
+        __syncthreads();
+        for (u32 s = s0; s < s1; s++) {
+            if (s + 1 < s1) ask(s + 1);
+            const u32x4* const in = lds + (s & 1) * STAGE;
+            const u32* const mark = marks + (s & 1) * 4;
+#pragma unroll 1
+            for (int h = 0; h < 2; h++) {
+                const u32 p0 = s * 64 + h * 32;
+                if (p0 >= whi || p0 + 32 <= wlo) continue;
+                const u32 none = at_uni(mark[h]);
+                const bool edge = p0 < wlo_all || p0 + 32 > whi_all || none;
+                f32x4 sco[NT][2];
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) sco[nt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int c = 0; c < KC; c++) {
+                        const u32x4 y = in[((2 * h + i) * KC + c) * 64 + lane];
+#pragma unroll
+                        for (int q = 0; q < QP; q++)
+#pragma unroll
+                            for (int nt = 0; nt < NT; nt++) sco[nt][i] = at_mfma<BF>(y, qf[nt][q][c], sco[nt][i]);
+                    }
+                }
+                f32x4 ks[2], vs[2];
+                if constexpr (I8) {
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        ks[i] = *(const f32x4*)(scales + (s & 1) * 128 + h * 32 + 16 * i + 4 * g);
+                        vs[i] = *(const f32x4*)(scales + (s & 1) * 128 + 64 + h * 32 + 16 * i + 4 * g);
+                    }
+                    float big = fmaxf(fmaxf(fmaxf(vs[0][0], vs[0][1]), fmaxf(vs[0][2], vs[0][3])), fmaxf(fmaxf(vs[1][0], vs[1][1]), fmaxf(vs[1][2], vs[1][3])));
+                    big = at_max4(big);
+                    const int to = __builtin_amdgcn_readfirstlane(big > 0.f ? __builtin_amdgcn_frexp_expf(big) : -200);
+                    if (to > ve) {
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                            for (int j = 0; j < C; j++)
+#pragma unroll
+                                for (int r = 0; r < 4; r++) acc[nt][j][r] = __builtin_amdgcn_ldexpf(acc[nt][j][r], ve - to);
+                        ve = to;
+                    }
+                }
+                u32x4 pf[NT][PP];
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    float y[8], by = qs[nt];       // scores are y by
+                    u32 hidden = 0;
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        y[j] = sco[nt][j / 4][j % 4];
+                        if constexpr (I8) y[j] *= ks[j / 4][j % 4];
+                    }
+                    if (edge || p.cap != 0.f) {
+                        by = 1.f;
+#pragma unroll
+                        for (int j = 0; j < 8; j++) y[j] *= qs[nt];
+                        if (p.cap != 0.f) {
+#pragma unroll
+                            for (int j = 0; j < 8; j++) y[j] = p.cap * JL_AT_LOG2E * at_tanh(y[j]);
+                        }
+#pragma unroll
+                        for (int j = 0; j < 8; j++) {
+                            const u32 at0 = p0 + 16 * (j / 4) + 4 * g + j % 4;
+                            const bool sees = !(none >> (j / 4) & 1) && at0 >= clo[nt] && at0 < chi[nt];
+                            y[j] = sees ? y[j] : -inf;
+                            if (I8 && !sees) hidden |= 1u << j;
+                        }
+                    }
+                    float top = fmaxf(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])), fmaxf(fmaxf(y[4], y[5]), fmaxf(y[6], y[7])));
+                    top = fmaxf(at_max4(top) * by, m[nt]);
+                    if (__ballot(top > m[nt] + JL_AT_SLACK(BF))) {
+                        const float turn = m[nt] == top ? 1.f : __builtin_amdgcn_exp2f(m[nt] - top);   // (from -inf: 0)
+                        l[nt] *= turn;
+#pragma unroll
+                        for (int j = 0; j < C; j++) acc[nt][j] *= turn;
+                        m[nt] = top;
+                    }
+                    const float from = OFF - (m[nt] > -inf ? m[nt] : 0.f);
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        y[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(y[j], by, from));
+                        l[nt] += y[j];
+                        if constexpr (I8) y[j] = hidden >> j & 1 ? 0.f : y[j] * __builtin_amdgcn_ldexpf(vs[j / 4][j % 4], -ve);   // (a scale others see may be no number)
+                    }
+#pragma unroll
+                    for (int q = 0; q < PP; q++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) pf[nt][q][j] = at_piece<BF>(y[2 * j], y[2 * j + 1]);
+                }
+                const u32x4* const vin = in + (4 * KC + h * C) * 64 + lane;
+#pragma unroll
+                for (int j = 0; j < C; j++) {
+                    const u32x4 vt = vin[j * 64];
+#pragma unroll
+                    for (int q = 0; q < PP; q++)
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) acc[nt][j] = at_mfma<BF>(vt, pf[nt][q], acc[nt][j]);
+                }
+            }
+            if (s + 1 < s1) put(s + 1);
+            __syncthreads();
+        }
+
+        if (!I8 && only == ~0u && at_uni(marks[8])) {
+            u32 q0;
+            only = span.t0;
+            at_sees(p, only, q0, zlo, zhi);
+            zlo = at_uni(zlo); zhi = at_uni(zhi);
+            continue;
+        }
+        const u32 slot = 2 * w + (at == job.first ? 0u : 1u);
+        const bool whole = left == n_chunks;
+        if (c0 == 0 && !whole) join = AtJoin{span.t0, span.t1, plane, job.share.holder(at + n_chunks - 1) + 1, slot, {0, 0, 0}};
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            const float sum = at_sum4(l[nt]);
+            float by = I8 ? __builtin_amdgcn_ldexpf(1.f, ve) : 1.f;
+            if (!live[nt] || (only != ~0u && tok[nt] != only)) continue;
+            if (whole) by *= at_finish(p, tok[nt], head[nt], m[nt], sum, OFF, g == 0);
+            const u32 col = (u32)(wave * NT + nt) * 16 + n;
+            if (!whole && g == 0) *at_part_ml<DP>(p, slot, col) = f32x2{m[nt], sum};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int d0 = C * (4 * g + i);
+                float y[C];
+#pragma unroll
+                for (int j = 0; j < C; j++) y[j] = acc[nt][j][i] * by;
+                if (whole) {
+                    if (d0 < p.c.d) at_store<C>(p, tok[nt], head[nt], d0, y);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < C; j += 4) *(f32x4*)(at_part<DP>(p, slot, col) + d0 + j) = f32x4{y[j], y[j + 1], y[j + 2], y[j + 3]};
+                }
+            }
+        }
+        if (only == ~0u || ++only == span.t1) break;
+        u32 q0;
+        at_sees(p, only, q0, zlo, zhi);
+        zlo = at_uni(zlo); zhi = at_uni(zhi);
+        }
+        at += left;
+        job.off = 0;
+        if (p.whole) {
+            if (span.t1 == unit_end) break;
+            job.span = at_span<true>(p, span.t1);
+        } else if (at < job.end) {
+            at_next<true>(p, job);
+        }
+    }
+    if (!p.whole && threadIdx.x == 0) at_join_of<DP>(p)[w] = join;
+}

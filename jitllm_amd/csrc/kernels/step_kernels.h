@@ -1,6 +1,7 @@
 // The kernels of a decode step that stand between a block's projections and behind the last one.
 #pragma once
-#include "attend.h"
+#include "attend_many.h"
+#include "attend_one.h"
 #include "kv_cache.h"
 #include "sample.h"
 
@@ -8,24 +9,37 @@
 extern "C" __global__ __launch_bounds__(256) void jl_kv_write(KvRowsArgs p) { kv_rows_body<true>(p); }
 extern "C" __global__ __launch_bounds__(256) void jl_kv_read(KvRowsArgs p) { kv_rows_body<false>(p); }
 
-// grid = p.wgs, block = 256
-#define JL_ATTEND(T, TYPE, DP, QP, NT)                                                                                              \
-    extern "C" __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void jl_attend_##T##_d##DP##_q##QP##_n##NT(AttendArgs p) {      \
+// _q<pieces of q>; over a bf16 cache one piece of q goes with two of the weights (a 16-bit result), three with three
+// grid = p.wgs, block = 256; _m: units of several tokens
+#define JL_ATTEND_ONE_M(T, TYPE, DP, QP, PP, NAME, MANY)                                                                            \
+    extern "C" __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void jl_attend_one_##T##_d##DP##_q##QP##NAME(AttendArgs p) {    \
         __shared__ __attribute__((aligned(16))) float lds[4 * 16 * (DP + 4) + 128];                                                 \
         __shared__ uint64_t find[8];                                                                                                \
-        attend_body<TYPE, DP, QP, NT>(p, lds, find);                                                                                \
+        attend_one_body<TYPE, DP, QP, PP, MANY>(p, lds, find);                                                                      \
     }
-#define JL_ATTEND_Q(T, TYPE, QP)                                                                                                    \
-    JL_ATTEND(T, TYPE, 64, QP, 1) JL_ATTEND(T, TYPE, 64, QP, 2) JL_ATTEND(T, TYPE, 128, QP, 1) JL_ATTEND(T, TYPE, 128, QP, 2)       \
-    JL_ATTEND(T, TYPE, 256, QP, 1)
-JL_ATTEND_Q(f16, JL_F16, 1) JL_ATTEND_Q(f16, JL_F16, 2) JL_ATTEND_Q(i8, JL_I8, 1) JL_ATTEND_Q(i8, JL_I8, 2)
-JL_ATTEND_Q(bf16, JL_BF16, 1) JL_ATTEND_Q(bf16, JL_BF16, 3)
-#define JL_ATTEND_JOIN(DP, NT)                                                                                                      \
-    extern "C" __global__ __launch_bounds__(256) void jl_attend_join_d##DP##_n##NT(AttendArgs p) {                                  \
+#define JL_ATTEND_ONE(T, TYPE, DP, QP, PP) JL_ATTEND_ONE_M(T, TYPE, DP, QP, PP, , false) JL_ATTEND_ONE_M(T, TYPE, DP, QP, PP, _m, true)
+// grid = p.wgs, or p.units * planes where p.whole; block = 256.  Two tiles of columns a wavefront where they do not spill.
+#define JL_ATTEND_MANY(T, TYPE, DP, QP, PP, NT)                                                                                     \
+    extern "C" __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void jl_attend_many_##T##_d##DP##_q##QP##_n##NT(AttendArgs p) { \
+        __shared__ u32x4 lds[2 * at_stage_words<DP>() / 4 + 2 * 32 + 3];                                                            \
         __shared__ uint64_t find[8];                                                                                                \
-        attend_join_body<DP, NT>(p, find);                                                                                          \
+        attend_many_body<TYPE, DP, QP, PP, NT>(p, lds, find);                                                                       \
     }
-JL_ATTEND_JOIN(64, 1) JL_ATTEND_JOIN(64, 2) JL_ATTEND_JOIN(128, 1) JL_ATTEND_JOIN(128, 2) JL_ATTEND_JOIN(256, 1)
+#define JL_ATTEND_Q(T, TYPE, QP, PP)                                                                                                \
+    JL_ATTEND_ONE(T, TYPE, 64, QP, PP) JL_ATTEND_ONE(T, TYPE, 128, QP, PP) JL_ATTEND_ONE(T, TYPE, 256, QP, PP)                      \
+    JL_ATTEND_MANY(T, TYPE, 64, QP, PP, 1) JL_ATTEND_MANY(T, TYPE, 128, QP, PP, 1) JL_ATTEND_MANY(T, TYPE, 256, QP, PP, 1)
+JL_ATTEND_Q(f16, JL_F16, 1, 2) JL_ATTEND_Q(f16, JL_F16, 2, 2) JL_ATTEND_Q(i8, JL_I8, 1, 2) JL_ATTEND_Q(i8, JL_I8, 2, 2)
+JL_ATTEND_Q(bf16, JL_BF16, 1, 2) JL_ATTEND_Q(bf16, JL_BF16, 3, 3)
+JL_ATTEND_MANY(f16, JL_F16, 64, 1, 2, 2) JL_ATTEND_MANY(f16, JL_F16, 128, 1, 2, 2) JL_ATTEND_MANY(f16, JL_F16, 64, 2, 2, 2)
+JL_ATTEND_MANY(i8, JL_I8, 64, 1, 2, 2) JL_ATTEND_MANY(i8, JL_I8, 128, 1, 2, 2) JL_ATTEND_MANY(i8, JL_I8, 64, 2, 2, 2)
+JL_ATTEND_MANY(bf16, JL_BF16, 64, 1, 2, 2) JL_ATTEND_MANY(bf16, JL_BF16, 128, 1, 2, 2)
+// grid = (p.wgs, up to four), block = 256
+#define JL_ATTEND_JOIN(DP)                                                                                                          \
+    extern "C" __global__ __launch_bounds__(256) void jl_attend_join_d##DP(AttendArgs p) {                                          \
+        __shared__ __attribute__((aligned(16))) float lds[16 * DP + 16];                                                            \
+        attend_join_body<DP>(p, lds);                                                                                               \
+    }
+JL_ATTEND_JOIN(64) JL_ATTEND_JOIN(128) JL_ATTEND_JOIN(256)
 
 // grid = rows, block = 1024
 extern "C" __global__ __launch_bounds__(1024) void jl_sample(SampleArgs p) {

@@ -11,7 +11,8 @@ import numpy as np
 import pytest
 
 from jitllm_amd import quant
-from jitllm_amd.hipmem import DeviceArray, Graph, Stream
+from jitllm_amd.device import Device
+from jitllm_amd.hipmem import DeviceArray, Graph, Stream, mem_info
 from test_gpu_kv_cache import KINDS, PLAIN, Cache, table_of
 from test_gpu_norm_rows import STEP, at_offset, dtype, stored, values
 
@@ -325,6 +326,20 @@ def test_captured_replayed_and_on_other_streams(dev):
     finally:
         st.destroy()
     del other
+
+
+def test_a_reserved_workspace_and_two_launches():
+    with Device(device=0) as d:
+        d.reserve_attend(256)
+        table, n_page = table_of(np.random.default_rng(1), [4000] * 8, 64)
+        for dim, t in ((64, quant.I8), (128, quant.F16), (256, quant.BF16)):
+            c = Cache(t, 4, dim, 64, table, n_page)
+            q, ld = DeviceArray(np.ones((8, 16, dim), np.float32)), DeviceArray(np.full(8, 4000, np.uint32))
+            out = DeviceArray(np.zeros((8, 16, dim), np.float32))
+            before, n = mem_info()[0], d.launch_count()
+            assert d.attend_dev(c.handle(d), out.ptr, q.ptr, 16, ld.ptr, 8, 0.1)
+            d.synchronize()
+            assert mem_info()[0] == before and d.launch_count() - n <= 2
 
 
 def test_a_token_alone_and_among_others(dev):
