@@ -178,7 +178,7 @@ int jl_forget(jl_ctx *ctx, const void *p, size_t n);
 /* Threads.  The host-pointer entry points (no _dev in the name) may be called from any
  * thread: each holds the context's lock for its whole synchronous run.  The *_dev entry
  * points take no lock and share the context's workspaces (activation fragments, K-split
- * slabs, the mixture block's lists, the adapters' sums and lists, the attention's partial sums, the flag word of
+ * slabs, the mixture block's lists, the adapters' sums and lists, the attention's partial sums, the sampling's bins and lists, the flag word of
  * jl_pack_weights_dev and jl_fold_admit_dev): a context's *_dev calls are made by one thread
  * at a time, on one stream at a time -- replays of graphs that hold such calls among them: two
  * of a context's, or one and a call, do not run at the same time --, as the reference's tier makes its device calls (jit/gpu/tier/tier.go:2831-2843);
@@ -661,7 +661,8 @@ int jl_reserve_attend(jl_ctx *ctx, int max_d);
  * T of 0 or less, or no number: the largest, the first of several.  An infinity is larger than the rest and shares with its equals; -infinity and NaN are never
  * taken; a row without anything else gets the token n and prob 0.  u of 1 or more, or no number: the last kept.  w is f64's to 2^-44, sums are exact in 64 bits whole numbers, so a
  * row's token does not depend on the call it is in.  temperature (null: ones), top_k, top_p, min_p (null: off) and u are device memory, [rows].
- * n up to 524288, rows up to 1048576. */
+ * n up to 524288, rows up to 1048576.  Three or four launches for every 1024 rows; the workspace (jl_reserve_sample) is the context's, and a buffer that is outgrown lives
+ * until the context goes. */
 typedef struct jl_sample {
     int rows, n;
     const void *logits;
@@ -674,6 +675,8 @@ typedef struct jl_sample {
     float *prob;
 } jl_sample;
 int jl_sample_dev(jl_ctx *ctx, const jl_sample *g, void *stream);
+/* Sizes the workspace for jl_sample_dev calls of up to max_rows rows (of any length). */
+int jl_reserve_sample(jl_ctx *ctx, int max_rows);
 
 /* ---- mixture of experts (device pointers) ----------------------------- */
 

@@ -179,6 +179,7 @@ SIGNATURES = {
     "jl_kv_read_dev": (_int, [_vp, C.POINTER(KvCache), C.POINTER(KvRows), _vp]),
     "jl_attend_dev": (_int, [_vp, C.POINTER(KvCache), C.POINTER(Attend), _vp]),
     "jl_reserve_attend": (_int, [_vp, _int]),
+    "jl_reserve_sample": (_int, [_vp, _int]),
     "jl_sample_dev": (_int, [_vp, C.POINTER(Sample), _vp]),
     "jl_moe_group_dev": (_int, [_vp, _vp, _int, _int, _int, _int, _vp, _vp, _vp, _vp]),
     "jl_moe_matvec_dev": (_int, [_vp, _vp, _vp, _int, _vp, _vp, _vp, _vp, _vp, _vp, _int, _int, _int, _int, _vp]),

@@ -221,6 +221,10 @@ struct jl_ctx {
     size_t attend_ws_bytes = 0;
     void* attend_old[64] = {};
     int attend_olds = 0;
+    void* sample_ws = nullptr;    // bins and lists of a sampling call's rows; likewise
+    size_t sample_ws_bytes = 0;
+    void* sample_old[64] = {};
+    int sample_olds = 0;
 
     // host-pointer seam state
     std::map<const void*, Resident> resident;
@@ -2247,7 +2251,7 @@ int jl_ctx_create(jl_ctx** out, const jl_options* opts) {
     for (const char* form : {"l16_1", "l32_1", "l64_1", "wg_1", "wg_2", "wg_4", "wg_8", "wg_16"})
         for (const char* any : {"", "_any"}) names.push_back(std::string("jl_norm_rows_") + form + any);
     for (const char* g : {"g1", "g2", "g3", "g4", "g3p", "g4p", "g6p", "g8p", "g12p", "g16p"}) names.push_back(std::string("jl_moe_select_") + g);
-    for (const char* n : {"jl_kv_write", "jl_kv_read", "jl_sample"}) names.push_back(n);
+    for (const char* n : {"jl_kv_write", "jl_kv_read", "jl_sample_max", "jl_sample_bins", "jl_sample_gather", "jl_sample_take"}) names.push_back(n);
     for (const char* d : {"64", "128", "256"}) names.push_back(std::string("jl_attend_join_d") + d);
     for (const char* t : {"f16", "i8", "bf16"})
         for (const char* d : {"_d64", "_d128", "_d256"})
@@ -2396,6 +2400,8 @@ void jl_ctx_destroy(jl_ctx* c) {
     for (int i = 0; i < c->adapter_olds; i++) (void)H->Free(c->adapter_old[i]);
     if (c->attend_ws) (void)H->Free(c->attend_ws);
     for (int i = 0; i < c->attend_olds; i++) (void)H->Free(c->attend_old[i]);
+    if (c->sample_ws) (void)H->Free(c->sample_ws);
+    for (int i = 0; i < c->sample_olds; i++) (void)H->Free(c->sample_old[i]);
     for (auto& kv : c->layers)
         if (kv.second.mem) (void)H->Free(kv.second.mem);
     if (c->one_group) (void)H->Free(c->one_group);
@@ -2569,6 +2575,7 @@ int kept_ws_ensure(jl_ctx* c, void** ws, size_t* have, void** old, int* olds, si
     return JL_OK;
 }
 int adapter_ws_ensure(jl_ctx* c, size_t need) { return kept_ws_ensure(c, &c->adapter_ws, &c->adapter_ws_bytes, c->adapter_old, &c->adapter_olds, need); }
+int sample_ws_ensure(jl_ctx* c, size_t need) { return kept_ws_ensure(c, &c->sample_ws, &c->sample_ws_bytes, c->sample_old, &c->sample_olds, need); }
 int attend_ws_ensure(jl_ctx* c, size_t need) { return kept_ws_ensure(c, &c->attend_ws, &c->attend_ws_bytes, c->attend_old, &c->attend_olds, need); }
 }  // namespace
 
@@ -3182,6 +3189,17 @@ int jl_attend_dev(jl_ctx* c, const jl_kv_cache* cache, const jl_attend* g, void*
     return launch(c, join, (unsigned)a.wgs, (unsigned)std::min(4, (std::min(a.part_cols, a.group * a.per) + 3) / 4), 256, 0, st, params);
 }
 
+namespace {
+constexpr int kSampleRows = 1024;   // rows a pass: the workspace is theirs
+}
+
+int jl_reserve_sample(jl_ctx* c, int max_rows) {
+    if (!c) return JL_ERR_ARG;
+    if (max_rows <= 0) return fail(c, JL_ERR_ARG, "reserve sample: %d rows", max_rows);
+    HIP_TRY(c, H->SetDevice(c->device));
+    return sample_ws_ensure(c, std::min(max_rows, kSampleRows) * sizeof(SampleRowWs));
+}
+
 int jl_sample_dev(jl_ctx* c, const jl_sample* g, void* stream) {
     if (!c) return JL_ERR_ARG;
     if (!g || !g->logits || !g->u || !g->token || g->rows <= 0 || g->n <= 0) return fail(c, JL_ERR_ARG, "sample: bad operand");
@@ -3194,12 +3212,36 @@ int jl_sample_dev(jl_ctx* c, const jl_sample* g, void* stream) {
         (((uintptr_t)g->temperature | (uintptr_t)g->top_k | (uintptr_t)g->top_p | (uintptr_t)g->min_p | (uintptr_t)g->u | (uintptr_t)g->token | (uintptr_t)g->prob) & 3))
         return JL_DECLINED;
     if (g->rows > 1 << 20) return JL_DECLINED;
-    a.logits = g->logits; a.temperature = g->temperature; a.top_k = g->top_k; a.top_p = g->top_p; a.min_p = g->min_p; a.u = g->u; a.token = g->token;
-    a.prob = g->prob; a.rows = g->rows; a.n = g->n; a.type = g->type;
-    a.vec = ((uintptr_t)g->logits & (4 * b - 1)) == 0 && a.stride % 4 == 0;
     HIP_TRY(c, H->SetDevice(c->device));
+    const int at_once = std::min(g->rows, kSampleRows);
+    int rc = sample_ws_ensure(c, at_once * sizeof(SampleRowWs));
+    if (rc != JL_OK) return rc;
+    // Slices: as many as give every CU two workgroups, of 4096 to 32768 elements.
+    const int most = (g->n + 4095) / 4096, least = (g->n + 32767) / 32768;
+    a.slices = std::clamp((2 * c->num_cu + at_once - 1) / at_once, least, std::min(most, JL_SA_SLICES));
+    a.slice_len = ((g->n + a.slices - 1) / a.slices + 3) / 4 * 4;
+    a.slices = (g->n + a.slice_len - 1) / a.slice_len;
+    a.n = g->n; a.type = g->type; a.ws = c->sample_ws;
+    const hipStream_t st = pick_stream(c, stream);
     void* params[] = {&a};
-    return launch(c, "jl_sample", (unsigned)g->rows, 1, 1024, 0, pick_stream(c, stream), params);
+    for (int row = 0; row < g->rows; row += at_once) {
+        a.rows = std::min(at_once, g->rows - row);
+        a.logits = (const char*)g->logits + (size_t)row * a.stride * b;
+        a.temperature = g->temperature ? g->temperature + row : nullptr;
+        a.top_k = g->top_k ? g->top_k + row : nullptr;
+        a.top_p = g->top_p ? g->top_p + row : nullptr;
+        a.min_p = g->min_p ? g->min_p + row : nullptr;
+        a.u = g->u + row;
+        a.token = g->token + row;
+        a.prob = g->prob ? g->prob + row : nullptr;
+        const unsigned slices = (unsigned)a.slices, rows = (unsigned)a.rows;
+        rc = launch(c, "jl_sample_max", slices, rows, 512, 0, st, params);
+        if (rc == JL_OK && (g->top_k || g->top_p || g->min_p)) rc = launch(c, "jl_sample_bins", slices, rows, 512, 0, st, params);
+        if (rc == JL_OK) rc = launch(c, "jl_sample_gather", slices, rows, 512, 0, st, params);
+        if (rc == JL_OK) rc = launch(c, "jl_sample_take", rows, 1, 1024, 0, st, params);
+        if (rc != JL_OK) return rc;
+    }
+    return JL_OK;
 }
 
 int jl_moe_logits_dev(jl_ctx* c, float* logits, int wtype, const void* w, const float* x, int n_expert, int k,

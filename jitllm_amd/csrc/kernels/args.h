@@ -680,6 +680,20 @@ struct AttendArgs {
     float scale, cap;
 };
 
+// A row's workspace of a sampling call (kernels/sample.h).
+#define JL_SA_BINS 2048      // (the last holds what is further than 32 temperatures off: its weights are under 2^-45)
+#define JL_SA_LIST 1024
+#define JL_SA_SLICES 64
+struct SampleRowWs {
+    uint32_t mode, bin, fill, before;      // before: candidates before the bin of the cut
+    uint64_t mass, all;                    // sum before that bin; of all candidates
+    uint32_t key[JL_SA_LIST], idx[JL_SA_LIST];
+    uint64_t sums[JL_SA_BINS];
+    uint32_t counts[JL_SA_BINS];
+    uint32_t top[JL_SA_SLICES], at[JL_SA_SLICES], many[JL_SA_SLICES];   // a slice's largest, its place; candidates
+    uint64_t slice[JL_SA_SLICES];          // the sum of what is kept for sure
+};
+
 // A token a row of logits (kernels/sample.h).
 struct SampleArgs {
     const void* logits;      // [rows][stride]
@@ -690,6 +704,8 @@ struct SampleArgs {
     const float* u;
     uint32_t* token;
     float* prob;
+    void* ws;                // a SampleRowWs a row
     size_t stride;
-    int rows, n, type, vec;  // vec: rows on 16-byte boundaries
+    int rows, n, type;
+    int slices, slice_len;   // of a row; a multiple of four
 };

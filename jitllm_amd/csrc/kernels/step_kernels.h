@@ -41,8 +41,23 @@ JL_ATTEND_MANY(bf16, JL_BF16, 64, 1, 2, 2) JL_ATTEND_MANY(bf16, JL_BF16, 128, 1,
     }
 JL_ATTEND_JOIN(64) JL_ATTEND_JOIN(128) JL_ATTEND_JOIN(256)
 
+// grid = (slices, rows), block = 512
+extern "C" __global__ __launch_bounds__(512) void jl_sample_max(SampleArgs p) {
+    __shared__ u32 lds[4];
+    sample_max_body(p, lds);
+}
+extern "C" __global__ __launch_bounds__(512) void jl_sample_bins(SampleArgs p) {
+    __shared__ uint64_t sums[JL_SA_BINS];
+    __shared__ u32 counts[JL_SA_BINS];
+    sample_bins_body(p, counts, sums);
+}
+extern "C" __global__ __launch_bounds__(512) void jl_sample_gather(SampleArgs p) {
+    __shared__ uint64_t scan[8];
+    __shared__ u32 told[8];
+    sample_gather_body(p, scan, told);
+}
 // grid = rows, block = 1024
-extern "C" __global__ __launch_bounds__(1024) void jl_sample(SampleArgs p) {
+extern "C" __global__ __launch_bounds__(1024) void jl_sample_take(SampleArgs p) {
     __shared__ SampleLds s;
-    sample_body(p, s);
+    sample_take_body(p, s);
 }

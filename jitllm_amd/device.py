@@ -148,6 +148,10 @@ class Device(_calls.Calls):
         """Size the workspace of attend_dev for rows of up to max_d elements."""
         self._served(self._l.jl_reserve_attend(self._ctx, max_d), "jl_reserve_attend")
 
+    def reserve_sample(self, max_rows):
+        """Size the workspace of sample_dev for up to max_rows rows."""
+        self._served(self._l.jl_reserve_sample(self._ctx, max_rows), "jl_reserve_sample")
+
     @staticmethod
     def kv_cache(t, n_kv, d, page_size, n_page, k, v, table, n_seq, table_pages, k_scale=None, v_scale=None, page_stride=0,
                  head_stride=0, row_stride=0, table_stride=0):
