@@ -3216,10 +3216,11 @@ int jl_sample_dev(jl_ctx* c, const jl_sample* g, void* stream) {
     const int at_once = std::min(g->rows, kSampleRows);
     int rc = sample_ws_ensure(c, at_once * sizeof(SampleRowWs));
     if (rc != JL_OK) return rc;
-    // Slices: as many as give every CU two workgroups, of 4096 to 32768 elements.
+    // Slices: as many as give every CU two workgroups, of 4096 to 32768 elements; in eight parts of whole steps of a wavefront.
     const int most = (g->n + 4095) / 4096, least = (g->n + 32767) / 32768;
     a.slices = std::clamp((2 * c->num_cu + at_once - 1) / at_once, least, std::min(most, JL_SA_SLICES));
-    a.slice_len = ((g->n + a.slices - 1) / a.slices + 3) / 4 * 4;
+    a.part_len = ((g->n + a.slices * JL_SA_PARTS - 1) / (a.slices * JL_SA_PARTS) + 255) / 256 * 256;
+    a.slice_len = a.part_len * JL_SA_PARTS;
     a.slices = (g->n + a.slice_len - 1) / a.slice_len;
     a.n = g->n; a.type = g->type; a.ws = c->sample_ws;
     const hipStream_t st = pick_stream(c, stream);
@@ -3238,7 +3239,7 @@ int jl_sample_dev(jl_ctx* c, const jl_sample* g, void* stream) {
         rc = launch(c, "jl_sample_max", slices, rows, 512, 0, st, params);
         if (rc == JL_OK && (g->top_k || g->top_p || g->min_p)) rc = launch(c, "jl_sample_bins", slices, rows, 512, 0, st, params);
         if (rc == JL_OK) rc = launch(c, "jl_sample_gather", slices, rows, 512, 0, st, params);
-        if (rc == JL_OK) rc = launch(c, "jl_sample_take", rows, 1, 1024, 0, st, params);
+        if (rc == JL_OK) rc = launch(c, "jl_sample_take", rows, 1, 256, 0, st, params);
         if (rc != JL_OK) return rc;
     }
     return JL_OK;

@@ -684,6 +684,7 @@ struct AttendArgs {
 #define JL_SA_BINS 2048      // (the last holds what is further than 32 temperatures off: its weights are under 2^-45)
 #define JL_SA_LIST 1024
 #define JL_SA_SLICES 64
+#define JL_SA_PARTS 8        // of a slice: a wavefront's
 struct SampleRowWs {
     uint32_t mode, bin, fill, before;      // before: candidates before the bin of the cut
     uint64_t mass, all;                    // sum before that bin; of all candidates
@@ -691,7 +692,7 @@ struct SampleRowWs {
     uint64_t sums[JL_SA_BINS];
     uint32_t counts[JL_SA_BINS];
     uint32_t top[JL_SA_SLICES], at[JL_SA_SLICES], many[JL_SA_SLICES];   // a slice's largest, its place; candidates
-    uint64_t slice[JL_SA_SLICES];          // the sum of what is kept for sure
+    uint64_t part[JL_SA_SLICES * JL_SA_PARTS];   // a wavefront's part of a slice: the sum of what is kept for sure
 };
 
 // A token a row of logits (kernels/sample.h).
@@ -707,5 +708,5 @@ struct SampleArgs {
     void* ws;                // a SampleRowWs a row
     size_t stride;
     int rows, n, type;
-    int slices, slice_len;   // of a row; a multiple of four
+    int slices, slice_len, part_len;   // of a row; elements of a slice and of its parts
 };

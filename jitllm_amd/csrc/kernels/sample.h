@@ -18,29 +18,14 @@
 #pragma once
 #include "args.h"
 #include "common.h"
-#include "moe_select.h"
 #include "norm_rows.h"
 
 #pragma clang fp contract(off)
-
-#define JL_SA_TILE 4096      // elements of a workgroup's pass in index order
 
 #define JL_SA_DONE 0
 #define JL_SA_LISTED 1
 #define JL_SA_LARGE 2
 #define JL_SA_SLOW 3
-
-struct SampleLds {
-    uint64_t mass[JL_SA_BINS];
-    u32 count[JL_SA_BINS];
-    u32 key[JL_SA_LIST], idx[JL_SA_LIST];
-    uint64_t tile[256];
-    uint64_t slices[JL_SA_SLICES];
-    uint64_t wsum[16];
-    uint64_t at_mass;
-    u32 wcnt[16];
-    u32 at, at_count, at_n, fill, lo, hi, res_key, res_idx;
-};
 
 // The row's values as ordered whole numbers; 0: no candidate.
 __device__ __forceinline__ u32 sample_key(float x) {
@@ -51,15 +36,32 @@ __device__ __forceinline__ float sample_value(u32 k) { return __uint_as_float(k 
 
 struct SampleRow {
     float max;        // of the row
-    double inv_t;     // 1 / temperature
+    double a;         // log2 e / temperature
     float fine;       // bins a unit of x
-    __device__ double weight(float x) const { return x == max ? 1.0 : select_exp(fmax(((double)x - (double)max) * inv_t, -800.0)); }
-    __device__ uint64_t whole(float x) const {   // round(w 2^44): the low bits of w 2^44 + 2^52
-        return __builtin_bit_cast(uint64_t, __builtin_fma(weight(x), 0x1p44, 0x1p52)) & ((1ull << 52) - 1);
+    // e^((x - max) / T) = 2^y, y = n + f with |f| <= 1/2: the series of 2^f up to (f ln2)^11 / 11! (the next term is under 2^-47).  Nothing for NaN, -infinity.
+    __device__ double weight(float x) const {
+        const double y = fmax(((double)x - (double)max) * a, -1000.0);
+        const double z = y + 0x1.8p52, f = y - (z - 0x1.8p52);     // (n in z's low bits)
+        double p = 0x1.e8cac7351bb25p-32;
+        p = __builtin_fma(p, f, 0x1.e4cf5158b8ecap-28);
+        p = __builtin_fma(p, f, 0x1.b5253d395e7c4p-24);
+        p = __builtin_fma(p, f, 0x1.62c0223a5c824p-20);
+        p = __builtin_fma(p, f, 0x1.ffcbfc588b0c7p-17);
+        p = __builtin_fma(p, f, 0x1.430912f86c787p-13);
+        p = __builtin_fma(p, f, 0x1.5d87fe78a6731p-10);
+        p = __builtin_fma(p, f, 0x1.3b2ab6fba4e77p-7);
+        p = __builtin_fma(p, f, 0x1.c6b08d704a0c0p-5);
+        p = __builtin_fma(p, f, 0x1.ebfbdff82c58fp-3);
+        p = __builtin_fma(p, f, 0x1.62e42fefa39efp-1);
+        p = __builtin_fma(p, f, 0x1.0000000000000p+0);
+        const double w = __builtin_ldexp(p, (int)(u32)__builtin_bit_cast(uint64_t, z));
+        return x == max ? 1.0 : w;       // (an infinity is its own largest)
     }
-    __device__ uint64_t kept(float x, u32 i, float low, u32 first) const {   // 0 where min_p takes it out
+    static __device__ uint64_t rounded(double w) { return __builtin_bit_cast(uint64_t, __builtin_fma(w, 0x1p44, 0x1p52)) & ((1ull << 52) - 1); }   // the low bits of w 2^44 + 2^52
+    __device__ uint64_t whole(float x) const { return rounded(weight(x)); }
+    __device__ uint64_t kept(float x, float low) const {   // 0 where min_p takes it out
         const double w = weight(x);
-        return low > 0.f && !(w >= (double)low) && i != first ? 0 : __builtin_bit_cast(uint64_t, __builtin_fma(w, 0x1p44, 0x1p52)) & ((1ull << 52) - 1);
+        return low > 0.f && !(w >= (double)low) ? 0 : rounded(w);
     }
     __device__ u32 bin(float x) const {          // falls as x rises
         const float d = (max - x) * fine;        // (infinities apart: NaN or infinite)
@@ -85,259 +87,67 @@ __device__ __forceinline__ f32x4 sample_load(const SampleArgs& p, size_t at, int
     }
     return v;
 }
-// f(value, index) for the elements from to end of a row, four in a row a thread; four such loads are on their way.
-template <int THREADS, class F> __device__ __forceinline__ void sample_range(const SampleArgs& p, size_t row, int from, int end, F f) {
+// f(value, index) for the elements from to end of a row, four in a row a lane, 4 * LANES together; four such loads are on their way.
+template <int LANES, class F> __device__ __forceinline__ void sample_range(const SampleArgs& p, size_t row, int from, int end, int lane, F f) {
     const size_t at = row * p.stride;
-    int i = from + 4 * (int)threadIdx.x;
-    for (; i + 3 * 4 * THREADS + 4 <= end; i += 4 * 4 * THREADS) {
+    int i = from + 4 * lane;
+    for (; i + 3 * 4 * LANES + 4 <= end; i += 4 * 4 * LANES) {
         f32x4 v[4];
 #pragma unroll
-        for (int k = 0; k < 4; k++) v[k] = sample_load(p, at + i + k * 4 * THREADS, 4);
+        for (int k = 0; k < 4; k++) v[k] = sample_load(p, at + i + k * 4 * LANES, 4);
 #pragma unroll
         for (int k = 0; k < 4; k++)
 #pragma unroll
-            for (int j = 0; j < 4; j++) f(v[k][j], (u32)(i + k * 4 * THREADS + j));
+            for (int j = 0; j < 4; j++) f(v[k][j], (u32)(i + k * 4 * LANES + j));
     }
-    for (; i < end; i += 4 * THREADS) {
+    for (; i < end; i += 4 * LANES) {
         const f32x4 v = sample_load(p, at + i, end - i);
 #pragma unroll
         for (int j = 0; j < 4; j++)
             if (i + j < end) f(v[j], (u32)(i + j));
     }
 }
-template <class F> __device__ __forceinline__ void sample_each(const SampleArgs& p, size_t row, F f) { sample_range<1024>(p, row, 0, p.n, f); }
+// A slice (a workgroup's) and the part of it that a wavefront has.
+__device__ __forceinline__ void sample_slice(const SampleArgs& p, int slice, int& from, int& end) {
+    from = min(slice * p.slice_len, p.n);
+    end = min(from + p.slice_len, p.n);
+}
+__device__ __forceinline__ void sample_part(const SampleArgs& p, int part, int& from, int& end) {
+    int s0, s1;
+    sample_slice(p, part / JL_SA_PARTS, s0, s1);
+    from = min(s0 + part % JL_SA_PARTS * p.part_len, s1);
+    end = min(from + p.part_len, s1);
+}
 
-// Inclusive sum over the workgroup's threads; total to every one.
-__device__ __forceinline__ uint64_t sample_scan(SampleLds& s, uint64_t v, uint64_t& total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+__device__ __forceinline__ uint64_t sample_scan64(uint64_t v) {      // inclusive sums over a wavefront
+    const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
         const uint64_t o = __shfl_up((unsigned long long)v, d, 64);
         if (lane >= d) v += o;
     }
+    return v;
+}
+// ... over WAVES of them; total to every thread.  LDS: WAVES words.
+template <int WAVES> __device__ __forceinline__ uint64_t sample_scan(uint64_t* lds, uint64_t v, uint64_t& total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    v = sample_scan64(v);
     __syncthreads();
-    if (lane == 63) s.wsum[wave] = v;
+    if (lane == 63) lds[wave] = v;
     __syncthreads();
     total = 0;
     uint64_t before = 0;
-    for (int w = 0; w < 16; w++) {
-        before += w < wave ? s.wsum[w] : 0;
-        total += s.wsum[w];
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) {
+        before += w < wave ? lds[w] : 0;
+        total += lds[w];
     }
     return v + before;
 }
-
-// The first element by index with crosses(sum of weight(x, i) up to and with it); ~0: none.  weight is 0 for elements that are not in the sum.
-// Of the elements from to end (from a multiple of four).
-template <class W, class X> __device__ __forceinline__ u32 sample_cross(const SampleArgs& p, SampleLds& s, size_t row, int from, int end, W weight, X crosses, uint64_t& total) {
-    const int tiles = (end - from + JL_SA_TILE - 1) / JL_SA_TILE;   // (256 at most)
-    __syncthreads();
-    if (threadIdx.x < 256) s.tile[threadIdx.x] = 0;
-    if (threadIdx.x == 0) s.at = ~0u;
-    __syncthreads();
-    const size_t at = row * p.stride;
-    auto load = [&](int i) { return sample_load(p, at + i, end - i); };
-    for (int i = from + 4 * (int)threadIdx.x, k = 0; k < tiles; k++, i += JL_SA_TILE) {
-        uint64_t sum = 0;
-        if (i < end) {
-            const f32x4 v = load(i);
+__device__ __forceinline__ u32 sample_wave_max(u32 v) {
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (i + j < end) sum += weight(v[j], (u32)(i + j));
-        }
-        if (sum) atomicAdd((unsigned long long*)&s.tile[k], (unsigned long long)sum);
-    }
-    __syncthreads();
-    uint64_t before = 0;
-    total = 0;
-    int tile = -1;
-    for (int k = 0; k < tiles; k++) {
-        const uint64_t t = s.tile[k];
-        if (tile < 0 && t && crosses(total + t)) {
-            tile = k;
-            before = total;
-        }
-        total += t;
-    }
-    if (tile >= 0) {   // uniform
-        const int i = from + tile * JL_SA_TILE + 4 * (int)threadIdx.x;
-        uint64_t part[4] = {0, 0, 0, 0}, mine = 0, all;
-        if (i < end) {
-            const f32x4 v = load(i);
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                if (i + j < end) part[j] = weight(v[j], (u32)(i + j));
-                mine += part[j];
-            }
-        }
-        uint64_t c = before + sample_scan(s, mine, all) - mine;
-        const bool had = c != 0 && crosses(c);
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const bool is = part[j] && crosses(c + part[j]);
-            if (is && !had) atomicMin(&s.at, (u32)(i + j));
-            c += part[j];
-        }
-    }
-    __syncthreads();
-    const u32 found = s.at;
-    __syncthreads();
-    return found;
-}
-
-// What is kept: elements not behind (key, idx) in the order.
-struct SampleCut {
-    u32 key, idx;
-    uint64_t mass;     // of those
-    __device__ bool keeps(u32 k, u32 i) const { return k > key || (k == key && i <= idx); }
-};
-
-// Counts and sums of the bins (bin(x, key) < BINS, or ~0: not in it), then over the bins before each.
-template <class B> __device__ __forceinline__ void sample_bins(const SampleArgs& p, SampleLds& s, size_t row, const SampleRow& r, B bin) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < JL_SA_BINS; i += 1024) {
-        s.mass[i] = 0;
-        s.count[i] = 0;
-    }
-    __syncthreads();
-    sample_each(p, row, [&](float x, u32) {
-        const u32 k = sample_key(x), b = k ? bin(x, k) : ~0u;
-        if (b < JL_SA_BINS) {
-            atomicAdd(&s.count[b], 1u);
-            atomicAdd((unsigned long long*)&s.mass[b], (unsigned long long)r.whole(x));
-        }
-    });
-    __syncthreads();
-}
-
-// The bin in which crosses(count, mass) with the bins up to it is first true, and what lies before it: s.at, s.at_count, s.at_mass, s.at_n.
-// None: s.at stays ~0.
-template <class X> __device__ __forceinline__ void sample_find(SampleLds& s, u32 count0, uint64_t mass0, X crosses) {
-    if (threadIdx.x == 0) s.at = ~0u;
-    constexpr int PER = JL_SA_BINS / 1024;
-    const int b0 = PER * threadIdx.x;
-    uint64_t c = 0, m = 0, all;
-#pragma unroll
-    for (int j = 0; j < PER; j++) {
-        c += s.count[b0 + j];
-        m += s.mass[b0 + j];
-    }
-    uint64_t cb = sample_scan(s, c, all) - c + count0, mb = sample_scan(s, m, all) - m + mass0;
-    if (c && crosses((u32)(cb + c), mb + m) && !(cb && crosses((u32)cb, mb))) {
-#pragma unroll
-        for (int j = 0; j < PER; j++) {
-            const u32 cj = s.count[b0 + j];
-            const uint64_t mj = s.mass[b0 + j];
-            if (cj && crosses((u32)(cb + cj), mb + mj) && !(cb && crosses((u32)cb, mb))) {
-                s.at = b0 + j;
-                s.at_count = (u32)cb;
-                s.at_mass = mb;
-                s.at_n = cj;
-            }
-            cb += cj;
-            mb += mj;
-        }
-    }
-    __syncthreads();
-}
-
-// The last element kept, in the order, such that crosses(count, mass) up to it is first true.  False: nothing crosses.
-template <class X> __device__ __forceinline__ bool sample_cut(const SampleArgs& p, SampleLds& s, size_t row, const SampleRow& r, X crosses, SampleCut& cut) {
-    sample_bins(p, s, row, r, [&](float x, u32) { return r.bin(x); });
-    sample_find(s, 0, 0, crosses);
-    if (s.at == ~0u) return false;   // uniform
-    const u32 bin0 = s.at;
-    u32 n = s.at_n, count = s.at_count, klo = 1, khi = ~0u;
-    uint64_t mass = s.at_mass;
-    __syncthreads();
-    if (n > JL_SA_LIST) {
-        if (threadIdx.x == 0) {
-            s.lo = ~0u;
-            s.hi = 0;
-        }
-        __syncthreads();
-        u32 lo = ~0u, hi = 0;
-        sample_each(p, row, [&](float x, u32) {
-            const u32 k = sample_key(x);
-            if (k && r.bin(x) == bin0) {
-                lo = min(lo, k);
-                hi = max(hi, k);
-            }
-        });
-        atomicMin(&s.lo, lo);
-        atomicMax(&s.hi, hi);
-        __syncthreads();
-        klo = s.lo;
-        khi = s.hi;
-        while (n > JL_SA_LIST && klo < khi) {
-            int shift = 0;
-            while ((khi - klo) >> shift >= JL_SA_BINS) shift++;
-            sample_bins(p, s, row, r, [&](float x, u32 k) { return r.bin(x) == bin0 && k >= klo && k <= khi ? (khi - k) >> shift : ~0u; });
-            sample_find(s, count, mass, crosses);
-            n = s.at_n;
-            count = s.at_count;
-            mass = s.at_mass;
-            const u32 top = khi - (s.at << shift), width = (1u << shift) - 1;
-            __syncthreads();
-            klo = top - klo > width ? top - width : klo;
-            khi = top;
-        }
-    }
-    if (n > JL_SA_LIST) {   // one key, many times: by index
-        const float x0 = sample_value(klo);
-        const uint64_t w0 = r.whole(x0);
-        uint64_t total;
-        // counted: sums of 1, the crossing by count and mass
-        cut.idx = sample_cross(p, s, row, 0, p.n, [&](float x, u32) { return (uint64_t)(sample_key(x) == klo); },
-                               [&](uint64_t c) { return crosses(count + (u32)c, mass + c * w0); }, total);
-        cut.key = klo;
-        // how many that are: again over those up to it
-        const u32 last = cut.idx;
-        sample_cross(p, s, row, 0, p.n, [&](float x, u32 i) { return (uint64_t)(sample_key(x) == klo && i <= last); }, [&](uint64_t) { return false; }, total);
-        cut.mass = mass + total * w0;
-        return true;
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) s.fill = 0;
-    __syncthreads();
-    sample_each(p, row, [&](float x, u32 i) {
-        const u32 k = sample_key(x);
-        if (k && k >= klo && k <= khi && r.bin(x) == bin0) {
-            const u32 at = atomicAdd(&s.fill, 1u);
-            if (at < JL_SA_LIST) {
-                s.key[at] = k;
-                s.idx[at] = i;
-            }
-        }
-    });
-    __syncthreads();
-    // a thread an element: those ahead of it, and their weights
-    const u32 tid = threadIdx.x;
-    uint64_t* const w = s.mass;   // (the bins have been read)
-    if (tid < n) w[tid] = r.whole(sample_value(s.key[tid]));
-    __syncthreads();
-    if (tid < n) {
-        const u32 k = s.key[tid], i = s.idx[tid];
-        u32 ahead = 0;
-        uint64_t m = 0;
-        for (u32 j = 0; j < n; j++) {
-            const bool is = s.key[j] > k || (s.key[j] == k && s.idx[j] < i);
-            ahead += is;
-            m += is ? w[j] : 0;
-        }
-        const u32 cb = count + ahead;
-        if (crosses(cb + 1, mass + m + w[tid]) && !(cb && crosses(cb, mass + m))) {
-            s.res_key = k;
-            s.res_idx = i;
-            s.at_mass = mass + m + w[tid];
-        }
-    }
-    __syncthreads();
-    cut.key = s.res_key;
-    cut.idx = s.res_idx;
-    cut.mass = s.at_mass;
-    __syncthreads();
-    return true;
+    for (int d = 1; d < 64; d *= 2) v = max(v, (u32)__shfl_xor((int)v, d, 64));
+    return v;
 }
 
 // Settings of a row, and what sample_max found.
@@ -353,34 +163,40 @@ __device__ __forceinline__ SampleSet sample_set(const SampleArgs& p, size_t row)
     const SampleRowWs& ws = ((const SampleRowWs*)p.ws)[row];
     const int lane = threadIdx.x & 63;     // a slice a lane
     const u32 top = lane < p.slices ? ws.top[lane] : 0u, at = lane < p.slices ? ws.at[lane] : 0u;
-    s.best = top;
+    const float t = p.temperature ? p.temperature[row] : 1.f;
+    const u32 k = p.top_k ? p.top_k[row] : 0u;
+    s.p = p.top_p ? p.top_p[row] : 1.f;
+    s.low = p.min_p ? p.min_p[row] : 0.f;
     s.valid = lane < p.slices ? ws.many[lane] : 0u;
+    s.best = sample_wave_max(top);
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        s.best = max(s.best, (u32)__shfl_xor((int)s.best, d, 64));
-        s.valid += (u32)__shfl_xor((int)s.valid, d, 64);
-    }
+    for (int d = 1; d < 64; d *= 2) s.valid += (u32)__shfl_xor((int)s.valid, d, 64);
     s.best = (u32)__builtin_amdgcn_readfirstlane((i32)s.best);
     s.valid = (u32)__builtin_amdgcn_readfirstlane((i32)s.valid);
     s.first = (u32)__builtin_amdgcn_readlane((i32)at, (int)__builtin_ctzll(__ballot(top == s.best)));   // the first slice that has it
-    const float t = p.temperature ? p.temperature[row] : 1.f;
-    s.greedy = s.best == 0 || !(t > 0.f);
+    s.greedy = s.best == 0 || !(t > 0.f) || s.low > 1.f;      // (nothing reaches a min_p above one: the first is left)
     s.r.max = sample_value(s.best);
-    s.r.inv_t = 1.0 / (double)t;
+    s.r.a = 1.4426950408889634074 / (double)t;
     s.r.fine = fminf(64.f / t, 1e30f);
-    const u32 k = p.top_k ? p.top_k[row] : 0u;
     s.k = k < s.valid ? k : 0u;
-    s.p = p.top_p ? p.top_p[row] : 1.f;
-    s.low = p.min_p ? p.min_p[row] : 0.f;
     s.nucleus = s.p < 1.f;
     return s;
 }
-__device__ __forceinline__ void sample_slice(const SampleArgs& p, int slice, int& from, int& end) {
-    from = slice * p.slice_len;
-    end = min(from + p.slice_len, p.n);
+// The smallest value that `holds` is true of, where it is true of all values from there on: 64 keys at a time.
+template <class F> __device__ __forceinline__ float sample_edge(F holds) {
+    u32 lo = 0x007fffffu;      // (the key of -infinity: false)
+    const u32 lane = threadIdx.x & 63;
+#pragma unroll
+    for (int shift = 26; ; shift = max(shift - 6, 0)) {
+        const uint64_t key = (uint64_t)lo + ((uint64_t)(lane + 1) << shift);
+        const uint64_t yes = __ballot(key > 0xff800000u || holds(sample_value((u32)key)));   // (the key of +infinity)
+        const u32 n = yes ? (u32)__builtin_ctzll(yes) : 64u;
+        if (shift == 0) return sample_value((u32)min(lo + (uint64_t)n + 1, (uint64_t)0xff800000u));
+        lo += n << shift;
+    }
 }
 
-// grid = (slices, rows), block = 512.  LDS: 4 words.
+// grid = (slices, rows), block = 512.  LDS: 3 words.
 __device__ __forceinline__ void sample_max_body(const SampleArgs& p, u32* lds) {
     const size_t row = blockIdx.y;
     SampleRowWs& ws = ((SampleRowWs*)p.ws)[row];
@@ -390,23 +206,20 @@ __device__ __forceinline__ void sample_max_body(const SampleArgs& p, u32* lds) {
         ws.sums[i] = 0;
     }
     if (slice == 0 && threadIdx.x == 0) ws.fill = 0;
-    if (threadIdx.x < 4) lds[threadIdx.x] = threadIdx.x == 1 ? ~0u : 0u;
+    if (threadIdx.x < 3) lds[threadIdx.x] = threadIdx.x == 1 ? ~0u : 0u;
     __syncthreads();
     int from, end;
     sample_slice(p, slice, from, end);
     u32 top = 0, many = 0, at = ~0u;
-    sample_range<512>(p, row, from, end, [&](float x, u32 i) {
+    sample_range<512>(p, row, from, end, threadIdx.x, [&](float x, u32 i) {
         const u32 k = sample_key(x);
         many += k != 0;
         at = k > top ? i : at;
         top = max(top, k);
     });
-    u32 best = top;
+    const u32 best = sample_wave_max(top);
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        best = max(best, (u32)__shfl_xor((int)best, d, 64));
-        many += (u32)__shfl_xor((int)many, d, 64);
-    }
+    for (int d = 1; d < 64; d *= 2) many += (u32)__shfl_xor((int)many, d, 64);
     if ((threadIdx.x & 63) == 0) {
         atomicMax(&lds[0], best);
         atomicAdd(&lds[2], many);
@@ -435,13 +248,20 @@ __device__ __forceinline__ void sample_bins_body(const SampleArgs& p, u32* count
     __syncthreads();
     int from, end;
     sample_slice(p, blockIdx.x, from, end);
-    sample_range<512>(p, row, from, end, [&](float x, u32) {
-        const u32 b = x > -__builtin_inff() ? s.r.bin(x) : (u32)JL_SA_BINS;
-        if (b < JL_SA_BINS - 1) {   // (the last bin's count is what is left over, its sum nothing)
-            atomicAdd(&counts[b], 1u);
-            if (weighs) atomicAdd((unsigned long long*)&sums[b], (unsigned long long)s.r.whole(x));
-        }
-    });
+    // (the last bin's count is what is left over, its sum nothing)
+    if (weighs)
+        sample_range<512>(p, row, from, end, threadIdx.x, [&](float x, u32) {
+            const u32 b = x > -__builtin_inff() ? s.r.bin(x) : (u32)JL_SA_BINS;
+            if (b < JL_SA_BINS - 1) {
+                atomicAdd(&counts[b], 1u);
+                atomicAdd((unsigned long long*)&sums[b], (unsigned long long)s.r.whole(x));
+            }
+        });
+    else
+        sample_range<512>(p, row, from, end, threadIdx.x, [&](float x, u32) {
+            const u32 b = x > -__builtin_inff() ? s.r.bin(x) : (u32)JL_SA_BINS;
+            if (b < JL_SA_BINS - 1) atomicAdd(&counts[b], 1u);
+        });
     __syncthreads();
     for (int i = threadIdx.x; i < JL_SA_BINS - 1; i += 512) {
         const u32 c = counts[i];
@@ -450,27 +270,6 @@ __device__ __forceinline__ void sample_bins_body(const SampleArgs& p, u32* count
             if (weighs && sums[i]) atomicAdd((unsigned long long*)&ws.sums[i], (unsigned long long)sums[i]);
         }
     }
-}
-
-// Inclusive sums over 512 threads.  LDS: 8 words.
-__device__ __forceinline__ uint64_t sample_scan512(uint64_t* lds, uint64_t v, uint64_t& total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const uint64_t o = __shfl_up((unsigned long long)v, d, 64);
-        if (lane >= d) v += o;
-    }
-    __syncthreads();
-    if (lane == 63) lds[wave] = v;
-    __syncthreads();
-    total = 0;
-    uint64_t before = 0;
-#pragma unroll
-    for (int w = 0; w < 8; w++) {
-        before += w < wave ? lds[w] : 0;
-        total += lds[w];
-    }
-    return v + before;
 }
 
 // grid = (slices, rows), block = 512.  LDS: 8 words of 8 bytes, then 8 of 4.
@@ -484,15 +283,15 @@ __device__ __forceinline__ void sample_gather_body(const SampleArgs& p, uint64_t
         return;
     }
     // The bin that min_p ends in, or one behind it: -ln(min_p) temperatures, 64 bins each.
-    const u32 low_bin = s.low > 0.f ? (u32)fminf((float)(JL_SA_BINS - 1), fmaxf(-__logf(fminf(s.low, 1.f)) * 64.f * 1.0001f + 2.f, 0.f)) : (u32)JL_SA_BINS - 1;
-    u32 mode = JL_SA_LARGE, cut = JL_SA_BINS, before = 0;    // the bin of the cut (LARGE) or the last bin (LIST); candidates before it
+    const u32 low_bin = s.low > 0.f ? (u32)fminf((float)(JL_SA_BINS - 1), -__logf(s.low) * 64.f * 1.0001f + 2.f) : (u32)JL_SA_BINS - 1;
+    u32 mode = JL_SA_LARGE, cut = JL_SA_BINS, before = 0;    // the bin of the cut (LARGE) or the last bin (LISTED); candidates before it
     uint64_t mass = 0;
     if (s.k || s.nucleus || s.low > 0.f) {
         constexpr int PER = JL_SA_BINS / 512;
         const bool weighs = s.nucleus && !s.k;      // (the bins have sums)
         const int b0 = PER * threadIdx.x;
         u32 c[PER];
-        uint64_t m[PER], cs = 0, ms = 0, all, mass_all;
+        uint64_t m[PER], cs = 0, ms = 0, all, mass_all = 0;
 #pragma unroll
         for (int j = 0; j < PER; j++) {
             c[j] = ws.counts[b0 + j];
@@ -500,40 +299,34 @@ __device__ __forceinline__ void sample_gather_body(const SampleArgs& p, uint64_t
             cs += c[j];
             ms += m[j];
         }
-        if (threadIdx.x < 8) told[threadIdx.x] = threadIdx.x < 2 ? (u32)JL_SA_BINS : 0u;
-        uint64_t cb = sample_scan512(scan, cs, all) - cs, mb = 0;
-        mass_all = 0;
-        if (weighs) mb = sample_scan512(scan, ms, mass_all) - ms;
+        if (threadIdx.x < 8) told[threadIdx.x] = threadIdx.x == 0 ? (u32)JL_SA_BINS : 0u;
+        uint64_t cb = sample_scan<8>(scan, cs, all) - cs, mb = 0;
+        if (weighs) mb = sample_scan<8>(scan, ms, mass_all) - ms;
         const double reach = (double)s.p * (double)mass_all;
-        // told: 0 the cut's bin, 1 low_bin's count through it, ... ; the last bin has what is left over
 #pragma unroll
         for (int j = 0; j < PER; j++) {
-            const u32 b = b0 + j, n = b == JL_SA_BINS - 1 ? s.valid - (u32)cb : c[j];
+            const u32 b = b0 + j, n = b == JL_SA_BINS - 1 ? s.valid - (u32)cb : c[j];      // (the last bin has what is left over)
             const uint64_t ce = cb + n, me = mb + m[j];
             const bool crossed = s.k ? ce >= s.k && cb < s.k : s.nucleus && n && (double)me >= reach && !(cb && (double)mb >= reach);
             if (crossed) {
                 told[0] = b;
-                told[2] = (u32)cb;
+                told[1] = (u32)cb;
+                told[2] = (u32)ce;
                 told[3] = (u32)mb;
                 told[4] = (u32)(mb >> 32);
-                told[5] = (u32)ce;
             }
-            if (b == low_bin) told[6] = (u32)ce;
+            if (b == low_bin) told[5] = (u32)ce;
             cb = ce;
             mb = me;
         }
         __syncthreads();
         cut = told[0];
-        before = told[2];
+        before = told[1];
         mass = (uint64_t)told[4] << 32 | told[3];
-        const u32 through = told[5], low_through = told[6];
+        const u32 through = told[2], low_through = told[5];
         if (s.low > 0.f && low_bin < cut && !(s.k && s.nucleus)) {   // min_p ends first
-            if (low_through <= JL_SA_LIST) {
-                mode = JL_SA_LISTED;
-                cut = low_bin;
-            } else {
-                cut = JL_SA_BINS;
-            }
+            mode = low_through <= JL_SA_LIST ? JL_SA_LISTED : JL_SA_LARGE;
+            cut = mode == JL_SA_LISTED ? low_bin : (u32)JL_SA_BINS;
         } else if (cut < JL_SA_BINS) {
             mode = through <= JL_SA_LIST ? JL_SA_LISTED : s.k && s.nucleus ? JL_SA_SLOW : through - before <= JL_SA_LIST ? JL_SA_LARGE : JL_SA_SLOW;
         }
@@ -546,80 +339,441 @@ __device__ __forceinline__ void sample_gather_body(const SampleArgs& p, uint64_t
         ws.mass = mass;
     }
     if (mode == JL_SA_SLOW) return;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, part = blockIdx.x * JL_SA_PARTS + wave;
     int from, end;
-    sample_slice(p, blockIdx.x, from, end);
-    uint64_t sum = 0, total;
-    sample_range<512>(p, row, from, end, [&](float x, u32 i) {
-        const u32 key = sample_key(x);
-        if (!key) return;
-        const u32 b = s.r.bin(x);
-        if (mode == JL_SA_LISTED ? b <= cut : b == cut) {
+    sample_part(p, part, from, end);
+    // by value: what goes into the list, from `list` on and below `sure`; what is kept for sure, from `sure` on (min_p's border in it)
+    const float none = __builtin_inff();
+    const bool cuts = cut < JL_SA_BINS;
+    const float list = cuts ? sample_edge([&](float x) { return s.r.bin(x) <= cut; }) : none;
+    float sure = none;
+    if (mode == JL_SA_LARGE) {
+        sure = cuts ? sample_edge([&](float x) { return s.r.bin(x) < cut; }) : -3.4028234663852886e38f;
+        if (s.low > 0.f) sure = fmaxf(sure, sample_edge([&](float x) { return s.r.weight(x) >= (double)s.low; }));
+    }
+    const float below = mode == JL_SA_LARGE && cuts ? sample_edge([&](float x) { return s.r.bin(x) < cut; }) : none;
+    const bool whole = !(below < none);       // no upper border of the list
+    uint64_t sum = 0;
+    sample_range<64>(p, row, from, end, lane, [&](float x, u32 i) {
+        if (cuts && x >= list && (whole || x < below)) {
             const u32 at = atomicAdd(&ws.fill, 1u);
             if (at < JL_SA_LIST) {
-                ws.key[at] = key;
+                ws.key[at] = sample_key(x);
                 ws.idx[at] = i;
             }
-        } else if (mode == JL_SA_LARGE && b < cut) {
-            sum += s.r.kept(x, i, s.low, s.first);
         }
+        if (mode == JL_SA_LARGE && x >= sure) sum += s.r.whole(x);
     });
     if (mode == JL_SA_LARGE) {
-        sample_scan512(scan, sum, total);
-        if (threadIdx.x == 0) ws.slice[blockIdx.x] = total;
+        sum = sample_scan64(sum);
+        if (lane == 63) ws.part[part] = sum;
     }
 }
 
-// The workgroup's list of up to 1024 (a thread an element), ascending.
-__device__ __forceinline__ uint64_t sample_sort(uint64_t* lds, uint64_t v, u32 n) {
-    const u32 tid = threadIdx.x;
+// ---- a workgroup a row ------------------------------------------------------------------
+
+#define JL_SA_WAVES 4
+#define JL_SA_THREADS 256
+struct SampleLds {
+    uint64_t mass[JL_SA_BINS];
+    u32 count[JL_SA_BINS];
+    u32 key[JL_SA_LIST], idx[JL_SA_LIST];
+    uint64_t tile[512];              // sums of tiles of a range, or of the row's parts
+    uint64_t scan[JL_SA_WAVES];
+    uint64_t at_mass;
+    u32 at, at_count, at_n, fill, lo, hi, res_key, res_idx;
+};
+#define JL_SA_TILE 1024      // elements of a workgroup's step in index order
+
+template <class F> __device__ __forceinline__ void sample_each(const SampleArgs& p, size_t row, F f) { sample_range<JL_SA_THREADS>(p, row, 0, p.n, threadIdx.x, f); }
+
+// The first element by index, of those from to end, with crosses(sum of weight(x, i) up to and with it); ~0: none.  weight is 0 for elements that are not in the sum.
+template <class W, class X> __device__ __forceinline__ u32 sample_cross(const SampleArgs& p, SampleLds& s, size_t row, int from, int end, W weight, X crosses, uint64_t& total) {
+    const int tiles = (end - from + JL_SA_TILE - 1) / JL_SA_TILE, lane = threadIdx.x & 63;   // (512 at most)
+    __syncthreads();
+    for (int i = threadIdx.x; i < 512; i += JL_SA_THREADS) s.tile[i] = 0;
+    if (threadIdx.x == 0) s.at = ~0u;
+    __syncthreads();
+    const size_t at = row * p.stride;
+    auto load = [&](int i) { return sample_load(p, at + i, end - i); };
+    for (int i = from + 4 * (int)threadIdx.x, k = 0; k < tiles; k++, i += JL_SA_TILE) {
+        uint64_t sum = 0;
+        if (i < end) {
+            const f32x4 v = load(i);
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (i + j < end) sum += weight(v[j], (u32)(i + j));
+        }
+        sum = sample_scan64(sum);
+        if (lane == 63 && sum) atomicAdd((unsigned long long*)&s.tile[k], (unsigned long long)sum);
+    }
+    __syncthreads();
+    // two tiles a thread
+    const uint64_t t0 = s.tile[2 * threadIdx.x], t1 = s.tile[2 * threadIdx.x + 1];
+    uint64_t c = sample_scan<JL_SA_WAVES>(s.scan, t0 + t1, total) - t0 - t1;
+    bool had = c != 0 && crosses(c);
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+        const uint64_t t = j ? t1 : t0;
+        if (t && !had && crosses(c + t)) {
+            s.at = 2 * threadIdx.x + j;
+            s.at_mass = c;
+            had = true;
+        }
+        c += t;
+    }
+    __syncthreads();
+    const u32 tile = s.at;
+    const uint64_t before = s.at_mass;
+    __syncthreads();
+    if (tile == ~0u) return ~0u;   // uniform
+    if (threadIdx.x == 0) s.at = ~0u;
+    const int i = from + (int)tile * JL_SA_TILE + 4 * (int)threadIdx.x;
+    uint64_t part[4] = {0, 0, 0, 0}, mine = 0, all;
+    if (i < end) {
+        const f32x4 v = load(i);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if (i + j < end) part[j] = weight(v[j], (u32)(i + j));
+            mine += part[j];
+        }
+    }
+    c = before + sample_scan<JL_SA_WAVES>(s.scan, mine, all) - mine;
+    had = c != 0 && crosses(c);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        if (part[j] && !had && crosses(c + part[j])) {
+            s.at = (u32)(i + j);
+            had = true;
+        }
+        c += part[j];
+    }
+    __syncthreads();
+    const u32 found = s.at;
+    __syncthreads();
+    return found;
+}
+
+// What is kept: elements not behind (key, idx) in the order.
+struct SampleCut {
+    u32 key, idx;
+    uint64_t mass;     // of those
+    __device__ bool keeps(u32 k, u32 i) const { return k > key || (k == key && i <= idx); }
+};
+
+// Counts and sums of the bins (bin(x, key) < BINS, or ~0: not in it).
+template <class B> __device__ __forceinline__ void sample_count(const SampleArgs& p, SampleLds& s, size_t row, const SampleRow& r, B bin) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < JL_SA_BINS; i += JL_SA_THREADS) {
+        s.mass[i] = 0;
+        s.count[i] = 0;
+    }
+    __syncthreads();
+    sample_each(p, row, [&](float x, u32) {
+        const u32 k = sample_key(x), b = k ? bin(x, k) : ~0u;
+        if (b < JL_SA_BINS) {
+            atomicAdd(&s.count[b], 1u);
+            atomicAdd((unsigned long long*)&s.mass[b], (unsigned long long)r.whole(x));
+        }
+    });
+    __syncthreads();
+}
+
+// The bin in which crosses(count, mass) with the bins up to it is first true, and what lies before it: s.at, s.at_count, s.at_mass, s.at_n.
+// None: s.at stays ~0.
+template <class X> __device__ __forceinline__ void sample_find(SampleLds& s, u32 count0, uint64_t mass0, X crosses) {
+    if (threadIdx.x == 0) s.at = ~0u;
+    constexpr int PER = JL_SA_BINS / JL_SA_THREADS;
+    const int b0 = PER * threadIdx.x;
+    uint64_t c = 0, m = 0, all;
+    for (int j = 0; j < PER; j++) {
+        c += s.count[b0 + j];
+        m += s.mass[b0 + j];
+    }
+    uint64_t cb = sample_scan<JL_SA_WAVES>(s.scan, c, all) - c + count0, mb = sample_scan<JL_SA_WAVES>(s.scan, m, all) - m + mass0;
+    for (int j = 0; j < PER; j++) {
+        const u32 cj = s.count[b0 + j];
+        const uint64_t mj = s.mass[b0 + j];
+        if (cj && crosses((u32)(cb + cj), mb + mj) && !(cb && crosses((u32)cb, mb))) {
+            s.at = b0 + j;
+            s.at_count = (u32)cb;
+            s.at_mass = mb;
+            s.at_n = cj;
+        }
+        cb += cj;
+        mb += mj;
+    }
+    __syncthreads();
+}
+
+// A SLOW row's cut: the last element kept, in the order, such that crosses(count, mass) up to it is first true.  False: nothing crosses.
+template <class X> __device__ __forceinline__ bool sample_cut(const SampleArgs& p, SampleLds& s, size_t row, const SampleRow& r, X crosses, SampleCut& cut) {
+    sample_count(p, s, row, r, [&](float x, u32) { return r.bin(x); });
+    sample_find(s, 0, 0, crosses);
+    if (s.at == ~0u) return false;   // uniform
+    const u32 bin0 = s.at;
+    u32 n = s.at_n, count = s.at_count, klo = 1, khi = ~0u;
+    uint64_t mass = s.at_mass;
+    __syncthreads();
+    if (n > JL_SA_LIST) {
+        if (threadIdx.x == 0) {
+            s.lo = ~0u;
+            s.hi = 0;
+        }
+        __syncthreads();
+        u32 lo = ~0u, hi = 0;
+        sample_each(p, row, [&](float x, u32) {
+            const u32 k = sample_key(x);
+            if (k && r.bin(x) == bin0) {
+                lo = min(lo, k);
+                hi = max(hi, k);
+            }
+        });
+        atomicMin(&s.lo, lo);
+        atomicMax(&s.hi, hi);
+        __syncthreads();
+        klo = s.lo;
+        khi = s.hi;
+        while (n > JL_SA_LIST && klo < khi) {
+            int shift = 0;
+            while ((khi - klo) >> shift >= JL_SA_BINS) shift++;
+            sample_count(p, s, row, r, [&](float x, u32 k) { return r.bin(x) == bin0 && k >= klo && k <= khi ? (khi - k) >> shift : ~0u; });
+            sample_find(s, count, mass, crosses);
+            n = s.at_n;
+            count = s.at_count;
+            mass = s.at_mass;
+            const u32 top = khi - (s.at << shift), width = (1u << shift) - 1;
+            __syncthreads();
+            klo = top - klo > width ? top - width : klo;
+            khi = top;
+        }
+    }
+    if (n > JL_SA_LIST) {   // one key, many times: by index
+        const uint64_t w0 = r.whole(sample_value(klo));
+        uint64_t total;
+        // counted: sums of 1, the crossing by count and mass
+        cut.idx = sample_cross(p, s, row, 0, p.n, [&](float x, u32) { return (uint64_t)(sample_key(x) == klo); },
+                               [&](uint64_t c) { return crosses(count + (u32)c, mass + c * w0); }, total);
+        cut.key = klo;
+        // how many that are: again over those up to it
+        const u32 last = cut.idx;
+        sample_cross(p, s, row, 0, p.n, [&](float x, u32 i) { return (uint64_t)(sample_key(x) == klo && i <= last); }, [&](uint64_t) { return false; }, total);
+        cut.mass = mass + total * w0;
+        return true;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) s.fill = 0;
+    __syncthreads();
+    sample_each(p, row, [&](float x, u32 i) {
+        const u32 k = sample_key(x);
+        if (k && k >= klo && k <= khi && r.bin(x) == bin0) {
+            const u32 at = atomicAdd(&s.fill, 1u);
+            if (at < JL_SA_LIST) {
+                s.key[at] = k;
+                s.idx[at] = i;
+            }
+        }
+    });
+    __syncthreads();
+    // an element at a time: those ahead of it, and their weights
+    uint64_t* const w = s.mass;   // (the bins have been read)
+    for (u32 i = threadIdx.x; i < n; i += JL_SA_THREADS) w[i] = r.whole(sample_value(s.key[i]));
+    __syncthreads();
+    for (u32 e = threadIdx.x; e < n; e += JL_SA_THREADS) {
+        const u32 k = s.key[e], i = s.idx[e];
+        u32 ahead = 0;
+        uint64_t m = 0;
+        for (u32 j = 0; j < n; j++) {
+            const bool is = s.key[j] > k || (s.key[j] == k && s.idx[j] < i);
+            ahead += is;
+            m += is ? w[j] : 0;
+        }
+        const u32 cb = count + ahead;
+        if (crosses(cb + 1, mass + m + w[e]) && !(cb && crosses(cb, mass + m))) {
+            s.res_key = k;
+            s.res_idx = i;
+            s.at_mass = mass + m + w[e];
+        }
+    }
+    __syncthreads();
+    cut.key = s.res_key;
+    cut.idx = s.res_idx;
+    cut.mass = s.at_mass;
+    __syncthreads();
+    return true;
+}
+
+// 64 NQ elements of a workgroup's (Q = 4), or a wavefront's (Q = 1) list, ascending; element e + THREADS q is thread e's q-th.  The network needs as many
+// as n rounded up to a power of two.
+template <int NQ, bool WG> __device__ __forceinline__ void sample_sort(uint64_t* lds, uint64_t (&v)[NQ], u32 n) {
+    constexpr u32 T = WG ? JL_SA_THREADS : 64;
+    const u32 tid = WG ? threadIdx.x : threadIdx.x & 63;
     u32 size = 64;
-    while (size < n) size *= 2;
+    while (WG && size < n) size *= 2;
     for (u32 k = 2; k <= size; k *= 2)
         for (u32 j = k / 2; j; j /= 2) {
-            uint64_t o;
-            if (j < 64) {
-                o = __shfl_xor((unsigned long long)v, (int)j, 64);
-            } else {
-                __syncthreads();
-                lds[tid] = v;
-                __syncthreads();
-                o = lds[tid ^ j];
+            if (j >= T) {      // between the thread's own
+#pragma unroll
+                for (u32 q = 0; q < NQ; q++) {
+                    const u32 o = q ^ (j / T);
+                    if (o > q && o < NQ) {
+                        const bool up = ((tid + T * q) & k) == 0;
+                        const uint64_t a = v[q], b = v[o];
+                        const bool turn = up ? a > b : a < b;
+                        v[q] = turn ? b : a;
+                        v[o] = turn ? a : b;
+                    }
+                }
+                continue;
             }
-            const bool up = (tid & k) == 0, lower = (tid & j) == 0;
-            v = (up == lower) == (v < o) ? v : o;
+            if (WG && j >= 64) {
+                __syncthreads();
+#pragma unroll
+                for (int q = 0; q < NQ; q++) lds[tid + T * q] = v[q];
+                __syncthreads();
+            }
+#pragma unroll
+            for (int q = 0; q < NQ; q++) {
+                const uint64_t o = WG && j >= 64 ? lds[(tid ^ j) + T * q] : (uint64_t)__shfl_xor((unsigned long long)v[q], (int)j, 64);
+                const bool up = ((tid + T * q) & k) == 0, lower = (tid & j) == 0;
+                v[q] = (up == lower) == (v[q] < o) ? v[q] : o;
+            }
         }
-    __syncthreads();
-    return v;
+    if (WG) __syncthreads();
 }
 
-// The same within a wavefront, and its inclusive sums.
-__device__ __forceinline__ uint64_t sample_sort64(uint64_t v) {
-    const u32 lane = threadIdx.x & 63;
+// The token of a LISTED row, or (LARGE) the cut's element and the kept of the list into their parts' sums.  NQ elements a thread; WG false: by one wavefront.
+template <int NQ, bool WG, class G>
+__device__ __forceinline__ void sample_list(const SampleArgs& p, SampleLds& s, const SampleRowWs& ws, const SampleSet& set, float u, u32 n, SampleCut& cut, G give) {
+    constexpr u32 T = WG ? JL_SA_THREADS : 64;
+    const u32 tid = WG ? threadIdx.x : threadIdx.x & 63;
+    const SampleRow& r = set.r;
+    const bool large = ws.mode == JL_SA_LARGE;
+    const uint64_t base = large ? ws.mass : 0, row_all = ws.all;
+    const u32 before = large ? ws.before : 0;
+    uint64_t v[NQ], w[NQ], through[NQ];
+    // descending by key, ascending by index: ascending by the key's complement
 #pragma unroll
-    for (u32 k = 2; k <= 64; k *= 2)
+    for (int q = 0; q < NQ; q++) v[q] = tid + T * q < n ? (uint64_t)~ws.key[tid + T * q] << 32 | ws.idx[tid + T * q] : ~0ull;
+    sample_sort<NQ, WG>(s.mass, v, n);
+    // sums up to and with each, and the number of kept
+    uint64_t sum = base;
 #pragma unroll
-        for (u32 j = k / 2; j; j /= 2) {
-            const uint64_t o = __shfl_xor((unsigned long long)v, (int)j, 64);
-            v = (((lane & k) == 0) == ((lane & j) == 0)) == (v < o) ? v : o;
+    for (int q = 0; q < NQ; q++) {
+        w[q] = tid + T * q < n ? r.whole(sample_value(~(u32)(v[q] >> 32))) : 0;
+        uint64_t all;
+        if (WG) through[q] = sum + sample_scan<JL_SA_WAVES>(s.scan, w[q], all);
+        else {
+            through[q] = sum + sample_scan64(w[q]);
+            all = 0;
         }
-    return v;
-}
-__device__ __forceinline__ uint64_t sample_scan64(uint64_t v) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const uint64_t o = __shfl_up((unsigned long long)v, d, 64);
-        if (lane >= d) v += o;
+        sum += all;
     }
-    return v;
+    u32 kept = set.k ? min(n, set.k - before) : n;
+    if (set.nucleus) {
+        uint64_t all = row_all;
+        if (set.k) {
+            if (WG) {
+                __syncthreads();
+#pragma unroll
+                for (int q = 0; q < NQ; q++)
+                    if (tid + T * q == kept - 1) s.at_mass = through[q];
+                __syncthreads();
+                all = s.at_mass;
+            } else {
+                all = __shfl((unsigned long long)through[0], (int)kept - 1, 64);
+            }
+        }
+        const double reach = (double)set.p * (double)all;
+        if (WG) {
+            __syncthreads();
+            if (tid == 0) s.at = kept;
+            __syncthreads();
+#pragma unroll
+            for (int q = 0; q < NQ; q++)
+                if (tid + T * q < kept && (double)through[q] >= reach) atomicMin(&s.at, tid + T * q + 1);
+            __syncthreads();
+            kept = s.at;
+        } else {
+            const uint64_t over = __ballot(tid < kept && (double)through[0] >= reach);
+            if (over) kept = (u32)__builtin_ctzll(over) + 1;
+        }
+    }
+    if (WG && large) {
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < NQ; q++) {
+            const u32 e = tid + T * q, idx = (u32)v[q];
+            if (e == kept - 1) {
+                s.res_key = ~(u32)(v[q] >> 32);
+                s.res_idx = idx;
+            }
+            if (e < kept && w[q] && (!(set.low > 0.f) || r.weight(sample_value(~(u32)(v[q] >> 32))) >= (double)set.low)) {
+                const u32 slice = idx / (u32)p.slice_len, part = slice * JL_SA_PARTS + (idx - slice * (u32)p.slice_len) / (u32)p.part_len;
+                atomicAdd((unsigned long long*)&s.tile[part], (unsigned long long)w[q]);
+            }
+        }
+        __syncthreads();
+        cut.key = s.res_key;
+        cut.idx = s.res_idx;
+        return;
+    }
+    // those that min_p keeps, by index; the place in the list goes along
+    uint64_t by[NQ], mine[NQ], c[NQ], total = 0;
+    if (WG) __syncthreads();
+#pragma unroll
+    for (int q = 0; q < NQ; q++) {
+        const u32 e = tid + T * q;
+        const bool in = e < kept && w[q] && (!(set.low > 0.f) || r.weight(sample_value(~(u32)(v[q] >> 32))) >= (double)set.low);
+        if (WG) s.mass[1024 + e] = w[q];
+        by[q] = in ? (v[q] & 0xffffffffu) << 32 | e : ~0ull;
+    }
+    if (WG) __syncthreads();
+    sample_sort<NQ, WG>(s.mass, by, n);
+#pragma unroll
+    for (int q = 0; q < NQ; q++) {
+        const uint64_t there = WG ? s.mass[1024 + ((u32)by[q] & 1023)] : (uint64_t)__shfl((unsigned long long)w[0], (int)(by[0] & 63), 64);
+        mine[q] = by[q] == ~0ull ? 0 : there;
+        uint64_t all;
+        if (WG) c[q] = total + sample_scan<JL_SA_WAVES>(s.scan, mine[q], all);
+        else {
+            c[q] = sample_scan64(mine[q]);
+            all = __shfl((unsigned long long)c[q], 63, 64);
+        }
+        total += all;
+    }
+    const double over = (double)u * (double)total;
+    u32 at;      // the first over it, or the last
+    if (WG) {
+        __syncthreads();
+        if (tid == 0) {
+            s.at = ~0u;
+            s.hi = 0;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < NQ; q++) {
+            if (mine[q] && (double)c[q] > over) atomicMin(&s.at, tid + T * q);
+            if (mine[q]) atomicMax(&s.hi, tid + T * q);
+        }
+        __syncthreads();
+        at = s.at != ~0u ? s.at : s.hi;
+    } else {
+        const uint64_t yes = __ballot(mine[0] && (double)c[0] > over), any = __ballot(mine[0] != 0);
+        at = (u32)(yes ? __builtin_ctzll(yes) : 63 - __builtin_clzll(any));
+    }
+#pragma unroll
+    for (int q = 0; q < NQ; q++)
+        if (tid + T * q == at) give((u32)(by[q] >> 32), (double)mine[q] / (double)total);
 }
 
-// grid = rows, block = 1024.
+// grid = rows, block = 256.
 __device__ __forceinline__ void sample_take_body(const SampleArgs& p, SampleLds& s) {
     const size_t row = blockIdx.x;
     const SampleRowWs& ws = ((const SampleRowWs*)p.ws)[row];
+    const u32 tid = threadIdx.x, mode = ws.mode, fill = min(ws.fill, (u32)JL_SA_LIST), bin = ws.bin;
+    const float u = p.u[row];
     const SampleSet set = sample_set(p, row);
-    const u32 tid = threadIdx.x, mode = ws.mode;
     const SampleRow& r = set.r;
     auto give = [&](u32 token, double prob) {
         p.token[row] = token;
@@ -629,98 +783,25 @@ __device__ __forceinline__ void sample_take_body(const SampleArgs& p, SampleLds&
         if (tid == 0) give(set.best ? set.first : (u32)p.n, set.best ? 1.0 : 0.0);
         return;
     }
-    const float u = p.u[row];
     SampleCut cut = {1u, ~0u, 0};
-    if (mode == JL_SA_LISTED && ws.fill <= 64) {   // by one wavefront
-        if (tid >= 64) return;
-        const u32 n = ws.fill;
-        uint64_t v = sample_sort64(tid < n ? (uint64_t)~ws.key[tid] << 32 | ws.idx[tid] : ~0ull);
-        const float x = sample_value(~(u32)(v >> 32));
-        const uint64_t w = tid < n ? r.whole(x) : 0, through = sample_scan64(w);
-        u32 kept = set.k ? min(n, set.k) : n;
-        if (set.nucleus) {
-            const uint64_t all = set.k ? (uint64_t)__shfl((unsigned long long)through, (int)kept - 1, 64) : ws.all;
-            const uint64_t over = __ballot(tid < kept && (double)through >= (double)set.p * (double)all);
-            if (over) kept = (u32)__builtin_ctzll(over) + 1;
+    if (mode == JL_SA_LISTED) {
+        if (fill <= 64) {
+            if (tid < 64) sample_list<1, false>(p, s, ws, set, u, fill, cut, give);
+        } else if (fill <= JL_SA_THREADS) {
+            sample_list<1, true>(p, s, ws, set, u, fill, cut, give);
+        } else {
+            sample_list<4, true>(p, s, ws, set, u, fill, cut, give);
         }
-        const bool in = tid < kept && (!(set.low > 0.f) || r.weight(x) >= (double)set.low || tid == 0);
-        // by index; the place in the list goes along
-        const uint64_t by = sample_sort64(in ? (v & 0xffffffffu) << 32 | tid : ~0ull);
-        const uint64_t there = __shfl((unsigned long long)w, (int)(by & 63), 64), mine = by == ~0ull ? 0 : there;
-        const uint64_t c = sample_scan64(mine), total = __shfl((unsigned long long)c, 63, 64);
-        const uint64_t over = __ballot(mine && (double)c > (double)u * (double)total), any = __ballot(mine != 0);
-        if (tid == (u32)(over ? __builtin_ctzll(over) : 63 - __builtin_clzll(any))) give((u32)(by >> 32), (double)mine / (double)total);
         return;
     }
-    if (mode == JL_SA_LISTED || (mode == JL_SA_LARGE && ws.bin < JL_SA_BINS)) {
-        const u32 n = min(ws.fill, (u32)JL_SA_LIST);
-        // descending by key, ascending by index: ascending by the key's complement
-        uint64_t v = tid < n ? (uint64_t)~ws.key[tid] << 32 | ws.idx[tid] : ~0ull;
-        v = sample_sort(s.mass, v, n);
-        const u32 key = ~(u32)(v >> 32), idx = (u32)v;
-        const bool live = tid < n;
-        const uint64_t w = live ? r.whole(sample_value(key)) : 0;
-        uint64_t all;
-        const uint64_t base = mode == JL_SA_LARGE ? ws.mass : 0;
-        const u32 before = mode == JL_SA_LARGE ? ws.before : 0;
-        const uint64_t through = base + sample_scan(s, w, all);      // sums up to and with this one
-        u32 kept = n;
-        if (set.k) kept = min(kept, set.k - before);
+    const int parts = p.slices * JL_SA_PARTS;
+    if (mode == JL_SA_LARGE) {
+        for (int i = tid; i < 512; i += JL_SA_THREADS) s.tile[i] = i < parts ? ws.part[i] : 0;
         __syncthreads();
-        if (tid == 0) s.at = kept;
-        if (tid == kept - 1) s.at_mass = through;
-        __syncthreads();
-        if (set.nucleus) {
-            const double reach = (double)set.p * (double)(set.k ? s.at_mass : ws.all);
-            if (tid < kept && (double)through >= reach) atomicMin(&s.at, tid + 1);
-            __syncthreads();
+        if (bin < JL_SA_BINS) {
+            if (fill <= JL_SA_THREADS) sample_list<1, true>(p, s, ws, set, u, fill, cut, give);
+            else sample_list<4, true>(p, s, ws, set, u, fill, cut, give);
         }
-        kept = s.at;
-        __syncthreads();
-        if (mode == JL_SA_LARGE) {
-            if (tid == kept - 1) {
-                s.res_key = key;
-                s.res_idx = idx;
-            }
-            __syncthreads();
-            cut.key = s.res_key;
-            cut.idx = s.res_idx;
-        } else {
-            // those of them that min_p keeps, by index
-            const bool in = tid < kept && (!(set.low > 0.f) || r.weight(sample_value(key)) >= (double)set.low || tid == 0);
-            __syncthreads();
-            if (tid < n) s.mass[1024 + tid] = in ? w : 0;
-            uint64_t by = in ? (uint64_t)idx << 32 | tid : ~0ull;
-            __syncthreads();
-            by = sample_sort(s.mass, by, n);
-            const bool has = by != ~0ull;
-            const uint64_t mine = has ? s.mass[1024 + (u32)by] : 0;
-            uint64_t total;
-            const uint64_t c = sample_scan(s, mine, total);
-            const double over = (double)u * (double)total;
-            __syncthreads();
-            if (tid == 0) {
-                s.at = ~0u;
-                s.hi = 0;
-            }
-            __syncthreads();
-            if (mine && (double)c > over) atomicMin(&s.at, tid);
-            if (mine) atomicMax(&s.hi, tid);
-            __syncthreads();
-            if (tid == (s.at != ~0u ? s.at : s.hi)) give((u32)(by >> 32), (double)mine / (double)total);
-            return;
-        }
-        // the list's kept into their slices' sums
-        if (tid < (u32)p.slices) s.tile[tid] = ws.slice[tid];
-        __syncthreads();
-        if (tid < kept) {
-            const uint64_t k = r.kept(sample_value(key), idx, set.low, set.first);
-            if (k) atomicAdd((unsigned long long*)&s.tile[idx / (u32)p.slice_len], (unsigned long long)k);
-        }
-        __syncthreads();
-    } else if (mode == JL_SA_LARGE) {
-        if (tid < (u32)p.slices) s.tile[tid] = ws.slice[tid];
-        __syncthreads();
     } else {
         if (set.k) sample_cut(p, s, row, r, [&](u32 c, uint64_t) { return c >= set.k; }, cut);
         if (set.nucleus) {
@@ -728,55 +809,66 @@ __device__ __forceinline__ void sample_take_body(const SampleArgs& p, SampleLds&
             if (!set.k) {
                 uint64_t sum = 0;
                 sample_each(p, row, [&](float x, u32) { sum += sample_key(x) ? r.whole(x) : 0; });
-                sample_scan(s, sum, all);
+                sample_scan<JL_SA_WAVES>(s.scan, sum, all);
             }
             const double reach = (double)set.p * (double)all;
             sample_cut(p, s, row, r, [&](u32, uint64_t m) { return (double)m >= reach; }, cut);
         }
-        for (int i = 0; i < p.slices; i++) {
+        __syncthreads();
+        for (int i = tid; i < 512; i += JL_SA_THREADS) s.tile[i] = 0;
+        __syncthreads();
+        for (int i = (int)tid >> 6; i < parts; i += JL_SA_WAVES) {
             int from, end;
-            sample_slice(p, i, from, end);
-            uint64_t sum = 0, all;
-            sample_range<1024>(p, row, from, end, [&](float x, u32 e) {
+            sample_part(p, i, from, end);
+            uint64_t sum = 0;
+            sample_range<64>(p, row, from, end, tid & 63, [&](float x, u32 e) {
                 const u32 key = sample_key(x);
-                if (key && cut.keeps(key, e)) sum += r.kept(x, e, set.low, set.first);
+                if (key && cut.keeps(key, e)) sum += r.kept(x, set.low);
             });
-            sample_scan(s, sum, all);
-            if (tid == 0) s.slices[i] = all;
+            sum = sample_scan64(sum);
+            if ((tid & 63) == 63) s.tile[i] = sum;
         }
         __syncthreads();
-        if (tid < (u32)p.slices) s.tile[tid] = s.slices[tid];
-        __syncthreads();
     }
-    // the slice in which the sum exceeds u of it, a slice a lane; and the token there
-    const int lane = tid & 63;
-    const uint64_t mine = lane < p.slices ? s.tile[lane] : 0;
-    uint64_t sum = mine;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const uint64_t o = __shfl_up((unsigned long long)sum, d, 64);
-        if (lane >= d) sum += o;
-    }
-    const uint64_t total = __shfl((unsigned long long)sum, 63, 64);
+    // the part in which the sum exceeds u of it, two parts a thread; and the token there
+    const uint64_t t0 = s.tile[2 * tid], t1 = s.tile[2 * tid + 1];
+    uint64_t total, c = sample_scan<JL_SA_WAVES>(s.scan, t0 + t1, total) - t0 - t1;
     const double over = (double)u * (double)total;
-    const uint64_t over_at = __ballot(mine && (double)sum > over), any = __ballot(mine != 0);
-    const int slice = over_at ? __builtin_ctzll(over_at) : -1, last = any ? 63 - __builtin_clzll(any) : 0;
-    const uint64_t before = __shfl((unsigned long long)(sum - mine), slice < 0 ? 0 : slice, 64);
+    if (tid == 0) {
+        s.at = ~0u;
+        s.hi = 0;
+    }
+    __syncthreads();
+    bool had = c && (double)c > over;
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+        const uint64_t t = j ? t1 : t0;
+        if (t) atomicMax(&s.hi, 2 * tid + j);
+        if (t && !had && (double)(c + t) > over) {
+            s.at = 2 * tid + j;
+            s.at_mass = c;
+            had = true;
+        }
+        c += t;
+    }
+    __syncthreads();
+    const bool found = s.at != ~0u;
+    const uint64_t before = s.at_mass;
+    int from, end;
+    sample_part(p, (int)(found ? s.at : s.hi), from, end);
     __syncthreads();
     auto weight = [&](float x, u32 i) -> uint64_t {
         const u32 key = sample_key(x);
-        return key && cut.keeps(key, i) ? r.kept(x, i, set.low, set.first) : 0;
+        return key && cut.keeps(key, i) ? r.kept(x, set.low) : 0;
     };
-    int from, end;
-    sample_slice(p, slice < 0 ? last : slice, from, end);
     u32 token = ~0u;
     uint64_t in;
-    if (slice >= 0) token = sample_cross(p, s, row, from, end, weight, [&](uint64_t c) { return (double)(before + c) > over; }, in);
+    if (found) token = sample_cross(p, s, row, from, end, weight, [&](uint64_t m) { return (double)(before + m) > over; }, in);
     if (token == ~0u) {   // u is 1 or more, or no number: the last that is kept
         if (tid == 0) s.hi = 0;
         __syncthreads();
         u32 at = 0;
-        sample_range<1024>(p, row, from, end, [&](float x, u32 i) { at = weight(x, i) ? max(at, i) : at; });
+        sample_range<JL_SA_THREADS>(p, row, from, end, tid, [&](float x, u32 i) { at = weight(x, i) ? max(at, i) : at; });
         atomicMax(&s.hi, at);
         __syncthreads();
         token = s.hi;

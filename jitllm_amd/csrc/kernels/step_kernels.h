@@ -43,7 +43,7 @@ JL_ATTEND_JOIN(64) JL_ATTEND_JOIN(128) JL_ATTEND_JOIN(256)
 
 // grid = (slices, rows), block = 512
 extern "C" __global__ __launch_bounds__(512) void jl_sample_max(SampleArgs p) {
-    __shared__ u32 lds[4];
+    __shared__ u32 lds[3];
     sample_max_body(p, lds);
 }
 extern "C" __global__ __launch_bounds__(512) void jl_sample_bins(SampleArgs p) {
@@ -56,8 +56,8 @@ extern "C" __global__ __launch_bounds__(512) void jl_sample_gather(SampleArgs p)
     __shared__ u32 told[8];
     sample_gather_body(p, scan, told);
 }
-// grid = rows, block = 1024
-extern "C" __global__ __launch_bounds__(1024) void jl_sample_take(SampleArgs p) {
+// grid = rows, block = 256
+extern "C" __global__ __launch_bounds__(256) void jl_sample_take(SampleArgs p) {
     __shared__ SampleLds s;
     sample_take_body(p, s);
 }
