@@ -34,28 +34,31 @@ __device__ __forceinline__ u32 sample_key(float x) {
 }
 __device__ __forceinline__ float sample_value(u32 k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
 
+// a b + c, c in scalar registers (the compiler makes the two-address form of it, with a copy of c each).
+__device__ __forceinline__ double sample_fma(double a, double b, double c) {
+    double d;
+    asm("v_fma_f64 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "s"(c));
+    return d;
+}
+
 struct SampleRow {
     float max;        // of the row
     double a;         // log2 e / temperature
     float fine;       // bins a unit of x
-    // e^((x - max) / T) = 2^y, y = n + f with |f| <= 1/2: the series of 2^f up to (f ln2)^11 / 11! (the next term is under 2^-47).  Nothing for NaN, -infinity.
+    // e^((x - max) / T) = 2^y, y = n + f with |f| <= 1/2: 2^f as 1 + f q(f), q of the eighth degree through (2^f - 1) / f at the nine Chebyshev points: off by
+    // under 2^-44.  x is a candidate.  (Largest infinities: their difference is no number, and counts as 0.)
     __device__ double weight(float x) const {
-        const double y = fmax(((double)x - (double)max) * a, -1000.0);
+        const double y = fmax(fmin(((double)x - (double)max) * a, 0.0), -1000.0);
         const double z = y + 0x1.8p52, f = y - (z - 0x1.8p52);     // (n in z's low bits)
-        double p = 0x1.e8cac7351bb25p-32;
-        p = __builtin_fma(p, f, 0x1.e4cf5158b8ecap-28);
-        p = __builtin_fma(p, f, 0x1.b5253d395e7c4p-24);
-        p = __builtin_fma(p, f, 0x1.62c0223a5c824p-20);
-        p = __builtin_fma(p, f, 0x1.ffcbfc588b0c7p-17);
-        p = __builtin_fma(p, f, 0x1.430912f86c787p-13);
-        p = __builtin_fma(p, f, 0x1.5d87fe78a6731p-10);
-        p = __builtin_fma(p, f, 0x1.3b2ab6fba4e77p-7);
-        p = __builtin_fma(p, f, 0x1.c6b08d704a0c0p-5);
-        p = __builtin_fma(p, f, 0x1.ebfbdff82c58fp-3);
-        p = __builtin_fma(p, f, 0x1.62e42fefa39efp-1);
-        p = __builtin_fma(p, f, 0x1.0000000000000p+0);
-        const double w = __builtin_ldexp(p, (int)(u32)__builtin_bit_cast(uint64_t, z));
-        return x == max ? 1.0 : w;       // (an infinity is its own largest)
+        double p = sample_fma(f, 0x1.b638718fee5a8p-24, 0x1.63d136366db24p-20);
+        p = sample_fma(p, f, 0x1.ffcb95269d85ap-17);
+        p = sample_fma(p, f, 0x1.4308ac85aa947p-13);
+        p = sample_fma(p, f, 0x1.5d87fe86f82cdp-10);
+        p = sample_fma(p, f, 0x1.3b2ab7181b755p-7);
+        p = sample_fma(p, f, 0x1.c6b08d7047e8bp-5);
+        p = sample_fma(p, f, 0x1.ebfbdff823cedp-3);
+        p = sample_fma(p, f, 0x1.62e42fefa39efp-1);
+        return __builtin_ldexp(__builtin_fma(p, f, 1.0), (int)(u32)__builtin_bit_cast(uint64_t, z));
     }
     static __device__ uint64_t rounded(double w) { return __builtin_bit_cast(uint64_t, __builtin_fma(w, 0x1p44, 0x1p52)) & ((1ull << 52) - 1); }   // the low bits of w 2^44 + 2^52
     __device__ uint64_t whole(float x) const { return rounded(weight(x)); }
@@ -343,26 +346,30 @@ __device__ __forceinline__ void sample_gather_body(const SampleArgs& p, uint64_t
     int from, end;
     sample_part(p, part, from, end);
     // by value: what goes into the list, from `list` on and below `sure`; what is kept for sure, from `sure` on (min_p's border in it)
-    const float none = __builtin_inff();
     const bool cuts = cut < JL_SA_BINS;
-    const float list = cuts ? sample_edge([&](float x) { return s.r.bin(x) <= cut; }) : none;
-    float sure = none;
-    if (mode == JL_SA_LARGE) {
-        sure = cuts ? sample_edge([&](float x) { return s.r.bin(x) < cut; }) : -3.4028234663852886e38f;
-        if (s.low > 0.f) sure = fmaxf(sure, sample_edge([&](float x) { return s.r.weight(x) >= (double)s.low; }));
-    }
-    const float below = mode == JL_SA_LARGE && cuts ? sample_edge([&](float x) { return s.r.bin(x) < cut; }) : none;
-    const bool whole = !(below < none);       // no upper border of the list
-    uint64_t sum = 0;
-    sample_range<64>(p, row, from, end, lane, [&](float x, u32 i) {
-        if (cuts && x >= list && (whole || x < below)) {
-            const u32 at = atomicAdd(&ws.fill, 1u);
-            if (at < JL_SA_LIST) {
-                ws.key[at] = sample_key(x);
-                ws.idx[at] = i;
-            }
+    auto append = [&](float x, u32 i) {
+        const u32 at = atomicAdd(&ws.fill, 1u);
+        if (at < JL_SA_LIST) {
+            ws.key[at] = sample_key(x);
+            ws.idx[at] = i;
         }
-        if (mode == JL_SA_LARGE && x >= sure) sum += s.r.whole(x);
+    };
+    uint64_t sum = 0;
+    float list = sample_edge([&](float x) { return s.r.bin(x) <= cut; });
+    if (mode == JL_SA_LISTED) {
+        sample_range<64>(p, row, from, end, lane, [&](float x, u32 i) {
+            if (x >= list) append(x, i);
+        });
+        return;
+    }
+    const float below = cuts ? sample_edge([&](float x) { return s.r.bin(x) < cut; }) : list;
+    const float sure = s.low > 0.f ? fmaxf(below, sample_edge([&](float x) { return s.r.weight(x) >= (double)s.low; })) : below;
+    if (!cuts) list = sure;
+    sample_range<64>(p, row, from, end, lane, [&](float x, u32 i) {
+        if (x >= list) {
+            if (x >= sure) sum += s.r.whole(x);
+            else if (x < below) append(x, i);
+        }
     });
     if (mode == JL_SA_LARGE) {
         sum = sample_scan64(sum);
