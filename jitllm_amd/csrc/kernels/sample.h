@@ -22,6 +22,7 @@
 
 #pragma clang fp contract(off)
 
+#define JL_SA_FEW 64
 #define JL_SA_DONE 0
 #define JL_SA_LISTED 1
 #define JL_SA_LARGE 2
@@ -275,8 +276,8 @@ __device__ __forceinline__ void sample_bins_body(const SampleArgs& p, u32* count
     }
 }
 
-// grid = (slices, rows), block = 512.  LDS: 8 words of 8 bytes, then 8 of 4.
-__device__ __forceinline__ void sample_gather_body(const SampleArgs& p, uint64_t* scan, u32* told) {
+// grid = (slices, rows), block = 512.  LDS: 8 words of 8 bytes, then 10 of 4, and a list of keys and of places.
+__device__ __forceinline__ void sample_gather_body(const SampleArgs& p, uint64_t* scan, u32* told, u32* keys, u32* places) {
     const size_t row = blockIdx.y;
     const SampleSet s = sample_set(p, row);
     SampleRowWs& ws = ((SampleRowWs*)p.ws)[row];
@@ -327,11 +328,13 @@ __device__ __forceinline__ void sample_gather_body(const SampleArgs& p, uint64_t
         before = told[1];
         mass = (uint64_t)told[4] << 32 | told[3];
         const u32 through = told[2], low_through = told[5];
+        // (a list is sorted twice: from JL_SA_FEW on, or so, its cut and the parts' sums are faster; 200 of 131072 13.4 us against 10.5)
+        const u32 few = s.k && s.nucleus ? JL_SA_LIST : JL_SA_FEW;
         if (s.low > 0.f && low_bin < cut && !(s.k && s.nucleus)) {   // min_p ends first
-            mode = low_through <= JL_SA_LIST ? JL_SA_LISTED : JL_SA_LARGE;
+            mode = low_through <= few ? JL_SA_LISTED : JL_SA_LARGE;
             cut = mode == JL_SA_LISTED ? low_bin : (u32)JL_SA_BINS;
         } else if (cut < JL_SA_BINS) {
-            mode = through <= JL_SA_LIST ? JL_SA_LISTED : s.k && s.nucleus ? JL_SA_SLOW : through - before <= JL_SA_LIST ? JL_SA_LARGE : JL_SA_SLOW;
+            mode = through <= few ? JL_SA_LISTED : s.k && s.nucleus ? JL_SA_SLOW : through - before <= JL_SA_LIST ? JL_SA_LARGE : JL_SA_SLOW;
         }
         if (writes) ws.all = mass_all;
     }
@@ -348,18 +351,35 @@ __device__ __forceinline__ void sample_gather_body(const SampleArgs& p, uint64_t
     // by value: what goes into the list, from `list` on and below `sure`; what is kept for sure, from `sure` on (min_p's border in it)
     const bool cuts = cut < JL_SA_BINS;
     auto append = [&](float x, u32 i) {
-        const u32 at = atomicAdd(&ws.fill, 1u);
+        const u32 at = atomicAdd(&told[8], 1u);
         if (at < JL_SA_LIST) {
-            ws.key[at] = sample_key(x);
-            ws.idx[at] = i;
+            keys[at] = sample_key(x);
+            places[at] = i;
         }
     };
+    // the workgroup's list behind those of the others (a word's atomic add an element, from all workgroups, took half of the launch)
+    auto flush = [&]() {
+        __syncthreads();
+        const u32 n = min(told[8], (u32)JL_SA_LIST);
+        if (threadIdx.x == 0) told[9] = n ? atomicAdd(&ws.fill, n) : 0u;
+        __syncthreads();
+        for (u32 i = threadIdx.x; i < n; i += 512) {
+            const u32 at = told[9] + i;
+            if (at < JL_SA_LIST) {
+                ws.key[at] = keys[i];
+                ws.idx[at] = places[i];
+            }
+        }
+    };
+    if (threadIdx.x == 0) told[8] = 0;
+    __syncthreads();
     uint64_t sum = 0;
     float list = sample_edge([&](float x) { return s.r.bin(x) <= cut; });
     if (mode == JL_SA_LISTED) {
         sample_range<64>(p, row, from, end, lane, [&](float x, u32 i) {
             if (x >= list) append(x, i);
         });
+        flush();
         return;
     }
     const float below = cuts ? sample_edge([&](float x) { return s.r.bin(x) < cut; }) : list;
@@ -371,6 +391,7 @@ __device__ __forceinline__ void sample_gather_body(const SampleArgs& p, uint64_t
             else if (x < below) append(x, i);
         }
     });
+    if (cuts) flush();
     if (mode == JL_SA_LARGE) {
         sum = sample_scan64(sum);
         if (lane == 63) ws.part[part] = sum;
@@ -698,7 +719,10 @@ __device__ __forceinline__ void sample_list(const SampleArgs& p, SampleLds& s, c
             __syncthreads();
 #pragma unroll
             for (int q = 0; q < NQ; q++)
-                if (tid + T * q < kept && (double)through[q] >= reach) atomicMin(&s.at, tid + T * q + 1);
+            {
+                const uint64_t over = __ballot(tid + T * q < kept && (double)through[q] >= reach);
+                if (over && (tid & 63) == (u32)__builtin_ctzll(over)) atomicMin(&s.at, tid + T * q + 1);
+            }
             __syncthreads();
             kept = s.at;
         } else {
@@ -760,8 +784,9 @@ __device__ __forceinline__ void sample_list(const SampleArgs& p, SampleLds& s, c
         __syncthreads();
 #pragma unroll
         for (int q = 0; q < NQ; q++) {
-            if (mine[q] && (double)c[q] > over) atomicMin(&s.at, tid + T * q);
-            if (mine[q]) atomicMax(&s.hi, tid + T * q);
+            const uint64_t yes = __ballot(mine[q] && (double)c[q] > over), any = __ballot(mine[q] != 0);
+            if (yes && (tid & 63) == (u32)__builtin_ctzll(yes)) atomicMin(&s.at, tid + T * q);
+            if (any && (tid & 63) == 63u - (u32)__builtin_clzll(any)) atomicMax(&s.hi, tid + T * q);
         }
         __syncthreads();
         at = s.at != ~0u ? s.at : s.hi;
@@ -772,6 +797,105 @@ __device__ __forceinline__ void sample_list(const SampleArgs& p, SampleLds& s, c
 #pragma unroll
     for (int q = 0; q < NQ; q++)
         if (tid + T * q == at) give((u32)(by[q] >> 32), (double)mine[q] / (double)total);
+}
+
+// A LARGE row's cut among the list, without sorting it: its keys' range in 256, and the few elements of the one in which the cut falls in order, by one
+// wavefront.  What is kept goes into the parts' sums.  False: that one has more than 64 (ties).
+__device__ __forceinline__ bool sample_near(const SampleArgs& p, SampleLds& s, const SampleRowWs& ws, const SampleSet& set, u32 n, SampleCut& cut) {
+    const u32 tid = threadIdx.x;
+    const SampleRow& r = set.r;
+    if (tid == 0) {
+        s.lo = ~0u;
+        s.hi = 0;
+        s.at = ~0u;
+        s.fill = 0;
+    }
+    s.mass[tid] = 0;
+    s.count[tid] = 0;
+    u32 key[4], idx[4], lo = ~0u, hi = 0;
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        const u32 e = tid + JL_SA_THREADS * q;
+        key[q] = e < n ? ws.key[e] : 0u;
+        idx[q] = e < n ? ws.idx[e] : 0u;
+        lo = min(lo, key[q] - 1u);       // (0: none)
+        hi = max(hi, key[q]);
+    }
+    lo = ~sample_wave_max(~lo);
+    hi = sample_wave_max(hi);
+    __syncthreads();
+    if ((tid & 63) == 0) {
+        atomicMin(&s.lo, lo);
+        atomicMax(&s.hi, hi);
+    }
+    __syncthreads();
+    hi = s.hi;
+    const u32 range = hi - (s.lo + 1u);
+    const int shift = max(0, 32 - (int)__builtin_clz(range | 1u) - 8);
+    uint64_t w[4];
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        if (!key[q]) continue;
+        w[q] = r.whole(sample_value(key[q]));
+        const u32 b = (hi - key[q]) >> shift;
+        atomicAdd(&s.count[b], 1u);
+        atomicAdd((unsigned long long*)&s.mass[b], (unsigned long long)w[q]);
+    }
+    __syncthreads();
+    const u32 c = s.count[tid];
+    const uint64_t m = s.mass[tid];
+    uint64_t all;
+    const uint64_t ce = ws.before + sample_scan<JL_SA_WAVES>(s.scan, c, all), me = ws.mass + sample_scan<JL_SA_WAVES>(s.scan, m, all);
+    const double reach = (double)set.p * (double)ws.all;
+    const uint64_t cb = ce - c, mb = me - m;
+    const bool crossed = c && (set.k ? ce >= set.k && cb < set.k : (double)me >= reach && !(cb && (double)mb >= reach));
+    if (crossed) {
+        s.at = tid;
+        s.at_count = (u32)cb;
+        s.at_mass = mb;
+        s.at_n = c;
+    }
+    __syncthreads();
+    const u32 at = s.at, many = s.at_n, before = s.at_count;
+    const uint64_t mass = s.at_mass;
+    if (at == ~0u || many > 64) {
+        __syncthreads();
+        return false;
+    }
+#pragma unroll
+    for (int q = 0; q < 4; q++)
+        if (key[q] && (hi - key[q]) >> shift == at) {
+            const u32 to = atomicAdd(&s.fill, 1u);
+            s.key[to] = key[q];
+            s.idx[to] = idx[q];
+        }
+    __syncthreads();
+    if (tid < 64) {
+        uint64_t v[1] = {tid < many ? (uint64_t)~s.key[tid] << 32 | s.idx[tid] : ~0ull};
+        sample_sort<1, false>(s.mass, v, many);
+        const uint64_t mine = tid < many ? r.whole(sample_value(~(u32)(v[0] >> 32))) : 0, through = mass + sample_scan64(mine);
+        u32 last = many - 1;
+        if (set.k) last = min(last, set.k - before - 1);
+        else {
+            const uint64_t over = __ballot(tid < many && (double)through >= reach);
+            if (over) last = (u32)__builtin_ctzll(over);
+        }
+        if (tid == last) {
+            s.res_key = ~(u32)(v[0] >> 32);
+            s.res_idx = (u32)v[0];
+        }
+    }
+    __syncthreads();
+    cut.key = s.res_key;
+    cut.idx = s.res_idx;
+#pragma unroll
+    for (int q = 0; q < 4; q++)
+        if (key[q] && cut.keeps(key[q], idx[q]) && w[q] && (!(set.low > 0.f) || r.weight(sample_value(key[q])) >= (double)set.low)) {
+            const u32 slice = idx[q] / (u32)p.slice_len, part = slice * JL_SA_PARTS + (idx[q] - slice * (u32)p.slice_len) / (u32)p.part_len;
+            atomicAdd((unsigned long long*)&s.tile[part], (unsigned long long)w[q]);
+        }
+    __syncthreads();
+    return true;
 }
 
 // grid = rows, block = 256.
@@ -805,7 +929,7 @@ __device__ __forceinline__ void sample_take_body(const SampleArgs& p, SampleLds&
     if (mode == JL_SA_LARGE) {
         for (int i = tid; i < 512; i += JL_SA_THREADS) s.tile[i] = i < parts ? ws.part[i] : 0;
         __syncthreads();
-        if (bin < JL_SA_BINS) {
+        if (bin < JL_SA_BINS && !sample_near(p, s, ws, set, fill, cut)) {
             if (fill <= JL_SA_THREADS) sample_list<1, true>(p, s, ws, set, u, fill, cut, give);
             else sample_list<4, true>(p, s, ws, set, u, fill, cut, give);
         }
@@ -850,7 +974,8 @@ __device__ __forceinline__ void sample_take_body(const SampleArgs& p, SampleLds&
 #pragma unroll
     for (int j = 0; j < 2; j++) {
         const uint64_t t = j ? t1 : t0;
-        if (t) atomicMax(&s.hi, 2 * tid + j);
+        const uint64_t any = __ballot(t != 0);
+        if (any && (tid & 63) == 63u - (u32)__builtin_clzll(any)) atomicMax(&s.hi, 2 * tid + j);
         if (t && !had && (double)(c + t) > over) {
             s.at = 2 * tid + j;
             s.at_mass = c;

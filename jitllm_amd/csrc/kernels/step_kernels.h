@@ -53,8 +53,8 @@ extern "C" __global__ __launch_bounds__(512) void jl_sample_bins(SampleArgs p) {
 }
 extern "C" __global__ __launch_bounds__(512) void jl_sample_gather(SampleArgs p) {
     __shared__ uint64_t scan[8];
-    __shared__ u32 told[8];
-    sample_gather_body(p, scan, told);
+    __shared__ u32 told[10], keys[JL_SA_LIST], places[JL_SA_LIST];
+    sample_gather_body(p, scan, told, keys, places);
 }
 // grid = rows, block = 256
 extern "C" __global__ __launch_bounds__(256) void jl_sample_take(SampleArgs p) {
