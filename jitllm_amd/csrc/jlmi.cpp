@@ -37,6 +37,7 @@ struct Tuning {
     int xpre = 0;               // decode matvec: 1 / 2 / 4 float4 groups of x a thread loads ahead of its weights
     int q8pair = 0;             // Q8_0 rows: 2 keeps one block a lane-slot (2-byte-aligned loads)
     int packed_rw = 0, packed_block = 0, moe_group = 0, moe_logits = 0;
+    int attend_whole = 0;       // many tokens: 1 a unit a workgroup, 2 equal shares of the chunks
     int moe_select = 0, adapter_form = 0, adapter_slices = 0, adapter_sets = 0;
     int moe_shares = 0;
     int gemm_rows = 0;
@@ -122,9 +123,6 @@ struct Name {
     }
     operator const char*() const { return s; }
 };
-
-// Whether jl_attend_many_* of rows of `row` and `pieces` of q has a form of two column tiles a wavefront (q's pieces and the sums fit its registers).
-bool attend_two_tiles(int row, int pieces) { return pieces == 1 ? row < 256 : pieces == 2 && row == 64; }
 
 struct Resident {
     void* dev = nullptr;
@@ -2252,13 +2250,12 @@ int jl_ctx_create(jl_ctx** out, const jl_options* opts) {
         for (const char* any : {"", "_any"}) names.push_back(std::string("jl_norm_rows_") + form + any);
     for (const char* g : {"g1", "g2", "g3", "g4", "g3p", "g4p", "g6p", "g8p", "g12p", "g16p"}) names.push_back(std::string("jl_moe_select_") + g);
     for (const char* n : {"jl_kv_write", "jl_kv_read", "jl_sample_max", "jl_sample_bins", "jl_sample_gather", "jl_sample_take"}) names.push_back(n);
-    for (const char* d : {"64", "128", "256"}) names.push_back(std::string("jl_attend_join_d") + d);
+    for (const char* d : {"64", "128", "256"}) for (const char* wide : {"", "wide_"}) names.push_back(std::string("jl_attend_join_") + wide + "d" + d);
     for (const char* t : {"f16", "i8", "bf16"})
         for (const char* d : {"_d64", "_d128", "_d256"})
             for (const char* q : {"_q1", strcmp(t, "bf16") ? "_q2" : "_q3"}) {
                 for (const char* m : {"", "_m"}) names.push_back(std::string("jl_attend_one_") + t + d + q + m);
-                names.push_back(std::string("jl_attend_many_") + t + d + q + "_n1");
-                if (attend_two_tiles(atoi(d + 2), atoi(q + 2))) names.push_back(std::string("jl_attend_many_") + t + d + q + "_n2");
+                for (const char* w : {"_w4", "_w8"}) names.push_back(std::string("jl_attend_many_") + t + d + q + w);
             }
     names.push_back("jl_adapter_sum");
     names.push_back("jl_adapter_group");
@@ -2443,6 +2440,7 @@ int jl_set_tuning(jl_ctx* c, const char* key, int value) {
     else if (!strcmp(key, "matvec.grid")) c->tune.grid = value;
     else if (!strcmp(key, "packed.rw")) c->tune.packed_rw = value;
     else if (!strcmp(key, "packed.block")) c->tune.packed_block = value;
+    else if (!strcmp(key, "attend.whole")) c->tune.attend_whole = value;
     else if (!strcmp(key, "moe.select")) c->tune.moe_select = value;
     else if (!strcmp(key, "adapter.form")) c->tune.adapter_form = value;
     else if (!strcmp(key, "adapter.slices")) c->tune.adapter_slices = value;
@@ -3131,7 +3129,7 @@ int jl_reserve_attend(jl_ctx* c, int max_d) {
     if (max_d <= 0) return fail(c, JL_ERR_ARG, "reserve attend: rows of %d", max_d);
     if (max_d > 256) return JL_DECLINED;
     HIP_TRY(c, H->SetDevice(c->device));
-    return attend_ws_ensure(c, attend_part_bytes(attend_wgs(c, 128), std::min(max_d, 128), 128));   // (rows above 128: half the workgroups, half the columns)
+    return attend_ws_ensure(c, attend_part_bytes(attend_wgs(c, 128), std::min(max_d, 128), 128));   // (rows above 128: half the workgroups)
 }
 
 int jl_attend_dev(jl_ctx* c, const jl_kv_cache* cache, const jl_attend* g, void* stream) {
@@ -3162,8 +3160,8 @@ int jl_attend_dev(jl_ctx* c, const jl_kv_cache* cache, const jl_attend* g, void*
     const bool bf = cache->type == JL_TYPE_BF16;
     // q in one piece where the cache's type holds it; over bf16 three pieces of the weights go with three of q, for a result of 32 bits
     const int pieces = bf ? (g->q_type == JL_TYPE_BF16 && g->out_type != JL_TYPE_F32 ? 1 : 3) : g->q_type == JL_TYPE_F32 ? 2 : 1;
-    const int nt = one ? 0 : attend_two_tiles(row, pieces) && (long)a.group * most > 64 ? 2 : 1;
-    a.part_cols = one ? 16 : 64 * nt;
+    const int waves = one || (long)a.group * most <= 64 ? 4 : 8;
+    a.part_cols = one ? 16 : 16 * waves;
     a.per = std::clamp(a.part_cols / a.group, 1, most);
     a.units = (g->ntok + a.per - 1) / a.per;
     a.blocks = a.per > 1 ? 1 : (a.group + a.part_cols - 1) / a.part_cols;
@@ -3171,22 +3169,23 @@ int jl_attend_dev(jl_ctx* c, const jl_kv_cache* cache, const jl_attend* g, void*
     // No more workgroups than there can be chunks of 128 positions.
     const unsigned long long per_head = ((unsigned long long)cache->table_pages * cache->page_size + 127) / 128 + 1, planes = (unsigned long long)cache->n_kv * a.blocks;
     a.wgs = (int)std::min<unsigned long long>(attend_wgs(c, cache->d), g->ntok * planes * per_head);
-    a.whole = !one && a.units * planes >= (unsigned)a.wgs;
-    if (a.units * planes > 0xffffffffull / 256) return JL_DECLINED;   // threads a launch can have
+    a.whole = !one && (c->tune.attend_whole ? c->tune.attend_whole == 1 : a.units * planes >= (unsigned)a.wgs);
+    if (a.units * planes > 0xffffffffull / 512) return JL_DECLINED;   // threads a launch can have
     HIP_TRY(c, H->SetDevice(c->device));
     rc = a.whole ? JL_OK : attend_ws_ensure(c, attend_part_bytes(a.wgs, cache->d, a.part_cols));
     if (rc != JL_OK) return rc;
     a.part = (float*)c->attend_ws;
     Name name, join;
     name << "jl_attend_" << (one ? "one_" : "many_") << (bf ? "bf16" : cache->type == JL_TYPE_F16 ? "f16" : "i8") << "_d" << row << "_q" << pieces;
-    if (!one) name << "_n" << nt;
+    if (!one) name << "_w" << waves;
     else if (a.per > 1) name << "_m";
-    join << "jl_attend_join_d" << row;
+    join << "jl_attend_join_" << (one ? "d" : "wide_d") << row;
     void* params[] = {&a};
     const hipStream_t st = pick_stream(c, stream);
-    rc = launch(c, name, a.whole ? (unsigned)(a.units * planes) : (unsigned)a.wgs, 1, 256, 0, st, params);
+    rc = launch(c, name, a.whole ? (unsigned)(a.units * planes) : (unsigned)a.wgs, 1, 64u * waves, 0, st, params);
     if (rc != JL_OK || a.whole) return rc;
-    return launch(c, join, (unsigned)a.wgs, (unsigned)std::min(4, (std::min(a.part_cols, a.group * a.per) + 3) / 4), 256, 0, st, params);
+    const int cols = std::min(a.part_cols, a.group * a.per);
+    return launch(c, join, (unsigned)a.wgs, (unsigned)(one ? std::min(4, (cols + 3) / 4) : (cols + 15) / 16), 256, 0, st, params);
 }
 
 namespace {

@@ -47,9 +47,10 @@ template <bool BF> __device__ __forceinline__ f32x4 at_mfma(u32x4 a, u32x4 b, f3
 template <bool BF> __device__ __forceinline__ u32 at_piece(float& x, float& y) {
     if constexpr (BF) {
         const at_bf16x2 h = {(__bf16)x, (__bf16)y};
-        x -= (float)h.x;
-        y -= (float)h.y;
-        return __builtin_bit_cast(u32, h);
+        const u32 b = __builtin_bit_cast(u32, h);
+        x -= __uint_as_float(b << 16);
+        y -= __uint_as_float(b & 0xffff0000u);
+        return b;
     } else {
         const f16x2 h = {(_Float16)x, (_Float16)y};
         x -= (float)h.x;
@@ -180,8 +181,8 @@ __device__ __forceinline__ AtShare at_share(uint64_t all, u32 wgs) {
 // Workgroups that follow each other share an L2 (eight of them, blockIdx modulo 8): neighbours' units often read the same rows.
 __device__ __forceinline__ u32 at_group_of(u32 b, u32 wgs) { return (wgs & 7) == 0 ? (b & 7) * (wgs >> 3) + (b >> 3) : b; }
 
-// Sums over the workgroup's 256 threads: those before this one, and all.  LDS: 4 words of 8 bytes.
-__device__ __forceinline__ uint64_t at_before(uint64_t mine, uint64_t* lds, uint64_t& total) {
+// Sums over the workgroup's WAVES wavefronts: before this thread, and all.  LDS: WAVES words of 8 bytes.
+template <int WAVES> __device__ __forceinline__ uint64_t at_before(uint64_t mine, uint64_t* lds, uint64_t& total) {
     const u32 tid = threadIdx.x;
     uint64_t s = mine;
 #pragma unroll
@@ -194,28 +195,28 @@ __device__ __forceinline__ uint64_t at_before(uint64_t mine, uint64_t* lds, uint
     uint64_t before = s - mine;
     total = 0;
 #pragma unroll
-    for (u32 w = 0; w < 4; w++) {
+    for (u32 w = 0; w < WAVES; w++) {
         before += w < tid >> 6 ? lds[w] : 0;
         total += lds[w];
     }
     return before;
 }
 
-// A workgroup's share: chunks first to end of all, and where the first lies.  LDS: 8 words of 8 bytes.  False: none (the whole workgroup alike).
+// A workgroup's share: chunks first to end of all, and where the first lies.  LDS: WAVES + 1 words of 8 bytes.  False: none (the whole workgroup alike).
 struct AtWork {
     uint64_t first, end;
     AtShare share;
     u32 plane, off;      // off: chunks of the span that are before it
     AtSpan span;
 };
-template <bool MANY> __device__ __forceinline__ bool at_work(const AttendArgs& p, u32 w, uint64_t* lds, AtWork& k) {
-    u32* const told = (u32*)(lds + 4);
+template <bool MANY, int WAVES> __device__ __forceinline__ bool at_work(const AttendArgs& p, u32 w, uint64_t* lds, AtWork& k) {
+    u32* const told = (u32*)(lds + WAVES);
     const u32 q = ((u32)p.units + 255) / 256, mine0 = threadIdx.x * q;
     uint64_t mine = 0, total;
     u32 from, off;
     for (u32 i = 0; i < q; i++)
         if (mine0 + i < (u32)p.units) mine += at_unit_chunks<MANY>(p, mine0 + i, ~0u, from, off);
-    const uint64_t before = at_before(mine, lds, total);
+    const uint64_t before = at_before<WAVES>(mine, lds, total);
     const u32 planes = (u32)p.c.n_kv * (u32)p.blocks;
     k.share = at_share(total * planes, (u32)p.wgs);
     if (w >= k.share.n) return false;
@@ -367,4 +368,34 @@ template <int DP> __device__ __forceinline__ void attend_join_body(const AttendA
         for (int i = 0; i < C; i++) out[i] *= inv;
         if (d0 < (u32)p.c.d) at_store<C>(p, tok, head, d0, out);
     }
+}
+
+// The same where a span has many columns: a wavefront four of them, over all parts.  grid = (wgs, columns / 16), block = 256.
+template <int DP> __device__ __forceinline__ void attend_join_wide_body(const AttendArgs& p) {
+    constexpr int C = DP / 16;
+    const u32 w = blockIdx.x;
+    const AtJoin j = at_join_of<DP>(p)[w];
+    if (j.last == 0) return;
+    const u32 lane = threadIdx.x & 63, x = lane & 15, d0 = C * x, col = blockIdx.y * 16 + (threadIdx.x >> 6) * 4 + (lane >> 4);
+    u32 tok, head;
+    if (!at_column(p, j.t0, j.t1, j.plane, col, tok, head)) return;
+    auto slot = [&](u32 k) { return k == w ? j.slot : 2 * k; };
+    float mm = -__builtin_inff(), l = 0.f, out[C];
+    f32x4 y[C / 4];
+#pragma unroll 4
+    for (u32 k = w; k < j.last; k++) mm = fmaxf(mm, (*at_part_ml<DP>(p, slot(k), col)).x);
+#pragma unroll
+    for (int i = 0; i < C / 4; i++) y[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (u32 k = w; k < j.last; k++) {
+        const f32x2 ml = *at_part_ml<DP>(p, slot(k), col);
+        const float turn = ml.x == mm ? 1.f : __builtin_amdgcn_exp2f(ml.x - mm);
+        l += ml.y * turn;
+#pragma unroll
+        for (int i = 0; i < C / 4; i++) y[i] += *(const f32x4*)(at_part<DP>(p, slot(k), col) + d0 + 4 * i) * turn;
+    }
+    const float inv = at_finish(p, tok, head, mm, l, p.c.type == JL_BF16 ? 0.f : JL_AT_OFF, d0 == 0);
+#pragma unroll
+    for (int i = 0; i < C; i++) out[i] = y[i / 4][i % 4] * inv;
+    if (d0 < (u32)p.c.d) at_store<C>(p, tok, head, d0, out);
 }

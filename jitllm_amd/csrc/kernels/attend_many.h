@@ -1,21 +1,20 @@
 // Many new tokens over a cache -- prompts, long drafts: more than sixteen columns a unit (attend.h).
 //
-// Each of a workgroup's four wavefronts has NT tiles of sixteen columns; the rows of 64 positions at a time go through LDS, as the fragments the matrix instruction
-// takes (a fragment a kilobyte, a lane's sixteen bytes behind the next lane's: no bank is met twice), so rows are read once for 64 NT columns, and 8-bit values
-// turned into f16 once.  Two wavefronts bring the values, two the keys, of the next 64 positions while all four multiply: one barrier a step.  A wavefront keeps its
-// columns' sums to the end, so nothing is exchanged.  What bounds it is the vector unit: about 120 instructions a tile of columns and 32 positions around the
-// exponentials, beside 24 matrix instructions (16 cycles each) with q in one piece.
+// Each of a workgroup's four or eight wavefronts has a tile of sixteen columns; the rows of 64 positions at a time go through LDS, as the fragments the matrix
+// instruction takes (a fragment a kilobyte, a lane's sixteen bytes behind the next lane's: no bank is met twice), so rows are read once for 64 or 128 columns, and 8-bit
+// values turned into f16 once.  Half of the wavefronts bring the values, half the keys, of the next 64 positions while all of them multiply: one barrier a step.  A
+// wavefront keeps its columns' sums to the end, so nothing is exchanged.
 #pragma once
 #include "attend.h"
 
 template <int DP> constexpr int at_stage_words() { return (4 * (DP / 32) + 2 * (DP / 16)) * 256; }   // 64 positions' fragments
 
 // lds: words [2][at_stage_words], then [2] of scales: keys' [64], values' [64]; then [2] of marks [4], and one mark of the span.
-template <int TYPE, int DP, int QP, int PP, int NT>
+template <int TYPE, int DP, int QP, int PP, int WAVES>
 __device__ __forceinline__ void attend_many_body(const AttendArgs& p, u32x4* lds, uint64_t* find) {
     constexpr bool BF = TYPE == JL_BF16, I8 = TYPE == JL_I8;
-    constexpr int C = DP / 16, KC = DP / 32, B = I8 ? 1 : 2, VB = C * B;
-    constexpr int KL = I8 ? KC / 2 : KC, VW = (VB + 3) / 4;
+    constexpr int C = DP / 16, KC = DP / 32, B = I8 ? 1 : 2, VB = C * B;   // elements of the values a lane, fragments of a key, bytes
+    constexpr int KL = I8 ? KC / 2 : KC, VW = (C * B * 4 / WAVES + 3) / 4;   // loads of a tile of keys; words of values a position and lane
     constexpr int STAGE = at_stage_words<DP>() / 4;       // in 16-byte pieces
     constexpr float OFF = BF ? 0.f : JL_AT_OFF;
     const float inf = __builtin_inff();
@@ -37,7 +36,7 @@ __device__ __forceinline__ void attend_many_body(const AttendArgs& p, u32x4* lds
         job.span = at_span<true>(p, unit * (u32)p.per);
     } else {
         w = at_group_of(blockIdx.x, (u32)p.wgs);
-        if (!at_work<true>(p, w, find, job)) {
+        if (!at_work<true, WAVES>(p, w, find, job)) {
             if (threadIdx.x == 0) at_join_of<DP>(p)[w] = join;
             return;
         }
@@ -45,8 +44,12 @@ __device__ __forceinline__ void attend_many_body(const AttendArgs& p, u32x4* lds
     const u32 row_bytes = (u32)p.c.row_stride * B;
     const size_t head_bytes = p.c.head_stride * B, page_bytes = p.c.page_stride * B;
     const u32 in_page = (1u << p.c.shift) - 1;
-    const int half = wave & 1;
-    const bool brings_keys = wave >= 2;
+    // What a wavefront brings of 64 positions: of four, two bring the values of 32 positions each and two the keys; of eight, four bring the values of 32 positions and
+    // half of the elements, four the keys of 16.
+    constexpr int VS = WAVES / 4, TILES = 2 / VS, CV = C / VS;      // shares of the values' elements; tiles of keys; elements a lane
+    const bool brings_keys = wave >= WAVES / 2;
+    const int half = brings_keys ? (wave - WAVES / 2) * TILES / 2 : wave & 1, share = wave >> 1;      // (share: of the values)
+    const int tile0 = brings_keys ? (wave - WAVES / 2) * TILES % 2 : 0;
     // a lane's bytes of a tile's rows, for what its wavefront brings
     u32 ko[KL];
 #pragma unroll
@@ -54,7 +57,7 @@ __device__ __forceinline__ void attend_many_body(const AttendArgs& p, u32x4* lds
         const int d = I8 ? 64 * c + 16 * g : 32 * c + 8 * g;
         ko[c] = d < p.c.d ? n * row_bytes + (u32)d * B : JL_AT_NOWHERE;
     }
-    const u32 vo = C * n < p.c.d ? 4 * g * row_bytes + (u32)n * VB : JL_AT_NOWHERE;
+    const u32 vo = C * n < p.c.d ? 4 * g * row_bytes + (u32)n * VB + (u32)(share & (VS - 1)) * CV * B : JL_AT_NOWHERE;
 
     for (uint64_t at = job.first; at < job.end;) {
         const AtSpan span = job.span;
@@ -76,44 +79,52 @@ __device__ __forceinline__ void attend_many_body(const AttendArgs& p, u32x4* lds
             const u32 at0 = (s + (lane >> 1)) * 64 + half * 32 + 16 * (lane & 1);
             pg = s + (lane >> 1) < s1 && at0 < hi && at0 + 16 > lo ? pages[at0 >> p.c.shift] : ~0u;
         };
-        u32 st[8 * (VW > KL ? VW : KL)];
+        u32 st[8 * VW > 4 * TILES * KL ? 8 * VW : 4 * TILES * KL];
         float sc = 0.f;
-        static_assert(2 * KL * 4 <= 8 * (VW > KL ? VW : KL), "the keys' registers");
         auto ask = [&](u32 s) {
             if (((s - s0) & 31) == 0) look(s);
             const u32 p0 = s * 64 + half * 32;
+            at_rsrc rs[2];
+            size_t sa[2];
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 page[i] = (u32)__builtin_amdgcn_readlane((i32)pg, (int)(2 * ((s - s0) & 31) + i));
                 const u32 slot = (p0 + 16 * i) & in_page, held = page[i] < p.c.n_page ? page[i] : 0u;
-                const at_rsrc rs = at_buffer(from + held * page_bytes + (size_t)slot * row_bytes);
-                if (brings_keys) {
+                rs[i] = at_buffer(from + held * page_bytes + (size_t)slot * row_bytes);
+                sa[i] = ((((size_t)held * p.c.n_kv + kv) << p.c.shift) + slot) + n;
+            }
+            if (brings_keys) {
+#pragma unroll
+                for (int i = 0; i < TILES; i++) {
+                    const at_rsrc r = TILES == 1 && tile0 ? rs[1] : rs[i];
 #pragma unroll
                     for (int c = 0; c < KL; c++) {
-                        const u32x4 y = __builtin_amdgcn_raw_buffer_load_b128(rs, ko[c], 0, 0);
+                        const u32x4 y = __builtin_amdgcn_raw_buffer_load_b128(r, ko[c], 0, 0);
 #pragma unroll
                         for (int e = 0; e < 4; e++) st[(i * KL + c) * 4 + e] = y[e];
                     }
-                } else {
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 2; i++)
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
-                        if constexpr (VW == 1) st[4 * i + r] = __builtin_amdgcn_raw_buffer_load_b32(rs, vo, r * row_bytes, 0);
+                        if constexpr (VW == 1 && CV * B == 2) st[4 * i + r] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(rs[i], vo, r * row_bytes, 0);
+                        else if constexpr (VW == 1) st[4 * i + r] = __builtin_amdgcn_raw_buffer_load_b32(rs[i], vo, r * row_bytes, 0);
                         else if constexpr (VW == 2) {
-                            const u32x2 y = __builtin_amdgcn_raw_buffer_load_b64(rs, vo, r * row_bytes, 0);
+                            const u32x2 y = __builtin_amdgcn_raw_buffer_load_b64(rs[i], vo, r * row_bytes, 0);
                             st[(4 * i + r) * 2] = y.x; st[(4 * i + r) * 2 + 1] = y.y;
                         } else {
 #pragma unroll
                             for (int e = 0; e < VW; e += 4) {
-                                const u32x4 y = __builtin_amdgcn_raw_buffer_load_b128(rs, vo + 4 * e, r * row_bytes, 0);
+                                const u32x4 y = __builtin_amdgcn_raw_buffer_load_b128(rs[i], vo + 4 * e, r * row_bytes, 0);
 #pragma unroll
                                 for (int f = 0; f < 4; f++) st[(4 * i + r) * VW + e + f] = y[f];
                             }
                         }
                     }
-                }
-                if constexpr (I8)
-                    if ((lane >> 4) == i) sc = from_scales[((((size_t)held * p.c.n_kv + kv) << p.c.shift) + slot) + n];
             }
+            if constexpr (I8) sc = from_scales[(lane >> 4) & 1 ? sa[1] : sa[0]];
         };
         auto put = [&](u32 s) {
             u32x4* const to = lds + (s & 1) * STAGE;
@@ -121,7 +132,7 @@ __device__ __forceinline__ void attend_many_body(const AttendArgs& p, u32x4* lds
             const bool none = max(page[0], page[1]) >= p.c.n_page;
             if (brings_keys) {
 #pragma unroll
-                for (int i = 0; i < 2; i++)
+                for (int i = 0; i < TILES; i++)
 #pragma unroll
                     for (int c = 0; c < KC; c++) {
                         u32x4 y;
@@ -134,11 +145,11 @@ __device__ __forceinline__ void attend_many_body(const AttendArgs& p, u32x4* lds
                         } else {
                             y = u32x4{st[(i * KL + c) * 4], st[(i * KL + c) * 4 + 1], st[(i * KL + c) * 4 + 2], st[(i * KL + c) * 4 + 3]};
                         }
-                        to[((2 * half + i) * KC + c) * 64 + lane] = y;
+                        to[((2 * half + tile0 + i) * KC + c) * 64 + lane] = y;
                     }
-                if (lane == 0) marks[(s & 1) * 4 + half] = (page[0] >= p.c.n_page ? 1u : 0u) | (page[1] >= p.c.n_page ? 2u : 0u);
+                if (lane == 0 && tile0 == 0) marks[(s & 1) * 4 + half] = (page[0] >= p.c.n_page ? 1u : 0u) | (page[1] >= p.c.n_page ? 2u : 0u);
                 if constexpr (I8)
-                    if (lane < 32) scales[(s & 1) * 128 + half * 32 + lane] = sc;
+                    if (lane < 32 && tile0 == 0) scales[(s & 1) * 128 + half * 32 + lane] = sc;
             } else {
                 if (none || p0 < zlo || p0 + 32 > zhi) {   // zeros for what no token sees: what lies there may be no number
 #pragma unroll
@@ -158,7 +169,7 @@ __device__ __forceinline__ void attend_many_body(const AttendArgs& p, u32x4* lds
                     if (max(big.x, big.y) >= (BF ? 0x7f80 : 0x7c00)) marks[8] = 1;
                 }
 #pragma unroll
-                for (int j = 0; j < C; j++) {
+                for (int j = 0; j < CV; j++) {
                     u32x4 vt;
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
@@ -170,31 +181,36 @@ __device__ __forceinline__ void attend_many_body(const AttendArgs& p, u32x4* lds
                             vt[r] = __builtin_amdgcn_perm(st[(2 * r + 1) * VW + j / 2], st[2 * r * VW + j / 2], j % 2 ? 0x07060302u : 0x05040100u);
                         }
                     }
-                    to[(4 * KC + half * C + j) * 64 + lane] = vt;
+                    to[(4 * KC + half * C + share * CV + j) * 64 + lane] = vt;
                 }
                 if constexpr (I8)
-                    if (lane < 32) scales[(s & 1) * 128 + 64 + half * 32 + lane] = sc;
+                    if (lane < 32 && share == 0) scales[(s & 1) * 128 + 64 + half * 32 + lane] = sc;
             }
         };
-        // the columns
-        u32 tok[NT], head[NT], clo[NT], chi[NT], wlo = ~0u, whi = 0;
-        bool live[NT];
-        u32x4 qf[NT][QP][KC];
-        float qs[NT];
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-            live[nt] = at_column(p, span.t0, span.t1, plane, (u32)(wave * NT + nt) * 16 + n, tok[nt], head[nt]);
+        // the column
+        u32 tok, head, clo, chi;
+        const bool live = at_column(p, span.t0, span.t1, plane, (u32)wave * 16 + n, tok, head);
+        {
             u32 q0;
-            at_sees(p, tok[nt], q0, clo[nt], chi[nt]);
-            if (!live[nt]) clo[nt] = chi[nt] = 0;
-            wlo = min(wlo, live[nt] ? clo[nt] : ~0u);
-            whi = max(whi, chi[nt]);
+            at_sees(p, tok, q0, clo, chi);
+        }
+        if (!live) clo = chi = 0;
+        u32 wlo = live ? clo : ~0u, whi = chi, wlo_all = clo, whi_all = live ? chi : ~0u;      // of the wavefront's columns
+#pragma unroll
+        for (int d = 1; d < 16; d *= 2) {
+            wlo = min(wlo, (u32)__shfl_xor((int)wlo, d, 64)); whi = max(whi, (u32)__shfl_xor((int)whi, d, 64));
+            wlo_all = max(wlo_all, (u32)__shfl_xor((int)wlo_all, d, 64)); whi_all = min(whi_all, (u32)__shfl_xor((int)whi_all, d, 64));
+        }
+        wlo = at_uni(wlo); whi = at_uni(whi); wlo_all = at_uni(wlo_all); whi_all = at_uni(whi_all);
+        u32x4 qf[QP][KC];
+        float qs;
+        {
             float x[KC][8], most = 0.f;
 #pragma unroll
             for (int c = 0; c < KC; c++) {
                 const int d = I8 ? 64 * (c / 2) + 16 * g + 8 * (c % 2) : 32 * c + 8 * g;
                 f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
-                if (live[nt] && d < p.c.d) kv_load8(p.q, tok[nt] * p.q_stride + (size_t)head[nt] * p.c.d + d, p.q_type, true, a, b);
+                if (live && d < p.c.d) kv_load8(p.q, tok * p.q_stride + (size_t)head * p.c.d + d, p.q_type, true, a, b);
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     x[c][j] = a[j];
@@ -207,8 +223,8 @@ __device__ __forceinline__ void attend_many_body(const AttendArgs& p, u32x4* lds
                 most = at_max4(most);
                 e = most > 0.f && most < inf ? 15 - __builtin_amdgcn_frexp_expf(most) : 0;
             }
-            qs[nt] = __builtin_amdgcn_ldexpf(fabsf(p.scale), -e);   // (a negative scale's sign goes to q: the largest score is the largest product)
-            qs[nt] = p.cap == 0.f ? qs[nt] * JL_AT_LOG2E : qs[nt] / p.cap;
+            qs = __builtin_amdgcn_ldexpf(fabsf(p.scale), -e);   // (a negative scale's sign goes to q: the largest score is the largest product)
+            qs = p.cap == 0.f ? qs * JL_AT_LOG2E : qs / p.cap;
             const u32 sign = __float_as_uint(p.scale) & 0x80000000u;
 #pragma unroll
             for (int c = 0; c < KC; c++) {
@@ -217,33 +233,16 @@ __device__ __forceinline__ void attend_many_body(const AttendArgs& p, u32x4* lds
 #pragma unroll
                 for (int k = 0; k < QP; k++)
 #pragma unroll
-                    for (int j = 0; j < 4; j++) qf[nt][k][c][j] = at_piece<BF>(x[c][2 * j], x[c][2 * j + 1]);
+                    for (int j = 0; j < 4; j++) qf[k][c][j] = at_piece<BF>(x[c][2 * j], x[c][2 * j + 1]);
             }
         }
-        u32 wlo_all = 0, whi_all = ~0u;
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-            wlo_all = max(wlo_all, live[nt] ? clo[nt] : 0u);
-            whi_all = min(whi_all, live[nt] ? chi[nt] : ~0u);
-        }
-#pragma unroll
-        for (int d = 1; d < 16; d *= 2) {
-            wlo = min(wlo, (u32)__shfl_xor((int)wlo, d, 64)); whi = max(whi, (u32)__shfl_xor((int)whi, d, 64));
-            wlo_all = max(wlo_all, (u32)__shfl_xor((int)wlo_all, d, 64)); whi_all = min(whi_all, (u32)__shfl_xor((int)whi_all, d, 64));
-        }
-        wlo = at_uni(wlo); whi = at_uni(whi); wlo_all = at_uni(wlo_all); whi_all = at_uni(whi_all);
 
         for (;;) {
-        f32x4 acc[NT][C];
-        float m[NT], l[NT];
+        f32x4 acc[C];
+        float m = -inf, l = 0.f;
         int ve = -200;          // 8-bit rows: acc is times 2^-ve
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-            m[nt] = -inf;
-            l[nt] = 0.f;
-#pragma unroll
-            for (int j = 0; j < C; j++) acc[nt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-        }
+        for (int j = 0; j < C; j++) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
         if (s0 < s1) ask(s0);
         __syncthreads();        // (the pass before has read its last stage)
@@ -261,19 +260,17 @@ __device__ __forceinline__ void attend_many_body(const AttendArgs& p, u32x4* lds
                 if (p0 >= whi || p0 + 32 <= wlo) continue;
                 const u32 none = at_uni(mark[h]);
                 const bool edge = p0 < wlo_all || p0 + 32 > whi_all || none;
-                f32x4 sco[NT][2];
+                const u32x4* const kin = in + 2 * h * KC * 64 + lane;
+                const u32x4* const vin = in + (4 * KC + h * C) * 64 + lane;
+                // (fragments two ahead of the products that take them)
+                f32x4 sco[2];
+                u32x4 kt[3] = {kin[0], kin[64], {0, 0, 0, 0}};
 #pragma unroll
-                for (int i = 0; i < 2; i++) {
+                for (int c = 0; c < 2 * KC; c++) {      // tile c % 2
+                    if (c + 2 < 2 * KC) kt[(c + 2) % 3] = kin[((c + 2) % 2 * KC + (c + 2) / 2) * 64];
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++) sco[nt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int c = 0; c < KC; c++) {
-                        const u32x4 y = in[((2 * h + i) * KC + c) * 64 + lane];
-#pragma unroll
-                        for (int q = 0; q < QP; q++)
-#pragma unroll
-                            for (int nt = 0; nt < NT; nt++) sco[nt][i] = at_mfma<BF>(y, qf[nt][q][c], sco[nt][i]);
-                    }
+                    for (int q = 0; q < QP; q++)
+                        sco[c % 2] = at_mfma<BF>(kt[c % 3], qf[q][c / 2], c / 2 || q ? sco[c % 2] : f32x4{0.f, 0.f, 0.f, 0.f});
                 }
                 f32x4 ks[2], vs[2];
                 if constexpr (I8) {
@@ -287,69 +284,64 @@ __device__ __forceinline__ void attend_many_body(const AttendArgs& p, u32x4* lds
                     const int to = __builtin_amdgcn_readfirstlane(big > 0.f ? __builtin_amdgcn_frexp_expf(big) : -200);
                     if (to > ve) {
 #pragma unroll
-                        for (int nt = 0; nt < NT; nt++)
+                        for (int j = 0; j < C; j++)
 #pragma unroll
-                            for (int j = 0; j < C; j++)
-#pragma unroll
-                                for (int r = 0; r < 4; r++) acc[nt][j][r] = __builtin_amdgcn_ldexpf(acc[nt][j][r], ve - to);
+                            for (int r = 0; r < 4; r++) acc[j][r] = __builtin_amdgcn_ldexpf(acc[j][r], ve - to);
                         ve = to;
                     }
                 }
-                u32x4 pf[NT][PP];
+                u32x4 vt[3] = {vin[0], vin[64], {0, 0, 0, 0}}, pf[PP];
+                float y[8], by = qs;       // scores are y by
+                u32 hidden = 0;
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    float y[8], by = qs[nt];       // scores are y by
-                    u32 hidden = 0;
+                for (int j = 0; j < 8; j++) {
+                    y[j] = sco[j / 4][j % 4];
+                    if constexpr (I8) y[j] *= ks[j / 4][j % 4];
+                }
+                if (edge || p.cap != 0.f) {
+                    by = 1.f;
 #pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        y[j] = sco[nt][j / 4][j % 4];
-                        if constexpr (I8) y[j] *= ks[j / 4][j % 4];
-                    }
-                    if (edge || p.cap != 0.f) {
-                        by = 1.f;
-#pragma unroll
-                        for (int j = 0; j < 8; j++) y[j] *= qs[nt];
-                        if (p.cap != 0.f) {
-#pragma unroll
-                            for (int j = 0; j < 8; j++) y[j] = p.cap * JL_AT_LOG2E * at_tanh(y[j]);
-                        }
+                    for (int j = 0; j < 8; j++) y[j] *= qs;
+                    if (p.cap != 0.f) {
 #pragma unroll
                         for (int j = 0; j < 8; j++) {
-                            const u32 at0 = p0 + 16 * (j / 4) + 4 * g + j % 4;
-                            const bool sees = !(none >> (j / 4) & 1) && at0 >= clo[nt] && at0 < chi[nt];
-                            y[j] = sees ? y[j] : -inf;
-                            if (I8 && !sees) hidden |= 1u << j;
+                            y[j] = p.cap * JL_AT_LOG2E * at_tanh(y[j]);
+                            asm volatile("" : "+v"(y[j]));     // (one after the other: side by side they take the loop's registers)
                         }
                     }
-                    float top = fmaxf(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])), fmaxf(fmaxf(y[4], y[5]), fmaxf(y[6], y[7])));
-                    top = fmaxf(at_max4(top) * by, m[nt]);
-                    if (__ballot(top > m[nt] + JL_AT_SLACK(BF))) {
-                        const float turn = m[nt] == top ? 1.f : __builtin_amdgcn_exp2f(m[nt] - top);   // (from -inf: 0)
-                        l[nt] *= turn;
-#pragma unroll
-                        for (int j = 0; j < C; j++) acc[nt][j] *= turn;
-                        m[nt] = top;
-                    }
-                    const float from = OFF - (m[nt] > -inf ? m[nt] : 0.f);
 #pragma unroll
                     for (int j = 0; j < 8; j++) {
-                        y[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(y[j], by, from));
-                        l[nt] += y[j];
-                        if constexpr (I8) y[j] = hidden >> j & 1 ? 0.f : y[j] * __builtin_amdgcn_ldexpf(vs[j / 4][j % 4], -ve);   // (a scale others see may be no number)
+                        const u32 at0 = p0 + 16 * (j / 4) + 4 * g + j % 4;
+                        const bool sees = !(none >> (j / 4) & 1) && at0 >= clo && at0 < chi;
+                        y[j] = sees ? y[j] : -inf;
+                        if (I8 && !sees) hidden |= 1u << j;
                     }
-#pragma unroll
-                    for (int q = 0; q < PP; q++)
-#pragma unroll
-                        for (int j = 0; j < 4; j++) pf[nt][q][j] = at_piece<BF>(y[2 * j], y[2 * j + 1]);
                 }
-                const u32x4* const vin = in + (4 * KC + h * C) * 64 + lane;
+                float top = fmaxf(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])), fmaxf(fmaxf(y[4], y[5]), fmaxf(y[6], y[7])));
+                top = fmaxf(at_max4(top) * by, m);
+                if (__ballot(top > m + JL_AT_SLACK(BF))) {
+                    const float turn = m == top ? 1.f : __builtin_amdgcn_exp2f(m - top);   // (from -inf: 0)
+                    l *= turn;
+#pragma unroll
+                    for (int j = 0; j < C; j++) acc[j] *= turn;
+                    m = top;
+                }
+                const float from = OFF - (m > -inf ? m : 0.f);
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    y[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(y[j], by, from));
+                    l += y[j];
+                    if constexpr (I8) y[j] = hidden >> j & 1 ? 0.f : y[j] * __builtin_amdgcn_ldexpf(vs[j / 4][j % 4], -ve);   // (a scale others see may be no number)
+                }
+#pragma unroll
+                for (int q = 0; q < PP; q++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) pf[q][j] = at_piece<BF>(y[2 * j], y[2 * j + 1]);
 #pragma unroll
                 for (int j = 0; j < C; j++) {
-                    const u32x4 vt = vin[j * 64];
+                    if (j + 2 < C) vt[(j + 2) % 3] = vin[(j + 2) * 64];
 #pragma unroll
-                    for (int q = 0; q < PP; q++)
-#pragma unroll
-                        for (int nt = 0; nt < NT; nt++) acc[nt][j] = at_mfma<BF>(vt, pf[nt][q], acc[nt][j]);
+                    for (int q = 0; q < PP; q++) acc[j] = at_mfma<BF>(vt[j % 3], pf[q], acc[j]);
                 }
             }
             if (s + 1 < s1) put(s + 1);
@@ -366,22 +358,20 @@ __device__ __forceinline__ void attend_many_body(const AttendArgs& p, u32x4* lds
         const u32 slot = 2 * w + (at == job.first ? 0u : 1u);
         const bool whole = left == n_chunks;
         if (c0 == 0 && !whole) join = AtJoin{span.t0, span.t1, plane, job.share.holder(at + n_chunks - 1) + 1, slot, {0, 0, 0}};
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-            const float sum = at_sum4(l[nt]);
+        const float sum = at_sum4(l);
+        if (live && (only == ~0u || tok == only)) {
             float by = I8 ? __builtin_amdgcn_ldexpf(1.f, ve) : 1.f;
-            if (!live[nt] || (only != ~0u && tok[nt] != only)) continue;
-            if (whole) by *= at_finish(p, tok[nt], head[nt], m[nt], sum, OFF, g == 0);
-            const u32 col = (u32)(wave * NT + nt) * 16 + n;
-            if (!whole && g == 0) *at_part_ml<DP>(p, slot, col) = f32x2{m[nt], sum};
+            if (whole) by *= at_finish(p, tok, head, m, sum, OFF, g == 0);
+            const u32 col = (u32)wave * 16 + n;
+            if (!whole && g == 0) *at_part_ml<DP>(p, slot, col) = f32x2{m, sum};
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const int d0 = C * (4 * g + i);
                 float y[C];
 #pragma unroll
-                for (int j = 0; j < C; j++) y[j] = acc[nt][j][i] * by;
+                for (int j = 0; j < C; j++) y[j] = acc[j][i] * by;
                 if (whole) {
-                    if (d0 < p.c.d) at_store<C>(p, tok[nt], head[nt], d0, y);
+                    if (d0 < p.c.d) at_store<C>(p, tok, head, d0, y);
                 } else {
 #pragma unroll
                     for (int j = 0; j < C; j += 4) *(f32x4*)(at_part<DP>(p, slot, col) + d0 + j) = f32x4{y[j], y[j + 1], y[j + 2], y[j + 3]};

@@ -20,7 +20,7 @@ __device__ __forceinline__ void attend_one_body(const AttendArgs& p, float* lds,
     const u32 w = at_group_of(blockIdx.x, (u32)p.wgs);
 
     AtWork job;
-    const bool any = at_work<MANY>(p, w, find, job);
+    const bool any = at_work<MANY, 4>(p, w, find, job);
     AtJoin join = {0, 0, 0, 0, 0, {0, 0, 0}};
     if (!any) {
         if (threadIdx.x == 0) at_join_of<DP>(p)[w] = join;
