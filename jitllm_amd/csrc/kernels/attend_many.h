@@ -254,32 +254,31 @@ __device__ __forceinline__ void attend_many_body(const AttendArgs& p, u32x4* lds
             if (s + 1 < s1) ask(s + 1);
             const u32x4* const in = lds + (s & 1) * STAGE;
             const u32* const mark = marks + (s & 1) * 4;
-#pragma unroll 1
-            for (int h = 0; h < 2; h++) {
-                const u32 p0 = s * 64 + h * 32;
-                if (p0 >= whi || p0 + 32 <= wlo) continue;
-                const u32 none = at_uni(mark[h]);
-                const bool edge = p0 < wlo_all || p0 + 32 > whi_all || none;
-                const u32x4* const kin = in + 2 * h * KC * 64 + lane;
-                const u32x4* const vin = in + (4 * KC + h * C) * 64 + lane;
+            const u32 p0 = s * 64;
+            if (p0 < whi && p0 + 64 > wlo) {
+                const u32 none = at_uni(mark[0] | mark[1] << 2);
+                const bool edge = p0 < wlo_all || p0 + 64 > whi_all || none;
+                const u32x4* const kin = in + lane;
+                const u32x4* const vin = in + 4 * KC * 64 + lane;
                 // (fragments two ahead of the products that take them)
-                f32x4 sco[2];
-                u32x4 kt[3] = {kin[0], kin[64], {0, 0, 0, 0}};
+                f32x4 sco[4];
+                u32x4 kt[3] = {kin[0], kin[KC * 64], {0, 0, 0, 0}};
 #pragma unroll
-                for (int c = 0; c < 2 * KC; c++) {      // tile c % 2
-                    if (c + 2 < 2 * KC) kt[(c + 2) % 3] = kin[((c + 2) % 2 * KC + (c + 2) / 2) * 64];
+                for (int i = 0; i < 4 * KC; i++) {      // tile i % 4, piece i / 4 of the row
+                    if (i + 2 < 4 * KC) kt[(i + 2) % 3] = kin[((i + 2) % 4 * KC + (i + 2) / 4) * 64];
 #pragma unroll
                     for (int q = 0; q < QP; q++)
-                        sco[c % 2] = at_mfma<BF>(kt[c % 3], qf[q][c / 2], c / 2 || q ? sco[c % 2] : f32x4{0.f, 0.f, 0.f, 0.f});
+                        sco[i % 4] = at_mfma<BF>(kt[i % 3], qf[q][i / 4], i / 4 || q ? sco[i % 4] : f32x4{0.f, 0.f, 0.f, 0.f});
                 }
-                f32x4 ks[2], vs[2];
+                f32x4 vs[4];
                 if constexpr (I8) {
+                    float big = 0.f;
 #pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        ks[i] = *(const f32x4*)(scales + (s & 1) * 128 + h * 32 + 16 * i + 4 * g);
-                        vs[i] = *(const f32x4*)(scales + (s & 1) * 128 + 64 + h * 32 + 16 * i + 4 * g);
+                    for (int i = 0; i < 4; i++) {
+                        sco[i] *= *(const f32x4*)(scales + (s & 1) * 128 + 16 * i + 4 * g);
+                        vs[i] = *(const f32x4*)(scales + (s & 1) * 128 + 64 + 16 * i + 4 * g);
+                        big = fmaxf(fmaxf(fmaxf(vs[i][0], vs[i][1]), fmaxf(vs[i][2], vs[i][3])), big);
                     }
-                    float big = fmaxf(fmaxf(fmaxf(vs[0][0], vs[0][1]), fmaxf(vs[0][2], vs[0][3])), fmaxf(fmaxf(vs[1][0], vs[1][1]), fmaxf(vs[1][2], vs[1][3])));
                     big = at_max4(big);
                     const int to = __builtin_amdgcn_readfirstlane(big > 0.f ? __builtin_amdgcn_frexp_expf(big) : -200);
                     if (to > ve) {
@@ -290,34 +289,29 @@ __device__ __forceinline__ void attend_many_body(const AttendArgs& p, u32x4* lds
                         ve = to;
                     }
                 }
-                u32x4 vt[3] = {vin[0], vin[64], {0, 0, 0, 0}}, pf[PP];
-                float y[8], by = qs;       // scores are y by
+                u32x4 vt[3] = {vin[0], vin[C * 64], {0, 0, 0, 0}}, pf[2][PP];
+                float y[16], by = qs;       // scores are y by
                 u32 hidden = 0;
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    y[j] = sco[j / 4][j % 4];
-                    if constexpr (I8) y[j] *= ks[j / 4][j % 4];
-                }
+                for (int j = 0; j < 16; j++) y[j] = sco[j / 4][j % 4];
                 if (edge || p.cap != 0.f) {
                     by = 1.f;
 #pragma unroll
-                    for (int j = 0; j < 8; j++) y[j] *= qs;
-                    if (p.cap != 0.f) {
-#pragma unroll
-                        for (int j = 0; j < 8; j++) {
+                    for (int j = 0; j < 16; j++) {
+                        y[j] *= qs;
+                        if (p.cap != 0.f) {
                             y[j] = p.cap * JL_AT_LOG2E * at_tanh(y[j]);
                             asm volatile("" : "+v"(y[j]));     // (one after the other: side by side they take the loop's registers)
                         }
-                    }
-#pragma unroll
-                    for (int j = 0; j < 8; j++) {
                         const u32 at0 = p0 + 16 * (j / 4) + 4 * g + j % 4;
                         const bool sees = !(none >> (j / 4) & 1) && at0 >= clo && at0 < chi;
                         y[j] = sees ? y[j] : -inf;
                         if (I8 && !sees) hidden |= 1u << j;
                     }
                 }
-                float top = fmaxf(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])), fmaxf(fmaxf(y[4], y[5]), fmaxf(y[6], y[7])));
+                float top = y[0];
+#pragma unroll
+                for (int j = 1; j < 16; j++) top = fmaxf(top, y[j]);
                 top = fmaxf(at_max4(top) * by, m);
                 if (__ballot(top > m + JL_AT_SLACK(BF))) {
                     const float turn = m == top ? 1.f : __builtin_amdgcn_exp2f(m - top);   // (from -inf: 0)
@@ -327,21 +321,25 @@ __device__ __forceinline__ void attend_many_body(const AttendArgs& p, u32x4* lds
                     m = top;
                 }
                 const float from = OFF - (m > -inf ? m : 0.f);
+                float sums[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
+                for (int j = 0; j < 16; j++) {
                     y[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(y[j], by, from));
-                    l += y[j];
+                    sums[j / 4] += y[j];
                     if constexpr (I8) y[j] = hidden >> j & 1 ? 0.f : y[j] * __builtin_amdgcn_ldexpf(vs[j / 4][j % 4], -ve);   // (a scale others see may be no number)
                 }
+                l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
 #pragma unroll
-                for (int q = 0; q < PP; q++)
+                for (int h = 0; h < 2; h++)
 #pragma unroll
-                    for (int j = 0; j < 4; j++) pf[q][j] = at_piece<BF>(y[2 * j], y[2 * j + 1]);
+                    for (int q = 0; q < PP; q++)
 #pragma unroll
-                for (int j = 0; j < C; j++) {
-                    if (j + 2 < C) vt[(j + 2) % 3] = vin[(j + 2) * 64];
+                        for (int j = 0; j < 4; j++) pf[h][q][j] = at_piece<BF>(y[8 * h + 2 * j], y[8 * h + 2 * j + 1]);
 #pragma unroll
-                    for (int q = 0; q < PP; q++) acc[j] = at_mfma<BF>(vt[j % 3], pf[q], acc[j]);
+                for (int i = 0; i < 2 * C; i++) {      // element i / 2, half i % 2
+                    if (i + 2 < 2 * C) vt[(i + 2) % 3] = vin[((i + 2) % 2 * C + (i + 2) / 2) * 64];
+#pragma unroll
+                    for (int q = 0; q < PP; q++) acc[i / 2] = at_mfma<BF>(vt[i % 3], pf[i % 2][q], acc[i / 2]);
                 }
             }
             if (s + 1 < s1) put(s + 1);
