@@ -84,9 +84,9 @@ __device__ __forceinline__ float at_tanh(float y) {
 // ---- which positions, units and chunks -----------------------------------------
 
 __device__ __forceinline__ void at_sees(const AttendArgs& p, u32 t, u32& seq, u32& lo, u32& hi) {
+    const u32 n = p.len[t];      // (both loads on their way together)
     seq = p.seq ? p.seq[t] : t;
-    hi = seq < p.c.n_seq ? p.len[t] : 0u;
-    hi = min((uint64_t)hi, (uint64_t)p.c.table_pages << p.c.shift);
+    hi = seq < p.c.n_seq ? min(n, p.c.table_pages << p.c.shift) : 0u;      // (2^31 positions at most)
     lo = p.window && hi > (u32)p.window ? hi - (u32)p.window : 0u;
 }
 // Chunks of what is seen, one at least: a token that sees nothing has its zeros written.
@@ -133,28 +133,26 @@ template <bool MANY> __device__ __forceinline__ AtSpan at_span(const AttendArgs&
     s.lo = at_uni(s.lo); s.hi = at_uni(s.hi); s.lo_all = at_uni(s.lo_all); s.hi_all = at_uni(s.hi_all);
     return s;
 }
-// The chunks of a unit's spans, by one thread; stops at the span that holds chunk `stop`: its first token and the chunks before it.
-template <bool MANY> __device__ __forceinline__ u32 at_unit_chunks(const AttendArgs& p, u32 unit, u32 stop, u32& from, u32& before) {
+// The chunks of a unit's spans, by one thread.
+template <bool MANY> __device__ __forceinline__ u32 at_unit_chunks(const AttendArgs& p, u32 unit) {
     u32 seq0, lo, hi;
     const u32 t0 = unit * (u32)p.per, end = min(t0 + (u32)p.per, (u32)p.ntok);
     at_sees(p, t0, seq0, lo, hi);
     u32 sum = 0;
-    from = t0;
-    before = 0;
-    bool found = false;
     if (MANY) {
-#pragma unroll 8
-        for (u32 t = t0 + 1; t < end; t++) {
-            u32 seq, l, h;
-            at_sees(p, t, seq, l, h);
-            const bool more = seq == seq0;
-            sum += more ? 0u : at_chunks(lo, hi);
-            lo = more ? min(lo, l) : l;
-            hi = more ? max(hi, h) : h;
-            seq0 = seq;
-            found = found || sum > stop;
-            from = more || found ? from : t;
-            before = found ? before : sum;
+#pragma unroll 1
+        for (u32 t = t0 + 1; t < end; t += 4) {
+            u32 seq[4], l[4], h[4];
+#pragma unroll
+            for (u32 i = 0; i < 4; i++) at_sees(p, min(t + i, end - 1), seq[i], l[i], h[i]);     // (the last again changes nothing)
+#pragma unroll
+            for (u32 i = 0; i < 4; i++) {
+                const bool more = seq[i] == seq0;
+                sum += more ? 0u : at_chunks(lo, hi);
+                lo = more ? min(lo, l[i]) : l[i];
+                hi = more ? max(hi, h[i]) : h[i];
+                seq0 = seq[i];
+            }
         }
     }
     return sum + at_chunks(lo, hi);
@@ -206,52 +204,50 @@ template <int WAVES> __device__ __forceinline__ uint64_t at_before(uint64_t mine
 struct AtWork {
     uint64_t first, end;
     AtShare share;
-    u32 plane, off;      // off: chunks of the span that are before it
-    AtSpan span;
+    u32 plane, tok, off;      // its unit's first token (later: the next span's), and the unit's chunks that are before it
 };
 template <bool MANY, int WAVES> __device__ __forceinline__ bool at_work(const AttendArgs& p, u32 w, uint64_t* lds, AtWork& k) {
     u32* const told = (u32*)(lds + WAVES);
     const u32 q = ((u32)p.units + 255) / 256, mine0 = threadIdx.x * q;
-    uint64_t mine = 0, total;
-    u32 from, off;
-    for (u32 i = 0; i < q; i++)
-        if (mine0 + i < (u32)p.units) mine += at_unit_chunks<MANY>(p, mine0 + i, ~0u, from, off);
-    const uint64_t before = at_before<WAVES>(mine, lds, total);
-    const u32 planes = (u32)p.c.n_kv * (u32)p.blocks;
-    k.share = at_share(total * planes, (u32)p.wgs);
-    if (w >= k.share.n) return false;
-    k.first = k.share.first(w);
-    k.end = k.share.first(w + 1);
-    k.plane = at_uni(planes == 1 ? 0u : (k.first >> 32) == 0 && (total >> 32) == 0 ? (u32)k.first / (u32)total : (u32)(k.first / total));
-    const uint64_t at = k.first - k.plane * total;
-    if (at >= before && at < before + mine) {
-        uint64_t b = before;
-        u32 i = 0;
-        if (q > 1)
-            for (;; i++) {
-                const u32 c = at_unit_chunks<MANY>(p, mine0 + i, ~0u, from, off);
-                if (at < b + c) break;
+    uint64_t mine = 0, total, before = 0, at = 0;
+    // twice: the sums, and the unit that has the first chunk, by the thread whose units have it
+#pragma unroll 1
+    for (int pass = 0; pass < 2; pass++) {
+        if (pass == 0 || (at >= before && at < before + mine)) {
+            uint64_t b = before;
+#pragma unroll 1
+            for (u32 i = 0; i < q; i++) {
+                if (mine0 + i >= (u32)p.units) break;
+                const u32 c = at_unit_chunks<MANY>(p, mine0 + i);
+                if (pass && at >= b && at < b + c) {
+                    told[0] = mine0 + i;
+                    told[1] = (u32)(at - b);
+                }
                 b += c;
             }
-        from = mine0 + i;
-        off = 0;
-        if (MANY) at_unit_chunks<MANY>(p, mine0 + i, (u32)(at - b), from, off);
-        told[0] = from;
-        told[1] = (u32)(at - b) - off;
+            if (pass == 0) mine = b;
+        }
+        if (pass) break;
+        before = at_before<WAVES>(mine, lds, total);
+        const u32 planes = (u32)p.c.n_kv * (u32)p.blocks;
+        k.share = at_share(total * planes, (u32)p.wgs);
+        if (w >= k.share.n) return false;
+        k.first = k.share.first(w);
+        k.end = k.share.first(w + 1);
+        k.plane = at_uni(planes == 1 ? 0u : (k.first >> 32) == 0 && (total >> 32) == 0 ? (u32)k.first / (u32)total : (u32)(k.first / total));
+        at = k.first - k.plane * total;
+        if (q == 1) {
+            if (at >= before && at < before + mine) {
+                told[0] = mine0;
+                told[1] = (u32)(at - before);
+            }
+            break;
+        }
     }
     __syncthreads();
     k.off = at_uni(told[1]);
-    k.span = at_span<MANY>(p, at_uni(told[0]));
+    k.tok = at_uni(told[0]) * (u32)p.per;
     return true;
-}
-// The span behind a span; plane is raised behind the last.
-template <bool MANY> __device__ __forceinline__ void at_next(const AttendArgs& p, AtWork& k) {
-    u32 t = k.span.t1;
-    if (t == (u32)p.ntok) {
-        t = 0;
-        k.plane++;
-    }
-    k.span = at_span<MANY>(p, t);
 }
 
 // Partial sums: [2 wgs][columns][DP], then [2 wgs][columns][2] of m and l, then a workgroup's word: what it is the first to have a part of.
@@ -282,14 +278,76 @@ typedef __amdgpu_buffer_rsrc_t at_rsrc;
 __device__ __forceinline__ at_rsrc at_buffer(const void* p) { return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, 0x7fffffff, 0x00020000); }
 #define JL_AT_NOWHERE 0x7fffffff      // an offset behind every buffer: reads zeros
 
-// A column's value written: c elements from d0 on.
+// C elements of a column written.
 template <int C> __device__ __forceinline__ void at_store(const AttendArgs& p, u32 t, u32 head, int d0, const float (&v)[C]) {
     const size_t at = t * p.out_stride + (size_t)head * p.c.d + d0;
+    if (p.out_type == JL_F32) {
+        float* const out = (float*)p.out + at;
+        if (p.out_vec) {
 #pragma unroll
-    for (int i = 0; i < C; i += 4) {
-        const f32x4 x = {v[i], v[i + 1], v[i + 2], v[i + 3]};
-        if (p.out_vec) norm_store<true>(p.out, at + i, p.out_type, 4, x);
-        else norm_store<false>(p.out, at + i, p.out_type, 4, x);
+            for (int i = 0; i < C; i += 4) *(f32x4*)(out + i) = f32x4{v[i], v[i + 1], v[i + 2], v[i + 3]};
+        } else {
+#pragma unroll
+            for (int i = 0; i < C; i++) out[i] = v[i];
+        }
+        return;
+    }
+    uint16_t* const out = (uint16_t*)p.out + at;
+    u32 b[C / 2];
+    if (p.out_type == JL_F16) {
+#pragma unroll
+        for (int i = 0; i < C / 2; i++) b[i] = __builtin_bit_cast(u32, f16x2{(_Float16)v[2 * i], (_Float16)v[2 * i + 1]});
+    } else {
+#pragma unroll
+        for (int i = 0; i < C / 2; i++) b[i] = __builtin_bit_cast(u32, at_bf16x2{(__bf16)v[2 * i], (__bf16)v[2 * i + 1]});
+    }
+    if (p.out_vec) {
+#pragma unroll
+        for (int i = 0; i < C / 2; i += 2) *(u32x2*)(out + 2 * i) = u32x2{b[i], b[i + 1]};
+    } else {
+#pragma unroll
+        for (int i = 0; i < C; i++) out[i] = (uint16_t)(b[i / 2] >> 16 * (i % 2));
+    }
+}
+// A column's q, a lane's eight elements of each piece of 32 (asked for ahead of the rows, which come behind it); then in QP pieces, as the matrix instruction takes
+// them, and what its scores are times.
+template <bool I8, int KC> __device__ __forceinline__ void at_load_query(const AttendArgs& p, bool live, u32 tok, u32 head, float (&x)[KC][8]) {
+    const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int c = 0; c < KC; c++) {
+        const int d = I8 ? 64 * (c / 2) + 16 * g + 8 * (c % 2) : 32 * c + 8 * g;
+        f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
+        if (live && d < p.c.d) kv_load8(p.q, tok * p.q_stride + (size_t)head * p.c.d + d, p.q_type, true, a, b);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            x[c][j] = a[j];
+            x[c][j + 4] = b[j];
+        }
+    }
+}
+template <bool BF, int QP, int KC>
+__device__ __forceinline__ void at_query(const AttendArgs& p, float (&x)[KC][8], u32x4 (&qf)[QP][KC], float& qs) {
+    float most = 0.f;
+    int e = 0;
+    if (!BF) {   // into f16's range: the column's largest to [2^14, 2^15)
+#pragma unroll
+        for (int c = 0; c < KC; c++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) most = fmaxf(most, fabsf(x[c][j]));
+        most = at_max4(most);
+        e = most > 0.f && most < __builtin_inff() ? 15 - __builtin_amdgcn_frexp_expf(most) : 0;
+    }
+    qs = __builtin_amdgcn_ldexpf(fabsf(p.scale), -e);    // (a negative scale's sign goes to q: the largest score is the largest product)
+    qs = p.cap == 0.f ? qs * JL_AT_LOG2E : qs / p.cap;
+    const u32 sign = __float_as_uint(p.scale) & 0x80000000u;
+#pragma unroll
+    for (int c = 0; c < KC; c++) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) x[c][j] = __uint_as_float(__float_as_uint(BF ? x[c][j] : __builtin_amdgcn_ldexpf(x[c][j], e)) ^ sign);
+#pragma unroll
+        for (int k = 0; k < QP; k++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) qf[k][c][j] = at_piece<BF>(x[c][2 * j], x[c][2 * j + 1]);
     }
 }
 // What a column's sums come to: 1 / (sum + sink), and lse.  m in units of log2, l times 2^OFF.

@@ -13,6 +13,7 @@ template <int DP> constexpr int at_stage_words() { return (4 * (DP / 32) + 2 * (
 template <int TYPE, int DP, int QP, int PP, int WAVES>
 __device__ __forceinline__ void attend_many_body(const AttendArgs& p, u32x4* lds, uint64_t* find) {
     constexpr bool BF = TYPE == JL_BF16, I8 = TYPE == JL_I8;
+    static_assert(WAVES * 16 * DP <= 2 * at_stage_words<DP>(), "the columns' rows in the stages' LDS");
     constexpr int C = DP / 16, KC = DP / 32, B = I8 ? 1 : 2, VB = C * B;   // elements of the values a lane, fragments of a key, bytes
     constexpr int KL = I8 ? KC / 2 : KC, VW = (C * B * 4 / WAVES + 3) / 4;   // loads of a tile of keys; words of values a position and lane
     constexpr int STAGE = at_stage_words<DP>() / 4;       // in 16-byte pieces
@@ -33,7 +34,7 @@ __device__ __forceinline__ void attend_many_body(const AttendArgs& p, u32x4* lds
         job.first = 0;
         job.end = ~0ull;
         unit_end = min((unit + 1) * (u32)p.per, (u32)p.ntok);
-        job.span = at_span<true>(p, unit * (u32)p.per);
+        job.tok = unit * (u32)p.per;
     } else {
         w = at_group_of(blockIdx.x, (u32)p.wgs);
         if (!at_work<true, WAVES>(p, w, find, job)) {
@@ -60,9 +61,19 @@ __device__ __forceinline__ void attend_many_body(const AttendArgs& p, u32x4* lds
     const u32 vo = C * n < p.c.d ? 4 * g * row_bytes + (u32)n * VB + (u32)(share & (VS - 1)) * CV * B : JL_AT_NOWHERE;
 
     for (uint64_t at = job.first; at < job.end;) {
-        const AtSpan span = job.span;
-        const u32 lo = span.lo, hi = span.hi, plane = job.plane, c0 = job.off;
-        const u32 n_chunks = at_chunks(lo, hi), left = (u32)min((uint64_t)(n_chunks - c0), job.end - at);
+        const AtSpan span = at_span<true>(p, job.tok);
+        const u32 lo = span.lo, hi = span.hi, plane = job.plane, c0 = job.off, n_chunks = at_chunks(lo, hi);
+        job.tok = span.t1;
+        if (!p.whole && job.tok == (u32)p.ntok) {
+            job.tok = 0;
+            job.plane++;
+        }
+        if (c0 >= n_chunks) {      // (a span of the first unit that others have)
+            job.off -= n_chunks;
+            continue;
+        }
+        job.off = 0;
+        const u32 left = (u32)min((uint64_t)(n_chunks - c0), job.end - at);
         const u32 kv = p.blocks > 1 ? plane / (u32)p.blocks : plane;
         // steps of 64 positions, from the chunk's first on, up to the last that any token sees
         const u32 s0 = max(2 * (lo / JL_AT_CHUNK + c0), lo / 64), s1 = min(2 * (lo / JL_AT_CHUNK + c0 + left), (hi + 63) / 64);
@@ -205,36 +216,9 @@ __device__ __forceinline__ void attend_many_body(const AttendArgs& p, u32x4* lds
         u32x4 qf[QP][KC];
         float qs;
         {
-            float x[KC][8], most = 0.f;
-#pragma unroll
-            for (int c = 0; c < KC; c++) {
-                const int d = I8 ? 64 * (c / 2) + 16 * g + 8 * (c % 2) : 32 * c + 8 * g;
-                f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
-                if (live && d < p.c.d) kv_load8(p.q, tok * p.q_stride + (size_t)head * p.c.d + d, p.q_type, true, a, b);
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    x[c][j] = a[j];
-                    x[c][j + 4] = b[j];
-                    most = fmaxf(most, fmaxf(fabsf(a[j]), fabsf(b[j])));
-                }
-            }
-            int e = 0;
-            if (!BF) {   // into f16's range: the column's largest to [2^14, 2^15)
-                most = at_max4(most);
-                e = most > 0.f && most < inf ? 15 - __builtin_amdgcn_frexp_expf(most) : 0;
-            }
-            qs = __builtin_amdgcn_ldexpf(fabsf(p.scale), -e);   // (a negative scale's sign goes to q: the largest score is the largest product)
-            qs = p.cap == 0.f ? qs * JL_AT_LOG2E : qs / p.cap;
-            const u32 sign = __float_as_uint(p.scale) & 0x80000000u;
-#pragma unroll
-            for (int c = 0; c < KC; c++) {
-#pragma unroll
-                for (int j = 0; j < 8; j++) x[c][j] = __uint_as_float(__float_as_uint(BF ? x[c][j] : __builtin_amdgcn_ldexpf(x[c][j], e)) ^ sign);
-#pragma unroll
-                for (int k = 0; k < QP; k++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) qf[k][c][j] = at_piece<BF>(x[c][2 * j], x[c][2 * j + 1]);
-            }
+            float x[KC][8];
+            at_load_query<I8, KC>(p, live, tok, head, x);
+            at_query<BF, QP, KC>(p, x, qf, qs);
         }
 
         for (;;) {
@@ -356,25 +340,28 @@ __device__ __forceinline__ void attend_many_body(const AttendArgs& p, u32x4* lds
         const u32 slot = 2 * w + (at == job.first ? 0u : 1u);
         const bool whole = left == n_chunks;
         if (c0 == 0 && !whole) join = AtJoin{span.t0, span.t1, plane, job.share.holder(at + n_chunks - 1) + 1, slot, {0, 0, 0}};
+        // through LDS, where each wavefront has its columns, so that rows leave whole
         const float sum = at_sum4(l);
-        if (live && (only == ~0u || tok == only)) {
-            float by = I8 ? __builtin_amdgcn_ldexpf(1.f, ve) : 1.f;
-            if (whole) by *= at_finish(p, tok, head, m, sum, OFF, g == 0);
-            const u32 col = (u32)wave * 16 + n;
-            if (!whole && g == 0) *at_part_ml<DP>(p, slot, col) = f32x2{m, sum};
+        float by = I8 ? __builtin_amdgcn_ldexpf(1.f, ve) : 1.f;
+        const bool gives = live && (only == ~0u || tok == only);
+        const u32 col0 = (u32)wave * 16;
+        if (whole && gives) by *= at_finish(p, tok, head, m, sum, OFF, g == 0);
+        if (!whole && gives && g == 0) *at_part_ml<DP>(p, slot, col0 + n) = f32x2{m, sum};
+        float* const mine = (float*)lds + wave * 16 * DP;
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int d0 = C * (4 * g + i);
-                float y[C];
+        for (int i = 0; i < 4; i++)
 #pragma unroll
-                for (int j = 0; j < C; j++) y[j] = acc[j][i] * by;
-                if (whole) {
-                    if (d0 < p.c.d) at_store<C>(p, tok, head, d0, y);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < C; j += 4) *(f32x4*)(at_part<DP>(p, slot, col) + d0 + j) = f32x4{y[j], y[j + 1], y[j + 2], y[j + 3]};
-                }
-            }
+            for (int j = 0; j < C; j += 4) *(f32x4*)(mine + n * DP + C * (4 * g + i) + j) = f32x4{acc[j][i], acc[j + 1][i], acc[j + 2][i], acc[j + 3][i]} * by;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // (a wavefront's own LDS)
+        const u32 out_tok = gives ? tok : ~0u, quad = (lane & (DP / 4 - 1)) * 4;
+#pragma unroll 1
+        for (int c = lane / (DP / 4); c < 16; c += 256 / DP) {       // a column's row of four-element pieces
+            const u32 t = (u32)__shfl((int)out_tok, c, 64), h = (u32)__shfl((int)head, c, 64);
+            const f32x4 y = *(const f32x4*)(mine + c * DP + quad);
+            const float v[4] = {y.x, y.y, y.z, y.w};
+            if (t == ~0u) continue;
+            if (!whole) *(f32x4*)(at_part<DP>(p, slot, col0 + c) + quad) = y;
+            else if (quad < (u32)p.c.d) at_store<4>(p, t, h, (int)quad, v);
         }
         if (only == ~0u || ++only == span.t1) break;
         u32 q0;
@@ -382,13 +369,7 @@ __device__ __forceinline__ void attend_many_body(const AttendArgs& p, u32x4* lds
         zlo = at_uni(zlo); zhi = at_uni(zhi);
         }
         at += left;
-        job.off = 0;
-        if (p.whole) {
-            if (span.t1 == unit_end) break;
-            job.span = at_span<true>(p, span.t1);
-        } else if (at < job.end) {
-            at_next<true>(p, job);
-        }
+        if (p.whole && span.t1 == unit_end) break;
     }
     if (!p.whole && threadIdx.x == 0) at_join_of<DP>(p)[w] = join;
 }

@@ -41,9 +41,19 @@ __device__ __forceinline__ void attend_one_body(const AttendArgs& p, float* lds,
     const u32 vo = C * n < p.c.d ? 4 * g * row_bytes + (u32)n * VB : JL_AT_NOWHERE;
 
     for (uint64_t at = job.first; at < job.end;) {
-        const AtSpan span = job.span;
-        const u32 lo = span.lo, hi = span.hi, plane = job.plane, c0 = job.off;
-        const u32 n_chunks = at_chunks(lo, hi), left = (u32)min((uint64_t)(n_chunks - c0), job.end - at);
+        const AtSpan span = at_span<MANY>(p, job.tok);
+        const u32 lo = span.lo, hi = span.hi, plane = job.plane, c0 = job.off, n_chunks = at_chunks(lo, hi);
+        job.tok = span.t1;
+        if (job.tok == (u32)p.ntok) {
+            job.tok = 0;
+            job.plane++;
+        }
+        if (MANY && c0 >= n_chunks) {      // (a span of the first unit that others have)
+            job.off -= n_chunks;
+            continue;
+        }
+        job.off = 0;
+        const u32 left = (u32)min((uint64_t)(n_chunks - c0), job.end - at);
         const u32 kv = p.blocks > 1 ? plane / (u32)p.blocks : plane;
         u32 tok, head, clo = lo, chi = hi;      // of this lane's column
         const bool col_live = at_column(p, span.t0, span.t1, plane, n, tok, head);
@@ -69,22 +79,8 @@ __device__ __forceinline__ void attend_one_body(const AttendArgs& p, float* lds,
         for (;;) {
         look(0);
 
-        // q
-        u32x4 qf[QP][KC];
-        float x[KC][8], most = 0.f;
-#pragma unroll
-        for (int c = 0; c < KC; c++) {
-            const int d = I8 ? 64 * (c / 2) + 16 * g + 8 * (c % 2) : 32 * c + 8 * g;
-            f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
-            if (col_live && d < p.c.d) kv_load8(p.q, tok * p.q_stride + (size_t)head * p.c.d + d, p.q_type, true, a, b);
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                x[c][j] = a[j];
-                x[c][j + 4] = b[j];
-                most = fmaxf(most, fmaxf(fabsf(a[j]), fabsf(b[j])));
-            }
-        }
-
+        float x[KC][8];
+        at_load_query<I8, KC>(p, col_live, tok, head, x);
         u32x4 kf[2][KL];
         u32 vw[8][VW];
         f32x4 ks[2], vs[2];
@@ -132,23 +128,9 @@ __device__ __forceinline__ void attend_one_body(const AttendArgs& p, float* lds,
         vpage[0] = page[0]; vpage[1] = page[1];
         ask_v(0);
 
-        int e = 0;
-        if (!BF) {   // into f16's range: the column's largest to [2^14, 2^15)
-            most = at_max4(most);
-            e = most > 0.f && most < inf ? 15 - __builtin_amdgcn_frexp_expf(most) : 0;
-        }
-        float qs = __builtin_amdgcn_ldexpf(fabsf(p.scale), -e);    // (a negative scale's sign goes to q: the largest score is the largest product)
-        qs = p.cap == 0.f ? qs * JL_AT_LOG2E : qs / p.cap;
-        const u32 sign = __float_as_uint(p.scale) & 0x80000000u;
-#pragma unroll
-        for (int c = 0; c < KC; c++) {
-#pragma unroll
-            for (int j = 0; j < 8; j++) x[c][j] = __uint_as_float(__float_as_uint(BF ? x[c][j] : __builtin_amdgcn_ldexpf(x[c][j], e)) ^ sign);
-#pragma unroll
-            for (int k = 0; k < QP; k++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) qf[k][c][j] = at_piece<BF>(x[c][2 * j], x[c][2 * j + 1]);
-        }
+        u32x4 qf[QP][KC];
+        float qs;
+        at_query<BF, QP, KC>(p, x, qf, qs);
 
         f32x4 acc[C];
         float m = -inf, l = 0.f;
@@ -352,8 +334,6 @@ __device__ __forceinline__ void attend_one_body(const AttendArgs& p, float* lds,
         }
         if (c0 == 0 && left < n_chunks) join = AtJoin{span.t0, span.t1, plane, job.share.holder(at + n_chunks - 1) + 1, 2 * w + (at == job.first ? 0u : 1u), {0, 0, 0}};
         at += left;
-        job.off = 0;
-        if (at < job.end) at_next<MANY>(p, job);
     }
     if (threadIdx.x == 0) at_join_of<DP>(p)[w] = join;
 }
