@@ -47,7 +47,8 @@ template <bool BF> __device__ __forceinline__ f32x4 at_mfma(u32x4 a, u32x4 b, f3
 template <bool BF> __device__ __forceinline__ u32 at_piece(float& x, float& y) {
     if constexpr (BF) {
         const at_bf16x2 h = {(__bf16)x, (__bf16)y};
-        const u32 b = __builtin_bit_cast(u32, h);
+        u32 b = __builtin_bit_cast(u32, h);
+        asm("" : "+v"(b));       // (else each half is converted once more, by itself)
         x -= __uint_as_float(b << 16);
         y -= __uint_as_float(b & 0xffff0000u);
         return b;

@@ -305,11 +305,11 @@ __device__ __forceinline__ void attend_many_body(const AttendArgs& p, u32x4* lds
                     m = top;
                 }
                 const float from = OFF - (m > -inf ? m : 0.f);
-                float sums[4] = {0.f, 0.f, 0.f, 0.f};
+                float sums[4];
 #pragma unroll
                 for (int j = 0; j < 16; j++) {
                     y[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(y[j], by, from));
-                    sums[j / 4] += y[j];
+                    sums[j / 4] = j % 4 ? sums[j / 4] + y[j] : y[j];
                     if constexpr (I8) y[j] = hidden >> j & 1 ? 0.f : y[j] * __builtin_amdgcn_ldexpf(vs[j / 4][j % 4], -ve);   // (a scale others see may be no number)
                 }
                 l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
