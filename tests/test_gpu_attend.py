@@ -355,3 +355,88 @@ def test_a_token_alone_and_among_others(dev):
     for t in range(4):
         got, lse = run(dev, c, q[t:t + 1], quant.F32, quant.F32, [t], [lens[t]], 0.09)
         check(got, lse, [a[t:t + 1] for a in ref], quant.F32)
+
+
+@pytest.fixture(params=[1, 2], ids=["units whole", "shares"])
+def form(dev, request):
+    """Which of the two ways more than sixteen columns a unit are divided among the workgroups."""
+    dev.set_tuning(attend__whole=request.param)
+    yield request.param
+    dev.set_tuning(attend__whole=0)
+
+
+@pytest.mark.parametrize("t", KINDS)
+@pytest.mark.parametrize("per, group, d", [(16, 2, 64), (17, 1, 80), (33, 4, 128), (64, 1, 256), (130, 2, 48), (9, 8, 192)])
+def test_prompts_in_both_divisions(dev, form, t, per, group, d):
+    """Units that end inside a sequence, sequences that end inside a unit, the last unit short; with and without what came before the prompt."""
+    lens = [per, per + 1, per + 200, per + 63, per + 64]
+    seq = np.repeat(np.arange(5), per)
+    length = np.concatenate([np.arange(n - per, n) + 1 for n in lens])
+    attend(dev, t, lens, seq, length, 2, group, d, qt=quant.F16, ot=quant.BF16)
+    attend(dev, t, lens, seq, length, 2, group, d, window=50, sinks=True, cap=20.0)
+    n = 3 * per // 2
+    attend(dev, t, lens, seq[:n], length[:n], 2, group, d)
+
+
+@pytest.mark.parametrize("t", KINDS)
+@pytest.mark.parametrize("ot", PLAIN)
+def test_prompts_of_each_type_in_both_divisions(dev, form, t, ot):
+    lens = [90, 70]
+    seq, length = np.repeat([0, 1], [60, 70]), np.concatenate([np.arange(31, 91), np.arange(1, 71)])
+    for qt in PLAIN:
+        attend(dev, t, lens, seq, length, 3, 2, 128, qt, ot)
+
+
+@pytest.mark.parametrize("t", KINDS)
+def test_hidden_places_in_both_divisions(dev, form, t):
+    """A prompt whose later positions hold NaN: only the tokens that see them have it.  Tokens that see nothing between those that do."""
+    rng = np.random.default_rng(21)
+    table, n_page = table_of(rng, [300, 80], 16)
+    c = Cache(t, 2, 64, 16, table, n_page)
+    seq, length = np.repeat([0, 1], [100, 40]), np.concatenate([np.arange(170, 270), np.arange(31, 71)])
+    length[[3, 50, 120]] = 0
+    seq[[7, 130]] = 9
+    q = rng.standard_normal((140, 4, 64)).astype(np.float32)
+    ref = reference(c, q, seq, length, 0.125)
+    for s, p in [(0, 200), (0, 257), (0, 269), (0, 275), (1, 60), (1, 71), (1, 79)]:
+        pg, at = c.place(s, p)
+        for pool, scales in ((c.k, c.ks), (c.v, c.vs)):
+            if t == quant.I8:
+                scales[pg, :, at] = np.nan
+            else:
+                pool[pg, :, at] = stored(np.full((2, 64), np.nan, np.float32), t)
+    c.upload()
+    got, lse = run(dev, c, q, quant.F32, quant.F32, seq, length, 0.125)
+    clean = (seq == 9) | ((seq == 0) & (length <= 200)) | ((seq == 1) & (length <= 60))
+    check(got[clean], lse[clean], [a[clean] for a in ref], quant.F32)
+    assert np.all(np.isnan(got[~clean])) and np.all(got[[3, 50, 120, 7, 130]] == 0)
+
+
+def test_prompts_on_a_stream_of_the_callers(dev, form):
+    """More than sixteen columns a unit captured and replayed over other lengths, between eager calls; the same bits as eager."""
+    rng = np.random.default_rng(22)
+    table, n_page = table_of(rng, [600, 300], 32)
+    c, st = Cache(quant.BF16, 2, 128, 32, table, n_page), Stream()
+    seq = np.repeat([0, 1], 45)
+    q = stored(rng.standard_normal((90, 8, 128)).astype(np.float32), quant.BF16)
+    qd, sd, ld, out = DeviceArray(q), DeviceArray(seq.astype(np.uint32)), DeviceArray(np.ones(90, np.uint32)), DeviceArray(np.zeros((90, 8, 128), np.uint16))
+    h = c.handle(dev)
+    dev.reserve_attend(128)
+    call = lambda s: dev.attend_dev(h, out.ptr, qd.ptr, 8, ld.ptr, 90, 0.1, seq=sd.ptr, q_type=quant.BF16, out_type=quant.BF16, stream=s)
+    try:
+        with Graph.capture(st.handle) as g:
+            assert call(st.handle)
+        for n in (45, 300, 64, 128):
+            length = np.concatenate([np.arange(2 * n - 45, 2 * n) + 1, np.arange(n - 45, n) + 1])
+            ld.put(length.astype(np.uint32))
+            g.launch()
+            st.synchronize()
+            first = out.get()
+            check(values(first, quant.BF16), None, reference(c, values(q, quant.BF16), seq, length, 0.1), quant.BF16)
+            attend(dev, quant.F16, [70], np.zeros(40, int), np.arange(31, 71), 2, 2, 64)
+            out.put(np.zeros_like(first))
+            assert call(st.handle)
+            st.synchronize()
+            assert np.array_equal(out.get(), first)
+    finally:
+        st.destroy()

@@ -5,7 +5,8 @@ import numpy as np
 import pytest
 
 from jitllm_amd import quant
-from jitllm_amd.hipmem import DeviceArray, Graph, Stream
+from jitllm_amd.device import Device
+from jitllm_amd.hipmem import DeviceArray, Graph, Stream, mem_info
 from test_gpu_kv_cache import PLAIN
 from test_gpu_norm_rows import STEP, at_offset, stored, values
 
@@ -191,3 +192,35 @@ def test_the_same_in_every_call(dev):
             run(dev, x[:7], quant.F32, rng.random(7).astype(np.float32), top_k=9)
     finally:
         st.destroy()
+
+
+@pytest.mark.parametrize("n", [200, 5000, 70001])
+@pytest.mark.parametrize("k", [63, 64, 65, 128, 700, 1023, 1024, 1025, 4000])
+def test_as_many_as_asked_for(dev, n, k):
+    """The k largest, alone and with a share of their sum, around the sizes at which they are held in another way."""
+    rng = np.random.default_rng(k)
+    x = logits(rng, 3, n, 1.0)
+    x[2] = np.round(x[2], 1)          # ties by the hundred
+    u = rng.random(3).astype(np.float32)
+    check(dev, x, quant.F32, u, top_k=k)
+    check(dev, x, quant.F32, u, top_k=k, top_p=0.97, min_p=0.001)
+    check(dev, x, quant.BF16, u, top_k=k, top_p=0.6, temperature=2.0)
+
+
+def test_more_rows_than_a_pass_has(dev):
+    rng = np.random.default_rng(31)
+    x = logits(rng, 2100, 300)
+    check(dev, x, quant.F16, rng.random(2100).astype(np.float32), top_k=rng.choice([0, 5, 90], 2100), top_p=rng.choice([0.5, 0.9, 1.0], 2100))
+
+
+def test_a_reserved_workspace():
+    with Device(device=0) as d:
+        d.reserve_sample(5000)          # (a pass's rows, whatever is asked for)
+        rng = np.random.default_rng(32)
+        for rows, n in ((1, 100), (1500, 2000), (7, 131072)):
+            xd, ud = DeviceArray(logits(rng, rows, n)), DeviceArray(rng.random(rows).astype(np.float32))
+            p, token = DeviceArray(np.full(rows, 0.9, np.float32)), DeviceArray(np.zeros(rows, np.uint32))
+            before = mem_info()[0]
+            assert d.sample_dev(xd.ptr, rows, n, ud.ptr, token.ptr, top_p=p.ptr) and d.sample_dev(xd.ptr, rows, n, ud.ptr, token.ptr)
+            d.synchronize()
+            assert mem_info()[0] == before and np.all(token.get() < n)

@@ -168,3 +168,5 @@ def test_sample_refusals(nodev, change, what):
 def test_reserve_refusals(nodev):
     _says(lambda: nodev.reserve_attend(128), None)
     _says(lambda: nodev.reserve_attend(0), "reserve attend")
+    _says(lambda: nodev.reserve_sample(64), None)
+    _says(lambda: nodev.reserve_sample(0), "reserve sample")
