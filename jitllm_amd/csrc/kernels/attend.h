@@ -43,20 +43,24 @@ template <bool BF> __device__ __forceinline__ f32x4 at_mfma(u32x4 a, u32x4 b, f3
     if constexpr (BF) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(at_bf16x8, a), __builtin_bit_cast(at_bf16x8, b), c, 0, 0, 0);
     else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(at_f16x8, a), __builtin_bit_cast(at_f16x8, b), c, 0, 0, 0);
 }
-// Two values in the type's bits, to nearest even, and what that leaves of them.
+// Two values in the type's bits, to nearest even, and what that leaves of them: of those very bits.  (Left to itself the compiler converts the values again for the
+// difference; where a value is a product, once from the product as it was rounded and once by an instruction that multiplies and converts: now and then the two are a
+// step apart, and a weight over 8-bit rows was off by 2^-11 of itself.)
 template <bool BF> __device__ __forceinline__ u32 at_piece(float& x, float& y) {
     if constexpr (BF) {
         const at_bf16x2 h = {(__bf16)x, (__bf16)y};
         u32 b = __builtin_bit_cast(u32, h);
-        asm("" : "+v"(b));       // (else each half is converted once more, by itself)
+        asm("" : "+v"(b));
         x -= __uint_as_float(b << 16);
         y -= __uint_as_float(b & 0xffff0000u);
         return b;
     } else {
-        const f16x2 h = {(_Float16)x, (_Float16)y};
+        u32 b = __builtin_bit_cast(u32, f16x2{(_Float16)x, (_Float16)y});
+        asm("" : "+v"(b));
+        const f16x2 h = __builtin_bit_cast(f16x2, b);
         x -= (float)h.x;
         y -= (float)h.y;
-        return __builtin_bit_cast(u32, h);
+        return b;
     }
 }
 // Largest of the four lanes of a column; every one of them has it.

@@ -440,3 +440,21 @@ def test_prompts_on_a_stream_of_the_callers(dev, form):
             assert np.array_equal(out.get(), first)
     finally:
         st.destroy()
+
+
+@pytest.mark.parametrize("per", [1, 24])
+def test_weights_of_an_int8_cache_are_split_as_they_are_rounded(dev, per):
+    """Tens of thousands of weights that each count, over scales of every size: where a weight times its row's scale falls next to a half step of f16, its two pieces
+    still add up to it."""
+    rng = np.random.default_rng(40)
+    lens = [12 + per] * (64 // per + 1)
+    table, n_page = table_of(rng, lens, 16)
+    c = Cache(quant.I8, 8, 64, 16, table, n_page)
+    c.k[:] //= 16
+    c.vs[:] = 0.01 + 0.03 * rng.random(c.vs.shape)
+    c.upload()
+    seq = np.repeat(np.arange(len(lens)), per)
+    length = np.concatenate([np.arange(12, 12 + per) + 1 for _ in lens])
+    q = rng.standard_normal((len(seq), 64, 64)).astype(np.float32)
+    got, lse = run(dev, c, q, quant.F32, quant.F32, seq, length, 0.125)
+    check(got, lse, reference(c, q, seq, length, 0.125), quant.F32)
