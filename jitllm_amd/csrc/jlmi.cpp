@@ -37,7 +37,8 @@ struct Tuning {
     int xpre = 0;               // decode matvec: 1 / 2 / 4 float4 groups of x a thread loads ahead of its weights
     int q8pair = 0;             // Q8_0 rows: 2 keeps one block a lane-slot (2-byte-aligned loads)
     int packed_rw = 0, packed_block = 0, moe_group = 0, moe_logits = 0;
-    int attend_whole = 0;       // many tokens: 1 a unit a workgroup, 2 equal shares of the chunks
+    int attend_form = 0;        // several tokens: 1 attend_one, 4 or 8 attend_many with as many wavefronts
+    int attend_whole = 0;       // attend_many: 1 a unit a workgroup, 2 equal shares of the chunks
     int moe_select = 0, adapter_form = 0, adapter_slices = 0, adapter_sets = 0;
     int moe_shares = 0;
     int gemm_rows = 0;
@@ -2440,6 +2441,7 @@ int jl_set_tuning(jl_ctx* c, const char* key, int value) {
     else if (!strcmp(key, "matvec.grid")) c->tune.grid = value;
     else if (!strcmp(key, "packed.rw")) c->tune.packed_rw = value;
     else if (!strcmp(key, "packed.block")) c->tune.packed_block = value;
+    else if (!strcmp(key, "attend.form")) c->tune.attend_form = value;
     else if (!strcmp(key, "attend.whole")) c->tune.attend_whole = value;
     else if (!strcmp(key, "moe.select")) c->tune.moe_select = value;
     else if (!strcmp(key, "adapter.form")) c->tune.adapter_form = value;
@@ -3122,6 +3124,71 @@ namespace {
 int attend_wgs(const jl_ctx* c, int d) { return (d > 128 ? 1 : 2) * c->num_cu; }
 int attend_row(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 size_t attend_part_bytes(int wgs, int d, int cols) { return (size_t)wgs * (2 * (size_t)cols * (attend_row(d) + 2) * 4 + 32); }   // (AtJoin: 32 bytes)
+
+// How the tokens of a call are put together and divided.
+struct AttendPlan {
+    int waves;                   // 0: attend_one
+    int cols, per, units, blocks;
+    bool whole;
+};
+// Columns are a token's heads that share a key head, and those of up to as many of a sequence's tokens as there are on average (`most`).  Single tokens take attend_one;
+// for several the five ways are set against each other by what they measured (us, 16-bit rows of 128, 4 heads a key head, 8 key heads), with S the
+// positions that a sequence can have (the table's, or the window's):
+//   attend_one: 20, and 2.5 a chunk of 128 positions that a workgroup has in turn; attend_many in shares: 32 and 2.1 a step of 64 (four wavefronts), 45 and 3.3
+//   (eight); units whole: 10 or 14, and of each round of workgroups 1.65 a step (four wavefronts; 1.8 where a CU has two), 1.85 or 2.7 (eight).
+//                          one    shares 4   shares 8   whole 4   whole 8    (sequences x tokens; shares and whole with four or eight wavefronts)
+//   8 x 5 of 2048           28       37         50        63        59
+//   2 x 16 of 8192          37       69         82       222       194
+//   8 x 32 of 2048          56       47         67        64        73
+//   64 x 16 of 2048        246      116        151        81        99
+//   64 x 32 of 2048        477      193        173       125       112
+//   1 x 512 of 512          45       41         44        24        29
+//   1 x 512 of 8192        302      169        151       225       244
+//   1 x 1024 of 1024       132       77         80        40        46
+//   3 x 683 of 2048        272      153        135       139       120
+//   1 x 2080 of 2080       388      179        154        99        89
+// Rows of 256 have half of the workgroups and 1.5 (shares) or 1.8 times (whole) as long a step.  Where units straddle sequences both of a unit's spans are work.
+// Of 80 such calls what is taken is the fastest or within a tenth of it but for three (16 x 24 of 2048 takes 72 for 56).  A table far larger than what the
+// sequences hold speaks for shares: 1 x 512 of 512 takes 41 for 24 then.
+AttendPlan attend_plan(const jl_ctx* c, int ntok, int n_seq, int n_kv, int group, int d, int most, int window, unsigned long long reach) {
+    const double wgs = attend_wgs(c, d);
+    AttendPlan best = {};
+    double least = 0;
+    for (int way = 0; way < 5; way++) {
+        AttendPlan a;
+        a.waves = way == 0 ? 0 : way % 2 ? 4 : 8;
+        a.whole = way > 2;
+        a.cols = a.waves ? 16 * a.waves : 16;
+        a.per = std::clamp(a.cols / group, 1, most);
+        a.units = (ntok + a.per - 1) / a.per;
+        a.blocks = a.per > 1 ? 1 : (group + a.cols - 1) / a.cols;
+        if (a.waves && most == 1) continue;
+        if (most > 1) {
+            const int form = c->tune.attend_form, whole = c->tune.attend_whole;
+            if (form && form != (a.waves ? a.waves : 1)) continue;
+            if (whole && a.waves && a.whole != (whole == 1)) continue;
+            if (whole && !form && !a.waves && (long)group * most > 16) continue;
+        }
+        const bool straddles = n_seq > 1 && most % a.per != 0, wide = attend_row(d) == 256;
+        const double seen = window ? std::min<double>(reach, (double)window + a.per) : (double)reach;
+        const double steps = seen / 64 + 1, work = (double)a.units * n_kv * a.blocks * (straddles ? 1 + (double)a.per / most : 1.0);
+        double us;
+        if (!a.waves) us = 20 + 2.5 * work * (steps / 2) / wgs;
+        else if (!a.whole) us = (a.waves == 4 ? 32 : 45) + (a.waves == 4 ? 2.1 : 3.3) * (wide ? 1.5 : 1) * work * steps / wgs;
+        else {
+            const double alone = (a.waves == 4 ? 1.65 : 1.85) * (wide ? 1.8 : 1), shared = (a.waves == 4 ? 1.8 : 2.7) * (wide ? 1.8 : 1);
+            const double rounds = std::floor(work / wgs), rest = work - rounds * wgs;
+            const double last = rest == 0 ? 0 : rounds > 0 ? std::max(alone / 2, shared * rest / wgs) : rest > wgs / 2 ? shared : alone;   // (behind others: units end one after the other)
+            const double all = steps * (rounds * shared + last);
+            us = (a.waves == 4 ? 10 : 14) + std::max(all, steps * alone * (straddles ? 2 : 1));
+        }
+        if (!best.cols || us < least) {
+            best = a;
+            least = us;
+        }
+    }
+    return best;
+}
 }  // namespace
 
 int jl_reserve_attend(jl_ctx* c, int max_d) {
@@ -3153,23 +3220,18 @@ int jl_attend_dev(jl_ctx* c, const jl_kv_cache* cache, const jl_attend* g, void*
     a.window = g->window; a.scale = g->scale; a.cap = g->softcap;
     a.out_vec = ((uintptr_t)g->out & (4 * ob - 1)) == 0 && a.out_stride % 4 == 0;
     const int row = attend_row(cache->d);
-    // Columns: a token's heads that share a key head, and with more tokens than sequences those of as many of a sequence's tokens as there are on average.  Up to
-    // sixteen of them take the form whose wavefronts share the positions, more the one whose wavefronts share the columns.
     const int most = std::max(1, g->seq ? g->ntok / cache->n_seq : 1);
-    const bool one = most == 1 || (long)a.group * most <= 16;
+    const AttendPlan plan = attend_plan(c, g->ntok, cache->n_seq, cache->n_kv, a.group, cache->d, most, g->window, (unsigned long long)cache->table_pages * cache->page_size);
+    const bool one = plan.waves == 0;
     const bool bf = cache->type == JL_TYPE_BF16;
     // q in one piece where the cache's type holds it; over bf16 three pieces of the weights go with three of q, for a result of 32 bits
     const int pieces = bf ? (g->q_type == JL_TYPE_BF16 && g->out_type != JL_TYPE_F32 ? 1 : 3) : g->q_type == JL_TYPE_F32 ? 2 : 1;
-    const int waves = one || (long)a.group * most <= 64 ? 4 : 8;
-    a.part_cols = one ? 16 : 16 * waves;
-    a.per = std::clamp(a.part_cols / a.group, 1, most);
-    a.units = (g->ntok + a.per - 1) / a.per;
-    a.blocks = a.per > 1 ? 1 : (a.group + a.part_cols - 1) / a.part_cols;
+    const int waves = one ? 4 : plan.waves;
+    a.part_cols = plan.cols; a.per = plan.per; a.units = plan.units; a.blocks = plan.blocks; a.whole = plan.whole;
     a.inv_group = 65536 / a.group + 1;
     // No more workgroups than there can be chunks of 128 positions.
     const unsigned long long per_head = ((unsigned long long)cache->table_pages * cache->page_size + 127) / 128 + 1, planes = (unsigned long long)cache->n_kv * a.blocks;
     a.wgs = (int)std::min<unsigned long long>(attend_wgs(c, cache->d), g->ntok * planes * per_head);
-    a.whole = !one && (c->tune.attend_whole ? c->tune.attend_whole == 1 : a.units * planes >= (unsigned)a.wgs);
     if (a.units * planes > 0xffffffffull / 512) return JL_DECLINED;   // threads a launch can have
     HIP_TRY(c, H->SetDevice(c->device));
     rc = a.whole ? JL_OK : attend_ws_ensure(c, attend_part_bytes(a.wgs, cache->d, a.part_cols));

@@ -458,3 +458,20 @@ def test_weights_of_an_int8_cache_are_split_as_they_are_rounded(dev, per):
     q = rng.standard_normal((len(seq), 64, 64)).astype(np.float32)
     got, lse = run(dev, c, q, quant.F32, quant.F32, seq, length, 0.125)
     check(got, lse, reference(c, q, seq, length, 0.125), quant.F32)
+
+
+@pytest.mark.parametrize("t", KINDS)
+@pytest.mark.parametrize("way", [dict(attend__form=1), dict(attend__form=4, attend__whole=1), dict(attend__form=4, attend__whole=2), dict(attend__form=8, attend__whole=1),
+                                 dict(attend__form=8, attend__whole=2)], ids=lambda w: " ".join(f"{k[8:]} {v}" for k, v in w.items()))
+def test_every_way_of_putting_tokens_together(dev, t, way):
+    """Few and many tokens in each of the forms, whichever would be taken for them."""
+    dev.set_tuning(**way)
+    try:
+        for per, group, d in ((2, 1, 64), (5, 3, 128), (19, 4, 256), (70, 20, 96)):
+            lens = [per, per + 150, per + 33]
+            seq = np.repeat(np.arange(3), per)
+            length = np.concatenate([np.arange(n - per, n) + 1 for n in lens])
+            attend(dev, t, lens, seq, length, 2, group, d, qt=quant.BF16, ot=quant.F16)
+            attend(dev, t, lens, seq, length, 2, group, d, window=70, sinks=True)
+    finally:
+        dev.set_tuning(attend__form=0, attend__whole=0)
