@@ -631,8 +631,9 @@ int jl_kv_read_dev(jl_ctx *ctx, const jl_kv_cache *cache, const jl_kv_rows *rows
  * A token that sees nothing (len 0, no such sequence, no pages) has zeros, lse -infinity or its sink.  len counts at most the table's positions.  Sums are f32, and q and the weights
  * keep 22 bits or more (16 of the weights over a bf16 cache where out is 16 bits wide); a token's result does not depend on the other tokens of the call but in the last bits, by
  * where the cache was cut among the workgroups.  Infinities and NaNs in rows that a token does not see change nothing of its result.
- * Tokens of one sequence share the reads of its rows where they follow each other.  q 16-byte aligned, its stride a multiple of 16 bytes; n_head a multiple of n_kv.  out overlaps no
- * other operand.  Two launches; the workspace (jl_reserve_attend) is the context's, of one size for a row width whatever the tokens, and a buffer that is outgrown
+ * Tokens of one sequence share the reads of its rows where they follow each other; how many of them are put together goes by ntok / n_seq, so a call over a few
+ * of many sequences gives the rows of the table that it needs.  q 16-byte aligned, its stride a multiple of 16 bytes; n_head a multiple of n_kv.  out overlaps no
+ * other operand.  One launch or two; the workspace (jl_reserve_attend) is the context's, of one size for a row width whatever the tokens, and a buffer that is outgrown
  * lives until the context goes, so a captured graph that holds its address stays valid.  The reference's attention is another part of its device seam
  * (engine/nn/device.go:1096-1176). */
 typedef struct jl_attend {
