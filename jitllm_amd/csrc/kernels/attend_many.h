@@ -6,10 +6,12 @@
 // wavefront keeps its columns' sums to the end, so nothing is exchanged; they leave through LDS as whole rows (64 tokens of a prompt 27.6 -> 22.9 us: the code that runs
 // once is fetched once, and is most of a short call).
 //
-// Bound by the matrix and vector units and LDS together: a step of 128 columns x 64 positions x 128 has 384 matrix instructions over four SIMDs (0.64 us at the peak rate),
-// about as many clocks of vector instructions, 290 KB through LDS, and takes 1.65.  Measured (32 heads over 8 of 128, bf16): a prompt of 8192 850 us, 647 TFLOP/s of
-// the product's operations, 970 of the instructions' (P in two pieces; a library's product of 8192^3 reaches 1400); of 2048 87, of 512 23; 3 x 683 over 2048 120.
-// Tried and not kept: every other span of a unit in a workgroup of its own (3 x 683: 141 for 133), a raised priority around the products (134 to 139 for 133).
+// A step of 128 columns x 64 positions x 128 has 384 matrix instructions over four SIMDs (0.64 us at the peak rate), 256 vector instructions a wavefront, 290 KB through LDS, and
+// takes 1.65: each unit is busy a fifth to a third of the time, and the rest is the wavefronts' waits at the same places (bringing the rows is a quarter of a call: 8192 tokens 850 us,
+// 600 with rows that stand in LDS already).  Measured (32 heads over 8 of 128, bf16): a prompt of 8192 850 us, 647 TFLOP/s of the product's operations, 970 of the
+// instructions' (P in two pieces; a library's product of 8192^3 reaches 1400); of 2048 87, of 512 23; 3 x 683 over 2048 120.
+// Tried and not kept: every other span of a unit in a workgroup of its own (3 x 683: 141 for 133), a raised priority around the products (134 to 139 for 133), keys by
+// loads that write LDS directly (150 for 133).
 #pragma once
 #include "attend.h"
 

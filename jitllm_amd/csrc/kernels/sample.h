@@ -16,8 +16,8 @@
 //   sample_take    a workgroup a row: the list sorted, the cuts, and the token, from the list or from the slice in which u falls.  SLOW rows are done here from
 //                  the start: the cut's bin divided again by keys and, where one key is left, by index.
 //
-// One row: four launches, each a few trips to memory (131072 values, the 40 largest and their nucleus: 19 us, 2.8 + 4 + 6 + 5).  Many: three reads of the row, the weights
-// behind the largest, the cut behind the weights' sums, and f64 beside them (256 x 200003, a nucleus of 0.95: 180 us, 43 + 63 + 63 + 11; a read alone is 43).
+// One row: four launches, each a few trips to memory (131072 values, the 40 largest and their nucleus: 19 us, 3.5 + 4.4 + 6.4 + 5.1).  Many: three reads of the row, the weights
+// behind the largest, the cut behind the weights' sums, and f64 beside them (256 x 200003, a nucleus of 0.95: 180 us back to back, by trace 44 + 66 + 75 + 19; a read alone is 43).
 #pragma once
 #include "args.h"
 #include "common.h"
