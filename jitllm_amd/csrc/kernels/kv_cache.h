@@ -4,8 +4,9 @@
 //   arithmetic (quantize.h) with the row as its window, d = amax / 127, q = round-half-away(f32(x * f32(1 / d))); read back as f32(q * d).
 //
 // A row takes `lanes` lanes of a wavefront, eight elements each: one or two 16-byte loads, one 16- or 8-byte store, and the amax
-// by lane moves.  Bytes bind: 8191 tokens of 8 heads of 128, f32 to 8 bits, 19.8 us (4.2 TB/s), back to bf16 12.0 (4.2), 50001 of 4 of 96, bf16 to f32, 59 (3.9; a large
-// copy has 5.0).  Two rows a thread side by side change nothing (19.9, 12.0, 59.1).  A token whose sequence, position or page is none of the cache's is written nowhere and read back as zeros.
+// by lane moves.  Bytes bind, in whole lines of rows that lie where the pages do: 8191 tokens of 8 heads of 128, f32 to 8 bits, 19.8 us (4.2 TB/s), back to bf16 12.0 (4.2);
+// 50001 tokens in any order of 4 heads of 96, bf16 to f32, 59 (3.9; rows of 192 bytes meet two lines of 128; a large copy has 5.0).  Two rows a thread side by side
+// change nothing (19.9, 12.0, 59.1), four elements a lane with stores of whole lines take 93.5 for 59.  A token whose sequence, position or page is none of the cache's is written nowhere and read back as zeros.
 #pragma once
 #include "args.h"
 #include "common.h"
