@@ -475,3 +475,20 @@ def test_every_way_of_putting_tokens_together(dev, t, way):
             attend(dev, t, lens, seq, length, 2, group, d, window=70, sinks=True)
     finally:
         dev.set_tuning(attend__form=0, attend__whole=0)
+
+
+@pytest.mark.parametrize("form", [1, 4, 8])
+def test_thousands_of_tokens(dev, form):
+    """More units than a workgroup has threads to count them, sequences in turn, and a few tokens that see nothing."""
+    rng = np.random.default_rng(50)
+    lens = [400, 37, 900]
+    seq = np.repeat([0, 2, 1, 2, 0], [1300, 1500, 37, 1100, 1200])
+    length = np.array([rng.integers(0, lens[s] + 1) for s in seq])
+    dev.set_tuning(attend__form=form, attend__whole=2)
+    try:
+        attend(dev, quant.F16, lens, seq, length, 1, 1, 16, ot=quant.F16)
+    finally:
+        dev.set_tuning(attend__form=0, attend__whole=0)
+    many = rng.integers(0, 38, 3000)
+    attend(dev, quant.I8, [37], np.zeros(3000, int), many, 1, 1, 16)
+    attend(dev, quant.BF16, lens * 700, None, np.array(lens * 700) // 20, 1, 2, 16, window=9)
