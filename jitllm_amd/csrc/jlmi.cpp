@@ -3247,7 +3247,7 @@ int jl_attend_dev(jl_ctx* c, const jl_kv_cache* cache, const jl_attend* g, void*
     rc = launch(c, name, a.whole ? (unsigned)(a.units * planes) : (unsigned)a.wgs, 1, 64u * waves, 0, st, params);
     if (rc != JL_OK || a.whole) return rc;
     const int cols = std::min(a.part_cols, a.group * a.per);
-    return launch(c, join, (unsigned)a.wgs, (unsigned)(one ? std::min(4, (cols + 3) / 4) : (cols + 15) / 16), 256, 0, st, params);
+    return launch(c, join, (unsigned)a.wgs, (unsigned)(one ? cols : (cols + 15) / 16), 256, 0, st, params);
 }
 
 namespace {

@@ -376,61 +376,58 @@ __device__ __forceinline__ float at_finish(const AttendArgs& p, u32 t, u32 head,
 
 // ---- partial sums joined ------------------------------------------------------------
 
-// grid = (wgs, up to four), block = 256: four columns at a time, a wavefront every fourth part of them.  LDS: floats [4][4][DP], [4][4].
+// grid = (wgs, columns), block = 256: a column's parts by sixteen groups of lanes.  (Four columns a workgroup, a wavefront every fourth part: 12.5 us for 7.4 where 64
+// parts a key head are joined, 7.7 for 5.6 with 8 parts of rows of 256.)  LDS: floats [4][DP], [4].
 template <int DP> __device__ __forceinline__ void attend_join_body(const AttendArgs& p, float* lds) {
     constexpr int C = DP / 16;
     const u32 w = blockIdx.x;
     const AtJoin j = at_join_of<DP>(p)[w];
     if (j.last == 0) return;
-    const u32 lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane >> 4, x = lane & 15, d0 = C * x;
-    const float inf = __builtin_inff(), off = p.c.type == JL_BF16 ? 0.f : JL_AT_OFF;
+    const u32 lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane >> 4, x = lane & 15, d0 = C * x, col = blockIdx.y;
+    u32 tok, head;
+    if (!at_column(p, j.t0, j.t1, j.plane, col, tok, head)) return;      // (the whole workgroup)
+    const float off = p.c.type == JL_BF16 ? 0.f : JL_AT_OFF;
     auto slot = [&](u32 k) { return k == w ? j.slot : 2 * k; };
-    for (u32 c0 = blockIdx.y * 4; c0 < (u32)p.part_cols; c0 += gridDim.y * 4) {
-        const u32 col = c0 + c;
-        u32 tok, head;
-        const bool live = at_column(p, j.t0, j.t1, j.plane, col, tok, head);
-        if (!__syncthreads_or(live)) return;
-        float mm = -inf, l = 0.f;
-        f32x4 y[C / 4];
+    float mm = -__builtin_inff(), l = 0.f;
+    f32x4 y[C / 4];
 #pragma unroll
-        for (int i = 0; i < C / 4; i++) y[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (live) {
-            for (u32 k = w + x; k < j.last; k += 16) mm = fmaxf(mm, (*at_part_ml<DP>(p, slot(k), col)).x);
-        }
-        mm = fmaxf(mm, dpp_f32_max<JL_DPP_QUAD_XOR1>(mm));
-        mm = fmaxf(mm, dpp_f32_max<JL_DPP_QUAD_XOR2>(mm));
-        mm = fmaxf(mm, dpp_f32_max<JL_DPP_ROW_HALF_MIRROR>(mm));
-        mm = fmaxf(mm, dpp_f32_max<JL_DPP_ROW_MIRROR>(mm));
-        if (live) {
+    for (int i = 0; i < C / 4; i++) y[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (u32 k = w + lane; k < j.last; k += 64) mm = fmaxf(mm, (*at_part_ml<DP>(p, slot(k), col)).x);
+    mm = fmaxf(mm, dpp_f32_max<JL_DPP_QUAD_XOR1>(mm));
+    mm = fmaxf(mm, dpp_f32_max<JL_DPP_QUAD_XOR2>(mm));
+    mm = fmaxf(mm, dpp_f32_max<JL_DPP_ROW_HALF_MIRROR>(mm));
+    mm = fmaxf(mm, dpp_f32_max<JL_DPP_ROW_MIRROR>(mm));
+    mm = at_max4(mm);
 #pragma unroll 4
-            for (u32 k = w + wave; k < j.last; k += 4) {
-                const f32x2 ml = *at_part_ml<DP>(p, slot(k), col);
-                const float turn = ml.x == mm ? 1.f : __builtin_amdgcn_exp2f(ml.x - mm);
-                l += ml.y * turn;
+    for (u32 k = w + 4 * wave + c; k < j.last; k += 16) {
+        const f32x2 ml = *at_part_ml<DP>(p, slot(k), col);
+        const float turn = ml.x == mm ? 1.f : __builtin_amdgcn_exp2f(ml.x - mm);
+        l += ml.y * turn;
 #pragma unroll
-                for (int i = 0; i < C / 4; i++) y[i] += *(const f32x4*)(at_part<DP>(p, slot(k), col) + d0 + 4 * i) * turn;
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < C / 4; i++) *(f32x4*)(lds + (wave * 4 + c) * DP + d0 + 4 * i) = y[i];
-        if (x == 0) lds[16 * DP + wave * 4 + c] = l;
-        __syncthreads();
-        if (wave || !live) continue;
-        float out[C];
-        l = 0.f;
-#pragma unroll
-        for (int k = 0; k < 4; k++) l += lds[16 * DP + k * 4 + c];
-#pragma unroll
-        for (int i = 0; i < C; i++) {
-            out[i] = lds[c * DP + d0 + i];
-#pragma unroll
-            for (int k = 1; k < 4; k++) out[i] += lds[(k * 4 + c) * DP + d0 + i];
-        }
-        const float inv = at_finish(p, tok, head, mm, l, off, d0 == 0);
-#pragma unroll
-        for (int i = 0; i < C; i++) out[i] *= inv;
-        if (d0 < (u32)p.c.d) at_store<C>(p, tok, head, d0, out);
+        for (int i = 0; i < C / 4; i++) y[i] += *(const f32x4*)(at_part<DP>(p, slot(k), col) + d0 + 4 * i) * turn;
     }
+    l = at_sum4(l);
+#pragma unroll
+    for (int i = 0; i < C / 4; i++) {
+#pragma unroll
+        for (int r = 0; r < 4; r++) y[i][r] = at_sum4(y[i][r]);
+        if (c == 0) *(f32x4*)(lds + wave * DP + d0 + 4 * i) = y[i];
+    }
+    if (lane == 0) lds[4 * DP + wave] = l;
+    __syncthreads();
+    if (threadIdx.x >= 16) return;
+    float out[C];
+    l = lds[4 * DP] + lds[4 * DP + 1] + lds[4 * DP + 2] + lds[4 * DP + 3];
+#pragma unroll
+    for (int i = 0; i < C; i++) {
+        out[i] = lds[d0 + i];
+#pragma unroll
+        for (int k = 1; k < 4; k++) out[i] += lds[k * DP + d0 + i];
+    }
+    const float inv = at_finish(p, tok, head, mm, l, off, d0 == 0);
+#pragma unroll
+    for (int i = 0; i < C; i++) out[i] *= inv;
+    if (d0 < (u32)p.c.d) at_store<C>(p, tok, head, d0, out);
 }
 
 // The same where a span has many columns: a wavefront four of them, over all parts.  grid = (wgs, columns / 16), block = 256.

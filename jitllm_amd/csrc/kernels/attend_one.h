@@ -3,8 +3,8 @@
 // MANY: units of several tokens.  A workgroup's wavefronts take 32 positions each of a chunk, with sums of their own that meet in LDS at a span's end.  What bounds it is
 // how many loads are on their way: a step's keys are asked for as soon as the ones before them have been multiplied, its values likewise, so a wavefront always has
 // a step of each in flight; the page numbers of 32 steps lie in its lanes.  q is asked for ahead of the rows (behind them its wait is theirs: 7.7 -> 9.4 us over 777).
-// Measured (8 key heads of 128; this kernel, then the join): 64 sequences to 8192 of 8-bit rows 119 + 5 us (4.7 TB/s), one of 131071 bf16 95 + 12 (5.6 TB/s), one
-// of 777 f16 7.7 + 4: launches and four trips to memory one after the other.
+// Measured (8 key heads of 128; this kernel, then the join): 64 sequences to 8192 of 8-bit rows 119 + 5 us (4.7 TB/s), one of 131071 bf16 97 + 7.4 (5.5 TB/s), one
+// of 777 f16 7.7 + 3.3: launches and four trips to memory one after the other.
 // Rows are read through buffer descriptors, whose bound gives zeros to the lanes behind a row that is no power of two wide.
 #pragma once
 #include "attend.h"

@@ -31,10 +31,10 @@ extern "C" __global__ __launch_bounds__(256) void jl_kv_read(KvRowsArgs p) { kv_
     JL_ATTEND_MANY(T, TYPE, 64, QP, PP, 8, 4) JL_ATTEND_MANY(T, TYPE, 128, QP, PP, 8, QP == 1 ? 4 : 2) JL_ATTEND_MANY(T, TYPE, 256, QP, PP, 8, 2)
 JL_ATTEND_Q(f16, JL_F16, 1, 2) JL_ATTEND_Q(f16, JL_F16, 2, 2) JL_ATTEND_Q(i8, JL_I8, 1, 2) JL_ATTEND_Q(i8, JL_I8, 2, 2)
 JL_ATTEND_Q(bf16, JL_BF16, 1, 2) JL_ATTEND_Q(bf16, JL_BF16, 3, 3)
-// grid = (p.wgs, up to four), block = 256
+// grid = (p.wgs, columns), block = 256; _wide: sixteen columns a workgroup
 #define JL_ATTEND_JOIN(DP)                                                                                                          \
     extern "C" __global__ __launch_bounds__(256) void jl_attend_join_d##DP(AttendArgs p) {                                          \
-        __shared__ __attribute__((aligned(16))) float lds[16 * DP + 16];                                                            \
+        __shared__ __attribute__((aligned(16))) float lds[4 * DP + 4];                                                              \
         attend_join_body<DP>(p, lds);                                                                                               \
     }
 #define JL_ATTEND_JOIN_WIDE(DP)                                                                                                     \
