@@ -38,7 +38,7 @@ struct Tuning {
     int q8pair = 0;             // Q8_0 rows: 2 keeps one block a lane-slot (2-byte-aligned loads)
     int packed_rw = 0, packed_block = 0, moe_group = 0, moe_logits = 0;
     int attend_form = 0;        // several tokens: 1 attend_one, 4 or 8 attend_many with as many wavefronts
-    int attend_whole = 0;       // attend_many: 1 a unit a workgroup, 2 equal shares of the chunks
+    int attend_whole = 0;       // 1 a unit a workgroup (attend_one: where attend_form is 1), 2 equal shares of the chunks
     int moe_select = 0, adapter_form = 0, adapter_slices = 0, adapter_sets = 0;
     int moe_shares = 0;
     int gemm_rows = 0;
@@ -3132,9 +3132,9 @@ struct AttendPlan {
     bool whole;
 };
 // Columns are a token's heads that share a key head, and those of up to as many of a sequence's tokens as there are on average (`most`).  Single tokens take attend_one;
-// for several the five ways are set against each other by what they measured (us, 16-bit rows of 128, 4 heads a key head, 8 key heads), with S the
+// for several its way and four of attend_many are set against each other by what they measured (us, 16-bit rows of 128, 4 heads a key head, 8 key heads), with S the
 // positions that a sequence can have (the table's, or the window's):
-//   attend_one: 20, and 2.5 a chunk of 128 positions that a workgroup has in turn; attend_many in shares: 32 and 2.1 a step of 64 (four wavefronts), 45 and 3.3
+//   attend_one: in shares 20, and 2.5 a chunk of 128 positions that a workgroup has in turn, units whole 6 and 3 (half of it while the chip is half empty); attend_many in shares: 32 and 2.1 a step of 64 (four wavefronts), 45 and 3.3
 //   (eight); units whole: 10 or 14, and of each round of workgroups 1.65 a step (four wavefronts; 1.8 where a CU has two), 1.85 or 2.7 (eight).
 //                          one    shares 4   shares 8   whole 4   whole 8    (sequences x tokens; shares and whole with four or eight wavefronts)
 //   8 x 5 of 2048           28       37         50        63        59
@@ -3150,6 +3150,11 @@ struct AttendPlan {
 // Rows of 256 have half of the workgroups and 1.5 (shares) or 1.8 times (whole) as long a step.  Where units straddle sequences both of a unit's spans are work.
 // Of 80 such calls what is taken is the fastest or within a tenth of it but for three (16 x 24 of 2048 takes 72 for 56).  A table far larger than what the
 // sequences hold speaks for shares: 1 x 512 of 512 takes 41 for 24 then.
+//
+// attend_one gives a workgroup a unit (no second launch) up to a number of chunks that grows with how many units there are, and shares beyond, where one sequence
+// would be waited for.  us, whole / shares, f16 rows of 128, 8 key heads, lengths evenly spread up to: 1 x 256 7.2 / 10.4, 512 9.4 / 10.4, 768 11.5 / 10.5; 32 x 256
+// 8.3 / 14.3, 768 14.4 / 21.1; 48 x 2048 50 / 54; 64 x 1024 29 / 38, 4096 112 / 111, int8 8192 144 / 126; 200 x 2048 152 / 179; 400 x 768 126 / 162; a window of 128, bf16 rows of
+// 64, 32 tokens 6.9 / 13.2; four tokens each, 32 x 500 14.4 / 30.4, 128 x 1000 61 / 97.
 AttendPlan attend_plan(const jl_ctx* c, int ntok, int n_seq, int n_kv, int group, int d, int most, int window, unsigned long long reach) {
     const double wgs = attend_wgs(c, d);
     AttendPlan best = {};
@@ -3173,7 +3178,11 @@ AttendPlan attend_plan(const jl_ctx* c, int ntok, int n_seq, int n_kv, int group
         const double seen = window ? std::min<double>(reach, (double)window + a.per) : (double)reach;
         const double steps = seen / 64 + 1, work = (double)a.units * n_kv * a.blocks * (straddles ? 1 + (double)a.per / most : 1.0);
         double us;
-        if (!a.waves) us = 20 + 2.5 * work * (steps / 2) / wgs;
+        if (!a.waves) {
+            const double chunks = std::ceil((seen + (window ? 127 : 0)) / 128), full = std::min(1.0, a.units * (double)n_kv * a.blocks / wgs);
+            a.whole = c->tune.attend_whole ? c->tune.attend_whole == 1 && c->tune.attend_form == 1 : chunks <= 3 + 32 * full * full;
+            us = a.whole ? 6 + 3 * chunks * std::max(0.5, work / wgs) : 20 + 2.5 * work * (steps / 2) / wgs;
+        }
         else if (!a.whole) us = (a.waves == 4 ? 32 : 45) + (a.waves == 4 ? 2.1 : 3.3) * (wide ? 1.5 : 1) * work * steps / wgs;
         else {
             const double alone = (a.waves == 4 ? 1.65 : 1.85) * (wide ? 1.8 : 1), shared = (a.waves == 4 ? 1.8 : 2.7) * (wide ? 1.8 : 1);

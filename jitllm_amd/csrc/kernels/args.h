@@ -674,7 +674,7 @@ struct AttendArgs {
     int part_cols;           // columns a block
     int inv_group;           // 2^16 / group + 1
     int wgs;                 // workgroups, or their shares of the chunks
-    int whole;               // a unit a workgroup (attend_many)
+    int whole;               // a unit a workgroup
     int window;
     int out_vec;             // out's rows on 16-byte boundaries
     float scale, cap;

@@ -18,7 +18,8 @@
 //
 // Two forms.  attend_one.h: up to sixteen columns, a workgroup's wavefronts take 32 positions each, bound by bytes.  attend_many.h: the wavefronts take columns each and
 // share the rows through LDS, bound by the matrix and vector units.  Work is cut in chunks of 128 positions, and the workgroups share the chunks of all
-// units and key heads evenly whatever their lengths, each a contiguous run of them; what ends up with more than one leaves partial sums that attend_join adds up.
+// units and key heads evenly whatever their lengths, each a contiguous run of them; what ends up with more than one leaves partial sums that attend_join adds up.  Where
+// units are many or short each is a workgroup's as it is, and nothing is joined.
 #pragma once
 #include "args.h"
 #include "common.h"

@@ -20,14 +20,23 @@ __device__ __forceinline__ void attend_one_body(const AttendArgs& p, float* lds,
     const float inf = __builtin_inff();
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const u32 w = at_group_of(blockIdx.x, (u32)p.wgs);
-
     AtWork job;
-    const bool any = at_work<MANY, 4>(p, w, find, job);
+    u32 unit_end = 0, w = 0;
     AtJoin join = {0, 0, 0, 0, 0, {0, 0, 0}};
-    if (!any) {
-        if (threadIdx.x == 0) at_join_of<DP>(p)[w] = join;
-        return;
+    if (p.whole) {
+        const u32 planes = (u32)p.c.n_kv * (u32)p.blocks, unit = blockIdx.x / planes;
+        job.plane = blockIdx.x - unit * planes;
+        job.off = 0;
+        job.first = 0;
+        job.end = ~0ull;
+        job.tok = unit * (u32)p.per;
+        unit_end = min(job.tok + (u32)p.per, (u32)p.ntok);
+    } else {
+        w = at_group_of(blockIdx.x, (u32)p.wgs);
+        if (!at_work<MANY, 4>(p, w, find, job)) {
+            if (threadIdx.x == 0) at_join_of<DP>(p)[w] = join;
+            return;
+        }
     }
 
     const u32 row_bytes = (u32)p.c.row_stride * B;      // (16 rows are less than 2^31 bytes)
@@ -47,7 +56,7 @@ __device__ __forceinline__ void attend_one_body(const AttendArgs& p, float* lds,
         const AtSpan span = at_span<MANY>(p, job.tok);
         const u32 lo = span.lo, hi = span.hi, plane = job.plane, c0 = job.off, n_chunks = at_chunks(lo, hi);
         job.tok = span.t1;
-        if (job.tok == (u32)p.ntok) {
+        if (!p.whole && job.tok == (u32)p.ntok) {
             job.tok = 0;
             job.plane++;
         }
@@ -337,6 +346,7 @@ __device__ __forceinline__ void attend_one_body(const AttendArgs& p, float* lds,
         }
         if (c0 == 0 && left < n_chunks) join = AtJoin{span.t0, span.t1, plane, job.share.holder(at + n_chunks - 1) + 1, 2 * w + (at == job.first ? 0u : 1u), {0, 0, 0}};
         at += left;
+        if (p.whole && span.t1 == unit_end) break;
     }
-    if (threadIdx.x == 0) at_join_of<DP>(p)[w] = join;
+    if (!p.whole && threadIdx.x == 0) at_join_of<DP>(p)[w] = join;
 }

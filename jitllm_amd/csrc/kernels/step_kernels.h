@@ -10,7 +10,7 @@ extern "C" __global__ __launch_bounds__(256) void jl_kv_write(KvRowsArgs p) { kv
 extern "C" __global__ __launch_bounds__(256) void jl_kv_read(KvRowsArgs p) { kv_rows_body<false>(p); }
 
 // _q<pieces of q>; over a bf16 cache one piece of q goes with two of the weights (a 16-bit result), three with three
-// grid = p.wgs, block = 256; _m: units of several tokens
+// grid = p.wgs, or p.units * planes where p.whole; block = 256; _m: units of several tokens
 #define JL_ATTEND_ONE_M(T, TYPE, DP, QP, PP, NAME, MANY)                                                                            \
     extern "C" __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void jl_attend_one_##T##_d##DP##_q##QP##NAME(AttendArgs p) {    \
         __shared__ __attribute__((aligned(16))) float lds[4 * 16 * (DP + 4) + 128];                                                 \

@@ -492,3 +492,19 @@ def test_thousands_of_tokens(dev, form):
     many = rng.integers(0, 38, 3000)
     attend(dev, quant.I8, [37], np.zeros(3000, int), many, 1, 1, 16)
     attend(dev, quant.BF16, lens * 700, None, np.array(lens * 700) // 20, 1, 2, 16, window=9)
+
+
+@pytest.mark.parametrize("t", KINDS)
+@pytest.mark.parametrize("whole", [1, 2])
+@pytest.mark.parametrize("d, group", [(64, 8), (128, 4), (256, 2), (80, 20)])
+def test_few_tokens_in_both_divisions(dev, t, whole, d, group):
+    """A unit a workgroup, and shares that are joined, for single tokens and for a few of a sequence, whichever would be taken for them."""
+    dev.set_tuning(attend__form=1, attend__whole=whole)
+    try:
+        for ot in PLAIN:
+            lens = [1, 37, 0, 300, 1500]
+            attend(dev, t, [max(n, 1) for n in lens], None, lens, 2, group, d, quant.BF16, ot, sinks=ot == quant.F16, window=200 if ot == quant.BF16 else 0)
+        lens = [3, 200, 700]
+        attend(dev, t, lens, np.repeat(np.arange(3), 3), np.concatenate([np.arange(n - 3, n) + 1 for n in lens]), 2, group, d)
+    finally:
+        dev.set_tuning(attend__form=0, attend__whole=0)
