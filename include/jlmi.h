@@ -585,7 +585,7 @@ int jl_matmul_mxfp4_packed_bf16_dev(jl_ctx *ctx, float *out, const uint32_t *qs,
 
 /* ---- between a block's projections, and behind the last one (device pointers) ---------------------------------------- */
 
-/* A paged cache of keys and values.  Rows of d elements of `type`: JL_TYPE_F16, JL_TYPE_BF16, or JL_TYPE_I8 with one f32 scale a row.  k and v are pools of
+/* A paged cache of keys and values.  Rows of d elements of `type`: JL_TYPE_F16, JL_TYPE_BF16, or JL_TYPE_I8 with one f32 scale a row, of either sign.  k and v are pools of
  * n_page pages of page_size positions (a power of two, 16 or more; one page a sequence makes a contiguous cache):
  *     row of page p, head h, place s:   p * page_stride + h * head_stride + s * row_stride    elements from k (v) on
  *     its scale:                        k_scale[(p * n_kv + h) * page_size + s]

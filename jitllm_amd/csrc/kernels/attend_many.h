@@ -269,7 +269,8 @@ __device__ __forceinline__ void attend_many_body(const AttendArgs& p, u32x4* lds
                     for (int i = 0; i < 4; i++) {
                         sco[i] *= *(const f32x4*)(scales + (s & 1) * 128 + 16 * i + 4 * g);
                         vs[i] = *(const f32x4*)(scales + (s & 1) * 128 + 64 + 16 * i + 4 * g);
-                        big = fmaxf(fmaxf(fmaxf(vs[i][0], vs[i][1]), fmaxf(vs[i][2], vs[i][3])), big);
+#pragma unroll
+                        for (int r = 0; r < 4; r++) big = fmaxf(big, fabsf(vs[i][r]));      // (a scale may be of either sign)
                     }
                     big = at_max4(big);
                     const int to = __builtin_amdgcn_readfirstlane(big > 0.f ? __builtin_amdgcn_frexp_expf(big) : -200);

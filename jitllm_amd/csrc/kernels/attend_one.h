@@ -229,7 +229,9 @@ __device__ __forceinline__ void attend_one_body(const AttendArgs& p, float* lds,
                 m = top;
             }
             if constexpr (I8) {   // the running power of two over the values' scales
-                float big = fmaxf(fmaxf(fmaxf(vs[0][0], vs[0][1]), fmaxf(vs[0][2], vs[0][3])), fmaxf(fmaxf(vs[1][0], vs[1][1]), fmaxf(vs[1][2], vs[1][3])));
+                float big = 0.f;      // (a scale may be of either sign)
+#pragma unroll
+                for (int j = 0; j < 8; j++) big = fmaxf(big, fabsf(vs[j / 4][j % 4]));
                 big = at_max4(big);
                 const int to = __builtin_amdgcn_readfirstlane(big > 0.f ? __builtin_amdgcn_frexp_expf(big) : -200);
                 if (to > ve) {

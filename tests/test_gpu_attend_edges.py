@@ -1,0 +1,41 @@
+"""Attention over a paged cache (jl_attend_dev) at the ends of what a cache and a call may hold, against the definition and the bars of test_gpu_attend."""
+import numpy as np
+import pytest
+
+from jitllm_amd import quant
+from test_gpu_attend import check, reference, run
+from test_gpu_kv_cache import Cache, table_of
+
+pytestmark = pytest.mark.gpu
+
+WAYS = [dict(attend__form=f, attend__whole=w) for f in (1, 4, 8) for w in (1, 2)]
+
+
+@pytest.fixture(params=WAYS, ids=lambda w: " ".join(f"{k[8:]} {v}" for k, v in w.items()))
+def way(dev, request):
+    """Each form, in units and in shares."""
+    dev.set_tuning(**request.param)
+    yield request.param
+    dev.set_tuning(attend__form=0, attend__whole=0)
+
+
+def causal(lens, per):
+    """The last `per` tokens of each sequence: their sequences, and the positions that they see."""
+    return np.repeat(np.arange(len(lens)), per), np.concatenate([np.arange(n - per, n) + 1 for n in lens])
+
+
+@pytest.mark.parametrize("signs", ["negative", "mixed", "largest negative"])
+@pytest.mark.parametrize("per, group, d", [(1, 4, 64), (3, 2, 128), (40, 2, 64), (24, 4, 256)])
+def test_scales_of_either_sign(dev, way, signs, per, group, d):
+    """A row of 8-bit values is its scale times them, whatever the scale's sign."""
+    rng = np.random.default_rng(60 + per)
+    lens = [per, per + 20, per + 300]
+    table, n_page = table_of(rng, lens, 16)
+    c = Cache(quant.I8, 2, d, 16, table, n_page)
+    sign = lambda s: -np.ones(s.shape) if signs == "negative" else rng.choice([-1.0, 1.0], s.shape) if signs == "mixed" else np.where(s > 0.015, -40.0, 1.0)
+    c.ks, c.vs = (c.ks * np.sign(sign(c.ks))).astype(np.float32), (c.vs * sign(c.vs)).astype(np.float32)
+    c.upload()
+    seq, length = causal(lens, per)
+    q = rng.standard_normal((len(seq), 2 * group, d)).astype(np.float32)
+    got, lse = run(dev, c, q, quant.F32, quant.F32, seq, length, 0.125)
+    check(got, lse, reference(c, q, seq, length, 0.125), quant.F32)
