@@ -629,7 +629,8 @@ int jl_kv_read_dev(jl_ctx *ctx, const jl_kv_cache *cache, const jl_kv_rows *rows
  *     lse = ln of that denominator                                   lse null: not wanted
  * q [ntok][q_stride] of q_type, out [ntok][out_stride] of out_type (JL_TYPE_F32, _F16, _BF16; strides in elements, 0: n_head * d), lse [ntok][n_head] f32.
  * A token that sees nothing (len 0, no such sequence, no pages) has zeros, lse -infinity or its sink.  len counts at most the table's positions.  Sums are f32, and q and the weights
- * keep 22 bits or more (16 of the weights over a bf16 cache where out is 16 bits wide); a token's result does not depend on the other tokens of the call but in the last bits, by
+ * keep 22 bits or more (16 of the weights over a bf16 cache where out is 16 bits wide; over f16 rows down to 2^-38 of the largest weight, over 8-bit rows weight times scale
+ * down to 2^-38 of the largest weight times the largest scale that the token sees); a token's result does not depend on the other tokens of the call but in the last bits, by
  * where the cache was cut among the workgroups.  Infinities and NaNs in rows that a token does not see change nothing of its result.
  * Tokens of one sequence share the reads of its rows where they follow each other; how many of them are put together goes by ntok / n_seq, so a call over a few
  * of many sequences gives the rows of the table that it needs.  q 16-byte aligned, its stride a multiple of 16 bytes; n_head a multiple of n_kv.  out overlaps no

@@ -13,7 +13,7 @@
 //     turns them into the c fragments of eight positions each by byte permutes: fragment j holds d = c n + j.
 //   A column's m, sum and O stay in the four lanes of its n: the running maximum is two lane swaps, rescaling is in-lane.
 //
-// Precision: K and V are exact in the instruction's type (8-bit rows as f16 integers, their scale applied to S, and to P relative to a running power of two); q and
+// Precision: K and V are exact in the instruction's type (8-bit rows as f16 integers, their scale applied to S, and to P relative to a running power of two over the scales that the column sees); q and
 // P are split into pieces that hold 22 (f16) or 24 and 16 or 24 (bf16) bits, so what rounds is the f32 sums, as in a plain product in f32.
 //
 // Two forms.  attend_one.h: up to sixteen columns, a workgroup's wavefronts take 32 positions each, bound by bytes.  attend_many.h: the wavefronts take columns each and

@@ -232,7 +232,7 @@ __device__ __forceinline__ void attend_many_body(const AttendArgs& p, u32x4* lds
         for (;;) {
         f32x4 acc[C];
         float m = -inf, l = 0.f;
-        int ve = -200;          // 8-bit rows: acc is times 2^-ve
+        int ve = -200;          // 8-bit rows: the column's acc is times 2^-ve
 #pragma unroll
         for (int j = 0; j < C; j++) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
@@ -264,27 +264,14 @@ __device__ __forceinline__ void attend_many_body(const AttendArgs& p, u32x4* lds
                 }
                 f32x4 vs[4];
                 if constexpr (I8) {
-                    float big = 0.f;
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         sco[i] *= *(const f32x4*)(scales + (s & 1) * 128 + 16 * i + 4 * g);
                         vs[i] = *(const f32x4*)(scales + (s & 1) * 128 + 64 + 16 * i + 4 * g);
-#pragma unroll
-                        for (int r = 0; r < 4; r++) big = fmaxf(big, fabsf(vs[i][r]));      // (a scale may be of either sign)
-                    }
-                    big = at_max4(big);
-                    const int to = __builtin_amdgcn_readfirstlane(big > 0.f ? __builtin_amdgcn_frexp_expf(big) : -200);
-                    if (to > ve) {
-#pragma unroll
-                        for (int j = 0; j < C; j++)
-#pragma unroll
-                            for (int r = 0; r < 4; r++) acc[j][r] = __builtin_amdgcn_ldexpf(acc[j][r], ve - to);
-                        ve = to;
                     }
                 }
                 u32x4 vt[3] = {vin[0], vin[C * 64], {0, 0, 0, 0}}, pf[2][PP];
                 float y[16], by = qs;       // scores are y by
-                u32 hidden = 0;
 #pragma unroll
                 for (int j = 0; j < 16; j++) y[j] = sco[j / 4][j % 4];
                 if (edge || p.cap != 0.f) {
@@ -299,7 +286,21 @@ __device__ __forceinline__ void attend_many_body(const AttendArgs& p, u32x4* lds
                         const u32 at0 = p0 + 16 * (j / 4) + 4 * g + j % 4;
                         const bool sees = !(none >> (j / 4) & 1) && at0 >= clo && at0 < chi;
                         y[j] = sees ? y[j] : -inf;
-                        if (I8 && !sees) hidden |= 1u << j;
+                        if constexpr (I8) vs[j / 4][j % 4] = sees ? vs[j / 4][j % 4] : 0.f;      // (this column's: others may see it)
+                    }
+                }
+                if constexpr (I8) {   // the running power of two over the scales of the values that the column sees
+                    float big = 0.f;      // (a scale may be of either sign)
+#pragma unroll
+                    for (int j = 0; j < 16; j++) big = fmaxf(big, fabsf(vs[j / 4][j % 4]));
+                    big = at_max4(big);
+                    const int to = max(ve, big > 0.f ? __builtin_amdgcn_frexp_expf(big) : -200);
+                    if (__ballot(to > ve)) {
+#pragma unroll
+                        for (int j = 0; j < C; j++)
+#pragma unroll
+                            for (int r = 0; r < 4; r++) acc[j][r] = __builtin_amdgcn_ldexpf(acc[j][r], ve - to);
+                        ve = to;
                     }
                 }
                 float top = y[0];
@@ -319,7 +320,7 @@ __device__ __forceinline__ void attend_many_body(const AttendArgs& p, u32x4* lds
                 for (int j = 0; j < 16; j++) {
                     y[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(y[j], by, from));
                     sums[j / 4] = j % 4 ? sums[j / 4] + y[j] : y[j];
-                    if constexpr (I8) y[j] = hidden >> j & 1 ? 0.f : y[j] * __builtin_amdgcn_ldexpf(vs[j / 4][j % 4], -ve);   // (a scale others see may be no number)
+                    if constexpr (I8) y[j] *= __builtin_amdgcn_ldexpf(vs[j / 4][j % 4], -ve);
                 }
                 l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
 #pragma unroll

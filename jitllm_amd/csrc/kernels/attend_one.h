@@ -146,7 +146,7 @@ __device__ __forceinline__ void attend_one_body(const AttendArgs& p, float* lds,
 
         f32x4 acc[C];
         float m = -inf, l = 0.f;
-        int ve = -200;          // 8-bit rows: acc is times 2^-ve
+        int ve = -200;          // 8-bit rows: the column's acc is times 2^-ve
 #pragma unroll
         for (int j = 0; j < C; j++) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
@@ -188,7 +188,6 @@ __device__ __forceinline__ void attend_one_body(const AttendArgs& p, float* lds,
                 y[j] = s[j / 4][j % 4];
                 if constexpr (I8) y[j] *= kx[j / 4][j % 4];
             }
-            u32 hidden = 0;
             const bool masks = edge || (MANY && only != ~0u);
             if (masks || p.cap != 0.f) {
                 by = 1.f;
@@ -204,10 +203,9 @@ __device__ __forceinline__ void attend_one_body(const AttendArgs& p, float* lds,
                         const u32 at0 = p0 + 16 * (j / 4) + 4 * g + j % 4;
                         const bool held = seen[j / 4] < p.c.n_page, sees = held && at0 >= clo && at0 < chi, one = MANY ? held && at0 >= zlo && at0 < zhi : sees;
                         y[j] = sees ? y[j] : -inf;
-                        if (MANY && !sees) hidden |= 1u << j;
 #pragma unroll
                         for (int e2 = 0; e2 < VW; e2++) vw[j][e2] = one ? vw[j][e2] : 0u;
-                        if constexpr (I8) vs[j / 4][j % 4] = one ? vs[j / 4][j % 4] : 0.f;
+                        if constexpr (I8) vs[j / 4][j % 4] = sees ? vs[j / 4][j % 4] : 0.f;      // (this column's: others may see it)
                     }
                 }
             }
@@ -228,13 +226,13 @@ __device__ __forceinline__ void attend_one_body(const AttendArgs& p, float* lds,
                 for (int j = 0; j < C; j++) acc[j] *= turn;
                 m = top;
             }
-            if constexpr (I8) {   // the running power of two over the values' scales
+            if constexpr (I8) {   // the running power of two over the scales of the values that the column sees
                 float big = 0.f;      // (a scale may be of either sign)
 #pragma unroll
                 for (int j = 0; j < 8; j++) big = fmaxf(big, fabsf(vs[j / 4][j % 4]));
                 big = at_max4(big);
-                const int to = __builtin_amdgcn_readfirstlane(big > 0.f ? __builtin_amdgcn_frexp_expf(big) : -200);
-                if (to > ve) {
+                const int to = max(ve, big > 0.f ? __builtin_amdgcn_frexp_expf(big) : -200);
+                if (__ballot(to > ve)) {
 #pragma unroll
                     for (int j = 0; j < C; j++)
 #pragma unroll
@@ -247,7 +245,7 @@ __device__ __forceinline__ void attend_one_body(const AttendArgs& p, float* lds,
             for (int j = 0; j < 8; j++) {
                 y[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(y[j], by, from));
                 l += y[j];
-                if constexpr (I8) y[j] = MANY && (hidden >> j & 1) ? 0.f : y[j] * __builtin_amdgcn_ldexpf(vs[j / 4][j % 4], -ve);   // (a scale others see may be no number)
+                if constexpr (I8) y[j] *= __builtin_amdgcn_ldexpf(vs[j / 4][j % 4], -ve);
             }
             u32x4 pf[PP];
 #pragma unroll

@@ -39,3 +39,29 @@ def test_scales_of_either_sign(dev, way, signs, per, group, d):
     q = rng.standard_normal((len(seq), 2 * group, d)).astype(np.float32)
     got, lse = run(dev, c, q, quant.F32, quant.F32, seq, length, 0.125)
     check(got, lse, reference(c, q, seq, length, 0.125), quant.F32)
+
+
+@pytest.mark.parametrize("per, group, d", [(3, 2, 128), (16, 1, 64), (40, 2, 64), (24, 4, 256)])
+@pytest.mark.parametrize("size", [2.0 ** 20, 2.0 ** 40, np.inf])
+def test_a_scale_that_only_a_later_token_sees(dev, way, size, per, group, d):
+    """The 8-bit row of a unit's last token may be larger than all others by any factor: the tokens before it, which do not see it, keep their bits."""
+    rng = np.random.default_rng(70 + per)
+    lens = [per, per + 20, per + 300]
+    table, n_page = table_of(rng, lens, 16)
+    c = Cache(quant.I8, 2, d, 16, table, n_page)
+    c.vs = (c.vs * np.float32(2.0 ** -30)).astype(np.float32)
+    for s, n in enumerate(lens):
+        page, at = c.place(s, n - 1)
+        c.vs[page, :, at] *= np.float32(size)
+    c.upload()
+    seq, length = causal(lens, per)
+    q = rng.standard_normal((len(seq), 2 * group, d)).astype(np.float32)
+    got, lse = run(dev, c, q, quant.F32, quant.F32, seq, length, 0.125)
+    last = length == np.array(lens)[seq]
+    with np.errstate(invalid="ignore"):
+        ref = reference(c, q, seq, length, 0.125)
+    check(got[~last], lse[~last], [a[~last] for a in ref], quant.F32)
+    if np.isinf(size):
+        assert np.all(np.isnan(got[last]) | np.isinf(got[last]))
+    else:
+        check(got[last], lse[last], [a[last] for a in ref], quant.F32)
