@@ -589,7 +589,9 @@ int jl_matmul_mxfp4_packed_bf16_dev(jl_ctx *ctx, float *out, const uint32_t *qs,
  * n_page pages of page_size positions (a power of two, 16 or more; one page a sequence makes a contiguous cache):
  *     row of page p, head h, place s:   p * page_stride + h * head_stride + s * row_stride    elements from k (v) on
  *     its scale:                        k_scale[(p * n_kv + h) * page_size + s]
- * (strides 0: back to back, [n_page][n_kv][page_size][d]; other orders by their strides, e.g. row_stride n_kv * d, head_stride d).  Position i of sequence s
+ * (strides 0: back to back, [n_page][n_kv][page_size][d]; other orders by their strides, e.g. row_stride n_kv * d, head_stride d for
+ * [n_page][page_size][n_kv][d]: page_stride 0 is the larger of n_kv * head_stride and page_size * row_stride.  No two rows may share elements: a stride is at least what the
+ * smaller ones span).  Position i of sequence s
  * lies on page table[s * table_stride + i / page_size], in place i modulo page_size; table is device memory, n_seq rows of table_pages entries
  * (table_stride 0: table_pages).  An entry of n_page or more is no page: what lies there is written nowhere, read as zeros, and seen by no one.
  * d a multiple of 16 up to 256; strides multiples of 16; k, v and the scales 16-byte aligned; table_pages * page_size up to 2^31.  Offsets are 64 bits wide.

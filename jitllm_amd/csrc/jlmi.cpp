@@ -3079,9 +3079,18 @@ int kv_view(jl_ctx* c, const jl_kv_cache* g, const char* what, KvArgs* a) {
     a->shift = __builtin_ctz((unsigned)g->page_size);
     a->row_stride = g->row_stride ? g->row_stride : (size_t)g->d;
     a->head_stride = g->head_stride ? g->head_stride : a->row_stride * g->page_size;
-    a->page_stride = g->page_stride ? g->page_stride : a->head_stride * g->n_kv;
+    a->page_stride = g->page_stride ? g->page_stride : std::max(a->head_stride * g->n_kv, a->row_stride * g->page_size);   // (whichever of the two is outer)
     if (a->row_stride < (size_t)g->d || a->head_stride < (size_t)g->d || a->page_stride < (size_t)g->d)
         return fail(c, JL_ERR_ARG, "%s: a stride is shorter than a row", what);
+    // No two rows share elements: in whatever order pages, heads and places lie, each stride is at least what the smaller ones span.
+    std::pair<size_t, int> dims[3] = {{a->row_stride, g->page_size}, {a->head_stride, g->n_kv}, {a->page_stride, g->n_page}};
+    std::sort(dims, dims + 3);
+    unsigned __int128 span = (unsigned)g->d;
+    for (const auto& [stride, count] : dims) {
+        if (count == 1) continue;
+        if (stride < span) return fail(c, JL_ERR_ARG, "%s: rows overlap by their strides (page %zu, head %zu, row %zu)", what, a->page_stride, a->head_stride, a->row_stride);
+        span += (unsigned __int128)stride * (unsigned)(count - 1);
+    }
     if (((a->row_stride | a->head_stride | a->page_stride) & 15) || a->row_stride >= 1u << 25) return JL_DECLINED;   // (sixteen rows: 32-bit offsets)
     if (!aligned16(g->k) || !aligned16(g->v) || !aligned16(g->k_scale) || !aligned16(g->v_scale) || ((uintptr_t)g->table & 3)) return JL_DECLINED;
     a->k = g->k; a->v = g->v; a->k_scale = g->k_scale; a->v_scale = g->v_scale; a->table = g->table;
