@@ -124,7 +124,7 @@ int jl_synchronize(jl_ctx *ctx);
  * a workgroup), "mxfp4.planes" (3 / 4: 64-token tiles of 64 / 96
  * rows over planes, rows turned into planes first; packed MXFP4: 2 restores rows first,
  * 64 / 32 / 16 rows a workgroup of the plane matvec), "attend.form" (calls of several tokens a sequence: 1 wavefronts
- * that share the positions, 4 or 8 so many that share the columns), "attend.whole" (1 a unit of tokens a workgroup,
+ * that share the positions, 4 or 8 so many that share the columns; another value is refused), "attend.whole" (1 a unit of tokens a workgroup,
  * of the first form only where it is asked for; 2 equal shares of the positions); value 0 restores the built-in choice.  These change launch shapes and f32 summation
  * order only.  Two keys change values, both off unless set: "mxfp4.scaled" = 1 runs
  * jl_matmul_mxfp4_packed_bf16_dev on the block-scaled fp8 x fp4 matrix instruction, which

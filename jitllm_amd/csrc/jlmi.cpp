@@ -2441,7 +2441,10 @@ int jl_set_tuning(jl_ctx* c, const char* key, int value) {
     else if (!strcmp(key, "matvec.grid")) c->tune.grid = value;
     else if (!strcmp(key, "packed.rw")) c->tune.packed_rw = value;
     else if (!strcmp(key, "packed.block")) c->tune.packed_block = value;
-    else if (!strcmp(key, "attend.form")) c->tune.attend_form = value;
+    else if (!strcmp(key, "attend.form")) {
+        if (value != 0 && value != 1 && value != 4 && value != 8) return fail(c, JL_ERR_ARG, "attend.form is 0, 1, 4 or 8, not %d", value);
+        c->tune.attend_form = value;
+    }
     else if (!strcmp(key, "attend.whole")) c->tune.attend_whole = value;
     else if (!strcmp(key, "moe.select")) c->tune.moe_select = value;
     else if (!strcmp(key, "adapter.form")) c->tune.adapter_form = value;
