@@ -183,7 +183,7 @@ __device__ __forceinline__ SampleSet sample_set(const SampleArgs& p, size_t row)
     s.first = (u32)__builtin_amdgcn_readlane((i32)at, (int)__builtin_ctzll(__ballot(top == s.best)));   // the first slice that has it
     s.greedy = s.best == 0 || !(t > 0.f) || s.low > 1.f;      // (nothing reaches a min_p above one: the first is left)
     s.r.max = sample_value(s.best);
-    s.r.a = 1.4426950408889634074 / (double)t;
+    s.r.a = fmax(1.4426950408889634074 / (double)t, 0x1p-200);      // (not 0: at an infinite temperature an infinite distance still weighs nothing, finite ones 1)
     s.r.fine = fminf(64.f / t, 1e30f);
     s.k = k < s.valid ? k : 0u;
     s.nucleus = s.p < 1.f;

@@ -1,0 +1,24 @@
+"""Sampling (jl_sample_dev) where a row's values and settings are both at an end of their range, against the definition."""
+import numpy as np
+import pytest
+
+from jitllm_amd import quant
+from test_gpu_sample import logits, run
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("settings", [dict(), dict(top_k=2), dict(top_k=40), dict(top_p=0.5), dict(min_p=0.3), dict(top_k=5, top_p=0.9, min_p=0.1)], ids=str)
+@pytest.mark.parametrize("n", [70, 5001])
+def test_infinities_at_an_infinite_temperature(dev, n, settings):
+    """An infinity is larger than the rest at every temperature and shares with its equals: of three, by thirds (of two where the first two are asked for or reach the half)."""
+    rng = np.random.default_rng(n)
+    at = [5, 33, n - 2]
+    u = np.array([0.0, 0.2, 0.4, 0.6, 0.9, 0.9999999], np.float32)
+    x = logits(rng, len(u), n)
+    x[:, at] = np.inf
+    for temperature in (np.inf, 3e38, 1.0, 1e-45):
+        token, prob = run(dev, x, quant.F32, u, temperature=np.float32(temperature), **settings)
+        share = 2 if settings.get("top_k") == 2 or settings.get("top_p") == 0.5 else 3
+        assert list(token) == [at[min(int(v * share), share - 1)] for v in u.astype(np.float64)], temperature
+        assert np.array_equal(prob, np.full(len(u), np.float32(1.0 / share)))
