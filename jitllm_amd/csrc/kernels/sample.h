@@ -71,7 +71,7 @@ struct SampleRow {
         return low > 0.f && !(w >= (double)low) ? 0 : rounded(w);
     }
     __device__ u32 bin(float x) const {          // falls as x rises
-        const float d = (max - x) * fine;        // (infinities apart: NaN or infinite)
+        const float d = __builtin_fmaf(x, -0.5f, 0.5f * max) * (2.f * fine);        // (by halves: max - x may be beyond f32; infinities apart: NaN or infinite)
         return x == max ? 0u : d < (float)(JL_SA_BINS - 1) ? (u32)d : (u32)JL_SA_BINS - 1u;
     }
 };

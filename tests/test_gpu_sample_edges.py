@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 from jitllm_amd import quant
-from test_gpu_sample import logits, run
+from test_gpu_sample import check, logits, run
 
 pytestmark = pytest.mark.gpu
 
@@ -22,3 +22,14 @@ def test_infinities_at_an_infinite_temperature(dev, n, settings):
         share = 2 if settings.get("top_k") == 2 or settings.get("top_p") == 0.5 else 3
         assert list(token) == [at[min(int(v * share), share - 1)] for v in u.astype(np.float64)], temperature
         assert np.array_equal(prob, np.full(len(u), np.float32(1.0 / share)))
+
+
+@pytest.mark.parametrize("settings", [dict(), dict(top_k=7), dict(top_p=0.6), dict(top_p=0.9), dict(min_p=0.3), dict(top_k=30, top_p=0.8), dict(top_p=0.7, min_p=0.05)], ids=str)
+@pytest.mark.parametrize("n", [70, 5001])
+@pytest.mark.parametrize("temperature", [1e38, 3e38, np.inf])
+def test_distances_beyond_the_type(dev, n, temperature, settings):
+    """Values at both ends of f32 and a temperature as large: the distance of two is no f32 number, its part of the temperature is a few."""
+    rng = np.random.default_rng(n + 1)
+    x = (3.3e38 * rng.uniform(-1, 1, (6, n))).astype(np.float32)
+    x[:, :2] = [3.3e38, -3.3e38]
+    check(dev, x, quant.F32, rng.random(6).astype(np.float32), temperature=np.float32(temperature), **settings)
