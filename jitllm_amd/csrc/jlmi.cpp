@@ -3135,7 +3135,7 @@ namespace {
 // Workgroups of an attention call: what the chip holds at once (two of four wavefronts a CU, by registers and LDS; one for rows above 128).
 int attend_wgs(const jl_ctx* c, int d) { return (d > 128 ? 1 : 2) * c->num_cu; }
 int attend_row(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
-size_t attend_part_bytes(int wgs, int d, int cols) { return (size_t)wgs * (2 * (size_t)cols * (attend_row(d) + 2) * 4 + 32); }   // (AtJoin: 32 bytes)
+size_t attend_part_bytes(int wgs, int d) { return (size_t)wgs * (2 * (size_t)128 * (attend_row(d) + 2) * 4 + 32); }   // (128 columns: whatever form comes next; AtJoin: 32 bytes)
 
 // How the tokens of a call are put together and divided.
 struct AttendPlan {
@@ -3217,7 +3217,7 @@ int jl_reserve_attend(jl_ctx* c, int max_d) {
     if (max_d <= 0) return fail(c, JL_ERR_ARG, "reserve attend: rows of %d", max_d);
     if (max_d > 256) return JL_DECLINED;
     HIP_TRY(c, H->SetDevice(c->device));
-    return attend_ws_ensure(c, attend_part_bytes(attend_wgs(c, 128), std::min(max_d, 128), 128));   // (rows above 128: half the workgroups)
+    return attend_ws_ensure(c, attend_part_bytes(attend_wgs(c, 128), std::min(max_d, 128)));   // (rows above 128: half the workgroups)
 }
 
 int jl_attend_dev(jl_ctx* c, const jl_kv_cache* cache, const jl_attend* g, void* stream) {
@@ -3255,7 +3255,7 @@ int jl_attend_dev(jl_ctx* c, const jl_kv_cache* cache, const jl_attend* g, void*
     a.wgs = (int)std::min<unsigned long long>(attend_wgs(c, cache->d), g->ntok * planes * per_head);
     if (a.units * planes > 0xffffffffull / 512) return JL_DECLINED;   // threads a launch can have
     HIP_TRY(c, H->SetDevice(c->device));
-    rc = a.whole ? JL_OK : attend_ws_ensure(c, attend_part_bytes(a.wgs, cache->d, a.part_cols));
+    rc = a.whole ? JL_OK : attend_ws_ensure(c, attend_part_bytes(attend_wgs(c, cache->d), cache->d));
     if (rc != JL_OK) return rc;
     a.part = (float*)c->attend_ws;
     Name name, join;

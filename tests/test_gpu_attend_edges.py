@@ -3,6 +3,8 @@ import numpy as np
 import pytest
 
 from jitllm_amd import quant
+from jitllm_amd.device import Device
+from jitllm_amd.hipmem import DeviceArray, mem_info
 from test_gpu_attend import check, reference, run
 from test_gpu_kv_cache import Cache, table_of
 
@@ -65,3 +67,24 @@ def test_a_scale_that_only_a_later_token_sees(dev, way, size, per, group, d):
         assert np.all(np.isnan(got[last]) | np.isinf(got[last]))
     else:
         check(got[last], lse[last], [a[last] for a in ref], quant.F32)
+
+
+def test_a_workspace_of_one_size_for_a_row_width():
+    """The first call that divides positions among the workgroups sizes the workspace for every other over rows of that width."""
+    with Device(device=0) as d:
+        table, n_page = table_of(np.random.default_rng(1), [3000] * 4, 64)
+        c = Cache(quant.F16, 4, 128, 64, table, n_page)
+        q, out = DeviceArray(np.ones((2000, 16, 128), np.float32)), DeviceArray(np.zeros((2000, 16, 128), np.float32))
+        seq, ld = DeviceArray(np.repeat(np.arange(4, dtype=np.uint32), 500)), DeviceArray(np.full(2000, 3000, np.uint32))
+        h = c.handle(d)
+        call = lambda ntok: d.attend_dev(h, out.ptr, q.ptr, 16, ld.ptr, ntok, 0.1, seq=seq.ptr)
+        d.set_tuning(attend__form=1, attend__whole=2)
+        assert call(1)
+        d.synchronize()
+        before = mem_info()[0]
+        for form in (1, 4, 8):
+            d.set_tuning(attend__form=form)
+            for ntok in (4, 100, 2000):
+                assert call(ntok)
+        d.synchronize()
+        assert mem_info()[0] == before
