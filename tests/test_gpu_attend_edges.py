@@ -6,7 +6,7 @@ from jitllm_amd import quant
 from jitllm_amd.device import Device
 from jitllm_amd.hipmem import DeviceArray, mem_info
 from test_gpu_attend import check, reference, run
-from test_gpu_kv_cache import Cache, table_of
+from test_gpu_kv_cache import KINDS, Cache, table_of
 
 pytestmark = pytest.mark.gpu
 
@@ -88,3 +88,55 @@ def test_a_workspace_of_one_size_for_a_row_width():
                 assert call(ntok)
         d.synchronize()
         assert mem_info()[0] == before
+
+
+@pytest.mark.parametrize("t", KINDS)
+@pytest.mark.parametrize("scale, cap", [(-0.125, 0.0), (-0.125, 20.0), (0.0, 0.0), (-0.0, 5.0), (-1e-30, 0.0)])
+def test_scales_of_the_scores(dev, way, t, scale, cap):
+    """Below zero: the smallest product has the most weight.  Zero: every position the same."""
+    rng = np.random.default_rng(80)
+    for per, group, d in ((1, 4, 64), (3, 2, 128), (40, 2, 64)):
+        lens = [per, per + 20, per + 300]
+        table, n_page = table_of(rng, lens, 16)
+        c = Cache(t, 2, d, 16, table, n_page)
+        seq, length = causal(lens, per)
+        q = rng.standard_normal((len(seq), 2 * group, d)).astype(np.float32)
+        got, lse = run(dev, c, q, quant.F32, quant.F32, seq, length, scale, cap=cap)
+        check(got, lse, reference(c, q, seq, length, scale, cap=cap), quant.F32)
+
+
+@pytest.mark.parametrize("t", KINDS)
+@pytest.mark.parametrize("pages", [3, 4000])
+def test_tables_longer_than_their_sequences(dev, t, pages):
+    """A table sized for far more positions than its sequences have, its rows apart: what lies behind a sequence's pages is no page, and what lies between the rows is not read."""
+    rng = np.random.default_rng(81)
+    for per, group, d in ((1, 4, 128), (3, 2, 64), (40, 2, 128), (300, 1, 64)):
+        lens = [per, per + 20, per + 300]
+        table, n_page = table_of(rng, lens, 16)
+        c = Cache(t, 2, d, 16, np.concatenate([table, np.full((3, pages), n_page, np.uint32)], 1), n_page)
+        wide = np.concatenate([c.table, np.zeros((3, 5), np.uint32)], 1)      # (page 0: read, it would be seen)
+        c.td = DeviceArray(wide)
+        make = c.handle
+        c.handle = lambda dev: make(dev, table_stride=wide.shape[1])
+        seq, length = causal(lens, per)
+        q = rng.standard_normal((len(seq), 2 * group, d)).astype(np.float32)
+        got, lse = run(dev, c, q, quant.F32, quant.F32, seq, length, 0.125)
+        check(got, lse, reference(c, q, seq, length, 0.125), quant.F32)
+        length[per - 1::per] = 0xFFFFFFFF          # behind the table: all that it holds
+        got, lse = run(dev, c, q, quant.F32, quant.F32, seq, length, 0.125)
+        check(got, lse, reference(c, q, seq, length, 0.125), quant.F32)
+
+
+@pytest.mark.parametrize("t", KINDS)
+def test_a_prompt_and_single_tokens_in_one_call(dev, way, t):
+    """One sequence's prompt between the next tokens of twenty others."""
+    rng = np.random.default_rng(82)
+    lens = [int(v) for v in rng.integers(1, 400, 21)]
+    lens[7] = 500
+    seq = np.concatenate([np.arange(7), np.full(120, 7), np.arange(8, 21)])
+    length = np.concatenate([lens[:7], np.arange(380, 500) + 1, lens[8:]])
+    table, n_page = table_of(rng, lens, 32)
+    c = Cache(t, 2, 64, 32, table, n_page)
+    q = rng.standard_normal((len(seq), 8, 64)).astype(np.float32)
+    got, lse = run(dev, c, q, quant.F32, quant.F32, seq, length, 0.125)
+    check(got, lse, reference(c, q, seq, length, 0.125), quant.F32)
