@@ -189,7 +189,7 @@ __device__ __forceinline__ SampleSet sample_set(const SampleArgs& p, size_t row)
     s.nucleus = s.p < 1.f;
     return s;
 }
-// The smallest value that `holds` is true of, where it is true of all values from there on: 64 keys at a time.
+// The smallest value that `holds` is true of, where it is true of all values from there on, or NaN: of none, not of an infinity either.  64 keys at a time.
 template <class F> __device__ __forceinline__ float sample_edge(F holds) {
     u32 lo = 0x007fffffu;      // (the key of -infinity: false)
     const u32 lane = threadIdx.x & 63;
@@ -198,7 +198,7 @@ template <class F> __device__ __forceinline__ float sample_edge(F holds) {
         const uint64_t key = (uint64_t)lo + ((uint64_t)(lane + 1) << shift);
         const uint64_t yes = __ballot(key > 0xff800000u || holds(sample_value((u32)key)));   // (the key of +infinity)
         const u32 n = yes ? (u32)__builtin_ctzll(yes) : 64u;
-        if (shift == 0) return sample_value((u32)min(lo + (uint64_t)n + 1, (uint64_t)0xff800000u));
+        if (shift == 0) return sample_value(lo + n + 1);      // (0xff800001 is a NaN)
         lo += n << shift;
     }
 }
@@ -351,7 +351,8 @@ __device__ __forceinline__ void sample_gather_body(const SampleArgs& p, uint64_t
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, part = blockIdx.x * JL_SA_PARTS + wave;
     int from, end;
     sample_part(p, part, from, end);
-    // by value: what goes into the list, from `list` on and below `sure`; what is kept for sure, from `sure` on (min_p's border in it)
+    // by value: what goes into the list, from `list` on and not from `below` on; what is kept for sure, from `sure` on (min_p's border in it; NaN: nothing, where the
+    // cut is in the largest's bin, which may hold infinities)
     const bool cuts = cut < JL_SA_BINS;
     auto append = [&](float x, u32 i) {
         const u32 at = atomicAdd(&told[8], 1u);
@@ -386,12 +387,16 @@ __device__ __forceinline__ void sample_gather_body(const SampleArgs& p, uint64_t
         return;
     }
     const float below = cuts ? sample_edge([&](float x) { return s.r.bin(x) < cut; }) : list;
-    const float sure = s.low > 0.f ? fmaxf(below, sample_edge([&](float x) { return s.r.weight(x) >= (double)s.low; })) : below;
+    float sure = below;
+    if (s.low > 0.f) {
+        const float edge = sample_edge([&](float x) { return s.r.weight(x) >= (double)s.low; });
+        if (edge > below) sure = edge;
+    }
     if (!cuts) list = sure;
     sample_range<64>(p, row, from, end, lane, [&](float x, u32 i) {
         if (x >= list) {
             if (x >= sure) sum += s.r.whole(x);
-            else if (x < below) append(x, i);
+            else if (!(x >= below)) append(x, i);
         }
     });
     if (cuts) flush();

@@ -33,3 +33,15 @@ def test_distances_beyond_the_type(dev, n, temperature, settings):
     x = (3.3e38 * rng.uniform(-1, 1, (6, n))).astype(np.float32)
     x[:, :2] = [3.3e38, -3.3e38]
     check(dev, x, quant.F32, rng.random(6).astype(np.float32), temperature=np.float32(temperature), **settings)
+
+
+@pytest.mark.parametrize("settings", [dict(), dict(top_k=6), dict(top_k=70), dict(top_k=700), dict(top_p=0.4), dict(top_p=0.4, min_p=0.2), dict(top_k=90, min_p=1.0),
+                                      dict(top_k=90, top_p=0.7, min_p=0.2)], ids=str)
+@pytest.mark.parametrize("many", [63, 64, 65, 480, 1024, 1025, 3000])
+def test_infinities_by_the_hundred(dev, many, settings):
+    """As many equals at the top as a list holds, or fewer or more, which are infinities, or the largest f32, or ones."""
+    rng = np.random.default_rng(many)
+    x = logits(rng, 6, 5001)
+    for r, top in enumerate((np.inf, np.inf, 3.4e38, 3.4e38, 30.0, 30.0)):
+        x[r, rng.permutation(5001)[:many]] = top
+    check(dev, x, quant.F32, rng.random(6).astype(np.float32), **settings)
