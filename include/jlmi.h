@@ -635,7 +635,8 @@ int jl_kv_read_dev(jl_ctx *ctx, const jl_kv_cache *cache, const jl_kv_rows *rows
  * down to 2^-38 of the largest weight times the largest scale that the token sees); a token's result does not depend on the other tokens of the call but in the last bits, by
  * where the cache was cut among the workgroups.  Infinities and NaNs in rows that a token does not see change nothing of its result.
  * Tokens of one sequence share the reads of its rows where they follow each other; how many of them are put together goes by ntok / n_seq, so a call over a few
- * of many sequences gives the rows of the table that it needs.  q 16-byte aligned, its stride a multiple of 16 bytes; n_head a multiple of n_kv.  out overlaps no
+ * of many sequences gives the rows of the table that it needs, and a prompt beside many single tokens is a call of its own (512 tokens of one sequence and 63 of others over up to
+ * 2048: 465 us in one call, 74 in two).  The form goes by what the table can hold: a table of little more than its sequences is faster.  q 16-byte aligned, its stride a multiple of 16 bytes; n_head a multiple of n_kv.  out overlaps no
  * other operand.  One launch or two; the workspace (jl_reserve_attend) is the context's: made by the first call whose positions are divided among workgroups (a call that gives each its
  * tokens needs none; which it is goes by sizes), of one size for a row width whatever the tokens, so jl_reserve_attend comes first where no call may allocate.  A buffer that is outgrown
  * lives until the context goes, so a captured graph that holds its address stays valid.  The reference's attention is another part of its device seam

@@ -676,7 +676,7 @@ struct AttendArgs {
     int wgs;                 // workgroups, or their shares of the chunks
     int whole;               // a unit a workgroup
     int window;
-    int out_vec;             // out's rows on 16-byte boundaries
+    int out_vec;             // out's rows on boundaries of four elements
     float scale, cap;
 };
 

@@ -8,8 +8,8 @@
 //
 // A step of 128 columns x 64 positions x 128 has 384 matrix instructions over four SIMDs (0.64 us at the peak rate), 256 vector instructions a wavefront, 290 KB through LDS, and
 // takes 1.65: each unit is busy a fifth to a third of the time, and the rest is the wavefronts' waits at the same places (bringing the rows is a quarter of a call: 8192 tokens 850 us,
-// 600 with rows that stand in LDS already).  Measured (32 heads over 8 of 128, bf16): a prompt of 8192 850 us, 647 TFLOP/s of the product's operations, 970 of the
-// instructions' (P in two pieces; a library's product of 8192^3 reaches 1400); of 2048 87, of 512 23; 3 x 683 over 2048 120.
+// 600 with rows that stand in LDS already).  Measured (32 heads over 8 of 128, bf16): a prompt of 8192 856 us, 642 TFLOP/s of the product's operations, 960 of the
+// instructions' (P in two pieces; a library's product of 8192^3 reaches 1400); of 2048 87, of 512 23; 3 x 683 over 2048 120 (f16 124, 8-bit rows with f32 q and out 172).
 // Tried and not kept: every other span of a unit in a workgroup of its own (3 x 683: 141 for 133), a raised priority around the products (134 to 139 for 133), keys by
 // loads that write LDS directly (150 for 133).
 #pragma once
