@@ -632,7 +632,7 @@ int jl_kv_read_dev(jl_ctx *ctx, const jl_kv_cache *cache, const jl_kv_rows *rows
  * q [ntok][q_stride] of q_type, out [ntok][out_stride] of out_type (JL_TYPE_F32, _F16, _BF16; strides in elements, 0: n_head * d), lse [ntok][n_head] f32.
  * A token that sees nothing (len 0, no such sequence, no pages) has zeros, lse -infinity or its sink.  len counts at most the table's positions.  Sums are f32, and q and the weights
  * keep 22 bits or more (16 of the weights over a bf16 cache where out is 16 bits wide; over f16 rows down to 2^-38 of the largest weight, over 8-bit rows weight times scale
- * down to 2^-38 of the largest weight times the largest scale that the token sees); a token's result does not depend on the other tokens of the call but in the last bits, by
+ * down to 2^-37 of the largest weight times the largest scale that the token sees); a token's result does not depend on the other tokens of the call but in the last bits, by
  * where the cache was cut among the workgroups.  Infinities and NaNs in rows that a token does not see change nothing of its result.
  * Tokens of one sequence share the reads of its rows where they follow each other; how many of them are put together goes by ntok / n_seq, so a call over a few
  * of many sequences gives the rows of the table that it needs, and a prompt beside many single tokens is a call of its own (512 tokens of one sequence and 63 of others over up to
@@ -667,7 +667,7 @@ int jl_reserve_attend(jl_ctx *ctx, int max_d);
  *     token = the first kept i, by index, for which the sum of the kept w up to i exceeds u times the sum of all kept
  *     prob = its w over that sum        (null: not wanted)
  * T of 0 or less, or no number: the largest, the first of several.  An infinity is larger than the rest and shares with its equals; -infinity and NaN are never
- * taken; a row without anything else gets the token n and prob 0.  u of 1 or more, or no number: the last kept.  w is f64's to 2^-44, sums are exact in 64 bits whole numbers, so a
+ * taken; a row without anything else gets the token n and prob 0.  u of 1 or more, or no number: the last kept.  w is f64's to 2^-44 (under 2^-45 it is nothing, and not taken), sums are exact in 64 bits whole numbers, so a
  * row's token does not depend on the call it is in.  temperature (null: ones), top_k, top_p, min_p (null: off) and u are device memory, [rows].
  * n up to 524288, rows up to 1048576.  Three or four launches for every 1024 rows; the workspace (jl_reserve_sample) is the context's, and a buffer that is outgrown lives
  * until the context goes. */
